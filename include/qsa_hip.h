@@ -485,6 +485,85 @@ int qsa_gdn_gated_norm(const void* o, const void* qkvz, int64_t qkvz_stride, con
                        float eps, int tokens, int key_heads, int value_heads, int head_dim,
                        void* y, void* stream);
 
+/* ------------------------------------------------------------------------ */
+/* A serving step over a few tokens: no counterpart in the reference          */
+/* ------------------------------------------------------------------------ */
+
+/* Linear layer with 4-bit weights: y[m][n] = round(sum_k x[m][k] *
+ * (c[n][k] - z[n][k / group]) * s[n][k / group] + bias[n]), fp32 sums.
+ * x [rows, in_features], y [rows, out_features], scales and bias bf16 (is_fp16
+ * 0) or fp16 (1), unit column strides; codes 0..15. The weight is laid out in
+ * tiles of 16 outputs x 128 inputs (out_features and in_features rounded up):
+ *   codes  [n tiles][k tiles][lane 64][word 4] uint32, 16-byte aligned: lane
+ *          16 g + n, word j holds output n's inputs 32 j + 8 g + 0..7 of the
+ *          tile, input 2 p in bits 4 p.., input 2 p + 1 in bits 16 + 4 p..;
+ *   scales [n tiles][groups][16]; zeros [n tiles][groups][16] uint8 0..15 or
+ *          null (8 everywhere), groups = k tiles * 128 / group_size.
+ * group_size 32, 64 or 128. bias may be null. A row of x that holds an infinity
+ * or NaN (or, in bf16, values past 2^112) has no defined result; other rows are
+ * not touched by it. Any alignment and row stride; 16-byte aligned rows and
+ * in_features a multiple of 8 are fastest. */
+int qsa_int4_linear(const void* x, int64_t x_row_stride, const void* codes, const void* scales,
+                    const void* zeros, const void* bias, void* y, int64_t y_row_stride, int rows,
+                    int out_features, int in_features, int group_size, int is_fp16, void* stream);
+
+/* Attention of drafted token trees over the paged cache. Request b owns rows
+ * query_start_loc[b] .. query_start_loc[b + 1] - 1 of q [rows, num_q_heads,
+ * head_dim] bf16, its nodes in order; cache positions 0 .. context_lens[b] - 1
+ * hold its committed tokens and position context_lens[b] + j node j (K/V [blocks,
+ * page, kv_heads, head_dim] bf16 through block_table). A row sees every
+ * committed position and node j of its request where bit j % 32 of its ancestor
+ * word j / 32 is set (ancestors [rows, ancestor_words]); nodes past the words
+ * are not seen, nor are positions without a page in the cache. out = softmax of
+ * the scaled scores times V, times sigmoid(gate) if gate is given, rounded once
+ * to bf16; zeros for a row that sees nothing. Rows of no request are not written.
+ * max_query_len bounds a request's nodes (further ones are not computed);
+ * max_context_len should bound context_lens: it shapes the launch only.
+ * head_dim 64 or 128. The workspace (0 bytes: none) holds the call's partial
+ * results until its work is done: calls that may overlap need one each. */
+size_t qsa_tree_attention_workspace_bytes(int rows, int requests, int num_q_heads,
+                                          int num_kv_heads, int head_dim, int max_query_len,
+                                          int max_context_len);
+int qsa_tree_attention(const void* q, int64_t q_row_stride, int64_t q_head_stride, int rows,
+                       int num_q_heads, int head_dim, const void* k_cache, int64_t k_block_stride,
+                       int64_t k_token_stride, int64_t k_head_stride, const void* v_cache,
+                       int64_t v_block_stride, int64_t v_token_stride, int64_t v_head_stride,
+                       int num_blocks, int page_size, int num_kv_heads,
+                       const int32_t* block_table, int64_t table_row_stride, int table_width,
+                       int num_requests, const int32_t* context_lens,
+                       const int32_t* query_start_loc, const int32_t* ancestors,
+                       int64_t ancestor_row_stride, int ancestor_words, void* out,
+                       int64_t out_row_stride, int64_t out_head_stride, const void* gate,
+                       int64_t gate_row_stride, int64_t gate_head_stride, int64_t gate_dim_stride,
+                       int max_query_len, int max_context_len, void* workspace,
+                       size_t workspace_bytes, void* stream);
+
+/* Rules on logits before sampling, fp32 out [rows, vocab] (may be the logits
+ * themselves when those are fp32). Column v is token vocab_start + v (a
+ * vocabulary shard). Row r belongs to request token_to_req[r] (null: r); rows of
+ * no request get their grammar mask alone. In this order:
+ *   tokens of the request's history (history [requests, history_width], the
+ *   first history_lens[b] valid, the first prompt_lens[b] the prompt) or, for a
+ *   drafted node, of its visible nodes: y = x > 0 ? x / repetition[b] : x *
+ *   repetition[b]; of those past the prompt, with count c: y -= frequency[b] * c
+ *   and y -= presence[b];
+ *   y += bias_values[b][i] for every i with bias_ids[b][i] == token (list order);
+ *   y = -inf where bit v % 32 of word v / 32 of allowed [rows, words] is 0.
+ * Ids outside the shard (negative ones pad) are passed over. Null pointers leave
+ * a rule out. ancestors [rows, ancestor_words] as in qsa_tree_attention, over
+ * draft_tokens [rows] and query_start_loc. logits_type: 0 fp32, 1 bf16, 2 fp16. */
+int qsa_process_logits(const void* logits, int logits_type, int64_t logits_row_stride, float* out,
+                       int64_t out_row_stride, int rows, int vocab, int64_t vocab_start,
+                       const int32_t* token_to_req, int num_requests, const int32_t* history,
+                       int64_t history_row_stride, int history_width, const int32_t* history_lens,
+                       const int32_t* prompt_lens, const float* repetition,
+                       const float* frequency, const float* presence, const int32_t* bias_ids,
+                       int64_t bias_id_row_stride, const float* bias_values,
+                       int64_t bias_value_row_stride, int num_biases, const int32_t* allowed,
+                       int64_t allowed_row_stride, const int32_t* draft_tokens,
+                       const int32_t* ancestors, int64_t ancestor_row_stride, int ancestor_words,
+                       const int32_t* query_start_loc, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

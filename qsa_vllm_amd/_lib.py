@@ -177,6 +177,21 @@ SIGNATURES = {
                                       c_ptr, c_size, c_ptr]),
     "qsa_gdn_gated_norm": (c_i32, [c_ptr, c_ptr, c_i64, c_ptr, ctypes.c_float, c_i32, c_i32,
                                    c_i32, c_i32, c_ptr, c_ptr]),
+    "qsa_int4_linear": (c_i32, [
+        c_ptr, c_i64, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_i64, c_i32, c_i32,
+        c_i32, c_i32, c_i32, c_ptr]),
+    "qsa_tree_attention_workspace_bytes": (c_size, [
+        c_i32, c_i32, c_i32, c_i32, c_i32, c_i32, c_i32]),
+    "qsa_tree_attention": (c_i32, [
+        c_ptr, c_i64, c_i64, c_i32, c_i32, c_i32, c_ptr, c_i64, c_i64, c_i64,
+        c_ptr, c_i64, c_i64, c_i64, c_i32, c_i32, c_i32, c_ptr, c_i64, c_i32,
+        c_i32, c_ptr, c_ptr, c_ptr, c_i64, c_i32, c_ptr, c_i64, c_i64, c_ptr,
+        c_i64, c_i64, c_i64, c_i32, c_i32, c_ptr, c_size, c_ptr]),
+    "qsa_process_logits": (c_i32, [
+        c_ptr, c_i32, c_i64, c_ptr, c_i64, c_i32, c_i32, c_i64, c_ptr, c_i32,
+        c_ptr, c_i64, c_i32, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_i64,
+        c_ptr, c_i64, c_i32, c_ptr, c_i64, c_ptr, c_ptr, c_i64, c_i32, c_ptr,
+        c_ptr]),
 }
 
 

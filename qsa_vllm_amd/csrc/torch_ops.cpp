@@ -787,6 +787,194 @@ void expand_block_indices_impl(const Tensor& block_indices, const Tensor& pos,
         "qsa_expand_block_indices");
 }
 
+// --- a serving step over a few tokens -------------------------------------------
+
+// Rows of a matrix: unit column stride and no overlap of rows that are written.
+void rows2d(const Tensor& t, const char* name) {
+  QSA_REQUIRE(t.dim() == 2 && (t.size(1) <= 1 || t.stride(1) == 1), name,
+              " must be [rows, columns] with unit column stride");
+}
+void own_rows(const Tensor& t, const char* name) {
+  QSA_REQUIRE(t.size(0) <= 1 || t.stride(0) >= t.size(1), name, " must not have overlapping rows");
+}
+int as_int(int64_t v, const char* name) {
+  QSA_REQUIRE(v >= 0 && v <= INT32_MAX, name, " is out of range: ", v);
+  return (int)v;
+}
+
+void int4_linear_impl(const Tensor& x, const Tensor& codes, const Tensor& scales,
+                      const OptTensor& zeros, const OptTensor& bias, const Tensor& out,
+                      int64_t in_features, int64_t out_features, int64_t group_size) {
+  const auto dev = on_gpu({&x, &codes, &scales, &out, opt(zeros), opt(bias)});
+  const at::ScalarType type = x.scalar_type();
+  QSA_REQUIRE(type == at::kBFloat16 || type == at::kHalf, "x must be bf16 or fp16, got ", type);
+  rows2d(x, "x");
+  QSA_REQUIRE(in_features > 0 && out_features >= 0, "the weight has no input features");
+  QSA_REQUIRE(x.size(1) == in_features, "x must have ", in_features, " columns, got ", x.size(1));
+  QSA_REQUIRE(group_size == 32 || group_size == 64 || group_size == 128,
+              "group size must be 32, 64 or 128, got ", group_size);
+  const int64_t n_tiles = (out_features + 15) / 16, k_tiles = (in_features + 127) / 128;
+  const int64_t groups = k_tiles * (128 / group_size);
+  dtype(codes, at::kInt, "codes");
+  QSA_REQUIRE(codes.is_contiguous() && codes.numel() == n_tiles * k_tiles * 256,
+              "codes must be the packed weight's");
+  dtype(scales, type, "scales");
+  QSA_REQUIRE(scales.is_contiguous() && scales.numel() == n_tiles * groups * 16,
+              "scales must be the packed weight's");
+  if (zeros) {
+    dtype(*zeros, at::kByte, "zeros");
+    QSA_REQUIRE(zeros->is_contiguous() && zeros->numel() == n_tiles * groups * 16,
+                "zeros must be the packed weight's");
+  }
+  if (bias) vec(*bias, type, "bias");
+  if (bias) QSA_REQUIRE(bias->numel() == out_features, "bias must have ", out_features, " entries");
+  dtype(out, type, "out");
+  rows2d(out, "out");
+  own_rows(out, "out");
+  QSA_REQUIRE(out.size(0) == x.size(0) && out.size(1) == out_features,
+              "out must be [rows, out_features]");
+  if (x.size(0) == 0 || out_features == 0) return;
+  c10::hip::HIPGuard guard(dev.index());
+  check(qsa_int4_linear(x.data_ptr(), sdim(x, 0), codes.data_ptr(), scales.data_ptr(),
+                        ptr_or_null(opt(zeros)), ptr_or_null(opt(bias)), out.data_ptr(),
+                        sdim(out, 0), as_int(x.size(0), "rows"),
+                        as_int(out_features, "out_features"), as_int(in_features, "in_features"),
+                        (int)group_size, type == at::kHalf ? 1 : 0, stream_of(dev)),
+        "qsa_int4_linear");
+}
+
+// Ancestor words of the rows of drafted trees.
+void ancestor_words(const Tensor& t, int64_t rows) {
+  dtype(t, at::kInt, "ancestors");
+  rows2d(t, "ancestors");
+  QSA_REQUIRE(t.size(0) >= rows, "ancestors must have a row for each query row");
+}
+
+void tree_attention_impl(const Tensor& q, const Tensor& k_cache, const Tensor& v_cache,
+                         const Tensor& block_table, const Tensor& context_lens,
+                         const Tensor& query_start_loc, const Tensor& ancestors, const Tensor& out,
+                         const OptTensor& output_gate, int64_t max_query_len,
+                         int64_t max_context_len) {
+  const auto dev = on_gpu({&q, &k_cache, &v_cache, &block_table, &context_lens, &query_start_loc,
+                           &ancestors, &out, opt(output_gate)});
+  dtype(q, at::kBFloat16, "q");
+  dtype(k_cache, at::kBFloat16, "k_cache");
+  dtype(v_cache, at::kBFloat16, "v_cache");
+  QSA_REQUIRE(q.dim() == 3 && q.stride(2) == 1, "q must be [rows, heads, dim] with unit dim stride");
+  const int64_t rows = q.size(0), hq = q.size(1), dim = q.size(2);
+  QSA_REQUIRE(k_cache.dim() == 4 && v_cache.dim() == 4 && k_cache.sizes() == v_cache.sizes(),
+              "k_cache/v_cache must be [blocks, page, kv_heads, dim] of one shape");
+  QSA_REQUIRE(k_cache.stride(3) == 1 && v_cache.stride(3) == 1, "k/v caches need a unit dim stride");
+  QSA_REQUIRE(k_cache.size(3) == dim, "cache head dim must match q");
+  check_out(out, rows, hq, dim);
+  table2d(block_table, "block_table");
+  const int64_t requests = block_table.size(0);
+  vec(context_lens, at::kInt, "context_lens", requests);
+  vec(query_start_loc, at::kInt, "query_start_loc", requests + 1);
+  ancestor_words(ancestors, rows);
+  const GateStrides g = gate_strides(output_gate, rows, hq, dim);
+  const int most = as_int(max_query_len, "max_query_len");
+  const int longest = as_int(max_context_len, "max_context_len");
+  if (rows == 0 || requests == 0) return;
+  c10::hip::HIPGuard guard(dev.index());
+  const int kv_heads = as_int(k_cache.size(2), "kv heads");
+  const size_t ws_bytes = qsa_tree_attention_workspace_bytes(
+      as_int(rows, "rows"), (int)requests, (int)hq, kv_heads, (int)dim, most, longest);
+  Tensor ws = ws_bytes ? workspace(ws_bytes, dev) : Tensor();
+  check(qsa_tree_attention(
+            q.data_ptr(), sdim(q, 0), sdim(q, 1), (int)rows, (int)hq, (int)dim, k_cache.data_ptr(),
+            sdim(k_cache, 0), sdim(k_cache, 1), sdim(k_cache, 2), v_cache.data_ptr(),
+            sdim(v_cache, 0), sdim(v_cache, 1), sdim(v_cache, 2),
+            as_int(k_cache.size(0), "blocks"), as_int(k_cache.size(1), "page size"), kv_heads,
+            at_elem<int32_t>(block_table), block_table.stride(0),
+            as_int(block_table.size(1), "table width"), as_int(requests, "requests"),
+            at_elem<int32_t>(context_lens), at_elem<int32_t>(query_start_loc),
+            at_elem<int32_t>(ancestors), ancestors.stride(0),
+            as_int(ancestors.size(1), "ancestor words"), out.data_ptr(), sdim(out, 0), sdim(out, 1),
+            ptr_or_null(opt(output_gate)), g.row, g.head, g.dim, most, longest,
+            ws_bytes ? ws.data_ptr() : nullptr, ws_bytes, stream_of(dev)),
+        "qsa_tree_attention");
+}
+
+void process_logits_impl(const Tensor& logits, const Tensor& out, const OptTensor& token_to_req,
+                         int64_t num_requests, const OptTensor& history,
+                         const OptTensor& history_lens, const OptTensor& prompt_lens,
+                         const OptTensor& repetition, const OptTensor& frequency,
+                         const OptTensor& presence, const OptTensor& bias_ids,
+                         const OptTensor& bias_values, const OptTensor& allowed,
+                         int64_t vocab_start, const OptTensor& draft_tokens,
+                         const OptTensor& ancestors, const OptTensor& query_start_loc) {
+  const auto dev = on_gpu({&logits, &out, opt(token_to_req), opt(history), opt(history_lens),
+                           opt(prompt_lens), opt(repetition), opt(frequency), opt(presence),
+                           opt(bias_ids), opt(bias_values), opt(allowed), opt(draft_tokens),
+                           opt(ancestors), opt(query_start_loc)});
+  const at::ScalarType type = logits.scalar_type();
+  QSA_REQUIRE(type == at::kFloat || type == at::kBFloat16 || type == at::kHalf,
+              "logits must be fp32, bf16 or fp16, got ", type);
+  rows2d(logits, "logits");
+  const int64_t rows = logits.size(0), vocab = logits.size(1);
+  dtype(out, at::kFloat, "out");
+  rows2d(out, "out");
+  own_rows(out, "out");
+  QSA_REQUIRE(out.size(0) == rows && out.size(1) == vocab, "out must have the shape of logits");
+  QSA_REQUIRE(vocab_start >= 0 && vocab_start <= INT32_MAX, "vocab_start is out of range");
+  if (token_to_req) vec(*token_to_req, at::kInt, "token_to_req", rows);
+  else QSA_REQUIRE(num_requests >= rows, "without token_to_req every row is a request: ", rows,
+                   " rows, ", num_requests, " requests");
+  QSA_REQUIRE(!history == !history_lens, "history and history_lens go together");
+  QSA_REQUIRE(!prompt_lens || history, "prompt_lens needs a history");
+  if (history) {
+    dtype(*history, at::kInt, "history");
+    rows2d(*history, "history");
+    QSA_REQUIRE(history->size(0) >= num_requests, "history must have a row for each request");
+    vec(*history_lens, at::kInt, "history_lens", num_requests);
+  }
+  if (prompt_lens) vec(*prompt_lens, at::kInt, "prompt_lens", num_requests);
+  if (repetition) vec(*repetition, at::kFloat, "repetition", num_requests);
+  if (frequency) vec(*frequency, at::kFloat, "frequency", num_requests);
+  if (presence) vec(*presence, at::kFloat, "presence", num_requests);
+  QSA_REQUIRE(!bias_ids == !bias_values, "bias_ids and bias_values go together");
+  if (bias_ids) {
+    dtype(*bias_ids, at::kInt, "bias_ids");
+    rows2d(*bias_ids, "bias_ids");
+    dtype(*bias_values, at::kFloat, "bias_values");
+    rows2d(*bias_values, "bias_values");
+    QSA_REQUIRE(bias_ids->size(0) >= num_requests && bias_values->size(0) >= num_requests &&
+                    bias_ids->size(1) == bias_values->size(1),
+                "bias_ids and bias_values must be [requests, biases]");
+  }
+  if (allowed) {
+    dtype(*allowed, at::kInt, "allowed");
+    rows2d(*allowed, "allowed");
+    QSA_REQUIRE(allowed->size(0) >= rows && allowed->size(1) >= (vocab + 31) / 32,
+                "allowed must be [rows, ceil(vocab / 32)]");
+  }
+  QSA_REQUIRE(!ancestors == !draft_tokens && !ancestors == !query_start_loc,
+              "ancestors, draft_tokens and query_start_loc go together");
+  if (ancestors) {
+    ancestor_words(*ancestors, rows);
+    vec(*draft_tokens, at::kInt, "draft_tokens", rows);
+    vec(*query_start_loc, at::kInt, "query_start_loc", num_requests + 1);
+  }
+  if (rows == 0 || vocab == 0) return;
+  c10::hip::HIPGuard guard(dev.index());
+  auto row_of = [](const OptTensor& t) { return t ? t->stride(0) : 0; };
+  auto cols_of = [](const OptTensor& t, const char* name) { return t ? as_int(t->size(1), name) : 0; };
+  auto i32 = [](const OptTensor& t) { return t ? at_elem<int32_t>(*t) : nullptr; };
+  auto f32 = [](const OptTensor& t) { return t ? at_elem<float>(*t) : nullptr; };
+  check(qsa_process_logits(
+            logits.data_ptr(), type == at::kFloat ? 0 : type == at::kBFloat16 ? 1 : 2,
+            sdim(logits, 0), at_elem<float>(out), sdim(out, 0), as_int(rows, "rows"),
+            as_int(vocab, "vocab"), vocab_start, i32(token_to_req),
+            as_int(num_requests, "requests"), i32(history), row_of(history),
+            cols_of(history, "history width"), i32(history_lens), i32(prompt_lens),
+            f32(repetition), f32(frequency), f32(presence), i32(bias_ids), row_of(bias_ids),
+            f32(bias_values), row_of(bias_values), cols_of(bias_ids, "biases"), i32(allowed),
+            row_of(allowed), i32(draft_tokens), i32(ancestors), row_of(ancestors),
+            cols_of(ancestors, "ancestor words"), i32(query_start_loc), stream_of(dev)),
+        "qsa_process_logits");
+}
+
 }  // namespace
 
 TORCH_LIBRARY_FRAGMENT(yulan_qsa_kernels, m) {
@@ -852,6 +1040,19 @@ TORCH_LIBRARY_FRAGMENT(yulan_qsa_kernels, m) {
       "Tensor q, Tensor k_cache, Tensor v_cache, Tensor table, Tensor token_to_req, "
       "Tensor positions, Tensor sequence_lengths, int count, int columns, int ratio, "
       "Tensor(a!) indices, Tensor(b!) counts, Tensor(c!) out, Tensor? output_gate) -> ()");
+  m.def(
+      "int4_linear(Tensor x, Tensor codes, Tensor scales, Tensor? zeros, Tensor? bias, "
+      "Tensor(a!) out, int in_features, int out_features, int group_size) -> ()");
+  m.def(
+      "tree_attention(Tensor q, Tensor k_cache, Tensor v_cache, Tensor block_table, "
+      "Tensor context_lens, Tensor query_start_loc, Tensor ancestors, Tensor(a!) out, "
+      "Tensor? output_gate, int max_query_len, int max_context_len) -> ()");
+  m.def(
+      "process_logits(Tensor logits, Tensor(a!) out, Tensor? token_to_req, int num_requests, "
+      "Tensor? history, Tensor? history_lens, Tensor? prompt_lens, Tensor? repetition, "
+      "Tensor? frequency, Tensor? presence, Tensor? bias_ids, Tensor? bias_values, "
+      "Tensor? allowed, int vocab_start, Tensor? draft_tokens, Tensor? ancestors, "
+      "Tensor? query_start_loc) -> ()");
 }
 
 TORCH_LIBRARY_IMPL(yulan_qsa_kernels, CUDA, m) {
@@ -870,6 +1071,9 @@ TORCH_LIBRARY_IMPL(yulan_qsa_kernels, CUDA, m) {
   m.impl("sparse_attention_merge", &sparse_attention_merge_impl);
   m.impl("decode_select_attend", &decode_select_attend_impl);
   m.impl("decode_layer", &decode_layer_impl);
+  m.impl("int4_linear", &int4_linear_impl);
+  m.impl("tree_attention", &tree_attention_impl);
+  m.impl("process_logits", &process_logits_impl);
 }
 
 // Shape-only tracing (fake / meta tensors): the ops mutate their outputs in
@@ -920,4 +1124,14 @@ TORCH_LIBRARY_IMPL(yulan_qsa_kernels, Meta, m) {
             const Tensor&, const Tensor&, int64_t, int64_t, int64_t, bool, bool) {});
   m.impl("indexer_norm_rope", [](const Tensor&, const Tensor&, const Tensor&, const Tensor&,
                                  double, int64_t, const Tensor&) {});
+  m.impl("int4_linear", [](const Tensor&, const Tensor&, const Tensor&, const OptTensor&,
+                           const OptTensor&, const Tensor&, int64_t, int64_t, int64_t) {});
+  m.impl("tree_attention", [](const Tensor&, const Tensor&, const Tensor&, const Tensor&,
+                              const Tensor&, const Tensor&, const Tensor&, const Tensor&,
+                              const OptTensor&, int64_t, int64_t) {});
+  m.impl("process_logits",
+         [](const Tensor&, const Tensor&, const OptTensor&, int64_t, const OptTensor&,
+            const OptTensor&, const OptTensor&, const OptTensor&, const OptTensor&,
+            const OptTensor&, const OptTensor&, const OptTensor&, const OptTensor&, int64_t,
+            const OptTensor&, const OptTensor&, const OptTensor&) {});
 }

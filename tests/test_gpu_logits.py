@@ -1,0 +1,289 @@
+"""Rules on logits on the GPU against a 64-bit statement, token by token.
+
+Tolerance: fp32 operations in the stated order, each off by 2^-24 of a value no
+larger than m = |x| max(r, 1 / r) + f c + p + sum |bias|: at most five of them
+and one per listed bias (2^-149 for subnormal results)."""
+
+import math
+
+import pytest
+import torch
+
+from qsa_vllm_amd.ops import process_logits, tree_ancestors
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+
+
+def _rules(gen, nreq, vocab, width, nb, first=0, total=None):
+    total = total or vocab
+    lens = torch.randint(0, width + 1, (nreq,), generator=gen, dtype=torch.int32)
+    lens[0] = width
+    return dict(
+        history=(torch.rand(nreq, width, generator=gen) ** 2 * total).to(torch.int32),
+        history_lens=lens, prompt_lens=(lens * torch.rand(nreq, generator=gen)).to(torch.int32),
+        repetition=torch.rand(nreq, generator=gen) + 0.7,
+        frequency=torch.rand(nreq, generator=gen) - 0.2,
+        presence=torch.rand(nreq, generator=gen) - 0.2,
+        bias_ids=torch.randint(-2, total, (nreq, nb), generator=gen, dtype=torch.int32) if nb else None,
+        bias_values=torch.randn(nreq, nb, generator=gen) * 3 if nb else None, vocab_start=first)
+
+
+def _want(logits, rules, token_to_req=None, allowed=None, draft_tokens=None, ancestors=None,
+          query_start_loc=None):
+    rows, vocab = logits.shape
+    y = logits.double().clone()
+    tol = torch.full((rows, vocab), 2.0 ** -149, dtype=torch.float64)
+    get = rules.get
+    first = get("vocab_start", 0)
+    sized = [t for t in (get("history"), get("repetition"), get("frequency"), get("presence"),
+                         get("bias_ids")) if t is not None]
+    nreq = min((t.shape[0] for t in sized), default=rows)
+    for row in range(rows):
+        b = row if token_to_req is None else int(token_to_req[row])
+        if 0 <= b < nreq:
+            ever, said = {}, {}
+            if get("history") is not None:
+                n = max(0, min(int(rules["history_lens"][b]), rules["history"].shape[1]))
+                prompt = int(get("prompt_lens")[b]) if get("prompt_lens") is not None else 0
+                for i, t in enumerate(rules["history"][b, :n].tolist()):
+                    ever[t] = True
+                    if i >= prompt:
+                        said[t] = said.get(t, 0) + 1
+            if ancestors is not None:
+                s, e = int(query_start_loc[b]), int(query_start_loc[b + 1])
+                for j in range(min(e - s, 32 * ancestors.shape[1])):
+                    if (int(ancestors[row, j // 32]) >> (j % 32)) & 1:
+                        t = int(draft_tokens[s + j])
+                        ever[t] = True
+                        said[t] = said.get(t, 0) + 1
+            r = float(get("repetition")[b]) if get("repetition") is not None else 1.0
+            f = float(get("frequency")[b]) if get("frequency") is not None else 0.0
+            p = float(get("presence")[b]) if get("presence") is not None else 0.0
+            for t in ever:
+                if 0 <= t - first < vocab:
+                    x = float(y[row, t - first])
+                    c = said.get(t, 0)
+                    z = (x / r if x > 0 else x * r) - f * c - (p if c else 0.0)
+                    y[row, t - first] = z
+                    m = abs(x) * max(r, 1 / r) + abs(f) * c + abs(p)
+                    tol[row, t - first] += 5 * 2.0 ** -24 * m if math.isfinite(m) else 0
+            if get("bias_ids") is not None:
+                for t, value in zip(rules["bias_ids"][b].tolist(), rules["bias_values"][b].tolist()):
+                    if 0 <= t - first < vocab:
+                        before = float(y[row, t - first])
+                        y[row, t - first] = before + value
+                        m = abs(before) + abs(value)
+                        tol[row, t - first] += 2 * 2.0 ** -24 * m if math.isfinite(m) else 0
+        if allowed is not None:
+            for v in range(vocab):
+                if not (int(allowed[row, v // 32]) >> (v % 32)) & 1:
+                    y[row, v] = -math.inf
+    return y, tol
+
+
+def _run(logits, rules, **kw):
+    move = lambda t: t.to(DEV) if isinstance(t, torch.Tensor) else t
+    return process_logits(move(logits), **{k: move(v) for k, v in {**rules, **kw}.items()})
+
+
+def _check(got, want):
+    y, tol = want
+    g = got.cpu().double()
+    fine = torch.isfinite(y)
+    assert torch.equal(g[~fine].nan_to_num(nan=7.0), y[~fine].nan_to_num(nan=7.0))
+    assert ((g - y).abs()[fine] <= tol[fine]).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("rows,vocab,width,nb", [
+    (1, 1, 5, 1), (1, 31, 0, 0), (3, 64, 1, 3), (4, 1000, 300, 40), (2, 8191, 50, 7),
+    (2, 8192, 2000, 0), (2, 8193, 900, 600), (3, 16421, 5000, 33), (1, 40000, 20, 2)])
+def test_matches_64_bits(rows, vocab, width, nb, dtype):
+    gen = torch.Generator().manual_seed(rows + vocab)
+    rules = _rules(gen, rows, vocab, width, nb)
+    logits = (torch.randn(rows, vocab, generator=gen) * 4).to(dtype)
+    allowed = torch.randint(-2**31, 2**31, (rows, -(-vocab // 32)), generator=gen).to(torch.int32)
+    _check(_run(logits, rules, allowed=allowed), _want(logits, rules, allowed=allowed))
+
+
+def test_each_rule_alone_and_none():
+    gen = torch.Generator().manual_seed(1)
+    full = _rules(gen, 3, 500, 60, 9)
+    logits = torch.randn(3, 500, generator=gen)
+    seen = ("history", "history_lens")
+    for keys in ((), ("bias_ids", "bias_values"), seen + ("repetition",), seen + ("frequency",),
+                 seen + ("presence",), seen + ("prompt_lens", "frequency", "repetition"), seen,
+                 ("repetition",)):
+        rules = {k: full[k] for k in keys}
+        _check(_run(logits, rules), _want(logits, rules))
+    assert torch.equal(_run(logits, {}).cpu(), logits)
+    half = logits.bfloat16()
+    assert torch.equal(_run(half, {}).cpu(), half.float())
+
+
+def test_shard_takes_its_own_tokens():
+    """Two shards of a vocabulary give what the whole does; ids of the other one
+    are passed over."""
+    gen = torch.Generator().manual_seed(2)
+    rules = _rules(gen, 4, 3000, 400, 50)
+    logits = torch.randn(4, 3000, generator=gen)
+    whole = _run(logits, rules)
+    for first, last in ((0, 1700), (1700, 3000), (1001, 1003)):
+        part = _run(logits[:, first:last].contiguous(), {**rules, "vocab_start": first})
+        assert torch.equal(part, whole[:, first:last])
+
+
+def test_listed_twice_adds_in_order():
+    ids = torch.tensor([[5, 7, 5, -1, 5, 7, 900, 2**31 - 1, 4]], dtype=torch.int32)
+    values = torch.tensor([[1e8, 0.25, 1.0, 3.0, -1e8, 0.5, 2.0, 9.0, float("-inf")]])
+    got = _run(torch.zeros(1, 10), dict(bias_ids=ids, bias_values=values))
+    # in fp32 and list order: (1e8 + 1) - 1e8 = 0
+    assert got[0].tolist() == [0, 0, 0, 0, -math.inf, 0.0, 0, 0.75, 0, 0]
+    many = torch.randint(0, 40, (2, 1500), dtype=torch.int32,
+                         generator=torch.Generator().manual_seed(3))
+    vals = torch.randint(-8, 9, (2, 1500), generator=torch.Generator().manual_seed(4)).float()
+    want = torch.zeros(2, 50).scatter_add_(1, many.long(), vals)     # whole numbers: any order
+    assert torch.equal(_run(torch.zeros(2, 50), dict(bias_ids=many, bias_values=vals)).cpu(), want)
+    nan = torch.tensor([[0xFFFFFFFF - (1 << 32)]], dtype=torch.int32).view(torch.float32)
+    got = _run(torch.zeros(1, 4), dict(bias_ids=ids[:, 8:], bias_values=nan)).cpu()
+    assert not got.isnan().any()                                     # id 4 is past the row
+    got = _run(torch.zeros(1, 5), dict(bias_ids=ids[:, 8:], bias_values=nan)).cpu()
+    assert got.isnan().tolist() == [[False] * 4 + [True]]
+
+
+def test_special_logits():
+    """Infinities and NaN: masked ones become -inf, others follow the rules."""
+    inf, nan = math.inf, math.nan
+    logits = torch.tensor([[inf, -inf, nan, 1.0, inf, -inf, nan, -0.0]])
+    rules = dict(history=torch.tensor([[0, 1, 2, 7, 7]], dtype=torch.int32),
+                 history_lens=torch.tensor([5], dtype=torch.int32),
+                 repetition=torch.tensor([2.0]), frequency=torch.tensor([0.5]),
+                 presence=torch.tensor([1.0]))
+    got = _run(logits, rules, allowed=torch.tensor([[0b10001111]], dtype=torch.int32)).cpu()[0]
+    assert got[0] == inf and got[1] == -inf and got[2].isnan() and got[3] == 1.0
+    assert (got[4:7] == -inf).all() and got[7] == -2.0
+    none = _run(logits, rules, allowed=torch.zeros(1, 1, dtype=torch.int32))
+    assert (none == -inf).all()                    # a row that allows nothing
+
+
+def test_rows_of_requests_and_padding():
+    """Rows in any order, several to a request, padding rows: no penalties."""
+    gen = torch.Generator().manual_seed(5)
+    rules = _rules(gen, 3, 9000, 700, 20)
+    req = torch.tensor([2, 0, -1, 2, 3, 1, 1, -2**31, 0], dtype=torch.int32)
+    logits = torch.randn(9, 9000, generator=gen)
+    allowed = torch.randint(-2**31, 2**31, (9, 282), generator=gen).to(torch.int32)
+    _check(_run(logits, rules, token_to_req=req, allowed=allowed),
+           _want(logits, rules, token_to_req=req, allowed=allowed))
+
+
+def test_lengths_out_of_range_are_kept_inside():
+    gen = torch.Generator().manual_seed(6)
+    rules = _rules(gen, 3, 300, 50, 0)
+    rules["history_lens"] = torch.tensor([1000, -4, 50], dtype=torch.int32)
+    rules["prompt_lens"] = torch.tensor([2000, 3, -9], dtype=torch.int32)
+    rules["history"][2, ::3] = -1
+    rules["history"][2, 1::3] = 2**31 - 1
+    logits = torch.randn(3, 300, generator=gen)
+    _check(_run(logits, rules), _want(logits, rules))
+
+
+@pytest.mark.parametrize("nodes", [[1], [5, 0, 9], [33, 64, 2], [70]])
+def test_drafted_nodes_count_their_ancestors(nodes):
+    gen = torch.Generator().manual_seed(sum(nodes))
+    nreq, rows, vocab = len(nodes), sum(nodes), 8300
+    qsl = torch.tensor([0] + torch.tensor(nodes).cumsum(0).tolist(), dtype=torch.int32)
+    parents = torch.tensor([int(torch.randint(-1, j, (1,), generator=gen)) if j else -1
+                            for t in nodes for j in range(t)])
+    anc = tree_ancestors(parents, qsl, max(nodes))
+    rules = _rules(gen, nreq, vocab, 200, 5, first=100, total=vocab + 200)
+    draft = (torch.rand(rows, generator=gen) ** 3 * 300).to(torch.int32)   # repeats, some outside
+    req = torch.repeat_interleave(torch.arange(nreq, dtype=torch.int32), torch.tensor(nodes))
+    logits = torch.randn(rows, vocab, generator=gen).bfloat16()
+    kw = dict(token_to_req=req, draft_tokens=draft, ancestors=anc, query_start_loc=qsl)
+    _check(_run(logits, rules, **kw), _want(logits, rules, **kw))
+    # without a history the path alone counts
+    path = {k: rules[k] for k in ("frequency", "presence", "repetition", "vocab_start")}
+    _check(_run(logits, path, **kw), _want(logits, path, **kw))
+
+
+def test_strides_alignment_and_in_place():
+    gen = torch.Generator().manual_seed(7)
+    rules = _rules(gen, 3, 777, 90, 8)
+    for dtype in (torch.float32, torch.bfloat16):
+        for offset, stride in ((0, 780), (1, 801), (5, 777), (4, 778)):
+            big = torch.randn(4 * stride, generator=gen).to(dtype)
+            x = big.as_strided((3, 777), (stride, 1), offset)
+            got = process_logits(big.to(DEV).as_strided((3, 777), (stride, 1), offset),
+                                 **{k: v.to(DEV) if isinstance(v, torch.Tensor) else v
+                                    for k, v in rules.items()})
+            _check(got, _want(x, rules))
+    wide = torch.full((5, 1000), 9.0, device=DEV)
+    wide[1:4, 11:788] = x.float().to(DEV)
+    inner = wide[1:4, 11:788]
+    want = _run(x.float(), rules)
+    moved = {k: v.to(DEV) if isinstance(v, torch.Tensor) else v for k, v in rules.items()}
+    assert process_logits(inner, inner, **moved) is inner
+    assert torch.equal(inner, want)
+    wide[1:4, 11:788] = 9.0
+    assert (wide == 9.0).all()
+    pad = torch.zeros(3, 40, dtype=torch.int32)
+    pad[:, 3:28] = torch.randint(-2**31, 2**31, (3, 25), generator=gen).to(torch.int32)
+    kw = dict(allowed=pad[:, 3:28])
+    _check(process_logits(x.float().to(DEV), **moved, allowed=pad.to(DEV)[:, 3:28]),
+           _want(x.float(), rules, **kw))
+    assert _run(x[:0], rules).shape == (0, 777)
+    assert _run(x[:, :0], rules).shape == (3, 0)
+
+
+def test_streams_and_graphs():
+    gen = torch.Generator().manual_seed(8)
+    rules = {k: v.to(DEV) if isinstance(v, torch.Tensor) else v
+             for k, v in _rules(gen, 4, 20000, 3000, 30).items()}
+    logits = torch.randn(4, 20000, generator=gen).to(DEV)
+    first = process_logits(logits, **rules)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        other = process_logits(logits, **rules)
+    torch.cuda.synchronize()
+    assert torch.equal(first, other)
+    out = torch.empty_like(logits)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        process_logits(logits, out, **rules)
+    for step in range(4):
+        logits.mul_(1.1)
+        rules["history_lens"].add_(-100).clamp_(min=0)
+        rules["frequency"].add_(0.1)
+        graph.replay()
+        want = process_logits(logits.clone(), **rules)
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+
+
+def test_refusals():
+    x = torch.zeros(3, 100, device=DEV)
+    i32 = lambda *s: torch.zeros(*s, dtype=torch.int32, device=DEV)
+    f32 = lambda *s: torch.zeros(*s, device=DEV)
+    for kw, match in ((dict(history=i32(3, 5)), "go together"),
+                      (dict(history=i32(3, 5).long(), history_lens=i32(3)), "history"),
+                      (dict(prompt_lens=i32(3)), "history"),
+                      (dict(repetition=f32(2)), "every row is a request"),
+                      (dict(repetition=f32(3).double()), "repetition"),
+                      (dict(bias_ids=i32(3, 4)), "go together"),
+                      (dict(bias_ids=i32(3, 4), bias_values=f32(3, 5)), "biases"),
+                      (dict(allowed=i32(3, 3)), "allowed"), (dict(allowed=i32(2, 4)), "allowed"),
+                      (dict(ancestors=i32(3, 1)), "go together"),
+                      (dict(token_to_req=i32(2)), "token_to_req"),
+                      (dict(vocab_start=-1), "vocab_start"),
+                      (dict(out=f32(3, 99)), "shape of logits"),
+                      (dict(out=f32(3, 100).half()), "out"),
+                      (dict(out=f32(1, 100).expand(3, 100)), "overlapping")):
+        with pytest.raises(RuntimeError, match=match):
+            process_logits(x, **kw)
+    with pytest.raises(RuntimeError, match="fp32, bf16 or fp16"):
+        process_logits(x.double())
+    with pytest.raises(RuntimeError, match="unit column"):
+        process_logits(x.t())

@@ -1,0 +1,359 @@
+"""Tree attention on the GPU against a 64-bit statement of it, row by row.
+
+Tolerance. Each weight is rounded to bf16 (2^-8 of it at most) before it meets V,
+so a result is off by at most 2^-8 sum p |v|; a score's fp32 sum of D products
+passes at most 36 roundings of 2^-24 on sum |q k|, scaled by D^-0.5, which moves
+a weight by as much (numerator and sum: twice); the fp32 exponentials and sums
+stay under 2^-19 of a weight. The gate's factor is at most 1 and off by 2^-20.
+Then one rounding to bf16, 2^-8 of the value."""
+
+import math
+
+import pytest
+import torch
+
+from qsa_vllm_amd.ops import qsa_sparse_paged_attention, qsa_tree_paged_attention, tree_ancestors
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+
+
+class Case:
+    """Random requests: committed lengths, node counts, random trees, a shuffled
+    paged cache whose unused slots (and pages) hold NaN."""
+
+    def __init__(self, ctx, nodes, heads=4, kv_heads=2, dim=128, page=16, gate=False, seed=0,
+                 layout="token_major", chain=False, scale=1.0, words=None):
+        gen = torch.Generator().manual_seed(seed)
+        self.gen, self.ctx, self.nodes, self.page, self.dim = gen, ctx, nodes, page, dim
+        self.heads, self.kv_heads = heads, kv_heads
+        rows = sum(nodes)
+        self.starts = [0]
+        for t in nodes:
+            self.starts.append(self.starts[-1] + t)
+        self.parents = [j - 1 if chain else (int(torch.randint(-1, j, (1,), generator=gen)) if j else -1)
+                        for t in nodes for j in range(t)]
+        pages = [-(-(c + t) // page) for c, t in zip(ctx, nodes)]
+        order = torch.randperm(sum(pages) + 2, generator=gen).to(torch.int32)
+        self.table = torch.full((len(ctx), max(max(pages), 1)), -1, dtype=torch.int32)
+        kv = torch.full((len(order), page, kv_heads, 2 * dim), float("nan"), dtype=torch.bfloat16)
+        at = 0
+        for b, p in enumerate(pages):
+            self.table[b, :p] = order[at:at + p]
+            at += p
+            for pos in range(ctx[b] + nodes[b]):
+                kv[self.table[b, pos // page], pos % page] = (
+                    torch.randn(kv_heads, 2 * dim, generator=gen) * scale).bfloat16()
+        self.q = (torch.randn(rows, heads, dim, generator=gen) * scale).bfloat16()
+        self.gate = torch.randn(rows, heads, dim, generator=gen).bfloat16() if gate else None
+        self.kv, self.layout = kv, layout
+        self.qsl = torch.tensor(self.starts, dtype=torch.int32)
+        most = max(max(nodes), 1)
+        self.anc = tree_ancestors(torch.tensor(self.parents, dtype=torch.int64), self.qsl, most)
+        if words is not None:
+            self.anc = torch.nn.functional.pad(self.anc, (0, words - self.anc.shape[1]))
+
+    def device_cache(self):
+        if self.layout == "head_major":   # [blocks, kv_heads, page, 2 D] storage
+            kv = self.kv.permute(0, 2, 1, 3).contiguous().to(DEV).permute(0, 2, 1, 3)
+        else:
+            kv = self.kv.to(DEV)
+        return kv[..., :self.dim], kv[..., self.dim:]
+
+    def run(self, out=None, q=None, max_query_len=None, max_context_len=None, anc=None, table=None):
+        k, v = self.device_cache()
+        return qsa_tree_paged_attention(
+            self.q.to(DEV) if q is None else q, k, v,
+            (self.table if table is None else table).to(DEV),
+            torch.tensor(self.ctx, dtype=torch.int32, device=DEV), self.qsl.to(DEV),
+            (self.anc if anc is None else anc).to(DEV), out,
+            output_gate=self.gate.to(DEV) if self.gate is not None else None,
+            max_query_len=max(self.nodes) if max_query_len is None else max_query_len,
+            max_context_len=max(self.ctx) if max_context_len is None else max_context_len)
+
+    def want(self, anc=None, table=None):
+        """(result, tolerance), 64 bits: each row over its own list of slots."""
+        anc = self.anc if anc is None else anc
+        table = self.table if table is None else table
+        out = torch.zeros(self.q.shape, dtype=torch.float64)
+        tol = torch.zeros_like(out)
+        group = self.heads // self.kv_heads
+        blocks = self.kv.shape[0]
+        for b, (c, t) in enumerate(zip(self.ctx, self.nodes)):
+            for r in range(self.starts[b], self.starts[b + 1]):
+                seen = list(range(c)) + [c + j for j in range(min(t, 32 * anc.shape[1]))
+                                         if (int(anc[r, j // 32]) >> (j % 32)) & 1]
+                slots = [(int(table[b, p // self.page]), p % self.page) for p in seen
+                         if p // self.page < table.shape[1]]
+                slots = [s for s in slots if 0 <= s[0] < blocks]
+                if not slots:
+                    continue
+                kv = self.kv[[s[0] for s in slots], [s[1] for s in slots]].double()
+                for h in range(self.heads):
+                    k, v = kv[:, h // group, :self.dim], kv[:, h // group, self.dim:]
+                    q = self.q[r, h].double()
+                    score = k @ q / math.sqrt(self.dim)
+                    p = torch.softmax(score, 0)
+                    spread = (k.abs() @ q.abs()).max().item() / math.sqrt(self.dim)
+                    rel = 2 ** -8 + 2 * 36 * 2 ** -24 * spread + 2 ** -18
+                    o, mass = p @ v, p @ v.abs()
+                    if self.gate is not None:
+                        s = torch.sigmoid(self.gate[r, h].double())
+                        o, mass = o * s, mass * s
+                    out[r, h] = o
+                    tol[r, h] = rel * mass + 2 ** -8 * (o.abs() + rel * mass) + 2 ** -100
+        return out, tol
+
+    def check(self, got, **kw):
+        want, tol = self.want(**kw)
+        off = (got.cpu().double() - want).abs()
+        assert torch.isfinite(got).all()
+        assert (off <= tol).all(), f"{(off / tol).max().item():.2f} times the tolerance"
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("ctx,nodes,heads,kv_heads,page", [
+    ([0], [1], 1, 1, 16),                      # the node itself is all there is
+    ([1], [1], 8, 1, 16),
+    ([37], [5], 4, 2, 16),                     # under one stage
+    ([128, 127, 129], [1, 1, 1], 16, 2, 16),   # single tokens about a stage's end
+    ([300], [3], 16, 2, 272),
+    ([64, 0, 63, 200], [2, 4, 1, 7], 8, 4, 48),
+    ([500, 20], [8, 8], 16, 2, 16),            # 64 rows a kv head
+    ([130, 700], [17, 33], 4, 1, 16),          # 132 rows: two tiles
+    ([90], [64], 8, 1, 1),                     # pages of one token
+    ([0, 5, 2], [40, 0, 70], 6, 2, 16),        # no context, an empty request, three words
+    ([33], [100], 3, 3, 16),                   # no sharing of kv heads
+])
+def test_matches_64_bits(ctx, nodes, heads, kv_heads, page, dim):
+    c = Case(ctx, nodes, heads, kv_heads, dim, page, gate=len(ctx) % 2 == 1, seed=sum(ctx) + dim)
+    c.check(c.run())
+
+
+@pytest.mark.parametrize("max_context_len", [3000, 0, 100000])
+@pytest.mark.parametrize("nodes", [[1, 3, 2], [9, 2, 20], [12, 64, 1]])
+def test_long_contexts_split(nodes, max_context_len):
+    """Several chunks a request, of ragged lengths; the bound on the context only
+    shapes the launch."""
+    c = Case([3000, 1, 1111], nodes, heads=4, kv_heads=1, gate=True, seed=7)
+    c.check(c.run(max_context_len=max_context_len))
+
+
+def test_layouts_and_strides():
+    c = Case([50, 200], [6, 3], heads=8, kv_heads=2, dim=64, layout="head_major", seed=8)
+    c.check(c.run())
+    big = torch.full((9, 8, 3 * 64), 3.0, dtype=torch.bfloat16, device=DEV)
+    out = big[:, :, 64:128]
+    q = torch.zeros(9, 8, 128, dtype=torch.bfloat16, device=DEV)
+    q[..., 64:] = c.q.to(DEV)
+    assert c.run(out=out, q=q[..., 64:]) is out
+    c.check(out)
+    assert (big[:, :, :64] == 3).all() and (big[:, :, 128:] == 3).all()
+    wide = torch.zeros(9, 5, dtype=torch.int32)
+    wide[:, 1:2] = c.anc
+    c.check(c.run(anc=wide[:, 1:2]))
+    c.check(c.run(anc=torch.nn.functional.pad(c.anc, (0, 3))))     # more words than nodes
+
+
+def test_rows_that_see_nothing_are_zero():
+    c = Case([0, 30], [4, 3], seed=9)
+    anc = c.anc.clone()
+    anc[:3] = 0
+    anc[5] = 0                        # sees the context alone
+    got = c.run(anc=anc)
+    assert (got[:3] == 0).all()
+    c.check(got, anc=anc)
+    # no words at all: nothing drafted is seen
+    none = torch.zeros(7, 0, dtype=torch.int32)
+    got = c.run(anc=none)
+    assert (got[:4] == 0).all()
+    c.check(got, anc=none)
+
+
+def test_any_mask_is_taken():
+    """Not only trees: later nodes, arbitrary subsets, bits past the nodes."""
+    c = Case([20, 7], [40, 33], heads=2, kv_heads=1, seed=10)
+    anc = torch.randint(-2**31, 2**31, (73, 2), generator=c.gen).to(torch.int32)
+    c.check(c.run(anc=anc), anc=anc)
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+@pytest.mark.parametrize("ctx", [100, 0, 61])
+@pytest.mark.parametrize("nodes", [6, 60])
+def test_unseen_nodes_may_hold_anything(bad, ctx, nodes):
+    """A node whose K/V are not finite is seen by its descendants only; every
+    other row has the bits that it has without it."""
+    c = Case([ctx], [nodes], heads=8, kv_heads=2, seed=11)
+    clean = c.run()
+    node = 1
+    pos = ctx + node
+    c.kv[c.table[0, pos // 16], pos % 16] = bad
+    got = c.run()
+    sees = (c.anc[:, 0] >> node) & 1 != 0
+    assert sees.any() and not sees.all()
+    off = (got.float() - clean.float())[~sees.to(DEV)].abs()
+    c_want, tol = c.want()
+    assert torch.isfinite(got[~sees.to(DEV)]).all()
+    assert ((got.cpu().double() - c_want).abs() <= tol)[~sees].all()
+    assert got[sees.to(DEV)].isnan().all()
+    assert off.max() <= 2 * tol[~sees].max()
+
+
+def test_positions_without_a_page_are_not_seen():
+    c = Case([100, 70], [3, 2], heads=4, kv_heads=1, seed=12)
+    table = c.table.clone()
+    table[0, 2] = -1
+    table[1, 0] = c.kv.shape[0]          # past the cache
+    table[0, 4] = -2**31
+    table[1, 3] = 2**31 - 1
+    c.check(c.run(table=table), table=table)
+    short = c.table[:, :5]               # a table that ends inside the first context
+    c.check(c.run(table=short), table=short)
+    empty = c.table[:, :0]
+    assert (c.run(table=empty) == 0).all()
+
+
+def test_lengths_on_the_device_stay_within_the_tensors():
+    """Starts outside the rows, falling starts, negative and huge contexts: no
+    access outside the tensors, and the requests that are sound are right."""
+    c = Case([40, 25], [4, 4], heads=4, kv_heads=1, seed=13)
+    want = c.run()
+    k, v = c.device_cache()
+
+    def call(ctx, qsl):
+        out = torch.full((8, 4, 128), 5.0, dtype=torch.bfloat16, device=DEV)
+        return qsa_tree_paged_attention(
+            c.q.to(DEV), k, v, c.table.to(DEV), torch.tensor(ctx, dtype=torch.int32, device=DEV),
+            torch.tensor(qsl, dtype=torch.int32, device=DEV), c.anc.to(DEV), out,
+            max_query_len=4, max_context_len=40)
+
+    got = call([40, 25], [0, 4, 4])
+    assert torch.equal(got[:4], want[:4]) and (got[4:] == 5).all()   # rows of no request
+    got = call([40, -3], [0, 4, 2])
+    assert torch.equal(got[:4], want[:4]) and (got[4:] == 5).all()
+    got = call([40, 2**31 - 1], [0, 4, 8])
+    assert torch.equal(got[:4], want[:4])
+    got = call([-2**31, 25], [-5, 4, 1 << 30])
+    assert torch.equal(got[4:], want[4:])
+
+
+def test_more_nodes_than_said_are_left():
+    c = Case([30], [20], heads=2, kv_heads=1, seed=14)
+    out = torch.full((20, 2, 128), 5.0, dtype=torch.bfloat16, device=DEV)
+    c.run(out=out, max_query_len=8)
+    full = c.run()
+    assert torch.equal(out[:8], full[:8])
+
+
+def test_a_chain_equals_the_sparse_attention_over_every_slot():
+    """Single tokens: the sparse op with every slot of the context selected does
+    the same sum (its own tolerance: two bf16 roundings of the weights)."""
+    c = Case([90, 33], [1, 1], heads=16, kv_heads=2, seed=15)
+    k, v = c.device_cache()
+    idx = torch.full((2, 91), -1, dtype=torch.int32)
+    for b, n in enumerate((91, 34)):
+        for p in range(n):
+            idx[b, p] = int(c.table[b, p // 16]) * 16 + p % 16
+    other = qsa_sparse_paged_attention(
+        c.q.to(DEV), k, v, idx.to(DEV), c.table.to(DEV),
+        torch.arange(2, dtype=torch.int32, device=DEV), use_decode_kernel=True,
+        indices_are_physical=True, valid_counts=torch.tensor([91, 34], dtype=torch.int32, device=DEV))
+    got = c.run()
+    _, tol = c.want()
+    assert ((got.cpu().double() - other.cpu().double()).abs() <= 2 * tol).all()
+
+
+def test_large_scores():
+    """Scores of hundreds: one weight takes all, nothing overflows."""
+    c = Case([200, 50], [4, 9], heads=4, kv_heads=2, scale=6.0, seed=16)
+    c.check(c.run())
+
+
+def test_offsets_past_32_bits():
+    """Pages whose byte offsets pass 4 GiB."""
+    blocks, page, heads, dim = 300000, 16, 2, 128
+    if torch.cuda.mem_get_info()[0] < (12 << 30):
+        pytest.skip("needs 12 GiB of free GPU memory")
+    c = Case([40, 70], [3, 5], heads=4, kv_heads=heads, seed=17)
+    kv = torch.empty(blocks, page, heads, 2 * dim, dtype=torch.bfloat16, device=DEV)
+    far = c.table.clone()
+    for b in range(2):
+        for i in range(c.table.shape[1]):
+            if c.table[b, i] >= 0:
+                far[b, i] = blocks - 1 - int(c.table[b, i]) * 7
+                kv[far[b, i]] = c.kv[c.table[b, i]].to(DEV)
+    got = qsa_tree_paged_attention(
+        c.q.to(DEV), kv[..., :dim], kv[..., dim:], far.to(DEV),
+        torch.tensor(c.ctx, dtype=torch.int32, device=DEV), c.qsl.to(DEV), c.anc.to(DEV),
+        max_query_len=5, max_context_len=70)
+    assert torch.equal(got, c.run())
+
+
+def test_streams_and_graphs():
+    """The same bits on another stream and in every replay of a graph, whose
+    lengths, tables and ancestors are read anew each time."""
+    c = Case([900, 60], [7, 12], heads=8, kv_heads=2, seed=18)
+    k, v = c.device_cache()
+    q, table, qsl, anc = (t.to(DEV) for t in (c.q, c.table, c.qsl, c.anc))
+    ctx = torch.tensor(c.ctx, dtype=torch.int32, device=DEV)
+    out = torch.zeros_like(q)
+
+    def step():
+        return qsa_tree_paged_attention(q, k, v, table, ctx, qsl, anc, out, max_query_len=12,
+                                        max_context_len=900)
+    first = step().clone()
+    c.check(first)
+    a, b = torch.cuda.Stream(), torch.cuda.Stream()
+    outs = [torch.zeros_like(q) for _ in range(2)]
+    for s, o in zip((a, b), outs):
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            for _ in range(5):
+                qsa_tree_paged_attention(q, k, v, table, ctx, qsl, anc, o, max_query_len=12,
+                                         max_context_len=900)
+    torch.cuda.synchronize()
+    assert torch.equal(outs[0], first) and torch.equal(outs[1], first)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    for shorter in (0, 100, 333, 0):
+        ctx.copy_(torch.tensor([900 - shorter, 60 - shorter // 10], dtype=torch.int32))
+        graph.replay()
+        got = out.clone()
+        out.zero_()
+        want = step().clone()
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)
+
+
+def test_refusals():
+    c = Case([20], [3], seed=19)
+    k, v = c.device_cache()
+    i32 = dict(dtype=torch.int32, device=DEV)
+    args = [c.q.to(DEV), k, v, c.table.to(DEV), torch.tensor([20], **i32), c.qsl.to(DEV),
+            c.anc.to(DEV)]
+
+    def call(**over):
+        a = list(args)
+        kw = dict(max_query_len=3, max_context_len=20)
+        for key, value in over.items():
+            if key.startswith("a"):
+                a[int(key[1:])] = value
+            else:
+                kw[key] = value
+        return qsa_tree_paged_attention(*a, **kw)
+
+    call()
+    for over, match in ((dict(a0=args[0].half()), "q must be"), (dict(a1=k.half()), "k_cache"),
+                        (dict(a0=args[0][..., :64]), "cache head dim"),
+                        (dict(a2=v[:, :8]), "one shape"), (dict(a3=args[3].long()), "block_table"),
+                        (dict(a4=args[4].long()), "context_lens"), (dict(a4=args[4][:0]), "entries"),
+                        (dict(a5=args[5][:1]), "entries"), (dict(a6=args[6][:2]), "each query row"),
+                        (dict(a6=args[6].long()), "ancestors"), (dict(max_query_len=-1), "max_query"),
+                        (dict(max_context_len=1 << 40), "max_context"),
+                        (dict(out=torch.empty(2, 4, 128, dtype=torch.bfloat16, device=DEV)), "out"),
+                        (dict(output_gate=args[0][:2]), "output_gate"),
+                        (dict(a0=args[0][:, :3]), "multiple of kv heads"),
+                        (dict(a6=args[6].cpu()), "GPU")):
+        with pytest.raises(RuntimeError, match=match):
+            call(**over)
