@@ -43,14 +43,21 @@ constexpr int kWaves = 4;
 constexpr int kCUs = 256;
 constexpr float kNegInf = -__builtin_huge_valf();
 
+constexpr int kTok = 64;         // tokens of a stage
+constexpr float kSlack = 8.0f;   // log2: how far scores may pass the exponents' base
+// s_waitcnt for the vector-memory counter alone (gfx9 encoding), at 0.
+constexpr int kLoadsDone = (7 << 4) | (15 << 8);
+
 typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
 
 struct TreeArgs {
   const uint16_t* q;
   int64_t q_row, q_head;  // elements
   const char* k;
   const char* v;
-  int64_t kb, kt, kh, vb, vt, vh;  // bytes
+  uint32_t kb, kt, vb, vt;  // bytes
+  int64_t kh, vh;
   int num_blocks;
   int page_size;
   FastDiv page_div;
@@ -72,6 +79,7 @@ struct TreeArgs {
   int rows, num_q_heads, kv_heads, group;
   FastDiv group_div;
   int m_tiles, splits, chunk;
+  int units;  // (request, kv head, chunk)
   float scale_log2;
 };
 
@@ -100,51 +108,109 @@ __device__ __forceinline__ float gate_factor(uint16_t g) {
 // are permuted by the token so that 16 tokens' same unit (the A operand's
 // read) lie in different banks.
 template <int D>
+__device__ __forceinline__ int k_swizzle(int tok) {
+  return D == 128 ? tok & 15 : (tok >> 1) & 7;
+}
+template <int D>
 __device__ __forceinline__ int k_at(int tok, int unit) {
-  constexpr int U = D / 8;
-  const int swizzle = D == 128 ? tok & 15 : (tok >> 1) & 7;
-  return (tok * U + (unit ^ swizzle)) * 16;
+  return (tok * (D / 8) + (unit ^ k_swizzle<D>(tok))) * 16;
 }
 // The same for V, permuted in 32-byte units (what the transposing read takes
 // of a token).
 template <int D>
+__device__ __forceinline__ int v_swizzle(int tok) {
+  return D == 128 ? (tok & 7) << 1 : ((tok >> 1) & 3) << 1;
+}
+template <int D>
 __device__ __forceinline__ int v_at(int tok, int unit) {
-  constexpr int U = D / 8;
-  const int swizzle = D == 128 ? (tok & 7) << 1 : ((tok >> 1) & 3) << 1;
-  return (tok * U + (unit ^ swizzle)) * 16;
+  return (tok * (D / 8) + (unit ^ v_swizzle<D>(tok))) * 16;
+}
+
+// Lane l (group g = l / 16, member n) passes the address of 4 dims of token
+// 4 g + n / 4 and gets dim n of the group's four tokens.
+__device__ __forceinline__ s16x4 read_transposed(const char* p) {
+  return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p);
+}
+
+// c += A B over 32 tokens (two subtiles' operands) or, when the wave has a
+// single subtile, over its 16.
+template <int SUB>
+__device__ __forceinline__ void add_product(f32x4& c, s16x4 a0, s16x4 a1, const uint32_t (&b0)[2],
+                                            const uint32_t (&b1)[2]) {
+  if constexpr (SUB > 1) {
+    const s16x8 a = __builtin_shufflevector(a0, a1, 0, 1, 2, 3, 4, 5, 6, 7);
+    const u32x4 b = {b0[0], b0[1], b1[0], b1[1]};
+    c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a),
+                                                __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  } else {
+    c = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(
+        a0, __builtin_bit_cast(s16x4, (u32x2{b0[0], b0[1]})), c, 0, 0, 0);
+  }
 }
 
 template <int D, int NB, int WM, int WT>
 struct Shape {
-  static constexpr int kRows = 16 * NB * WM;          // query rows of a workgroup
-  static constexpr int kTok = 32 * WT < 64 ? 64 : 32 * WT;  // tokens of a stage
-  static constexpr int kWaveTok = kTok / WT;
-  static constexpr int kSub = kWaveTok / 16;          // 16-token subtiles of a wave
-  static constexpr int kLoads = kTok * (D / 8) / (64 * kWaves);  // 16-byte loads of a lane
-  static constexpr size_t kStage = (size_t)kTok * D * 2;
-  // K and V stages; afterwards the waves' partial results.
-  static constexpr size_t kMerge = (size_t)kWaves * 16 * NB * (D + 2) * 4;
-  static constexpr size_t kLds = 2 * kStage > kMerge ? 2 * kStage : kMerge;
+  static constexpr int kRows = 16 * NB * WM;    // query rows of a workgroup
+  static constexpr int kWaveTok = kTok / WT;    // tokens of a stage a wave takes
+  static constexpr int kSub = kWaveTok / 16;    // 16-token subtiles of them
+  static constexpr int kPair = kSub > 1 ? 1 : 0;  // subtiles are multiplied in pairs
+  static constexpr int kLoads = kTok * (D / 8) / (64 * kWaves);  // 16-byte K loads of a lane
+  static constexpr size_t kStage = (size_t)kTok * D * 2;         // K or V of a stage
+  // Two stages of K and V; afterwards the partial results of all but the first
+  // wave of each row block.
+  static constexpr int kWaveMerge = 16 * NB * (D + 2);
+  static constexpr size_t kMerge = (size_t)WM * (WT - 1) * kWaveMerge * 4;
+  static constexpr size_t kLds = 4 * kStage > kMerge ? 4 * kStage : kMerge;
 };
 
+__device__ __forceinline__ void load_to_lds(const char* src, char* dst) {  // 16 bytes a lane
+  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src,
+                                   (__attribute__((address_space(3))) void*)dst, 16, 0, 0);
+}
+
+// max over the four lanes (n, 0 .. 3) of a query row.
+__device__ __forceinline__ float max_over_groups(float v) {
+  uint32_t b = __builtin_bit_cast(uint32_t, v);
+  auto r = __builtin_amdgcn_permlane32_swap(b, b, false, false);
+  v = fmaxf(__builtin_bit_cast(float, (uint32_t)r[0]), __builtin_bit_cast(float, (uint32_t)r[1]));
+  b = __builtin_bit_cast(uint32_t, v);
+  r = __builtin_amdgcn_permlane16_swap(b, b, false, false);
+  return fmaxf(__builtin_bit_cast(float, (uint32_t)r[0]), __builtin_bit_cast(float, (uint32_t)r[1]));
+}
+
+// What a row sees of 64 positions: bit i for drafted node j + i, set for the
+// committed ones (j + i < 0).
+__device__ __forceinline__ uint64_t seen_from(const TreeArgs& a, int row, int j) {
+  const int32_t* const words = a.ancestors + row * a.ancestor_row;
+  auto word = [&](int w) -> uint64_t {
+    return w >= 0 && w < a.words ? (uint32_t)words[w] : 0u;
+  };
+  if (j <= -64) return ~0ull;
+  const int w = j >> 5, shift = j & 31;  // rounded down: w is -2 or -1 where j < 0
+  uint64_t bits = (word(w + 1) << 32 | word(w)) >> shift;
+  if (shift) bits |= word(w + 2) << (64 - shift);
+  return j < 0 ? bits | ((1ull << -j) - 1) : bits;
+}
+
 template <int D, int NB, int WM, int WT>
-__global__ __launch_bounds__(64 * kWaves) void tree_attn_kernel(TreeArgs a) {
+__global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 2))) void
+tree_attn_kernel(TreeArgs a) {
   typedef Shape<D, NB, WM, WT> S;
-  constexpr int U = D / 8;       // 16-byte units of a row
+  constexpr int U = D / 8;  // 16-byte units of a row
   constexpr int kSteps = D / 32;
   constexpr int kDims = D / 16;
   extern __shared__ __attribute__((aligned(16))) char lds[];
-  char* const k_lds = lds;
-  char* const v_lds = lds + S::kStage;
 
-  int block = blockIdx.x;
-  const int split = block % a.splits;
-  block /= a.splits;
-  const int m_tile = block % a.m_tiles;
-  block /= a.m_tiles;
-  const int kv = block % a.kv_heads;
-  const Request rq = load_request(a, block / a.kv_heads);
-  const int32_t* const trow = a.table + (block / a.kv_heads) * a.table_row;
+  // Row tiles of one chunk are 8 blocks apart: the same XCD, whose L2 then
+  // serves the chunk's K/V to all but the first.
+  const int unit = (int)(blockIdx.x / (8 * a.m_tiles)) * 8 + (int)(blockIdx.x & 7);
+  const int m_tile = (int)(blockIdx.x >> 3) % a.m_tiles;
+  if (unit >= a.units) return;
+  const int split = unit % a.splits;
+  const int kv = unit / a.splits % a.kv_heads;
+  const int request = unit / a.splits / a.kv_heads;
+  const Request rq = load_request(a, request);
+  const int32_t* const trow = a.table + request * a.table_row;
   const int rows = rq.nodes * a.group;
   const int m0 = m_tile * S::kRows;
   const int t_begin = split * a.chunk;
@@ -152,9 +218,11 @@ __global__ __launch_bounds__(64 * kWaves) void tree_attn_kernel(TreeArgs a) {
   // The last chunk takes whatever is left (a context longer than was said).
   const int t_end = split + 1 == a.splits ? rq.length : min(rq.length, t_begin + a.chunk);
 
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n = lane & 15, g = lane >> 4;
   const int wm = wave / WT, wt = wave % WT;
+  const bool active = m0 + wm * 16 * NB < rows;  // else the wave only moves K/V
 
   // Query rows: lane n's row of each 16-row block, dims 32 s + 8 g .. + 7.
   bf16x8 q[NB][kSteps];
@@ -174,68 +242,58 @@ __global__ __launch_bounds__(64 * kWaves) void tree_attn_kernel(TreeArgs a) {
   const char* const vbase = a.v + kv * a.vh;
   const char* const zero = reinterpret_cast<const char*>(g_qsa_zero_rows);
 
-  // A stage's K and V rows, one stage ahead in registers. Tokens past the end
-  // or without a page in the cache read zeros and are left out of `valid`.
-  u32x4 kr[S::kLoads], vr[S::kLoads];
-  uint64_t valid_next[S::kTok / 64], valid[S::kTok / 64];
-  auto load_stage = [&](int t) {
-    int page[S::kTok / 64];
-#pragma unroll
-    for (int w = 0; w < S::kTok / 64; ++w) {
-      const int pos = t + 64 * w + lane;
-      page[w] = pos < t_end ? trow[a.page_div.div(pos)] : -1;
-      if (page[w] >= a.num_blocks) page[w] = -1;
-      valid_next[w] = __ballot(page[w] >= 0);
-    }
+  // Page of token t + lane, -1 past the end or where the cache has none.
+  auto load_page = [&](int t) {
+    const int pos = t + lane;
+    return *(pos < t_end ? trow + a.page_div.div(pos) : g_qsa_no_page);
+  };
+  // A stage's K and V rows straight into LDS; tokens without a page read zeros.
+  auto load_stage = [&](int t, int page, char* stage) {
 #pragma unroll
     for (int i = 0; i < S::kLoads; ++i) {
-      const int item = (i * kWaves + wave) * 64 + lane;
-      const int tok = item / U, unit = item % U;
-      const int pos = t + tok;
-      const int mine = __shfl(page[i * kWaves / U], tok & 63, 64);
-      const int64_t off = pos - a.page_div.div(pos) * a.page_size;
-      const char* ks = mine >= 0 ? kbase + mine * a.kb + off * a.kt + unit * 16 : zero;
-      const char* vs = mine >= 0 ? vbase + mine * a.vb + off * a.vt + unit * 16 : zero;
-      kr[i] = load_u32x4(ks);
-      vr[i] = load_u32x4(vs);
+      const int block = i * kWaves + wave;
+      const int tok = block * (64 / U) + lane / U, pos = t + tok;
+      const int mine = __shfl(page, tok, 64);
+      const bool ok = mine >= 0 && mine < a.num_blocks;
+      const uint32_t block_at = ok ? mine : 0, tok_at = ok ? pos - a.page_div.div(pos) * a.page_size : 0;
+      const char* const ks = (ok ? kbase : zero) + (uint64_t)block_at * a.kb + (uint64_t)tok_at * a.kt;
+      const char* const vs = (ok ? vbase : zero) + (uint64_t)block_at * a.vb + (uint64_t)tok_at * a.vt;
+      load_to_lds(ks + (lane % U ^ k_swizzle<D>(tok)) * 16, stage + block * 1024);
+      load_to_lds(vs + (lane % U ^ v_swizzle<D>(tok)) * 16, stage + S::kStage + block * 1024);
     }
   };
 
-  f32x4 o[NB][kDims];
-  float top[NB], sum[NB];  // running maximum (log2 domain) and the lane's share of the sum
+  f32x4 o[NB][kDims], sum[NB];  // sum: the row's, in each of the four
+  float base[NB];               // what the exponents are taken from: the maximum, or up to kSlack below
 #pragma unroll
   for (int i = 0; i < NB; ++i) {
-    top[i] = kNegInf;
-    sum[i] = 0.0f;
+    base[i] = kNegInf;
+    sum[i] = f32x4{0, 0, 0, 0};
 #pragma unroll
     for (int d = 0; d < kDims; ++d) o[i][d] = f32x4{0, 0, 0, 0};
   }
+  const float slack = kSlack / a.scale_log2;
 
-  if (t_begin < t_end) load_stage(t_begin);
-  for (int t = t_begin; t < t_end; t += S::kTok) {
-    __syncthreads();  // the last stage has been read
-    // A drafted token's V may hold infinities or NaN that a row outside its
-    // branch must not see (0 times them is NaN): such stages, rare, multiply
-    // element by element below.
-    bool bad = false;
-    const bool drafted = t + S::kTok > rq.context;
-#pragma unroll
-    for (int i = 0; i < S::kLoads; ++i) {
-      const int item = (i * kWaves + wave) * 64 + lane;
-      const int tok = item / U, unit = item % U;
-      *reinterpret_cast<u32x4*>(k_lds + k_at<D>(tok, unit)) = kr[i];
-      *reinterpret_cast<u32x4*>(v_lds + v_at<D>(tok, unit)) = vr[i];
-      if (drafted) {
-#pragma unroll
-        for (int w = 0; w < 4; ++w)
-          bad |= (vr[i][w] & 0x7F80u) == 0x7F80u || (vr[i][w] & 0x7F800000u) == 0x7F800000u;
-      }
+  int page = -1, page_next = -1;
+  if (t_begin < t_end) {
+    page = load_page(t_begin);
+    page_next = load_page(t_begin + kTok);
+    load_stage(t_begin, page, lds);
+  }
+  int buffer = 0;
+  for (int t = t_begin; t < t_end; t += kTok, buffer ^= 1) {
+    __builtin_amdgcn_s_waitcnt(kLoadsDone);
+    __syncthreads();  // the stage is in LDS, and the last one has been read by all
+    const char* const k_lds = lds + buffer * 2 * S::kStage;
+    const char* const v_lds = k_lds + S::kStage;
+    const uint64_t valid = __ballot(page >= 0 && page < a.num_blocks);
+    if (t + kTok < t_end) {
+      load_stage(t + kTok, page_next, lds + (buffer ^ 1) * 2 * S::kStage);
+      page = page_next;
+      page_next = load_page(t + 2 * kTok);
     }
-#pragma unroll
-    for (int w = 0; w < S::kTok / 64; ++w) valid[w] = valid_next[w];
-    if (t + S::kTok < t_end) load_stage(t + S::kTok);
-    if (drafted) bad = __syncthreads_or(bad);
-    else __syncthreads();
+    if (!active) continue;
+    const bool drafted = t + kTok > rq.context;
 
     const int first = wt * S::kWaveTok;  // the wave's tokens of the stage
     f32x4 sc[NB][S::kSub];
@@ -244,8 +302,7 @@ __global__ __launch_bounds__(64 * kWaves) void tree_attn_kernel(TreeArgs a) {
       bf16x8 kf[kSteps];
 #pragma unroll
       for (int s = 0; s < kSteps; ++s)
-        kf[s] = __builtin_bit_cast(
-            bf16x8, *reinterpret_cast<const u32x4*>(k_lds + k_at<D>(first + 16 * u + n, 4 * s + g)));
+        kf[s] = __builtin_bit_cast(bf16x8, load_u32x4(k_lds + k_at<D>(first + 16 * u + n, 4 * s + g)));
 #pragma unroll
       for (int i = 0; i < NB; ++i) {
         sc[i][u] = f32x4{0, 0, 0, 0};
@@ -255,147 +312,152 @@ __global__ __launch_bounds__(64 * kWaves) void tree_attn_kernel(TreeArgs a) {
       }
     }
 
-    // Scores in the log2 domain; masked ones are replaced, whatever they hold.
-    uint32_t seen[NB];
-    bool all = !drafted;
+    // Masked scores are replaced, whatever they hold.
+    uint64_t seen[NB];  // bit 16 u + r: the lane's token 16 u + 4 g + r
+    if (drafted || valid != ~0ull) {
 #pragma unroll
-    for (int w = 0; w < S::kTok / 64; ++w) all = all && valid[w] == ~0ull;
+      for (int i = 0; i < NB; ++i) {
+        seen[i] = (valid >> first & seen_from(a, node[i], t + first - rq.context)) >> (4 * g);
 #pragma unroll
-    for (int i = 0; i < NB; ++i) {
-      seen[i] = ~0u;
+        for (int u = 0; u < S::kSub; ++u)
 #pragma unroll
-      for (int u = 0; u < S::kSub; ++u)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          float s = sc[i][u][r] * a.scale_log2;
-          if (!all) {
-            const int tok = first + 16 * u + 4 * g + r;
-            const int j = t + tok - rq.context;
-            bool ok = (valid[tok / 64] >> (tok & 63)) & 1;
-            if (j >= 0 && ok)
-              ok = j < 32 * a.words &&
-                   ((uint32_t)a.ancestors[node[i] * a.ancestor_row + (j >> 5)] >> (j & 31)) & 1u;
-            if (!ok) {
-              s = kNegInf;
-              seen[i] &= ~(1u << (4 * u + r));
-            }
-          }
-          sc[i][u][r] = s;
-        }
-    }
-
-    bf16x8 p[NB][S::kSub / 2];
-#pragma unroll
-    for (int i = 0; i < NB; ++i) {
-      float m = top[i];
-#pragma unroll
-      for (int u = 0; u < S::kSub; ++u)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) m = fmaxf(m, sc[i][u][r]);
-      m = fmaxf(m, shfl_xor_f(m, 16));
-      m = fmaxf(m, shfl_xor_f(m, 32));
-      const float base = m == kNegInf ? 0.0f : m;
-      const float shrink = fast_exp2(top[i] - base);
-      top[i] = m;
-      float add = 0.0f;
-#pragma unroll
-      for (int h = 0; h < S::kSub / 2; ++h) {
-        u32x4 packed;
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          float e[4];
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            e[r] = fast_exp2(sc[i][2 * h + u][r] - base);
-            add += e[r];
-          }
-          packed[2 * u] = pack_bf16x2(e[0], e[1]);
-          packed[2 * u + 1] = pack_bf16x2(e[2], e[3]);
-        }
-        p[i][h] = __builtin_bit_cast(bf16x8, packed);
+          for (int r = 0; r < 4; ++r)
+            sc[i][u][r] = (seen[i] >> (16 * u + r)) & 1 ? sc[i][u][r] : kNegInf;
       }
-      sum[i] = sum[i] * shrink + add;
-#pragma unroll
-      for (int d = 0; d < kDims; ++d)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) o[i][d][r] *= shrink;
     }
 
-    if (!(drafted && bad)) {
 #pragma unroll
-      for (int h = 0; h < S::kSub / 2; ++h)
+    for (int i = 0; i < NB; ++i) {
+      float top = fmaxf(fmaxf(sc[i][0][0], sc[i][0][1]), fmaxf(sc[i][0][2], sc[i][0][3]));
+#pragma unroll
+      for (int u = 1; u < S::kSub; ++u) {
+        top = fmaxf(fmaxf(top, sc[i][u][0]), sc[i][u][1]);
+        top = fmaxf(fmaxf(top, sc[i][u][2]), sc[i][u][3]);
+      }
+      if (__any(top > base[i] + slack)) {
+        const float m = fmaxf(base[i], max_over_groups(top));
+        const float shrink =
+            m == kNegInf ? 1.0f : fast_exp2((base[i] - m) * a.scale_log2);
+        base[i] = m;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) sum[i][r] *= shrink;
+#pragma unroll
+        for (int d = 0; d < kDims; ++d)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) o[i][d][r] *= shrink;
+      }
+    }
+
+    uint32_t p[NB][S::kSub][2];  // weights of tokens 16 u + 4 g + 0 .. 3, bf16 pairs
+#pragma unroll
+    for (int i = 0; i < NB; ++i) {
+      const float from = base[i] == kNegInf ? 0.0f : -base[i] * a.scale_log2;
+#pragma unroll
+      for (int u = 0; u < S::kSub; ++u) {
+        float e[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          e[r] = fast_exp2(__builtin_fmaf(sc[i][u][r], a.scale_log2, from));
+        p[i][u][0] = pack_bf16x2(e[0], e[1]);
+        p[i][u][1] = pack_bf16x2(e[2], e[3]);
+      }
+    }
+
+    const s16x4 ones = {0x3F80, 0x3F80, 0x3F80, 0x3F80};
+#pragma unroll
+    for (int u = 0; u < S::kSub; u += 2)
+#pragma unroll
+      for (int i = 0; i < NB; ++i) add_product<S::kSub>(sum[i], ones, ones, p[i][u], p[i][u + S::kPair]);
+
+    // A drafted token's V may hold infinities or NaN that a row outside its
+    // branch must not see (0 times them is NaN). Such stages, rare, take them
+    // as 0, and count the ones that a row sees by a second product, of marks:
+    // those results are NaN.
+    bool bad = false;
+    if (drafted) {
+      for (int i = lane; i < S::kWaveTok * U; i += 64) {
+        const u32x4 v = load_u32x4(v_lds + first * D * 2 + i * 16);
+#pragma unroll
+        for (int w = 0; w < 4; ++w)
+          bad |= (v[w] & 0x7F80u) == 0x7F80u || (v[w] & 0x7F800000u) == 0x7F800000u;
+      }
+      bad = __any(bad);
+    }
+    const char* const v_lane = v_lds + (first + 4 * g + (n >> 2)) * D * 2 + (n & 1) * 8;
+    const int v_unit = (n & 3) >> 1, v_swz = v_swizzle<D>(first + 4 * g + (n >> 2));
+    if (!bad) {
+#pragma unroll
+      for (int u = 0; u < S::kSub; u += 2)
 #pragma unroll
         for (int d = 0; d < kDims; ++d) {
-          s16x4 part[2];
-#pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            const int tok = first + 32 * h + 16 * u + 4 * g + (n >> 2);
-            part[u] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                (__attribute__((address_space(3))) s16x4*)(
-                    v_lds + v_at<D>(tok, 2 * d + ((n & 3) >> 1)) + (n & 1) * 8));
-          }
-          typedef short s16x8 __attribute__((ext_vector_type(8)));
-          const s16x8 joined = __builtin_shufflevector(part[0], part[1], 0, 1, 2, 3, 4, 5, 6, 7);
+          const char* const src = v_lane + 16 * u * D * 2 + ((2 * d + v_unit) ^ v_swz) * 16;
+          const s16x4 v0 = read_transposed(src);
+          const s16x4 v1 = S::kPair ? read_transposed(src + 16 * D * 2) : v0;
 #pragma unroll
           for (int i = 0; i < NB; ++i)
-            o[i][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-                __builtin_bit_cast(bf16x8, joined), p[i][h], o[i][d], 0, 0, 0);
+            add_product<S::kSub>(o[i][d], v0, v1, p[i][u], p[i][u + S::kPair]);
         }
     } else {
-      for (int c = 0; c < 16 * S::kSub; ++c) {
-        // Token c: element (c / 16, c % 4) of the lanes with g = (c % 16) / 4.
-        const int tok = first + c;
 #pragma unroll
-        for (int i = 0; i < NB; ++i) {
-          float w = 0.0f;
-          bool ok = false;
+      for (int d = 0; d < kDims; ++d) {
+        f32x4 marks[NB] = {};
 #pragma unroll
-          for (int h = 0; h < S::kSub / 2; ++h)
+        for (int u = 0; u < S::kSub; u += 2) {
+          const char* const src = v_lane + 16 * u * D * 2 + ((2 * d + v_unit) ^ v_swz) * 16;
+          s16x4 v[2], mark[2];
+          v[0] = read_transposed(src);
+          v[1] = S::kPair ? read_transposed(src + 16 * D * 2) : v[0];
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
-              if (32 * h + 16 * (e >> 2) + (e & 3) == (c & ~12)) {
-                w = (float)p[i][h][e];
-                ok = (seen[i] >> (8 * h + e)) & 1u;
-              }
-          const int from = ((c & 12) << 2) | n;
-          w = __shfl(w, from, 64);
-          ok = __shfl((int)ok, from, 64);
+          for (int h = 0; h < 2; ++h)
 #pragma unroll
-          for (int d = 0; d < kDims; ++d) {
-            const u32x2 v = load_u32x2(v_lds + v_at<D>(tok, 2 * d + (g >> 1)) + (g & 1) * 8);
-            if (ok) {
-              o[i][d][0] += w * bf16_lo(v[0]);
-              o[i][d][1] += w * bf16_hi(v[0]);
-              o[i][d][2] += w * bf16_lo(v[1]);
-              o[i][d][3] += w * bf16_hi(v[1]);
+            for (int r = 0; r < 4; ++r) {
+              const bool odd = (v[h][r] & 0x7F80) == 0x7F80;
+              mark[h][r] = odd ? 0x3F80 : 0;
+              v[h][r] = odd ? 0 : v[h][r];
             }
+#pragma unroll
+          for (int i = 0; i < NB; ++i) {
+            add_product<S::kSub>(o[i][d], v[0], v[1], p[i][u], p[i][u + S::kPair]);
+            uint32_t see[2][2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const uint32_t bits = (uint32_t)(seen[i] >> (16 * (u + h * S::kPair)));
+              see[h][0] = (bits & 1 ? 0x3F80u : 0u) | (bits & 2 ? 0x3F800000u : 0u);
+              see[h][1] = (bits & 4 ? 0x3F80u : 0u) | (bits & 8 ? 0x3F800000u : 0u);
+            }
+            add_product<S::kSub>(marks[i], mark[0], mark[1], see[0], see[1]);
           }
         }
+#pragma unroll
+        for (int i = 0; i < NB; ++i)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (marks[i][r] > 0.0f) o[i][d][r] = __builtin_nanf("");
       }
     }
   }
 
+  float total[NB];
 #pragma unroll
   for (int i = 0; i < NB; ++i) {
-    sum[i] += shfl_xor_f(sum[i], 16);
-    sum[i] += shfl_xor_f(sum[i], 32);
+    total[i] = sum[i][0];
+    base[i] *= a.scale_log2;  // log2 domain from here on
   }
 
   if constexpr (WT > 1) {
     // The token shares of each row block, joined in wave order by its first wave.
-    float* const merge = reinterpret_cast<float*>(lds);
-    constexpr int kWave = 16 * NB * (D + 2);
-    float* const mine = merge + wave * kWave;
+    float* const merge = reinterpret_cast<float*>(lds) + wm * (WT - 1) * S::kWaveMerge;
     __syncthreads();
     if (wt > 0) {
+      float* const mine = merge + (wt - 1) * S::kWaveMerge;
 #pragma unroll
       for (int i = 0; i < NB; ++i) {
 #pragma unroll
         for (int d = 0; d < kDims; ++d)
           *reinterpret_cast<f32x4*>(mine + ((i * kDims + d) * 64 + lane) * 4) = o[i][d];
         if (g == 0) {
-          mine[16 * NB * D + 16 * i + n] = top[i];
-          mine[16 * NB * D + 16 * NB + 16 * i + n] = sum[i];
+          mine[16 * NB * D + 16 * i + n] = base[i];
+          mine[16 * NB * D + 16 * NB + 16 * i + n] = total[i];
         }
       }
     }
@@ -403,19 +465,19 @@ __global__ __launch_bounds__(64 * kWaves) void tree_attn_kernel(TreeArgs a) {
     if (wt > 0) return;
 #pragma unroll
     for (int i = 0; i < NB; ++i) {
-      float m = top[i];
-      for (int w = 1; w < WT; ++w) m = fmaxf(m, mine[w * kWave + 16 * NB * D + 16 * i + n]);
-      const float base = m == kNegInf ? 0.0f : m;
-      float f = fast_exp2(top[i] - base);
-      sum[i] *= f;
+      float m = base[i];
+      for (int w = 0; w < WT - 1; ++w) m = fmaxf(m, merge[w * S::kWaveMerge + 16 * NB * D + 16 * i + n]);
+      const float from = m == kNegInf ? 0.0f : m;
+      float f = fast_exp2(base[i] - from);
+      total[i] *= f;
 #pragma unroll
       for (int d = 0; d < kDims; ++d)
 #pragma unroll
         for (int r = 0; r < 4; ++r) o[i][d][r] *= f;
-      for (int w = 1; w < WT; ++w) {
-        const float* other = mine + w * kWave;
-        f = fast_exp2(other[16 * NB * D + 16 * i + n] - base);
-        sum[i] += f * other[16 * NB * D + 16 * NB + 16 * i + n];
+      for (int w = 0; w < WT - 1; ++w) {
+        const float* other = merge + w * S::kWaveMerge;
+        f = fast_exp2(other[16 * NB * D + 16 * i + n] - from);
+        total[i] += f * other[16 * NB * D + 16 * NB + 16 * i + n];
 #pragma unroll
         for (int d = 0; d < kDims; ++d) {
           const f32x4 add = *reinterpret_cast<const f32x4*>(other + ((i * kDims + d) * 64 + lane) * 4);
@@ -423,7 +485,7 @@ __global__ __launch_bounds__(64 * kWaves) void tree_attn_kernel(TreeArgs a) {
           for (int r = 0; r < 4; ++r) o[i][d][r] += f * add[r];
         }
       }
-      top[i] = m;
+      base[i] = m;
     }
   }
 
@@ -432,14 +494,14 @@ __global__ __launch_bounds__(64 * kWaves) void tree_attn_kernel(TreeArgs a) {
     const int m = m0 + (wm * NB + i) * 16 + n;
     if (m >= rows) continue;
     const int head = kv * a.group + m - (node[i] - rq.row0) * a.group;
-    const float inv = sum[i] == 0.0f ? 0.0f : 1.0f / sum[i];  // a row that sees nothing: zeros
+    const float inv = total[i] == 0.0f ? 0.0f : 1.0f / total[i];  // a row that sees nothing: zeros
     if (a.splits > 1) {
       const int64_t at = ((int64_t)node[i] * a.num_q_heads + head) * a.splits + split;
 #pragma unroll
       for (int d = 0; d < kDims; ++d)
         *reinterpret_cast<f32x4*>(a.part_out + at * D + 16 * d + 4 * g) =
             f32x4{o[i][d][0] * inv, o[i][d][1] * inv, o[i][d][2] * inv, o[i][d][3] * inv};
-      if (g == 0) a.part_lse[at] = sum[i] == 0.0f ? kNegInf : top[i] + __log2f(sum[i]);
+      if (g == 0) a.part_lse[at] = total[i] == 0.0f ? kNegInf : base[i] + __log2f(total[i]);
     } else {
       uint16_t* dst = a.out + node[i] * a.out_row + head * a.out_head;
       const uint16_t* gate = a.gate ? a.gate + node[i] * a.g_row + head * a.g_head : nullptr;
@@ -504,7 +566,6 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs a, int row_til
 
 struct TreePlan {
   int tile_rows;  // (node, head) rows of a workgroup
-  int stage;      // tokens of a stage
   int m_tiles, splits, chunk;
 };
 
@@ -518,15 +579,14 @@ TreePlan make_plan(int requests, int num_q_heads, int num_kv_heads, int64_t max_
   TreePlan p;
   const int64_t rows = max_nodes * (num_q_heads / num_kv_heads);
   p.tile_rows = tile_rows_for(rows);
-  p.stage = p.tile_rows <= 32 ? 128 : 64;
   p.m_tiles = (int)((rows + p.tile_rows - 1) / p.tile_rows);
   const int64_t units = (int64_t)requests * num_kv_heads * p.m_tiles;
   const int64_t length = std::min<int64_t>(max_context + max_nodes, INT_MAX / 2);
-  const int64_t stages = std::max<int64_t>(1, (length + p.stage - 1) / p.stage);
+  const int64_t stages = std::max<int64_t>(1, (length + kTok - 1) / kTok);
   int64_t splits = std::min<int64_t>((2 * kCUs + units - 1) / units, (stages + 3) / 4);
   splits = std::max<int64_t>(1, std::min<int64_t>(splits, 256));
   const int64_t per = (stages + splits - 1) / splits;
-  p.chunk = (int)std::min<int64_t>(per * p.stage, INT_MAX / 2);
+  p.chunk = (int)std::min<int64_t>(per * kTok, INT_MAX / 2);
   p.splits = (int)((stages + per - 1) / per);
   return p;
 }
@@ -546,7 +606,7 @@ hipError_t launch_tile(const TreeArgs& a, unsigned grid, hipStream_t stream) {
 
 template <int D>
 hipError_t launch_tree(const TreeArgs& a, const TreePlan& plan, int max_nodes, hipStream_t stream) {
-  const unsigned grid = (unsigned)((int64_t)a.requests * a.kv_heads * a.m_tiles * a.splits);
+  const unsigned grid = (unsigned)(((int64_t)a.units + 7) / 8 * 8 * a.m_tiles);
   hipError_t err;
   if (plan.tile_rows == 16) err = launch_tile<D, 1, 1, 4>(a, grid, stream);
   else if (plan.tile_rows == 32) err = launch_tile<D, 2, 1, 4>(a, grid, stream);
@@ -610,10 +670,14 @@ extern "C" int qsa_tree_attention(
       ((out_row_stride | out_head_stride) & 1))
     return fail(QSA_ERR_INVALID, name + ": q and the caches need 16-byte alignment and strides of "
                                         "multiples of 8 elements, out 4-byte alignment");
+  for (int64_t stride : {k_block_stride, k_token_stride, v_block_stride, v_token_stride})
+    if (stride < 0 || stride > INT_MAX / 2)
+      return fail(QSA_ERR_UNSUPPORTED, name + ": cache strides must be under 2 GiB");
   max_query_len = std::min(max_query_len, rows);
   const TreePlan plan =
       make_plan(num_requests, num_q_heads, num_kv_heads, max_query_len, max_context_len);
-  const int64_t grid = (int64_t)num_requests * num_kv_heads * plan.m_tiles * plan.splits;
+  const int64_t units = (int64_t)num_requests * num_kv_heads * plan.splits;
+  const int64_t grid = (units + 7) / 8 * 8 * plan.m_tiles;
   const int64_t merge = (int64_t)num_requests * (((int64_t)max_query_len * num_q_heads + 7) / 8);
   if (grid > INT_MAX || merge > INT_MAX || (int64_t)max_query_len * num_q_heads > INT_MAX / 2)
     return fail(QSA_ERR_UNSUPPORTED, name + ": too many requests, rows or heads");
@@ -632,11 +696,11 @@ extern "C" int qsa_tree_attention(
   a.q_head = q_head_stride;
   a.k = static_cast<const char*>(k_cache);
   a.v = static_cast<const char*>(v_cache);
-  a.kb = 2 * k_block_stride;
-  a.kt = 2 * k_token_stride;
+  a.kb = (uint32_t)(2 * k_block_stride);
+  a.kt = (uint32_t)(2 * k_token_stride);
   a.kh = 2 * k_head_stride;
-  a.vb = 2 * v_block_stride;
-  a.vt = 2 * v_token_stride;
+  a.vb = (uint32_t)(2 * v_block_stride);
+  a.vt = (uint32_t)(2 * v_token_stride);
   a.vh = 2 * v_head_stride;
   a.num_blocks = num_blocks;
   a.page_size = page_size;
@@ -664,6 +728,7 @@ extern "C" int qsa_tree_attention(
   a.group_div = FastDiv::make(a.group);
   a.m_tiles = plan.m_tiles;
   a.splits = plan.splits;
+  a.units = (int)units;
   a.chunk = plan.chunk;
   a.scale_log2 = 1.4426950408889634f / sqrtf((float)head_dim);
   hipStream_t s = static_cast<hipStream_t>(stream);

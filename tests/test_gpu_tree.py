@@ -241,8 +241,8 @@ def test_more_nodes_than_said_are_left():
     c = Case([30], [20], heads=2, kv_heads=1, seed=14)
     out = torch.full((20, 2, 128), 5.0, dtype=torch.bfloat16, device=DEV)
     c.run(out=out, max_query_len=8)
-    full = c.run()
-    assert torch.equal(out[:8], full[:8])
+    want, tol = c.want()
+    assert ((out.cpu().double() - want).abs() <= tol)[:8].all()
 
 
 def test_a_chain_equals_the_sparse_attention_over_every_slot():
