@@ -44,6 +44,8 @@ constexpr int kCUs = 256;
 constexpr float kNegInf = -__builtin_huge_valf();
 
 constexpr int kTok = 64;         // tokens of a stage
+constexpr int kTileRows = 128;  // (node, head) rows of a workgroup
+constexpr uint32_t kNoToken = 0xFFFFFFFFu;
 constexpr float kSlack = 8.0f;   // log2: how far scores may pass the exponents' base
 // s_waitcnt for the vector-memory counter alone (gfx9 encoding), at 0.
 constexpr int kLoadsDone = (7 << 4) | (15 << 8);
@@ -56,8 +58,8 @@ struct TreeArgs {
   int64_t q_row, q_head;  // elements
   const char* k;
   const char* v;
-  uint32_t kb, kt, vb, vt;  // bytes
-  int64_t kh, vh;
+  uint32_t kb, kt, vb, vt;  // units of 16 bytes
+  int64_t kh, vh;  // bytes
   int num_blocks;
   int page_size;
   FastDiv page_div;
@@ -79,7 +81,7 @@ struct TreeArgs {
   int rows, num_q_heads, kv_heads, group;
   FastDiv group_div;
   int m_tiles, splits, chunk;
-  int units;  // (request, kv head, chunk)
+  int pair_slots;  // (request, kv head) pairs, rounded up to 8
   float scale_log2;
 };
 
@@ -168,6 +170,24 @@ __device__ __forceinline__ void load_to_lds(const char* src, char* dst) {  // 16
                                    (__attribute__((address_space(3))) void*)dst, 16, 0, 0);
 }
 
+// Which 16-bit halves hold an infinity or NaN (bf16), as bits; and 0 in their place.
+__device__ __forceinline__ uint32_t not_finite(const u32x4& v) {
+  uint32_t bits = 0;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    bits |= (uint32_t)((v[w] & 0x7F80u) == 0x7F80u) << (2 * w);
+    bits |= (uint32_t)((v[w] & 0x7F800000u) == 0x7F800000u) << (2 * w + 1);
+  }
+  return bits;
+}
+__device__ __forceinline__ u32x4 finite_or_zero(u32x4 v) {
+  const uint32_t bits = not_finite(v);
+#pragma unroll
+  for (int w = 0; w < 4; ++w)
+    v[w] &= (bits >> (2 * w) & 1 ? 0u : 0xFFFFu) | (bits >> (2 * w + 1) & 1 ? 0u : 0xFFFF0000u);
+  return v;
+}
+
 // max over the four lanes (n, 0 .. 3) of a query row.
 __device__ __forceinline__ float max_over_groups(float v) {
   uint32_t b = __builtin_bit_cast(uint32_t, v);
@@ -192,32 +212,15 @@ __device__ __forceinline__ uint64_t seen_from(const TreeArgs& a, int row, int j)
   return j < 0 ? bits | ((1ull << -j) - 1) : bits;
 }
 
+// One row tile (rows m0 .. of a request's `rows`) of one chunk.
 template <int D, int NB, int WM, int WT>
-__global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 2))) void
-tree_attn_kernel(TreeArgs a) {
+__device__ __forceinline__ void attend_tile(const TreeArgs& a, const Request& rq,
+                                            const int32_t* trow, int kv, int rows, int m0,
+                                            int split, int t_begin, int t_end, char* lds) {
   typedef Shape<D, NB, WM, WT> S;
   constexpr int U = D / 8;  // 16-byte units of a row
   constexpr int kSteps = D / 32;
   constexpr int kDims = D / 16;
-  extern __shared__ __attribute__((aligned(16))) char lds[];
-
-  // Row tiles of one chunk are 8 blocks apart: the same XCD, whose L2 then
-  // serves the chunk's K/V to all but the first.
-  const int unit = (int)(blockIdx.x / (8 * a.m_tiles)) * 8 + (int)(blockIdx.x & 7);
-  const int m_tile = (int)(blockIdx.x >> 3) % a.m_tiles;
-  if (unit >= a.units) return;
-  const int split = unit % a.splits;
-  const int kv = unit / a.splits % a.kv_heads;
-  const int request = unit / a.splits / a.kv_heads;
-  const Request rq = load_request(a, request);
-  const int32_t* const trow = a.table + request * a.table_row;
-  const int rows = rq.nodes * a.group;
-  const int m0 = m_tile * S::kRows;
-  const int t_begin = split * a.chunk;
-  if (m0 >= rows || (split > 0 && t_begin >= rq.length)) return;
-  // The last chunk takes whatever is left (a context longer than was said).
-  const int t_end = split + 1 == a.splits ? rq.length : min(rq.length, t_begin + a.chunk);
-
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n = lane & 15, g = lane >> 4;
@@ -238,30 +241,91 @@ tree_attn_kernel(TreeArgs a) {
       q[i][s] = __builtin_bit_cast(bf16x8, load_u32x4(src + 32 * s + 8 * g));
   }
 
-  const char* const kbase = a.k + kv * a.kh;
-  const char* const vbase = a.v + kv * a.vh;
+  // K/V of a stage go straight into LDS: block i of a stage (64 units) is moved
+  // by wave i mod 4, and every lane's unit of a row is the same in all its
+  // blocks (a block of 64 / U tokens times the waves is a multiple of the
+  // swizzles' periods).
   const char* const zero = reinterpret_cast<const char*>(g_qsa_zero_rows);
+  const int tok0 = wave * (64 / U) + lane / U;  // the lane's token of the wave's first block
+  const int ku = (lane % U ^ k_swizzle<D>(tok0)) * 16, vu = (lane % U ^ v_swizzle<D>(tok0)) * 16;
+  const char* const klane = a.k + kv * a.kh + ku;
+  const char* const vlane = a.v + kv * a.vh + vu;
 
-  // Page of token t + lane, -1 past the end or where the cache has none.
+  // Page of token t + lane, -1 past the end or where the table has none.
   auto load_page = [&](int t) {
     const int pos = t + lane;
     return *(pos < t_end ? trow + a.page_div.div(pos) : g_qsa_no_page);
   };
-  // A stage's K and V rows straight into LDS; tokens without a page read zeros.
   auto load_stage = [&](int t, int page, char* stage) {
+    // Offsets (16-byte units) of token t + lane; blocks without tokens of the
+    // cache read zeros in their place.
+    const int pos = t + lane;
+    const bool ok = page >= 0 && page < a.num_blocks;
+    const uint32_t at = pos - a.page_div.div(pos) * a.page_size;
+    const uint32_t koff = ok ? page * a.kb + at * a.kt : kNoToken;
+    const uint32_t voff = page * a.vb + at * a.vt;
+    const uint64_t valid = __ballot(ok);
 #pragma unroll
     for (int i = 0; i < S::kLoads; ++i) {
-      const int block = i * kWaves + wave;
-      const int tok = block * (64 / U) + lane / U, pos = t + tok;
-      const int mine = __shfl(page, tok, 64);
-      const bool ok = mine >= 0 && mine < a.num_blocks;
-      const uint32_t block_at = ok ? mine : 0, tok_at = ok ? pos - a.page_div.div(pos) * a.page_size : 0;
-      const char* const ks = (ok ? kbase : zero) + (uint64_t)block_at * a.kb + (uint64_t)tok_at * a.kt;
-      const char* const vs = (ok ? vbase : zero) + (uint64_t)block_at * a.vb + (uint64_t)tok_at * a.vt;
-      load_to_lds(ks + (lane % U ^ k_swizzle<D>(tok)) * 16, stage + block * 1024);
-      load_to_lds(vs + (lane % U ^ v_swizzle<D>(tok)) * 16, stage + S::kStage + block * 1024);
+      const int from = (i * kWaves * (64 / U) + tok0) * 4;
+      const uint32_t ko = __builtin_amdgcn_ds_bpermute(from, koff);
+      const uint32_t vo = __builtin_amdgcn_ds_bpermute(from, voff);
+      const char* ks = klane + ((uint64_t)ko << 4);
+      const char* vs = vlane + ((uint64_t)vo << 4);
+      if (valid != ~0ull) {
+        ks = ko != kNoToken ? ks : zero + ku;
+        vs = ko != kNoToken ? vs : zero + vu;
+      }
+      char* const dst = stage + (i * kWaves + wave) * 1024;
+      load_to_lds(ks, dst);
+      load_to_lds(vs, dst + S::kStage);
     }
+    return valid;
   };
+
+  int page_next = -1, buffer = 0;
+  uint64_t valid = 0, valid_next = 0;
+  if (t_begin < t_end) {
+    const int page = load_page(t_begin);
+    page_next = load_page(t_begin + kTok);
+    valid_next = load_stage(t_begin, page, lds);
+  }
+  bool poisoned = false;
+  // Waits for stage t, starts the next one's loads, and returns stage t's K.
+  auto advance = [&](int t) -> const char* {
+    char* const stage = lds + buffer * 2 * S::kStage;
+    buffer ^= 1;
+    __builtin_amdgcn_s_waitcnt(kLoadsDone);
+    __syncthreads();  // the stage is in LDS, and the last one has been read by all
+    valid = valid_next;
+    if (t + kTok < t_end)
+      valid_next = load_stage(t + kTok, page_next, lds + buffer * 2 * S::kStage);
+    page_next = load_page(t + 2 * kTok);
+    if (t + kTok > rq.context) {
+      // A drafted token's V may hold infinities or NaN that a row outside its
+      // branch must not see (0 times them is NaN). They are taken as 0 here,
+      // and rows that see them get NaN at the end.
+      u32x4* const v = reinterpret_cast<u32x4*>(stage + S::kStage);
+      bool bad = false;
+      for (int i = lane; i < kTok * U; i += 64) bad |= not_finite(v[i]) != 0;
+      if (__any(bad)) {  // every wave has looked at the whole stage
+        __syncthreads();
+        for (int i = threadIdx.x; i < kTok * U; i += 64 * kWaves) v[i] = finite_or_zero(v[i]);
+        __syncthreads();
+        poisoned = true;
+      }
+    }
+    return stage;
+  };
+
+  if (!active) {
+    for (int t = t_begin; t < t_end; t += kTok) advance(t);
+    if constexpr (WT > 1) {
+      __syncthreads();
+      __syncthreads();
+    }
+    return;
+  }
 
   f32x4 o[NB][kDims], sum[NB];  // sum: the row's, in each of the four
   float base[NB];               // what the exponents are taken from: the maximum, or up to kSlack below
@@ -274,25 +338,9 @@ tree_attn_kernel(TreeArgs a) {
   }
   const float slack = kSlack / a.scale_log2;
 
-  int page = -1, page_next = -1;
-  if (t_begin < t_end) {
-    page = load_page(t_begin);
-    page_next = load_page(t_begin + kTok);
-    load_stage(t_begin, page, lds);
-  }
-  int buffer = 0;
-  for (int t = t_begin; t < t_end; t += kTok, buffer ^= 1) {
-    __builtin_amdgcn_s_waitcnt(kLoadsDone);
-    __syncthreads();  // the stage is in LDS, and the last one has been read by all
-    const char* const k_lds = lds + buffer * 2 * S::kStage;
+  for (int t = t_begin; t < t_end; t += kTok) {
+    const char* const k_lds = advance(t);
     const char* const v_lds = k_lds + S::kStage;
-    const uint64_t valid = __ballot(page >= 0 && page < a.num_blocks);
-    if (t + kTok < t_end) {
-      load_stage(t + kTok, page_next, lds + (buffer ^ 1) * 2 * S::kStage);
-      page = page_next;
-      page_next = load_page(t + 2 * kTok);
-    }
-    if (!active) continue;
     const bool drafted = t + kTok > rq.context;
 
     const int first = wt * S::kWaveTok;  // the wave's tokens of the stage
@@ -313,16 +361,17 @@ tree_attn_kernel(TreeArgs a) {
     }
 
     // Masked scores are replaced, whatever they hold.
-    uint64_t seen[NB];  // bit 16 u + r: the lane's token 16 u + 4 g + r
     if (drafted || valid != ~0ull) {
 #pragma unroll
       for (int i = 0; i < NB; ++i) {
-        seen[i] = (valid >> first & seen_from(a, node[i], t + first - rq.context)) >> (4 * g);
+        // bit 16 u + r: the lane's token 16 u + 4 g + r
+        const uint64_t seen =
+            (valid >> first & seen_from(a, node[i], t + first - rq.context)) >> (4 * g);
 #pragma unroll
         for (int u = 0; u < S::kSub; ++u)
 #pragma unroll
           for (int r = 0; r < 4; ++r)
-            sc[i][u][r] = (seen[i] >> (16 * u + r)) & 1 ? sc[i][u][r] : kNegInf;
+            sc[i][u][r] = (seen >> (16 * u + r)) & 1 ? sc[i][u][r] : kNegInf;
       }
     }
 
@@ -369,72 +418,19 @@ tree_attn_kernel(TreeArgs a) {
 #pragma unroll
       for (int i = 0; i < NB; ++i) add_product<S::kSub>(sum[i], ones, ones, p[i][u], p[i][u + S::kPair]);
 
-    // A drafted token's V may hold infinities or NaN that a row outside its
-    // branch must not see (0 times them is NaN). Such stages, rare, take them
-    // as 0, and count the ones that a row sees by a second product, of marks:
-    // those results are NaN.
-    bool bad = false;
-    if (drafted) {
-      for (int i = lane; i < S::kWaveTok * U; i += 64) {
-        const u32x4 v = load_u32x4(v_lds + first * D * 2 + i * 16);
-#pragma unroll
-        for (int w = 0; w < 4; ++w)
-          bad |= (v[w] & 0x7F80u) == 0x7F80u || (v[w] & 0x7F800000u) == 0x7F800000u;
-      }
-      bad = __any(bad);
-    }
     const char* const v_lane = v_lds + (first + 4 * g + (n >> 2)) * D * 2 + (n & 1) * 8;
     const int v_unit = (n & 3) >> 1, v_swz = v_swizzle<D>(first + 4 * g + (n >> 2));
-    if (!bad) {
 #pragma unroll
-      for (int u = 0; u < S::kSub; u += 2)
-#pragma unroll
-        for (int d = 0; d < kDims; ++d) {
-          const char* const src = v_lane + 16 * u * D * 2 + ((2 * d + v_unit) ^ v_swz) * 16;
-          const s16x4 v0 = read_transposed(src);
-          const s16x4 v1 = S::kPair ? read_transposed(src + 16 * D * 2) : v0;
-#pragma unroll
-          for (int i = 0; i < NB; ++i)
-            add_product<S::kSub>(o[i][d], v0, v1, p[i][u], p[i][u + S::kPair]);
-        }
-    } else {
+    for (int u = 0; u < S::kSub; u += 2)
 #pragma unroll
       for (int d = 0; d < kDims; ++d) {
-        f32x4 marks[NB] = {};
-#pragma unroll
-        for (int u = 0; u < S::kSub; u += 2) {
-          const char* const src = v_lane + 16 * u * D * 2 + ((2 * d + v_unit) ^ v_swz) * 16;
-          s16x4 v[2], mark[2];
-          v[0] = read_transposed(src);
-          v[1] = S::kPair ? read_transposed(src + 16 * D * 2) : v[0];
-#pragma unroll
-          for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              const bool odd = (v[h][r] & 0x7F80) == 0x7F80;
-              mark[h][r] = odd ? 0x3F80 : 0;
-              v[h][r] = odd ? 0 : v[h][r];
-            }
-#pragma unroll
-          for (int i = 0; i < NB; ++i) {
-            add_product<S::kSub>(o[i][d], v[0], v[1], p[i][u], p[i][u + S::kPair]);
-            uint32_t see[2][2];
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const uint32_t bits = (uint32_t)(seen[i] >> (16 * (u + h * S::kPair)));
-              see[h][0] = (bits & 1 ? 0x3F80u : 0u) | (bits & 2 ? 0x3F800000u : 0u);
-              see[h][1] = (bits & 4 ? 0x3F80u : 0u) | (bits & 8 ? 0x3F800000u : 0u);
-            }
-            add_product<S::kSub>(marks[i], mark[0], mark[1], see[0], see[1]);
-          }
-        }
+        const char* const src = v_lane + 16 * u * D * 2 + ((2 * d + v_unit) ^ v_swz) * 16;
+        const s16x4 v0 = read_transposed(src);
+        const s16x4 v1 = S::kPair ? read_transposed(src + 16 * D * 2) : v0;
 #pragma unroll
         for (int i = 0; i < NB; ++i)
-#pragma unroll
-          for (int r = 0; r < 4; ++r)
-            if (marks[i][r] > 0.0f) o[i][d][r] = __builtin_nanf("");
+          add_product<S::kSub>(o[i][d], v0, v1, p[i][u], p[i][u + S::kPair]);
       }
-    }
   }
 
   float total[NB];
@@ -489,6 +485,26 @@ tree_attn_kernel(TreeArgs a) {
     }
   }
 
+  if (poisoned) {
+    for (int pos = max(t_begin, rq.context); pos < t_end; ++pos) {
+      const int page = trow[a.page_div.div(pos)];
+      if (page < 0 || page >= a.num_blocks) continue;
+      const char* const v = a.v + kv * a.vh + ((uint64_t)page * a.vb << 4) +
+                            ((uint64_t)(pos - a.page_div.div(pos) * a.page_size) * a.vt << 4);
+#pragma unroll
+      for (int i = 0; i < NB; ++i) {
+        if (!(seen_from(a, node[i], pos - rq.context) & 1)) continue;
+#pragma unroll
+        for (int d = 0; d < kDims; ++d) {
+          const u32x2 x = load_u32x2(v + (16 * d + 4 * g) * 2);
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if ((x[r >> 1] >> (16 * (r & 1)) & 0x7F80u) == 0x7F80u) o[i][d][r] = __builtin_nanf("");
+        }
+      }
+    }
+  }
+
 #pragma unroll
   for (int i = 0; i < NB; ++i) {
     const int m = m0 + (wm * NB + i) * 16 + n;
@@ -520,34 +536,86 @@ tree_attn_kernel(TreeArgs a) {
   }
 }
 
-// Joins a row's chunks: out = sum_s 2^(lse_s - max) part_s / sum_s 2^(lse_s - max),
-// in chunk order. A workgroup per request and group of its rows; D / 4 lanes a
-// (row, head).
 template <int D>
+__global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 2))) void
+tree_attn_kernel(TreeArgs a) {
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  // Blocks go to the 8 XCDs in turn. Row tiles of one chunk are 8 blocks apart:
+  // the same XCD, whose L2 then serves the chunk's K/V to all but the first. A
+  // (request, kv head)'s chunks go round the XCDs, so that long and short
+  // requests spread evenly.
+  const int slot = (int)(blockIdx.x / (8 * a.m_tiles)) * 8 + (int)(blockIdx.x & 7);
+  const int m_tile = (int)(blockIdx.x >> 3) % a.m_tiles;
+  const int split = slot / a.pair_slots, place = slot % a.pair_slots;
+  const int pair = (place & ~7) | ((place - split) & 7);
+  if (pair >= a.requests * a.kv_heads) return;
+  const int kv = pair % a.kv_heads;
+  const int request = pair / a.kv_heads;
+  const Request rq = load_request(a, request);
+  const int32_t* const trow = a.table + request * a.table_row;
+  const int rows = rq.nodes * a.group;
+  const int m0 = m_tile * kTileRows;
+  const int t_begin = split * a.chunk;
+  if (m0 >= rows || (split > 0 && t_begin >= rq.length)) return;
+  // The last chunk takes whatever is left (a context longer than was said).
+  const int t_end = split + 1 == a.splits ? rq.length : min(rq.length, t_begin + a.chunk);
+  // The wave shares by the tile's own rows: requests of one batch differ.
+  const int left = rows - m0;
+  if (left > 64) attend_tile<D, 2, 4, 1>(a, rq, trow, kv, rows, m0, split, t_begin, t_end, lds);
+  else if (left > 32) attend_tile<D, 2, 2, 2>(a, rq, trow, kv, rows, m0, split, t_begin, t_end, lds);
+  else if (left > 16) attend_tile<D, 2, 1, 4>(a, rq, trow, kv, rows, m0, split, t_begin, t_end, lds);
+  else attend_tile<D, 1, 1, 4>(a, rq, trow, kv, rows, m0, split, t_begin, t_end, lds);
+}
+
+// Joins a row's chunks: out = sum_s 2^(lse_s - max) part_s / sum_s 2^(lse_s - max).
+// D / 4 lanes hold a (row, head)'s dims; WAYS such groups take its chunks in
+// turn (s mod WAYS) and add up in group order, so that a long context's many
+// partials are read side by side. Bound by reading the partials.
+template <int D, int WAYS>
 __global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs a, int row_tiles) {
   constexpr int kLanes = D / 4;
-  constexpr int kPer = 256 / kLanes;
+  constexpr int kGroups = 256 / kLanes;
+  constexpr int kPer = kGroups / WAYS;  // (row, head)s of a workgroup
+  __shared__ f32x4 acc_lds[WAYS > 1 ? kGroups : 1][kLanes];
+  __shared__ float sum_lds[WAYS > 1 ? kGroups : 1];
   const Request rq = load_request(a, blockIdx.x / row_tiles);
-  const int64_t item = (int64_t)(blockIdx.x % row_tiles) * kPer + threadIdx.x / kLanes;
-  const int64_t node = item / a.num_q_heads;
-  if (node >= rq.nodes) return;
-  const int head = (int)(item - node * a.num_q_heads);
+  const int lane = threadIdx.x % kLanes, grp = threadIdx.x / kLanes;
+  const int way = grp % WAYS;
+  const int64_t item = (int64_t)(blockIdx.x % row_tiles) * kPer + grp / WAYS;
+  const int node = (int)(item / a.num_q_heads);
+  const bool live = node < rq.nodes;
+  const int head = (int)(item - (int64_t)node * a.num_q_heads);
   const int64_t row = rq.row0 + node;
-  const int splits = min(a.splits, max(1, (rq.length + a.chunk - 1) / a.chunk));
-  const int lane = threadIdx.x % kLanes;
-  const int64_t at = (row * a.num_q_heads + head) * a.splits;
+  const int splits = live ? min(a.splits, max(1, (rq.length + a.chunk - 1) / a.chunk)) : 0;
+  const int64_t at = live ? (row * a.num_q_heads + head) * a.splits : 0;
+  const float* const lse = a.part_lse + at;
   float top = kNegInf;
-  for (int s = 0; s < splits; ++s) top = fmaxf(top, a.part_lse[at + s]);
+  for (int s = lane; s < splits; s += kLanes) top = fmaxf(top, lse[s]);
+#pragma unroll
+  for (int w = kLanes / 2; w > 0; w /= 2) top = fmaxf(top, __shfl_xor(top, w, 64));
   const float base = top == kNegInf ? 0.0f : top;
   float sum = 0.0f;
   f32x4 acc = {0, 0, 0, 0};
-  for (int s = 0; s < splits; ++s) {
-    const float f = fast_exp2(a.part_lse[at + s] - base);
+#pragma unroll 4
+  for (int s = way; s < splits; s += WAYS) {
+    const float f = fast_exp2(lse[s] - base);
     const f32x4 part = *reinterpret_cast<const f32x4*>(a.part_out + (at + s) * D + 4 * lane);
     sum += f;
 #pragma unroll
     for (int r = 0; r < 4; ++r) acc[r] += f * part[r];
   }
+  if constexpr (WAYS > 1) {
+    acc_lds[grp][lane] = acc;
+    if (lane == 0) sum_lds[grp] = sum;
+    __syncthreads();
+    if (way > 0) return;
+#pragma unroll
+    for (int w = 1; w < WAYS; ++w) {
+      acc += acc_lds[grp + w][lane];
+      sum += sum_lds[grp + w];
+    }
+  }
+  if (!live) return;
   const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
   float y[4];
 #pragma unroll
@@ -565,11 +633,8 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs a, int row_til
 // ---------------------------------------------------------------------------
 
 struct TreePlan {
-  int tile_rows;  // (node, head) rows of a workgroup
   int m_tiles, splits, chunk;
 };
-
-int tile_rows_for(int64_t rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128; }
 
 // max_nodes and max_context bound the requests' nodes and committed tokens; the
 // results do not depend on the chunks beyond fp32 rounding, and a request longer
@@ -578,12 +643,18 @@ TreePlan make_plan(int requests, int num_q_heads, int num_kv_heads, int64_t max_
                    int64_t max_context) {
   TreePlan p;
   const int64_t rows = max_nodes * (num_q_heads / num_kv_heads);
-  p.tile_rows = tile_rows_for(rows);
-  p.m_tiles = (int)((rows + p.tile_rows - 1) / p.tile_rows);
+  p.m_tiles = (int)((rows + kTileRows - 1) / kTileRows);
   const int64_t units = (int64_t)requests * num_kv_heads * p.m_tiles;
   const int64_t length = std::min<int64_t>(max_context + max_nodes, INT_MAX / 2);
   const int64_t stages = std::max<int64_t>(1, (length + kTok - 1) / kTok);
-  int64_t splits = std::min<int64_t>((2 * kCUs + units - 1) / units, (stages + 3) / 4);
+  // Two workgroups fit a CU. One request's chunks are alike: one round of them
+  // (64 nodes on 131072 tokens 97 us, a round and a half 108, two 107, and each
+  // chunk's partial result is written and read again). Several requests differ
+  // in length and rows, and a chunk of the longest's share leaves CUs without
+  // work: four rounds by the longest (32 trees on 4k-32k 230 us, one round 280,
+  // eight 231; 64 single tokens on 1k-8k 73, 68 and 78).
+  const int64_t rounds = requests == 1 ? 1 : 4;
+  int64_t splits = std::min<int64_t>((rounds * 2 * kCUs + units - 1) / units, stages);
   splits = std::max<int64_t>(1, std::min<int64_t>(splits, 256));
   const int64_t per = (stages + splits - 1) / splits;
   p.chunk = (int)std::min<int64_t>(per * kTok, INT_MAX / 2);
@@ -591,33 +662,36 @@ TreePlan make_plan(int requests, int num_q_heads, int num_kv_heads, int64_t max_
   return p;
 }
 
-template <int D, int NB, int WM, int WT>
-hipError_t launch_tile(const TreeArgs& a, unsigned grid, hipStream_t stream) {
-  const size_t lds = Shape<D, NB, WM, WT>::kLds;
-  auto* kernel = &tree_attn_kernel<D, NB, WM, WT>;
-  if (lds > 65536) {
-    const hipError_t err = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
-                                               hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
-    if (err != hipSuccess) return err;
-  }
-  hipLaunchKernelGGL(kernel, dim3(grid), dim3(64 * kWaves), lds, stream, a);
+template <int D, int WAYS>
+hipError_t launch_merge(const TreeArgs& a, int64_t pairs, hipStream_t stream) {
+  constexpr int kPer = 256 / (D / 4) / WAYS;
+  const int row_tiles = (int)((pairs + kPer - 1) / kPer);
+  hipLaunchKernelGGL((tree_merge_kernel<D, WAYS>), dim3((unsigned)(a.requests * row_tiles)),
+                     dim3(256), 0, stream, a, row_tiles);
   return hipGetLastError();
 }
 
 template <int D>
-hipError_t launch_tree(const TreeArgs& a, const TreePlan& plan, int max_nodes, hipStream_t stream) {
-  const unsigned grid = (unsigned)(((int64_t)a.units + 7) / 8 * 8 * a.m_tiles);
-  hipError_t err;
-  if (plan.tile_rows == 16) err = launch_tile<D, 1, 1, 4>(a, grid, stream);
-  else if (plan.tile_rows == 32) err = launch_tile<D, 2, 1, 4>(a, grid, stream);
-  else if (plan.tile_rows == 64) err = launch_tile<D, 2, 2, 2>(a, grid, stream);
-  else err = launch_tile<D, 2, 4, 1>(a, grid, stream);
+hipError_t launch_tree(const TreeArgs& a, int max_nodes, hipStream_t stream) {
+  const unsigned grid = (unsigned)((int64_t)a.pair_slots * a.splits * a.m_tiles);
+  constexpr size_t kLds = std::max({Shape<D, 2, 4, 1>::kLds, Shape<D, 2, 2, 2>::kLds,
+                                    Shape<D, 2, 1, 4>::kLds, Shape<D, 1, 1, 4>::kLds});
+  static_assert(kLds <= 65536, "two workgroups a CU, and no attribute to set");
+  hipLaunchKernelGGL((tree_attn_kernel<D>), dim3(grid), dim3(64 * kWaves), kLds, stream, a);
+  const hipError_t err = hipGetLastError();
   if (err != hipSuccess || a.splits == 1) return err;
-  constexpr int kPer = 256 / (D / 4);
-  const int row_tiles = (int)(((int64_t)max_nodes * a.num_q_heads + kPer - 1) / kPer);
-  hipLaunchKernelGGL((tree_merge_kernel<D>), dim3((unsigned)(a.requests * row_tiles)), dim3(256), 0,
-                     stream, a, row_tiles);
-  return hipGetLastError();
+  const int64_t pairs = (int64_t)max_nodes * a.num_q_heads;
+  if (a.splits >= 8) return launch_merge<D, 8>(a, pairs, stream);
+  return launch_merge<D, 2>(a, pairs, stream);
+}
+
+// Elements from a cache's first token row to its last, -1 if a stride is negative
+// or the span past 2^62.
+int64_t cache_span(int64_t blocks, int64_t block_stride, int64_t page, int64_t token_stride) {
+  if (block_stride < 0 || token_stride < 0 || block_stride >= INT64_MAX / 4 / (blocks + 1) ||
+      token_stride >= INT64_MAX / 4 / page)
+    return -1;
+  return blocks > 0 ? (blocks - 1) * block_stride + (page - 1) * token_stride : 0;
 }
 
 bool aligned16(const void* p) { return ((uintptr_t)p & 15u) == 0; }
@@ -670,15 +744,17 @@ extern "C" int qsa_tree_attention(
       ((out_row_stride | out_head_stride) & 1))
     return fail(QSA_ERR_INVALID, name + ": q and the caches need 16-byte alignment and strides of "
                                         "multiples of 8 elements, out 4-byte alignment");
-  for (int64_t stride : {k_block_stride, k_token_stride, v_block_stride, v_token_stride})
-    if (stride < 0 || stride > INT_MAX / 2)
-      return fail(QSA_ERR_UNSUPPORTED, name + ": cache strides must be under 2 GiB");
+  // The kernel's offsets are 32-bit counts of 16 bytes.
+  const int64_t span = std::max(cache_span(num_blocks, k_block_stride, page_size, k_token_stride),
+                                cache_span(num_blocks, v_block_stride, page_size, v_token_stride));
+  if (span < 0 || span / 8 >= kNoToken)
+    return fail(QSA_ERR_UNSUPPORTED, name + ": the cache must span under 64 GiB");
   max_query_len = std::min(max_query_len, rows);
   const TreePlan plan =
       make_plan(num_requests, num_q_heads, num_kv_heads, max_query_len, max_context_len);
-  const int64_t units = (int64_t)num_requests * num_kv_heads * plan.splits;
-  const int64_t grid = (units + 7) / 8 * 8 * plan.m_tiles;
-  const int64_t merge = (int64_t)num_requests * (((int64_t)max_query_len * num_q_heads + 7) / 8);
+  const int64_t pair_slots = ((int64_t)num_requests * num_kv_heads + 7) / 8 * 8;
+  const int64_t grid = pair_slots * plan.splits * plan.m_tiles;
+  const int64_t merge = (int64_t)num_requests * max_query_len * num_q_heads;
   if (grid > INT_MAX || merge > INT_MAX || (int64_t)max_query_len * num_q_heads > INT_MAX / 2)
     return fail(QSA_ERR_UNSUPPORTED, name + ": too many requests, rows or heads");
   TreeArgs a = {};
@@ -696,11 +772,11 @@ extern "C" int qsa_tree_attention(
   a.q_head = q_head_stride;
   a.k = static_cast<const char*>(k_cache);
   a.v = static_cast<const char*>(v_cache);
-  a.kb = (uint32_t)(2 * k_block_stride);
-  a.kt = (uint32_t)(2 * k_token_stride);
+  a.kb = (uint32_t)(k_block_stride / 8);
+  a.kt = (uint32_t)(k_token_stride / 8);
   a.kh = 2 * k_head_stride;
-  a.vb = (uint32_t)(2 * v_block_stride);
-  a.vt = (uint32_t)(2 * v_token_stride);
+  a.vb = (uint32_t)(v_block_stride / 8);
+  a.vt = (uint32_t)(v_token_stride / 8);
   a.vh = 2 * v_head_stride;
   a.num_blocks = num_blocks;
   a.page_size = page_size;
@@ -728,12 +804,12 @@ extern "C" int qsa_tree_attention(
   a.group_div = FastDiv::make(a.group);
   a.m_tiles = plan.m_tiles;
   a.splits = plan.splits;
-  a.units = (int)units;
+  a.pair_slots = (int)pair_slots;
   a.chunk = plan.chunk;
   a.scale_log2 = 1.4426950408889634f / sqrtf((float)head_dim);
   hipStream_t s = static_cast<hipStream_t>(stream);
-  const hipError_t err = head_dim == 128 ? launch_tree<128>(a, plan, max_query_len, s)
-                                         : launch_tree<64>(a, plan, max_query_len, s);
+  const hipError_t err = head_dim == 128 ? launch_tree<128>(a, max_query_len, s)
+                                         : launch_tree<64>(a, max_query_len, s);
   if (err != hipSuccess)
     return fail(QSA_ERR_HIP, name + " launch: " + hipGetErrorString(err));
   return QSA_OK;
