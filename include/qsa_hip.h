@@ -497,8 +497,8 @@ int qsa_gdn_gated_norm(const void* o, const void* qkvz, int64_t qkvz_stride, con
  *   codes  [n tiles][k tiles][lane 64][word 4] uint32, 16-byte aligned: lane
  *          16 g + n, word j holds output n's inputs 32 j + 8 g + 0..7 of the
  *          tile, input 2 p in bits 4 p.., input 2 p + 1 in bits 16 + 4 p..;
- *   scales [n tiles][groups][16]; zeros [n tiles][groups][16] uint8 0..15 or
- *          null (8 everywhere), groups = k tiles * 128 / group_size.
+ *   scales [n tiles][k tiles][16][128 / group_size], 8-byte aligned; zeros the
+ *          same in uint8 0..15, 4-byte aligned, or null (8 everywhere).
  * group_size 32, 64 or 128. bias may be null. A row of x that holds an infinity
  * or NaN (or, in bf16, values past 2^112) has no defined result; other rows are
  * not touched by it. Any alignment and row stride; 16-byte aligned rows and

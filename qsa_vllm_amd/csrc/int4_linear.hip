@@ -8,22 +8,30 @@
 // Mathematics. A group's scale is a factor of its whole sum, so the codes go
 // into the matrix product as small whole numbers and the scale multiplies the
 // group's fp32 sum: nothing is rounded before the output. With bf16 the code q
-// becomes 128 + q by one and-or (bf16 holds whole numbers to 256), and
-//   sum x (q - z) = sum x (128 + q) - (128 + z) sum x,
-// with sum x from the same matrix instruction against ones; both in fp32, whose
-// step is 2^-15 of bf16's. With fp16 the code becomes 1024 + q (or 1024 + 16 q)
-// and one packed add (or fma) gives q - z exactly.
+// becomes c0 + q - z by an and and an or (or add), c0 = 192 with zero points
+// and 136 without: bf16 holds whole numbers to 256. Then
+//   sum x (q - z) = sum x (c0 + q - z) - c0 sum x,
+// and the last term, the same for every output, is the accumulator's start: the
+// product of x with a constant. Both are summed in fp32, whose step is 2^-16 of
+// bf16's. With fp16 the code becomes 1024 + q (or 1024 + 16 q) and one packed
+// add (or fma) gives q - z exactly.
 //
 // Layout. Weights are stored in tiles of 16 outputs x 128 inputs, 1 KiB each:
 // lane (n, g) of a wave holds output n's codes of inputs 32 j + 8 g .. + 7 as
 // word j, the B operand of mfma_f32_16x16x32 after unpacking, element 2 p of a
 // word in bits 4 p and element 2 p + 1 in bits 16 + 4 p. So a wave reads a tile
-// with one 16-byte load a lane, and unpacking is shifts and and-ors alone.
+// with one 16-byte load a lane, unpacking is shifts, ands and ors, and a tile's
+// scales (zero points) of an output are one load.
 //
-// Work. A workgroup owns 16 NT outputs and 16 MT rows; its waves share the
-// inputs, tile t going to wave t mod waves, and add their sums through LDS in
-// wave order (no atomics, the same bits every time). Each weight is read once
-// per block of 16 MT rows.
+// Two kernels, by rows:
+//  * to 16 rows, bound by streaming the weight: a wave takes whole tiles, its
+//    workgroup's waves share the inputs (tile t to wave t mod waves), and
+//    activations come straight from L2;
+//  * more, where each workgroup's re-reading of the activations is the larger
+//    traffic: they go through LDS in whole 256-byte rows, shared by the waves
+//    that take different outputs (int4_rows_kernel).
+// Waves that share the inputs add their sums through LDS in wave order: no
+// atomics, the same bits every time.
 #include "qsa_common.h"
 #include "../../include/qsa_hip.h"
 
@@ -38,13 +46,16 @@ typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 constexpr int kTileN = 16;
 constexpr int kTileK = 128;
 
+// s_waitcnt for the vector-memory counter alone (gfx9 encoding), at 0.
+constexpr int loads_done() { return (7 << 4) | (15 << 8); }
+
 struct Int4Args {
   const uint16_t* x;
   int64_t x_row;
-  const u32x4* codes;       // [n tiles][k tiles][64 lanes]
-  const uint16_t* scales;   // [n tiles][groups][16]
-  const uint8_t* zeros;     // [n tiles][groups][16] or null
-  const uint16_t* bias;     // [n] or null
+  const u32x4* codes;     // [n tiles][k tiles][64 lanes]
+  const char* scales;     // [n tiles][k tiles][16][128 / G] 16-bit
+  const char* zeros;      // [n tiles][k tiles][16][128 / G] 8-bit, or null
+  const uint16_t* bias;   // [n] or null
   uint16_t* y;
   int64_t y_row;
   int rows, n, k;
@@ -52,22 +63,55 @@ struct Int4Args {
   int row_blocks;
 };
 
+// GROUPS values of 16 (8) bits of a tile's output, loaded at once.
+template <int GROUPS>
+struct GroupWords;
+template <>
+struct GroupWords<1> {
+  typedef uint16_t scales;
+  typedef uint8_t zeros;
+};
+template <>
+struct GroupWords<2> {
+  typedef uint32_t scales;
+  typedef uint16_t zeros;
+};
+template <>
+struct GroupWords<4> {
+  typedef u32x2 scales;
+  typedef uint32_t zeros;
+};
+__device__ __forceinline__ uint16_t scale_of(uint16_t v, int) { return v; }
+__device__ __forceinline__ uint16_t scale_of(uint32_t v, int q) { return (uint16_t)(v >> (16 * q)); }
+__device__ __forceinline__ uint16_t scale_of(const u32x2& v, int q) {
+  return (uint16_t)(v[q >> 1] >> (16 * (q & 1)));
+}
+
+// A type's matrix operand: unpacking a word of codes with a zero point's
+// constant, and what the accumulator's start takes off again.
+template <bool ZEROS>
 struct Bf16 {
   typedef bf16x8 frag;
-  static constexpr bool kOffset = true;  // unpacked codes are 128 + q
+  static constexpr bool kOffset = true;
   static __device__ __forceinline__ f32x4 mfma(frag a, frag b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
   }
-  static __device__ __forceinline__ frag unpack(uint32_t w, int) {
+  // 192 - z in both halves (128, to which a code is or-ed, without zero points).
+  static __device__ __forceinline__ uint32_t zero_word(int z) {
+    return ZEROS ? 0x43404340u - (uint32_t)z * 0x10001u : 0x43004300u;
+  }
+  static __device__ __forceinline__ frag unpack(uint32_t w, uint32_t zero) {
     u32x4 r;
-    r[0] = (w & 0x000F000Fu) | 0x43004300u;
-    r[1] = ((w >> 4) & 0x000F000Fu) | 0x43004300u;
-    r[2] = ((w >> 8) & 0x000F000Fu) | 0x43004300u;
-    r[3] = ((w >> 12) & 0x000F000Fu) | 0x43004300u;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t q = (w >> (4 * i)) & 0x000F000Fu;
+      r[i] = ZEROS ? q + zero : q | zero;
+    }
     return __builtin_bit_cast(frag, r);
   }
-  static __device__ __forceinline__ frag ones() {
-    return __builtin_bit_cast(frag, (u32x4{0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u}));
+  static __device__ __forceinline__ frag offset() {  // -192 or -136
+    const uint32_t c = ZEROS ? 0xC340C340u : 0xC308C308u;
+    return __builtin_bit_cast(frag, (u32x4{c, c, c, c}));
   }
   static __device__ __forceinline__ float to_float(uint16_t v) {
     return __builtin_bit_cast(float, (uint32_t)v << 16);
@@ -77,30 +121,35 @@ struct Bf16 {
   }
 };
 
+template <bool ZEROS>
 struct Fp16 {
   typedef f16x8 frag;
-  static constexpr bool kOffset = false;  // unpacked codes are q - z
+  static constexpr bool kOffset = false;
   static __device__ __forceinline__ f32x4 mfma(frag a, frag b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
   }
-  static __device__ __forceinline__ frag unpack(uint32_t w, int z) {
-    const _Float16 low = (_Float16)(-1024 - z), high = (_Float16)(-64 - z);
-    const f16x2 low2 = {low, low}, high2 = {high, high}, sixteenth = {(_Float16)0.0625f,
-                                                                      (_Float16)0.0625f};
+  static __device__ __forceinline__ uint32_t zero_word(int z) {  // -1024 - z in both halves
+    return 0xE400E400u + (uint32_t)z * 0x10001u;
+  }
+  static __device__ __forceinline__ frag unpack(uint32_t w, uint32_t zero) {
+    const f16x2 low = __builtin_bit_cast(f16x2, zero);
+    const f16x2 gap = {(_Float16)960.0f, (_Float16)960.0f};
+    const f16x2 high = low + gap;  // -64 - z
+    const f16x2 sixteenth = {(_Float16)0.0625f, (_Float16)0.0625f};
     union {
       f16x2 p[4];
       frag f;
     } r;
     const uint32_t v = w >> 8;
-    r.p[0] = __builtin_bit_cast(f16x2, (w & 0x000F000Fu) | 0x64006400u) + low2;
+    r.p[0] = __builtin_bit_cast(f16x2, (w & 0x000F000Fu) | 0x64006400u) + low;
     r.p[1] = __builtin_elementwise_fma(
-        __builtin_bit_cast(f16x2, (w & 0x00F000F0u) | 0x64006400u), sixteenth, high2);
-    r.p[2] = __builtin_bit_cast(f16x2, (v & 0x000F000Fu) | 0x64006400u) + low2;
+        __builtin_bit_cast(f16x2, (w & 0x00F000F0u) | 0x64006400u), sixteenth, high);
+    r.p[2] = __builtin_bit_cast(f16x2, (v & 0x000F000Fu) | 0x64006400u) + low;
     r.p[3] = __builtin_elementwise_fma(
-        __builtin_bit_cast(f16x2, (v & 0x00F000F0u) | 0x64006400u), sixteenth, high2);
+        __builtin_bit_cast(f16x2, (v & 0x00F000F0u) | 0x64006400u), sixteenth, high);
     return r.f;
   }
-  static __device__ __forceinline__ frag ones() { return frag{}; }  // not used
+  static __device__ __forceinline__ frag offset() { return frag{}; }  // not used
   static __device__ __forceinline__ float to_float(uint16_t v) {
     return (float)__builtin_bit_cast(_Float16, v);
   }
@@ -108,6 +157,85 @@ struct Fp16 {
     return __builtin_bit_cast(uint16_t, (_Float16)v);
   }
 };
+
+// A wave's weight tiles of one k tile: NT adjacent n tiles.
+template <int GROUP, bool ZEROS, int NT>
+struct Tiles {
+  static constexpr int kGroups = kTileK / GROUP;
+  typedef GroupWords<kGroups> Words;
+  u32x4 w[NT];
+  typename Words::scales s[NT];
+  typename Words::zeros z[NT];
+  // Tiles past the last (an odd end) are read as the last one; not stored.
+  __device__ __forceinline__ void load(const Int4Args& a, int tile0, int t, int lane) {
+#pragma unroll
+    for (int v = 0; v < NT; ++v) {
+      const int64_t at = (int64_t)min(tile0 + v, a.n_tiles - 1) * a.k_tiles + t;
+      w[v] = a.codes[at * 64 + lane];
+      const int64_t group = at * 16 + (lane & 15);
+      s[v] = *reinterpret_cast<const typename Words::scales*>(a.scales + group * (2 * kGroups));
+      if constexpr (ZEROS)
+        z[v] = *reinterpret_cast<const typename Words::zeros*>(a.zeros + group * kGroups);
+    }
+  }
+  __device__ __forceinline__ int zero(int v, int q) const {
+    return ZEROS ? (int)(((uint32_t)z[v] >> (8 * q)) & 0xFFu) : 8;
+  }
+};
+
+// acc += x (MT x 16 rows, the k tile's four operands each) times the tiles.
+template <typename T, int GROUP, bool ZEROS, int MT, int NT>
+__device__ __forceinline__ void multiply(const u32x4 (&x)[MT][4], const Tiles<GROUP, ZEROS, NT>& b,
+                                         f32x4 (&acc)[MT][NT]) {
+  typedef typename T::frag frag;
+  constexpr int kSteps = GROUP / 32;  // matrix instructions per group
+#pragma unroll
+  for (int q = 0; q < kTileK / GROUP; ++q) {
+    f32x4 start[MT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+      start[i] = f32x4{0, 0, 0, 0};
+      if constexpr (T::kOffset) {
+#pragma unroll
+        for (int j = 0; j < kSteps; ++j)
+          start[i] = T::mfma(__builtin_bit_cast(frag, x[i][q * kSteps + j]), T::offset(), start[i]);
+      }
+    }
+#pragma unroll
+    for (int v = 0; v < NT; ++v) {
+      const float scale = T::to_float(scale_of(b.s[v], q));
+      const uint32_t zero = T::zero_word(b.zero(v, q));
+      f32x4 d[MT];
+#pragma unroll
+      for (int i = 0; i < MT; ++i) d[i] = start[i];
+#pragma unroll
+      for (int j = 0; j < kSteps; ++j) {
+        const frag f = T::unpack(b.w[v][q * kSteps + j], zero);
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+          d[i] = T::mfma(__builtin_bit_cast(frag, x[i][q * kSteps + j]), f, d[i]);
+      }
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) acc[i][v][r] = __builtin_fmaf(scale, d[i][r], acc[i][v][r]);
+    }
+  }
+}
+
+// A tile's sums (a lane: rows 4 g + r of output n) to y.
+template <typename T>
+__device__ __forceinline__ void store(const Int4Args& a, int m0, int tile, int lane,
+                                      const f32x4& sum) {
+  const int col = tile * kTileN + (lane & 15);
+  if (col >= a.n) return;
+  const float b = a.bias ? T::to_float(a.bias[col]) : 0.0f;
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    const int m = m0 + 4 * (lane >> 4) + r;
+    if (m < a.rows) a.y[m * a.y_row + col] = T::from_float(sum[r] + b);
+  }
+}
 
 // Eight activations from input k on: VEC reads 16 bytes (row stride, width and
 // address multiples of 8 elements), otherwise element by element. Inputs past
@@ -130,9 +258,9 @@ __device__ __forceinline__ u32x4 load_x(const uint16_t* row, int k, int width, b
 
 template <typename T, int GROUP, bool ZEROS, int MT, int NT, bool VEC>
 __global__ __launch_bounds__(512) void int4_linear_kernel(Int4Args a) {
-  constexpr int kGroups = kTileK / GROUP;  // per k tile
-  constexpr int kSteps = GROUP / 32;       // matrix instructions per group
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+  typedef Tiles<GROUP, ZEROS, NT> Weights;
+  const int lane = threadIdx.x & 63, waves = blockDim.x >> 6;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n = lane & 15, g = lane >> 4;
   const int row0 = (blockIdx.x % a.row_blocks) * (16 * MT);
   const int tile0 = (blockIdx.x / a.row_blocks) * NT;
@@ -146,73 +274,37 @@ __global__ __launch_bounds__(512) void int4_linear_kernel(Int4Args a) {
     live[i] = m < a.rows;
     xrow[i] = a.x + (live[i] ? m : 0) * a.x_row;
   }
-  const int64_t groups = (int64_t)a.k_tiles * kGroups;
-
-  for (int t = wave; t < a.k_tiles; t += waves) {
-    u32x4 w[NT];
-    uint16_t s[NT][kGroups];
-    uint8_t z[NT][kGroups];
-#pragma unroll
-    for (int j = 0; j < NT; ++j) {
-      const int64_t tile = min(tile0 + j, a.n_tiles - 1);
-      w[j] = a.codes[(tile * a.k_tiles + t) * 64 + lane];
-#pragma unroll
-      for (int q = 0; q < kGroups; ++q) {
-        const int64_t at = (tile * groups + (int64_t)t * kGroups + q) * 16 + n;
-        s[j][q] = a.scales[at];
-        z[j][q] = ZEROS ? a.zeros[at] : 8;
-      }
-    }
-    u32x4 x[MT][4];
+  auto load_rows = [&](int t, u32x4 (&x)[MT][4]) {
 #pragma unroll
     for (int i = 0; i < MT; ++i)
 #pragma unroll
       for (int j = 0; j < 4; ++j)
         x[i][j] = load_x<VEC>(xrow[i], t * kTileK + 32 * j + 8 * g, a.k, live[i]);
-
-#pragma unroll
-    for (int q = 0; q < kGroups; ++q) {
-      f32x4 total[MT];
-#pragma unroll
-      for (int i = 0; i < MT; ++i) {
-        total[i] = f32x4{0, 0, 0, 0};
-        if constexpr (T::kOffset) {
-#pragma unroll
-          for (int j = 0; j < kSteps; ++j)
-            total[i] = T::mfma(__builtin_bit_cast(typename T::frag, x[i][q * kSteps + j]),
-                               T::ones(), total[i]);
-        }
-      }
-#pragma unroll
-      for (int v = 0; v < NT; ++v) {
-        const float scale = T::to_float(s[v][q]);
-        const float offset = -(float)(128 + z[v][q]);
-        f32x4 d[MT];
-#pragma unroll
-        for (int i = 0; i < MT; ++i) {
-          d[i] = f32x4{0, 0, 0, 0};
-          if constexpr (T::kOffset) {
-#pragma unroll
-            for (int r = 0; r < 4; ++r) d[i][r] = offset * total[i][r];
-          }
-        }
-#pragma unroll
-        for (int j = 0; j < kSteps; ++j) {
-          const typename T::frag b = T::unpack(w[v][q * kSteps + j], z[v][q]);
-#pragma unroll
-          for (int i = 0; i < MT; ++i)
-            d[i] = T::mfma(__builtin_bit_cast(typename T::frag, x[i][q * kSteps + j]), b, d[i]);
-        }
-#pragma unroll
-        for (int i = 0; i < MT; ++i)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) acc[i][v][r] = __builtin_fmaf(scale, d[i][r], acc[i][v][r]);
-      }
+  };
+  // Two tiles in flight: the next one's loads are issued before this one's
+  // product.
+  Weights b0, b1;
+  u32x4 x0[MT][4], x1[MT][4];
+  int t = wave;
+  b0.load(a, tile0, t, lane);
+  load_rows(t, x0);
+  while (true) {
+    int next = t + waves;
+    if (next < a.k_tiles) {
+      b1.load(a, tile0, next, lane);
+      load_rows(next, x1);
     }
+    multiply<T, GROUP, ZEROS, MT, NT>(x0, b0, acc);
+    if (next >= a.k_tiles) break;
+    t = next + waves;
+    if (t < a.k_tiles) {
+      b0.load(a, tile0, t, lane);
+      load_rows(t, x0);
+    }
+    multiply<T, GROUP, ZEROS, MT, NT>(x1, b1, acc);
+    if (t >= a.k_tiles) break;
   }
 
-  // The waves' sums, in wave order. A lane's accumulators are rows 4 g + r of
-  // output n.
   extern __shared__ f32x4 part[];  // [waves][MT * NT][64]
 #pragma unroll
   for (int i = 0; i < MT; ++i)
@@ -222,52 +314,172 @@ __global__ __launch_bounds__(512) void int4_linear_kernel(Int4Args a) {
   for (int u = wave; u < MT * NT; u += waves) {
     f32x4 sum = part[u * 64 + lane];
     for (int o = 1; o < waves; ++o) sum += part[(o * MT * NT + u) * 64 + lane];
-    const int col = (tile0 + u % NT) * kTileN + n;
-    if (col < a.n) {
-      const float b = a.bias ? T::to_float(a.bias[col]) : 0.0f;
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int m = row0 + 16 * (u / NT) + 4 * g + r;
-        if (m < a.rows) a.y[m * a.y_row + col] = T::from_float(sum[r] + b);
-      }
-    }
+    store<T>(a, row0 + 16 * (u / NT), tile0 + u % NT, lane, sum);
   }
 }
 
-template <typename T, int GROUP, bool ZEROS, int MT, int NT>
-void launch_vec(const Int4Args& a, bool vec, unsigned grid, int waves, hipStream_t stream) {
-  const size_t lds = (size_t)waves * MT * NT * 64 * sizeof(f32x4);
-  if (vec)
-    hipLaunchKernelGGL((int4_linear_kernel<T, GROUP, ZEROS, MT, NT, true>), dim3(grid),
-                       dim3(64 * waves), lds, stream, a);
-  else
-    hipLaunchKernelGGL((int4_linear_kernel<T, GROUP, ZEROS, MT, NT, false>), dim3(grid),
-                       dim3(64 * waves), lds, stream, a);
+// More than 16 rows: a workgroup of WN x WK waves takes 16 MT rows and 16 NT WN
+// outputs, wave (wn, wk) NT n tiles and KS of every WK KS k tiles. A step's
+// activations (WK KS tiles of 16 MT rows x 256 bytes) go straight into LDS, one
+// step ahead in the other of two buffers; weights one step ahead in registers.
+// Unit u (16 bytes) of a row sits at place u ^ (row mod 16), so that the A
+// operand's reads (16 rows' same unit) lie in different banks.
+template <typename T, int GROUP, bool ZEROS, int MT, int NT, int WN, int WK, int KS>
+__global__ __launch_bounds__(64 * WN * WK) __attribute__((amdgpu_waves_per_eu(2, 2))) void
+int4_rows_kernel(Int4Args a) {
+  typedef Tiles<GROUP, ZEROS, NT> Weights;
+  constexpr int kWaves = WN * WK;
+  constexpr int kStepTiles = WK * KS;
+  constexpr int kTileBytes = 16 * MT * 256;
+  constexpr int kBlocks = kStepTiles * 16 * MT / 4;  // 4 rows of 256 bytes an instruction
+  static_assert(kBlocks % kWaves == 0, "");
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int n = lane & 15, g = lane >> 4;
+  const int wn = wave % WN, wk = wave / WN;
+  // Row blocks of the same outputs are 8 blocks apart: one XCD, whose L2 then
+  // serves the weight to all but the first.
+  const int slot = (int)(blockIdx.x / (8 * a.row_blocks)) * 8 + (int)(blockIdx.x & 7);
+  const int row0 = ((int)(blockIdx.x >> 3) % a.row_blocks) * (16 * MT);
+  const int tile0 = (slot * WN + wn) * NT;
+  if (slot * WN * NT >= a.n_tiles) return;
+
+  const char* const zero = reinterpret_cast<const char*>(g_qsa_zero_rows);
+  const char* const xbase = reinterpret_cast<const char*>(a.x + row0 * a.x_row);
+  auto load_rows = [&](int step, char* stage) {
+#pragma unroll
+    for (int i = 0; i < kBlocks / kWaves; ++i) {
+      const int block = i * kWaves + wave;  // of tile block / (4 MT)
+      const int t = step * kStepTiles + block / (4 * MT);
+      const int row = block % (4 * MT) * 4 + g;
+      const int unit = n ^ (row & 15);
+      const int k = t * kTileK + unit * 8;
+      // Rows past the last repeat it (their results are not stored); inputs past
+      // the width are zero.
+      const uint32_t at = (uint32_t)min(row, a.rows - 1 - row0) * (uint32_t)(2 * a.x_row) +
+                          (uint32_t)unit * 16;
+      const char* src = xbase + (int64_t)t * (2 * kTileK) + at;
+      if ((t + 1) * kTileK > a.k) src = k < a.k ? src : zero;
+      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src,
+                                       (__attribute__((address_space(3))) void*)(stage + block * 1024),
+                                       16, 0, 0);
+    }
+  };
+  auto load_weights = [&](int step, Weights (&b)[KS]) {
+#pragma unroll
+    for (int c = 0; c < KS; ++c)
+      b[c].load(a, tile0, min(step * kStepTiles + wk * KS + c, a.k_tiles - 1), lane);
+  };
+
+  f32x4 acc[MT][NT] = {};
+  const int steps = (a.k_tiles + kStepTiles - 1) / kStepTiles;
+  auto run = [&](int step, Weights (&b)[KS], Weights (&ahead)[KS]) {
+    __builtin_amdgcn_s_waitcnt(loads_done());
+    __syncthreads();  // the step's rows are in LDS, the last ones have been read by all
+    char* const stage = lds + (step & 1) * kStepTiles * kTileBytes;
+    if (step + 1 < steps) load_rows(step + 1, lds + (~step & 1) * kStepTiles * kTileBytes);
+    load_weights(step + 1, ahead);
+#pragma unroll
+    for (int c = 0; c < KS; ++c) {
+      if (step * kStepTiles + wk * KS + c >= a.k_tiles) break;
+      const char* const tile = stage + (wk * KS + c) * kTileBytes;
+      u32x4 x[MT][4];
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          x[i][j] = load_u32x4(tile + (16 * i + n) * 256 + ((4 * j + g) ^ n) * 16);
+      multiply<T, GROUP, ZEROS, MT, NT>(x, b[c], acc);
+    }
+  };
+  Weights b0[KS], b1[KS];
+  load_rows(0, lds);
+  load_weights(0, b0);
+  for (int step = 0; step < steps; step += 2) {
+    run(step, b0, b1);
+    if (step + 1 < steps) run(step + 1, b1, b0);
+  }
+
+  if constexpr (WK > 1) {
+    f32x4* const part = reinterpret_cast<f32x4*>(lds);  // [WK][WN][MT * NT][64]
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int v = 0; v < NT; ++v)
+        part[((wk * WN + wn) * MT * NT + i * NT + v) * 64 + lane] = acc[i][v];
+    __syncthreads();
+    for (int u = wk; u < MT * NT; u += WK) {
+      f32x4 sum = part[(wn * MT * NT + u) * 64 + lane];
+#pragma unroll
+      for (int o = 1; o < WK; ++o) sum += part[((o * WN + wn) * MT * NT + u) * 64 + lane];
+      if (tile0 + u % NT < a.n_tiles)
+        store<T>(a, row0 + 16 * (u / NT), tile0 + u % NT, lane, sum);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int v = 0; v < NT; ++v)
+        if (tile0 + v < a.n_tiles) store<T>(a, row0 + 16 * i, tile0 + v, lane, acc[i][v]);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Host side
+// ---------------------------------------------------------------------------
+
+template <typename T, int GROUP, bool ZEROS, int MT, int NT, bool VEC>
+hipError_t launch_few(Int4Args a, hipStream_t stream) {
+  const int waves = std::min(8, a.k_tiles);
+  a.row_blocks = (a.rows + 16 * MT - 1) / (16 * MT);
+  const unsigned grid = (unsigned)((int64_t)a.row_blocks * ((a.n_tiles + NT - 1) / NT));
+  hipLaunchKernelGGL((int4_linear_kernel<T, GROUP, ZEROS, MT, NT, VEC>), dim3(grid),
+                     dim3(64 * waves), (size_t)waves * MT * NT * 64 * sizeof(f32x4), stream, a);
+  return hipGetLastError();
+}
+
+template <typename T, int GROUP, bool ZEROS, int MT, int NT, int WN, int WK, int KS>
+hipError_t launch_many(Int4Args a, hipStream_t stream) {
+  constexpr size_t kLds = std::max<size_t>((size_t)2 * WK * KS * 16 * MT * 256,
+                                           WK > 1 ? (size_t)WK * WN * MT * NT * 1024 : 0);
+  auto* kernel = &int4_rows_kernel<T, GROUP, ZEROS, MT, NT, WN, WK, KS>;
+  if (kLds > 65536) {
+    const hipError_t err = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
+                                               hipFuncAttributeMaxDynamicSharedMemorySize, (int)kLds);
+    if (err != hipSuccess) return err;
+  }
+  a.row_blocks = (a.rows + 16 * MT - 1) / (16 * MT);
+  const int64_t n_blocks = (a.n_tiles + NT * WN - 1) / (NT * WN);
+  hipLaunchKernelGGL(kernel, dim3((unsigned)((n_blocks + 7) / 8 * 8 * a.row_blocks)),
+                     dim3(64 * WN * WK), kLds, stream, a);
+  return hipGetLastError();
 }
 
 template <typename T, int GROUP, bool ZEROS>
-void launch_rows(Int4Args a, bool vec, hipStream_t stream) {
-  const int waves = std::min(8, a.k_tiles);
-  auto grid = [&](int mt, int nt) {
-    a.row_blocks = (a.rows + 16 * mt - 1) / (16 * mt);
-    return (unsigned)((int64_t)a.row_blocks * ((a.n_tiles + nt - 1) / nt));
-  };
-  if (a.rows <= 16)
-    launch_vec<T, GROUP, ZEROS, 1, 1>(a, vec, grid(1, 1), waves, stream);
-  else if (a.rows <= 32)
-    launch_vec<T, GROUP, ZEROS, 2, 1>(a, vec, grid(2, 1), waves, stream);
-  else
-    launch_vec<T, GROUP, ZEROS, 4, 2>(a, vec, grid(4, 2), waves, stream);
+hipError_t launch_rows(const Int4Args& a, bool vec, hipStream_t stream) {
+  if (!vec)  // rows that no 16-byte load can take
+    return a.rows <= 16 ? launch_few<T, GROUP, ZEROS, 1, 1, false>(a, stream)
+                        : launch_few<T, GROUP, ZEROS, 2, 1, false>(a, stream);
+  if (a.rows <= 16) return launch_few<T, GROUP, ZEROS, 1, 1, true>(a, stream);
+  if (a.rows <= 32) return launch_many<T, GROUP, ZEROS, 2, 2, 2, 4, 1>(a, stream);
+  if ((int64_t)((a.rows + 63) / 64) * ((a.n_tiles + 15) / 16) >= 192)
+    return launch_many<T, GROUP, ZEROS, 4, 4, 4, 1, 2>(a, stream);
+  return launch_many<T, GROUP, ZEROS, 4, 2, 2, 4, 1>(a, stream);
 }
 
-template <typename T>
-void launch(const Int4Args& a, int group, bool vec, hipStream_t stream) {
-  if (group == 32)
-    a.zeros ? launch_rows<T, 32, true>(a, vec, stream) : launch_rows<T, 32, false>(a, vec, stream);
-  else if (group == 64)
-    a.zeros ? launch_rows<T, 64, true>(a, vec, stream) : launch_rows<T, 64, false>(a, vec, stream);
-  else
-    a.zeros ? launch_rows<T, 128, true>(a, vec, stream) : launch_rows<T, 128, false>(a, vec, stream);
+template <template <bool> class T, int GROUP>
+hipError_t launch_zeros(const Int4Args& a, bool vec, hipStream_t stream) {
+  return a.zeros ? launch_rows<T<true>, GROUP, true>(a, vec, stream)
+                 : launch_rows<T<false>, GROUP, false>(a, vec, stream);
+}
+
+template <template <bool> class T>
+hipError_t launch(const Int4Args& a, int group, bool vec, hipStream_t stream) {
+  if (group == 32) return launch_zeros<T, 32>(a, vec, stream);
+  if (group == 64) return launch_zeros<T, 64>(a, vec, stream);
+  return launch_zeros<T, 128>(a, vec, stream);
 }
 
 bool aligned(const void* p, uintptr_t bytes) { return ((uintptr_t)p & (bytes - 1)) == 0; }
@@ -291,7 +503,7 @@ extern "C" int qsa_int4_linear(const void* x, int64_t x_row_stride, const void* 
     return fail(QSA_ERR_UNSUPPORTED, std::string(name) + ": no input features");
   if (!x || !codes || !scales || !y)
     return fail(QSA_ERR_INVALID, std::string(name) + ": null tensor pointer");
-  if (!aligned(codes, 16) || !aligned(x, 2) || !aligned(scales, 2) || !aligned(bias, 2) ||
+  if (!aligned(codes, 16) || !aligned(x, 2) || !aligned(scales, 8) || !aligned(zeros, 4) || !aligned(bias, 2) ||
       !aligned(y, 2))
     return fail(QSA_ERR_INVALID, std::string(name) + ": misaligned tensor");
   if (rows > 1 && y_row_stride < out_features)
@@ -300,8 +512,8 @@ extern "C" int qsa_int4_linear(const void* x, int64_t x_row_stride, const void* 
   a.x = static_cast<const uint16_t*>(x);
   a.x_row = x_row_stride;
   a.codes = static_cast<const u32x4*>(codes);
-  a.scales = static_cast<const uint16_t*>(scales);
-  a.zeros = static_cast<const uint8_t*>(zeros);
+  a.scales = static_cast<const char*>(scales);
+  a.zeros = static_cast<const char*>(zeros);
   a.bias = static_cast<const uint16_t*>(bias);
   a.y = static_cast<uint16_t*>(y);
   a.y_row = y_row_stride;
@@ -312,9 +524,13 @@ extern "C" int qsa_int4_linear(const void* x, int64_t x_row_stride, const void* 
   a.k_tiles = (int)(((int64_t)in_features + kTileK - 1) / kTileK);
   if ((int64_t)a.n_tiles * ((rows + 15) / 16) > 0x7fffffffLL / 2)
     return fail(QSA_ERR_UNSUPPORTED, std::string(name) + ": too many output tiles");
-  const bool vec = aligned(x, 16) && x_row_stride % 8 == 0 && in_features % 8 == 0;
+  // 16-byte loads of whole rows, whose offsets within a block fit 32 bits.
+  const bool vec = aligned(x, 16) && x_row_stride % 8 == 0 && in_features % 8 == 0 &&
+                   x_row_stride < (1 << 24);
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (is_fp16) launch<Fp16>(a, group_size, vec, s);
-  else launch<Bf16>(a, group_size, vec, s);
-  return check_launch(name);
+  const hipError_t err = is_fp16 ? launch<Fp16>(a, group_size, vec, s)
+                                 : launch<Bf16>(a, group_size, vec, s);
+  if (err != hipSuccess)
+    return fail(QSA_ERR_HIP, std::string(name) + " launch: " + hipGetErrorString(err));
+  return QSA_OK;
 }

@@ -28,8 +28,8 @@ class Int4Weight:
     (the layout is the C ABI's, ``qsa_int4_linear``)."""
 
     codes: torch.Tensor            # int32 [n tiles, k tiles, 64, 4]
-    scales: torch.Tensor           # bf16 / fp16 [n tiles, groups, 16]
-    zeros: torch.Tensor | None     # uint8 [n tiles, groups, 16]
+    scales: torch.Tensor           # bf16 / fp16 [n tiles, k tiles, 16, 128 / group size]
+    zeros: torch.Tensor | None     # uint8, shaped like scales
     out_features: int
     in_features: int
     group_size: int
@@ -51,7 +51,7 @@ class Int4Weight:
         c = c.permute(0, 3, 1, 4, 2, 5).reshape(nt * _TILE_N, kt * _TILE_K).float()
 
         def spread(t):
-            t = t.permute(0, 2, 1).reshape(nt * _TILE_N, -1).float()
+            t = t.permute(0, 2, 1, 3).reshape(nt * _TILE_N, -1).float()
             return t.repeat_interleave(self.group_size, dim=1)
 
         zero = 8.0 if self.zeros is None else spread(self.zeros)
@@ -99,7 +99,7 @@ def int4_pack(codes: torch.Tensor, scales: torch.Tensor, zeros: torch.Tensor | N
     def by_tile(t):
         full = t.new_zeros(nt * _TILE_N, all_groups)
         full[:n, :groups] = t
-        return full.view(nt, _TILE_N, all_groups).permute(0, 2, 1).contiguous()
+        return full.view(nt, _TILE_N, kt, -1).permute(0, 2, 1, 3).contiguous()
 
     return Int4Weight(packed, by_tile(scales), None if zeros is None else by_tile(zeros & 15), n, k,
                       group_size)

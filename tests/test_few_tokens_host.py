@@ -20,7 +20,7 @@ def test_packed_words_hold_each_code_at_its_place():
     scales = torch.rand(n, 10, generator=gen).bfloat16()
     zeros = torch.randint(0, 16, (n, 10), generator=gen, dtype=torch.uint8)
     w = int4_pack(codes, scales, zeros, group_size=32)
-    assert tuple(w.codes.shape) == (2, 3, 64, 4) and tuple(w.scales.shape) == (2, 12, 16)
+    assert tuple(w.codes.shape) == (2, 3, 64, 4) and tuple(w.scales.shape) == (2, 3, 16, 4)
     words = w.codes.numpy().view(np.uint32)
     for out in range(32):
         for inp in range(384):
@@ -30,8 +30,8 @@ def test_packed_words_hold_each_code_at_its_place():
             assert got == (int(codes[out, inp]) if out < n and inp < k else 0), (out, inp)
     for out in range(n):
         for group in range(10):
-            assert w.scales[out // 16, group, out % 16] == scales[out, group]
-            assert w.zeros[out // 16, group, out % 16] == zeros[out, group]
+            place = (out // 16, group // 4, out % 16, group % 4)
+            assert w.scales[place] == scales[out, group] and w.zeros[place] == zeros[out, group]
     want = (codes.float() - zeros.float().repeat_interleave(32, 1)[:, :k]) * (
         scales.float().repeat_interleave(32, 1)[:, :k])
     assert torch.equal(w.dequantize(), want)
@@ -58,7 +58,7 @@ def test_quantized_weight_is_the_nearest_code(dtype, zero_points, group):
     w[3, :group] = 0
     q = int4_quantize(w, group_size=group, zero_points=zero_points)
     nt = q.scales.shape[0]
-    steps = q.scales.permute(0, 2, 1).reshape(nt * 16, -1)[:19].float()
+    steps = q.scales.permute(0, 2, 1, 3).reshape(nt * 16, -1)[:19].float()
     step = steps.repeat_interleave(group, 1)[:, :330]
     off = (q.dequantize() - w.float()).abs()
     end = torch.finfo(dtype).eps / 2 * (15 if zero_points else 7)
