@@ -498,7 +498,8 @@ int qsa_gdn_gated_norm(const void* o, const void* qkvz, int64_t qkvz_stride, con
  *          16 g + n, word j holds output n's inputs 32 j + 8 g + 0..7 of the
  *          tile, input 2 p in bits 4 p.., input 2 p + 1 in bits 16 + 4 p..;
  *   scales [n tiles][k tiles][16][128 / group_size], 8-byte aligned; zeros the
- *          same in uint8 0..15, 4-byte aligned, or null (8 everywhere).
+ *          same in uint8 0..15, 4-byte aligned, or null (8 everywhere). Codes of
+ *          inputs past in_features hold their zero point.
  * group_size 32, 64 or 128. bias may be null. A row of x that holds an infinity
  * or NaN (or, in bf16, values past 2^112) has no defined result; other rows are
  * not touched by it. Any alignment and row stride; 16-byte aligned rows and

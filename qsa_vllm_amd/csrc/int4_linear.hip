@@ -45,9 +45,23 @@ typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 
 constexpr int kTileN = 16;
 constexpr int kTileK = 128;
+constexpr int kCUs = 256;  // compute units of an MI355X
 
-// s_waitcnt for the vector-memory counter alone (gfx9 encoding), at 0.
-constexpr int loads_done() { return (7 << 4) | (15 << 8); }
+// s_waitcnt immediate (gfx9 encoding): at most n vector-memory operations in
+// flight, no LDS operation.
+constexpr int loads_left(int n) { return (n & 15) | (7 << 4) | ((n >> 4) << 14); }
+
+// Barrier after the wave's LDS reads and all but its last N loads. (A fence
+// would wait for those too.)
+template <int N>
+__device__ __forceinline__ void stage_barrier() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_sched_barrier(0);
+  __builtin_amdgcn_s_waitcnt(loads_left(N));
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_sched_barrier(0);
+  asm volatile("" ::: "memory");
+}
 
 struct Int4Args {
   const uint16_t* x;
@@ -87,6 +101,14 @@ __device__ __forceinline__ uint16_t scale_of(const u32x2& v, int q) {
   return (uint16_t)(v[q >> 1] >> (16 * (q & 1)));
 }
 
+// (w & 0x000F000F) | c in one instruction (the compiler makes two of it: a VOP3
+// instruction takes no literal, and at most one scalar).
+__device__ __forceinline__ uint32_t nibbles_or(uint32_t w, uint32_t c) {
+  uint32_t r;
+  asm("v_and_or_b32 %0, %1, %2, %3" : "=v"(r) : "v"(w), "s"(0x000F000Fu), "v"(c));
+  return r;
+}
+
 // A type's matrix operand: unpacking a word of codes with a zero point's
 // constant, and what the accumulator's start takes off again.
 template <bool ZEROS>
@@ -104,8 +126,8 @@ struct Bf16 {
     u32x4 r;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const uint32_t q = (w >> (4 * i)) & 0x000F000Fu;
-      r[i] = ZEROS ? q + zero : q | zero;
+      if constexpr (ZEROS) r[i] = ((w >> (4 * i)) & 0x000F000Fu) + zero;
+      else r[i] = nibbles_or(w >> (4 * i), zero);
     }
     return __builtin_bit_cast(frag, r);
   }
@@ -141,10 +163,10 @@ struct Fp16 {
       frag f;
     } r;
     const uint32_t v = w >> 8;
-    r.p[0] = __builtin_bit_cast(f16x2, (w & 0x000F000Fu) | 0x64006400u) + low;
+    r.p[0] = __builtin_bit_cast(f16x2, nibbles_or(w, 0x64006400u)) + low;
     r.p[1] = __builtin_elementwise_fma(
         __builtin_bit_cast(f16x2, (w & 0x00F000F0u) | 0x64006400u), sixteenth, high);
-    r.p[2] = __builtin_bit_cast(f16x2, (v & 0x000F000Fu) | 0x64006400u) + low;
+    r.p[2] = __builtin_bit_cast(f16x2, nibbles_or(v, 0x64006400u)) + low;
     r.p[3] = __builtin_elementwise_fma(
         __builtin_bit_cast(f16x2, (v & 0x00F000F0u) | 0x64006400u), sixteenth, high);
     return r.f;
@@ -158,6 +180,11 @@ struct Fp16 {
   }
 };
 
+template <typename V>
+__device__ __forceinline__ V load_at(const char* base, uint32_t offset) {
+  return *reinterpret_cast<const V*>(base + offset);
+}
+
 // A wave's weight tiles of one k tile: NT adjacent n tiles.
 template <int GROUP, bool ZEROS, int NT>
 struct Tiles {
@@ -167,15 +194,17 @@ struct Tiles {
   typename Words::scales s[NT];
   typename Words::zeros z[NT];
   // Tiles past the last (an odd end) are read as the last one; not stored.
+  // tile0 and t are the same in the whole wave: scalar addresses, and a lane's
+  // offset from them that never changes.
   __device__ __forceinline__ void load(const Int4Args& a, int tile0, int t, int lane) {
+    const uint32_t n = lane & 15;
 #pragma unroll
     for (int v = 0; v < NT; ++v) {
       const int64_t at = (int64_t)min(tile0 + v, a.n_tiles - 1) * a.k_tiles + t;
-      w[v] = a.codes[at * 64 + lane];
-      const int64_t group = at * 16 + (lane & 15);
-      s[v] = *reinterpret_cast<const typename Words::scales*>(a.scales + group * (2 * kGroups));
+      w[v] = load_at<u32x4>(reinterpret_cast<const char*>(a.codes) + at * 1024, lane * 16u);
+      s[v] = load_at<typename Words::scales>(a.scales + at * (32 * kGroups), n * (2 * kGroups));
       if constexpr (ZEROS)
-        z[v] = *reinterpret_cast<const typename Words::zeros*>(a.zeros + group * kGroups);
+        z[v] = load_at<typename Words::zeros>(a.zeros + at * (16 * kGroups), n * kGroups);
     }
   }
   __device__ __forceinline__ int zero(int v, int q) const {
@@ -237,25 +266,18 @@ __device__ __forceinline__ void store(const Int4Args& a, int m0, int tile, int l
   }
 }
 
-// Eight activations from input k on: VEC reads 16 bytes (row stride, width and
-// address multiples of 8 elements), otherwise element by element. Inputs past
-// the width and rows past the last are zero and not read.
-template <bool VEC>
-__device__ __forceinline__ u32x4 load_x(const uint16_t* row, int k, int width, bool live) {
-  if constexpr (VEC) {
-    if (live && k < width) return load_u32x4(row + k);
-    return u32x4{0, 0, 0, 0};
-  } else {
-    u32x4 r = {0, 0, 0, 0};
-    if (live) {
+// Eight activations from input k on, element by element: rows that 16-byte
+// loads cannot take. Inputs past the width are zero and not read.
+__device__ __forceinline__ u32x4 gather_x(const uint16_t* row, int k, int width) {
+  u32x4 r = {0, 0, 0, 0};
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (k + i < width) r[i / 2] |= (uint32_t)row[k + i] << (16 * (i & 1));
-    }
-    return r;
-  }
+  for (int i = 0; i < 8; ++i)
+    if (k + i < width) r[i / 2] |= (uint32_t)row[k + i] << (16 * (i & 1));
+  return r;
 }
 
+// To 16 MT rows a workgroup. VEC: row stride, width and address are multiples of
+// 8 elements.
 template <typename T, int GROUP, bool ZEROS, int MT, int NT, bool VEC>
 __global__ __launch_bounds__(512) void int4_linear_kernel(Int4Args a) {
   typedef Tiles<GROUP, ZEROS, NT> Weights;
@@ -266,20 +288,27 @@ __global__ __launch_bounds__(512) void int4_linear_kernel(Int4Args a) {
   const int tile0 = (blockIdx.x / a.row_blocks) * NT;
 
   f32x4 acc[MT][NT] = {};
-  const uint16_t* xrow[MT];
-  bool live[MT];
+  const uint16_t* const xblock = a.x + row0 * a.x_row;
+  // Rows past the last repeat it (their results are not stored), and inputs past
+  // the width the row's first ones (their codes are the zero point): no load
+  // depends on a condition, which would make it wait for the ones before it.
+  uint32_t at[MT];  // the lane's byte offset in the block
 #pragma unroll
-  for (int i = 0; i < MT; ++i) {
-    const int m = row0 + 16 * i + n;
-    live[i] = m < a.rows;
-    xrow[i] = a.x + (live[i] ? m : 0) * a.x_row;
-  }
+  for (int i = 0; i < MT; ++i)
+    at[i] = (uint32_t)min(16 * i + n, a.rows - 1 - row0) * (uint32_t)(2 * a.x_row);
   auto load_rows = [&](int t, u32x4 (&x)[MT][4]) {
 #pragma unroll
-    for (int i = 0; i < MT; ++i)
+    for (int j = 0; j < 4; ++j) {
+      const int k = t * kTileK + 32 * j + 8 * g;
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        x[i][j] = load_x<VEC>(xrow[i], t * kTileK + 32 * j + 8 * g, a.k, live[i]);
+      for (int i = 0; i < MT; ++i)
+        if constexpr (VEC)
+          x[i][j] = load_at<u32x4>(reinterpret_cast<const char*>(xblock),
+                                   at[i] + (k < a.k ? 2 * k : 0));
+        else
+          x[i][j] = gather_x(reinterpret_cast<const uint16_t*>(
+                                 reinterpret_cast<const char*>(xblock) + at[i]), k, a.k);
+    }
   };
   // Two tiles in flight: the next one's loads are issued before this one's
   // product.
@@ -319,20 +348,21 @@ __global__ __launch_bounds__(512) void int4_linear_kernel(Int4Args a) {
 }
 
 // More than 16 rows: a workgroup of WN x WK waves takes 16 MT rows and 16 NT WN
-// outputs, wave (wn, wk) NT n tiles and KS of every WK KS k tiles. A step's
-// activations (WK KS tiles of 16 MT rows x 256 bytes) go straight into LDS, one
-// step ahead in the other of two buffers; weights one step ahead in registers.
-// Unit u (16 bytes) of a row sits at place u ^ (row mod 16), so that the A
-// operand's reads (16 rows' same unit) lie in different banks.
-template <typename T, int GROUP, bool ZEROS, int MT, int NT, int WN, int WK, int KS>
-__global__ __launch_bounds__(64 * WN * WK) __attribute__((amdgpu_waves_per_eu(2, 2))) void
+// outputs, wave (wn, wk) NT n tiles and one of every WK k tiles. A step's
+// activations (WK tiles of 16 MT rows x 256 bytes) go straight into LDS, AHEAD
+// steps before they are used, in a ring of AHEAD + 1 buffers; weights as far
+// ahead in registers. Unit u (16 bytes) of a row sits at place u ^ (row mod 16),
+// so that the A operand's reads (16 rows' same unit) lie in different banks.
+template <typename T, int GROUP, bool ZEROS, int MT, int NT, int WN, int WK, int AHEAD>
+__global__ __launch_bounds__(64 * WN * WK) __attribute__((amdgpu_waves_per_eu(MT > 2 ? 2 : 4))) void
 int4_rows_kernel(Int4Args a) {
   typedef Tiles<GROUP, ZEROS, NT> Weights;
   constexpr int kWaves = WN * WK;
-  constexpr int kStepTiles = WK * KS;
   constexpr int kTileBytes = 16 * MT * 256;
-  constexpr int kBlocks = kStepTiles * 16 * MT / 4;  // 4 rows of 256 bytes an instruction
-  static_assert(kBlocks % kWaves == 0, "");
+  constexpr int kStageBytes = WK * kTileBytes;
+  constexpr int kBlocks = WK * 16 * MT / 4;  // 4 rows of 256 bytes an instruction
+  constexpr int kOps = kBlocks / kWaves + NT * (ZEROS ? 3 : 2);  // a step's loads of a wave
+  static_assert(kBlocks % kWaves == 0 && (AHEAD - 1) * kOps < 64, "");
   extern __shared__ __attribute__((aligned(16))) char lds[];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -344,62 +374,70 @@ int4_rows_kernel(Int4Args a) {
   const int row0 = ((int)(blockIdx.x >> 3) % a.row_blocks) * (16 * MT);
   const int tile0 = (slot * WN + wn) * NT;
   if (slot * WN * NT >= a.n_tiles) return;
+  const int steps = (a.k_tiles + WK - 1) / WK;
 
   const char* const zero = reinterpret_cast<const char*>(g_qsa_zero_rows);
   const char* const xbase = reinterpret_cast<const char*>(a.x + row0 * a.x_row);
-  auto load_rows = [&](int step, char* stage) {
+  // Block i of a step (4 rows of tile i / (4 MT)) is moved by wave i mod waves;
+  // the lane's byte offset in its blocks. Rows past the last repeat it (their
+  // results are not stored).
+  uint32_t at[kBlocks / kWaves];
 #pragma unroll
-    for (int i = 0; i < kBlocks / kWaves; ++i) {
-      const int block = i * kWaves + wave;  // of tile block / (4 MT)
-      const int t = step * kStepTiles + block / (4 * MT);
-      const int row = block % (4 * MT) * 4 + g;
-      const int unit = n ^ (row & 15);
-      const int k = t * kTileK + unit * 8;
-      // Rows past the last repeat it (their results are not stored); inputs past
-      // the width are zero.
-      const uint32_t at = (uint32_t)min(row, a.rows - 1 - row0) * (uint32_t)(2 * a.x_row) +
-                          (uint32_t)unit * 16;
-      const char* src = xbase + (int64_t)t * (2 * kTileK) + at;
-      if ((t + 1) * kTileK > a.k) src = k < a.k ? src : zero;
-      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src,
-                                       (__attribute__((address_space(3))) void*)(stage + block * 1024),
-                                       16, 0, 0);
+  for (int i = 0; i < kBlocks / kWaves; ++i) {
+    const int row = (i * kWaves + wave) % (4 * MT) * 4 + g;
+    at[i] = (uint32_t)min(row, a.rows - 1 - row0) * (uint32_t)(2 * a.x_row) +
+            (uint32_t)(n ^ (row & 15)) * 16;
+  }
+  // Loads past the last step repeat it: the number of loads in flight is fixed.
+  auto load_step = [&](int step, char* stage, Weights& b) {
+    const int s = min(step, steps - 1);
+    auto move = [&](int i, const char* src) {
+      __builtin_amdgcn_global_load_lds(
+          (const __attribute__((address_space(1))) void*)src,
+          (__attribute__((address_space(3))) void*)(stage + (i * kWaves + wave) * 1024), 16, 0, 0);
+    };
+    const char* const base = xbase + (int64_t)s * (2 * WK * kTileK);
+    if ((s + 1) * WK * kTileK <= a.k) {
+#pragma unroll
+      for (int i = 0; i < kBlocks / kWaves; ++i)
+        move(i, base + (i * kWaves + wave) / (4 * MT) * (2 * kTileK) + at[i]);
+    } else {  // inputs past the width are zero
+#pragma unroll
+      for (int i = 0; i < kBlocks / kWaves; ++i) {
+        const int block = i * kWaves + wave, tile = block / (4 * MT);
+        const int k = (s * WK + tile) * kTileK + (n ^ ((block % (4 * MT) * 4 + g) & 15)) * 8;
+        move(i, k < a.k ? base + tile * (2 * kTileK) + at[i] : zero);
+      }
     }
-  };
-  auto load_weights = [&](int step, Weights (&b)[KS]) {
-#pragma unroll
-    for (int c = 0; c < KS; ++c)
-      b[c].load(a, tile0, min(step * kStepTiles + wk * KS + c, a.k_tiles - 1), lane);
+    b.load(a, tile0, min(s * WK + wk, a.k_tiles - 1), lane);
   };
 
   f32x4 acc[MT][NT] = {};
-  const int steps = (a.k_tiles + kStepTiles - 1) / kStepTiles;
-  auto run = [&](int step, Weights (&b)[KS], Weights (&ahead)[KS]) {
-    __builtin_amdgcn_s_waitcnt(loads_done());
-    __syncthreads();  // the step's rows are in LDS, the last ones have been read by all
-    char* const stage = lds + (step & 1) * kStepTiles * kTileBytes;
-    if (step + 1 < steps) load_rows(step + 1, lds + (~step & 1) * kStepTiles * kTileBytes);
-    load_weights(step + 1, ahead);
+  Weights b[AHEAD + 1];
 #pragma unroll
-    for (int c = 0; c < KS; ++c) {
-      if (step * kStepTiles + wk * KS + c >= a.k_tiles) break;
-      const char* const tile = stage + (wk * KS + c) * kTileBytes;
+  for (int i = 0; i < AHEAD; ++i) load_step(i, lds + i * kStageBytes, b[i]);
+  for (int step = 0;; step += AHEAD + 1) {
+#pragma unroll
+    for (int i = 0; i <= AHEAD; ++i) {
+      if (step + i >= steps) goto done;
+      // This step's loads are done, and the buffer that the next loads go to
+      // has been read by all.
+      stage_barrier<(AHEAD - 1) * kOps>();
+      load_step(step + i + AHEAD, lds + (i + AHEAD) % (AHEAD + 1) * kStageBytes,
+                b[(i + AHEAD) % (AHEAD + 1)]);
+      if ((step + i) * WK + wk >= a.k_tiles) continue;
+      const char* const tile = lds + i * kStageBytes + wk * kTileBytes;
       u32x4 x[MT][4];
 #pragma unroll
-      for (int i = 0; i < MT; ++i)
+      for (int m = 0; m < MT; ++m)
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-          x[i][j] = load_u32x4(tile + (16 * i + n) * 256 + ((4 * j + g) ^ n) * 16);
-      multiply<T, GROUP, ZEROS, MT, NT>(x, b[c], acc);
+          x[m][j] = load_u32x4(tile + (16 * m + n) * 256 + ((4 * j + g) ^ n) * 16);
+      multiply<T, GROUP, ZEROS, MT, NT>(x, b[i], acc);
     }
-  };
-  Weights b0[KS], b1[KS];
-  load_rows(0, lds);
-  load_weights(0, b0);
-  for (int step = 0; step < steps; step += 2) {
-    run(step, b0, b1);
-    if (step + 1 < steps) run(step + 1, b1, b0);
   }
+done:
+  __builtin_amdgcn_s_waitcnt(loads_left(0));  // no load into LDS outlives the wave
 
   if constexpr (WK > 1) {
     f32x4* const part = reinterpret_cast<f32x4*>(lds);  // [WK][WN][MT * NT][64]
@@ -431,8 +469,8 @@ int4_rows_kernel(Int4Args a) {
 // ---------------------------------------------------------------------------
 
 template <typename T, int GROUP, bool ZEROS, int MT, int NT, bool VEC>
-hipError_t launch_few(Int4Args a, hipStream_t stream) {
-  const int waves = std::min(8, a.k_tiles);
+hipError_t launch_few(Int4Args a, int waves, hipStream_t stream) {
+  waves = std::min(waves, a.k_tiles);
   a.row_blocks = (a.rows + 16 * MT - 1) / (16 * MT);
   const unsigned grid = (unsigned)((int64_t)a.row_blocks * ((a.n_tiles + NT - 1) / NT));
   hipLaunchKernelGGL((int4_linear_kernel<T, GROUP, ZEROS, MT, NT, VEC>), dim3(grid),
@@ -440,11 +478,11 @@ hipError_t launch_few(Int4Args a, hipStream_t stream) {
   return hipGetLastError();
 }
 
-template <typename T, int GROUP, bool ZEROS, int MT, int NT, int WN, int WK, int KS>
+template <typename T, int GROUP, bool ZEROS, int MT, int NT, int WN, int WK, int AHEAD>
 hipError_t launch_many(Int4Args a, hipStream_t stream) {
-  constexpr size_t kLds = std::max<size_t>((size_t)2 * WK * KS * 16 * MT * 256,
+  constexpr size_t kLds = std::max<size_t>((size_t)(AHEAD + 1) * WK * 16 * MT * 256,
                                            WK > 1 ? (size_t)WK * WN * MT * NT * 1024 : 0);
-  auto* kernel = &int4_rows_kernel<T, GROUP, ZEROS, MT, NT, WN, WK, KS>;
+  auto* kernel = &int4_rows_kernel<T, GROUP, ZEROS, MT, NT, WN, WK, AHEAD>;
   if (kLds > 65536) {
     const hipError_t err = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
                                                hipFuncAttributeMaxDynamicSharedMemorySize, (int)kLds);
@@ -457,16 +495,60 @@ hipError_t launch_many(Int4Args a, hipStream_t stream) {
   return hipGetLastError();
 }
 
+// More than 16 rows: workgroups of 16 MT rows x 16 NT WN outputs. Time goes by
+// how many of them a CU gets: one costs `one`, two at a time `two` (us at 4096
+// inputs, in proportion to them otherwise; measured at 17 - 256 rows, 2048 -
+// 49536 outputs, groups of 128):
+//   rows x outputs     32 x 32   32 x 64   32 x 96   64 x 128   64 x 192
+//   one / two a CU    8.3/12.5   10.1/16  12.3/20.5  28.5/45     35/58
+// A larger block unpacks each weight for more rows and loads less, a smaller
+// one fills the card sooner: the least max(one, two ceil(blocks / CUs) / 2).
+enum RowsShape { k32x32, k32x64, k32x96, k64x128, k64x192, kRowsShapes };
+RowsShape pick_rows_shape(int rows, int n_tiles) {
+  static constexpr struct {
+    int rows, tiles;
+    float one, two;
+  } kShapes[kRowsShapes] = {
+      {32, 2, 8.3f, 12.5f}, {32, 4, 10.1f, 16.0f}, {32, 6, 12.3f, 20.5f}, {64, 8, 28.5f, 45.0f},
+      {64, 12, 35.0f, 58.0f}};
+  int best = 0;
+  float least = 0.0f;
+  for (int i = 0; i < kRowsShapes; ++i) {
+    const int64_t blocks = (int64_t)((rows - 1) / kShapes[i].rows + 1) *
+                           ((n_tiles - 1) / kShapes[i].tiles + 1);
+    const float us = std::max(kShapes[i].one,
+                              kShapes[i].two * 0.5f * (float)((blocks + kCUs - 1) / kCUs));
+    if (i == 0 || us < least) {
+      best = i;
+      least = us;
+    }
+  }
+  return (RowsShape)best;
+}
+
 template <typename T, int GROUP, bool ZEROS>
 hipError_t launch_rows(const Int4Args& a, bool vec, hipStream_t stream) {
   if (!vec)  // rows that no 16-byte load can take
-    return a.rows <= 16 ? launch_few<T, GROUP, ZEROS, 1, 1, false>(a, stream)
-                        : launch_few<T, GROUP, ZEROS, 2, 1, false>(a, stream);
-  if (a.rows <= 16) return launch_few<T, GROUP, ZEROS, 1, 1, true>(a, stream);
-  if (a.rows <= 32) return launch_many<T, GROUP, ZEROS, 2, 2, 2, 4, 1>(a, stream);
-  if ((int64_t)((a.rows + 63) / 64) * ((a.n_tiles + 15) / 16) >= 192)
-    return launch_many<T, GROUP, ZEROS, 4, 4, 4, 1, 2>(a, stream);
-  return launch_many<T, GROUP, ZEROS, 4, 2, 2, 4, 1>(a, stream);
+    return a.rows <= 16 ? launch_few<T, GROUP, ZEROS, 1, 1, false>(a, 8, stream)
+                        : launch_few<T, GROUP, ZEROS, 2, 1, false>(a, 8, stream);
+  // To 16 rows: more outputs a wave (and fewer waves) share the activations'
+  // loads and the closing sum, once there are enough of them for every CU
+  // (K = 4096, us for 1 / 2 / 4 n tiles a wave. 1 row: 11264 outputs 7.1 / 8.0 /
+  // 8.4, 22528 11.8 / 10.8 / 12.0, 49536 28.4 / 21.9 / 22.5; 16 rows: 2048
+  // 6.7 / 7.0 / 8.3, 8832 14.5 / 11.2 / 9.2, 49536 52 / 35 / 28).
+  if (a.rows <= 4)
+    return a.n_tiles < 1024 ? launch_few<T, GROUP, ZEROS, 1, 1, true>(a, 8, stream)
+                            : launch_few<T, GROUP, ZEROS, 1, 2, true>(a, 4, stream);
+  if (a.rows <= 16)
+    return a.n_tiles < 384 ? launch_few<T, GROUP, ZEROS, 1, 1, true>(a, 8, stream)
+                           : launch_few<T, GROUP, ZEROS, 1, 4, true>(a, 4, stream);
+  switch (pick_rows_shape(a.rows, a.n_tiles)) {
+    case k32x32: return launch_many<T, GROUP, ZEROS, 2, 1, 2, 4, 1>(a, stream);
+    case k32x64: return launch_many<T, GROUP, ZEROS, 2, 2, 2, 4, 1>(a, stream);
+    case k32x96: return launch_many<T, GROUP, ZEROS, 2, 3, 2, 4, 1>(a, stream);
+    case k64x128: return launch_many<T, GROUP, ZEROS, 4, 2, 4, 1, 1>(a, stream);
+    default: return launch_many<T, GROUP, ZEROS, 4, 3, 4, 1, 1>(a, stream);
+  }
 }
 
 template <template <bool> class T, int GROUP>

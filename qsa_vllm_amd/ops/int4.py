@@ -87,8 +87,12 @@ def int4_pack(codes: torch.Tensor, scales: torch.Tensor, zeros: torch.Tensor | N
     for t in range(0, nt, step):
         part = codes[t * _TILE_N:(t + step) * _TILE_N]
         tiles = min(step, nt - t)
-        full = codes.new_zeros(tiles * _TILE_N, kt * _TILE_K)
+        full = codes.new_full((tiles * _TILE_N, kt * _TILE_K), 8 if zeros is None else 0)
         full[:part.shape[0], :k] = part
+        if zeros is not None and k < groups * group_size:
+            # a short last group is filled up with its zero point
+            last = zeros[t * _TILE_N:(t + step) * _TILE_N, -1:]
+            full[:part.shape[0], k:groups * group_size] = last
         # [tile, n, k tile, j, g, i] -> words [tile, k tile, g, n, j]
         c = full.view(tiles, _TILE_N, kt, 4, 4, 8).permute(0, 2, 4, 1, 3, 5).to(torch.int32) & 15
         word = c[..., 0].clone()
