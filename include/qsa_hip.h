@@ -552,7 +552,8 @@ int qsa_tree_attention(const void* q, int64_t q_row_stride, int64_t q_head_strid
  *   y = -inf where bit v % 32 of word v / 32 of allowed [rows, words] is 0.
  * Ids outside the shard (negative ones pad) are passed over. Null pointers leave
  * a rule out. ancestors [rows, ancestor_words] as in qsa_tree_attention, over
- * draft_tokens [rows] and query_start_loc. logits_type: 0 fp32, 1 bf16, 2 fp16. */
+ * draft_tokens [rows] and query_start_loc. At most 1024 biases and 1024 nodes (32
+ * ancestor words) a request. logits_type: 0 fp32, 1 bf16, 2 fp16. */
 int qsa_process_logits(const void* logits, int logits_type, int64_t logits_row_stride, float* out,
                        int64_t out_row_stride, int rows, int vocab, int64_t vocab_start,
                        const int32_t* token_to_req, int num_requests, const int32_t* history,

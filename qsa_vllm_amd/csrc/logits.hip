@@ -12,12 +12,21 @@
 // a drafted node, its visible ancestors' tokens (itself among them).
 //
 // The pass is bound by memory: a logit read (2 or 4 bytes), its result written
-// (4), a grammar bit. What a token's penalties need is kept in LDS for a chunk
-// of the vocabulary: a workgroup counts its request's history within its chunk
-// with LDS atomics (whole numbers: any order gives the same counts), sums the
-// biases in list order, then streams the chunk of its rows. The rows of a
-// request that share a workgroup (a drafted tree's) share the table: a node's
-// ancestors are added to it before its row and taken off after.
+// (4), a grammar bit. A workgroup takes a chunk of the vocabulary for one row, or
+// for several rows of one request (a drafted tree's):
+//
+//   1. it counts the request's history within the chunk in LDS, with LDS atomics
+//      (whole numbers: any order gives the same counts);
+//   2. it lists the chunk's special columns, those of biases and of drafted
+//      tokens, whose values differ by row or need a sum, and marks them in the
+//      table;
+//   3. it streams its rows, four vectors of a thread in flight, each logit by its
+//      count alone, and leaves the special columns;
+//   4. it computes those, one (row, column) a thread: the visible nodes' tokens
+//      on top of the count, the biases in list order.
+//
+// A history is scanned once per chunk, so chunks are as large as LDS allows for
+// two workgroups a CU, unless there would be too few workgroups.
 #include "qsa_common.h"
 #include "../../include/qsa_hip.h"
 
@@ -28,12 +37,16 @@ namespace qsa {
 namespace {
 
 constexpr int kThreads = 512;
-constexpr int kChunk = 8192;            // vocabulary entries of a workgroup
-constexpr int kTreeRows = 8;            // rows of a workgroup with drafted trees
-constexpr uint32_t kPrompt = 1u << 31;  // count table: in the prompt
-constexpr uint32_t kNoBias = 0xFFFFFFFFu;
-constexpr uint32_t kTwice = 1u << 30;   // bias table, while it is built: an id listed twice
-constexpr int kMaxBiases = 64 * kThreads;
+constexpr int kCUs = 256;
+constexpr int kMinChunk = 2048;   // vocabulary entries of a workgroup, at least; at most
+constexpr int kMaxChunk = 25344;  // what fits 64 KiB of LDS (two workgroups a CU) with 16-bit
+constexpr int kMaxChunkWide = 13440;  // counts, and with 32-bit ones
+constexpr int kRounds = 2;            // workgroups wanted for each CU
+constexpr int kMaxNarrow = 65535;     // history tokens that 16 bits count
+constexpr int kTreeRows = 8;          // rows of a workgroup with drafted trees
+constexpr int kMaxNodes = 1024;       // a request's nodes and biases: what the list holds
+constexpr int kMaxBiases = 1024;
+constexpr int kBatch = 4;             // vectors of a thread in flight
 constexpr float kNegInf = -__builtin_huge_valf();
 
 enum LogitType { kFp32 = 0, kBf16 = 1, kFp16 = 2 };
@@ -66,7 +79,7 @@ struct LogitsArgs {
   int64_t ancestor_row;
   int words;
   const int32_t* query_start_loc;
-  int chunks, group_rows;
+  int chunks, chunk, group_rows;
 };
 
 template <int TYPE>
@@ -77,167 +90,318 @@ __device__ __forceinline__ float load_logit(const void* p, int64_t i) {
   else return (float)static_cast<const _Float16*>(p)[i];
 }
 
+// 16 bytes of logits (4 or 8) as they lie in memory, 4-byte aligned; and one of them.
 template <int TYPE>
-__device__ __forceinline__ f32x4 load_logit4(const void* p, int64_t i) {
+constexpr int kVec = TYPE == kFp32 ? 4 : 8;
+__device__ __forceinline__ u32x4 load_16(const void* p) {
+  u32x4 v;
+  __builtin_memcpy(&v, __builtin_assume_aligned(p, 4), 16);
+  return v;
+}
+template <int TYPE>
+__device__ __forceinline__ float logit_of(const u32x4& v, int e) {
   if constexpr (TYPE == kFp32) {
-    return *reinterpret_cast<const f32x4*>(static_cast<const float*>(p) + i);
-  } else if constexpr (TYPE == kBf16) {
-    const u32x2 v = load_u32x2(static_cast<const uint16_t*>(p) + i);
-    return f32x4{bf16_lo(v[0]), bf16_hi(v[0]), bf16_lo(v[1]), bf16_hi(v[1])};
+    return __builtin_bit_cast(float, (uint32_t)v[e]);
   } else {
-    typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
-    const f16x4 v = *reinterpret_cast<const f16x4*>(static_cast<const _Float16*>(p) + i);
-    return f32x4{(float)v[0], (float)v[1], (float)v[2], (float)v[3]};
+    const uint32_t pair = v[e >> 1];
+    if constexpr (TYPE == kBf16) return e & 1 ? bf16_hi(pair) : bf16_lo(pair);
+    return (float)__builtin_bit_cast(_Float16, (uint16_t)(pair >> (16 * (e & 1))));
   }
 }
 
 struct RowRules {
   float repetition, frequency, presence;
-  bool count, bias;
 };
 
-__device__ __forceinline__ float apply(float x, uint32_t c, uint32_t b, const RowRules& r) {
-  if (r.count && c) {
-    const uint32_t spoken = c & ~kPrompt;
-    x = x > 0.0f ? x / r.repetition : x * r.repetition;
-    if (spoken) x = x - r.frequency * (float)spoken - r.presence;
-  }
-  if (r.bias && b != kNoBias) x += __builtin_bit_cast(float, b);
+// A logit of a token said `spoken` times (and seen: in the prompt or spoken).
+__device__ __forceinline__ float penalised(float x, bool seen, uint32_t spoken, const RowRules& r) {
+  if (seen) x = x > 0.0f ? x / r.repetition : x * r.repetition;
+  if (spoken) x = x - r.frequency * (float)spoken - r.presence;
   return x;
 }
 
-template <int TYPE, bool VEC>
-__global__ __launch_bounds__(kThreads) void logits_kernel(LogitsArgs a) {
-  extern __shared__ uint32_t table[];  // [kChunk] counts, [kChunk] biases (whichever are used)
-  const bool penalise = a.repetition || a.frequency || a.presence;
-  const bool biased = a.biases > 0;
-  uint32_t* const counts = table;
-  uint32_t* const bias = table + (penalise ? kChunk : 0);
-  const int base = (blockIdx.x % a.chunks) * kChunk;
-  const int size = min(kChunk, a.vocab - base);
-  const int64_t first = a.vocab_start + base;  // the chunk's first token id
-  const int row_begin = (blockIdx.x / a.chunks) * a.group_rows;
-  const int row_end = min(a.rows, row_begin + a.group_rows);
+// Special columns of a chunk: entry e < nodes is drafted node `source`'s token,
+// the others are biases, in list order.
+struct Specials {
+  uint16_t column[kMaxNodes + kMaxBiases];
+  uint16_t source[kMaxNodes + kMaxBiases];
+  int wave[kThreads / 64];
+};
 
-  int held = -1;  // the request whose tokens and biases the tables hold
-  for (int row = row_begin; row < row_end; ++row) {
+// Appends the threads' entries in thread order; returns the list's new length.
+__device__ __forceinline__ int append(Specials& list, int length, uint32_t column, uint32_t size,
+                                      int source) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const bool take = column < size;
+  const uint64_t mask = __ballot(take);
+  if (lane == 0) list.wave[wave] = __popcll(mask);
+  __syncthreads();
+  int at = length;
+#pragma unroll
+  for (int w = 0; w < kThreads / 64; ++w) {
+    const int n = list.wave[w];
+    at += w < wave ? n : 0;
+    length += n;
+  }
+  if (take) {
+    at += __popcll(mask & ((1ull << lane) - 1));
+    list.column[at] = (uint16_t)column;
+    list.source[at] = (uint16_t)source;
+  }
+  __syncthreads();
+  return length;
+}
+
+// The chunk's table in LDS: how often each token was said (WIDE: 32 bits, else
+// 16), which were in the prompt, and which columns are special.
+template <bool WIDE>
+struct Table {
+  uint32_t *counts, *prompt, *special;
+  static __host__ __device__ __forceinline__ int words(int chunk) {
+    return (WIDE ? chunk : chunk / 2) + 2 * (chunk / 32);
+  }
+  __device__ __forceinline__ Table(uint32_t* lds, int chunk)
+      : counts(lds), prompt(lds + (WIDE ? chunk : chunk / 2)), special(prompt + chunk / 32) {}
+  __device__ __forceinline__ void say(uint32_t at) {
+    if constexpr (WIDE) atomicAdd(&counts[at], 1u);
+    else atomicAdd(&counts[at >> 1], at & 1 ? 0x10000u : 1u);
+  }
+  __device__ __forceinline__ void see(uint32_t at) { atomicOr(&prompt[at >> 5], 1u << (at & 31)); }
+  __device__ __forceinline__ void mark(uint32_t at) { atomicOr(&special[at >> 5], 1u << (at & 31)); }
+  __device__ __forceinline__ uint32_t said(int at) const {
+    return WIDE ? counts[at] : (counts[at >> 1] >> (16 * (at & 1))) & 0xFFFFu;
+  }
+  __device__ __forceinline__ u32x4 said4(int at) const {  // at a multiple of 4
+    if constexpr (WIDE) {
+      return *reinterpret_cast<const u32x4*>(counts + at);
+    } else {
+      const u32x2 c = *reinterpret_cast<const u32x2*>(counts + at / 2);
+      return u32x4{c[0] & 0xFFFFu, c[0] >> 16, c[1] & 0xFFFFu, c[1] >> 16};
+    }
+  }
+};
+
+template <int TYPE, bool VEC, bool WIDE>
+__global__ __launch_bounds__(kThreads) void logits_kernel(LogitsArgs a) {
+  extern __shared__ __attribute__((aligned(16))) uint32_t lds[];
+  __shared__ Specials list;
+  Table<WIDE> table(lds, a.chunk);
+  const bool penalise = a.repetition || a.frequency || a.presence;
+  const bool ruled = penalise || a.biases > 0;
+  const int base = (blockIdx.x % a.chunks) * a.chunk;
+  const int size = min(a.chunk, a.vocab - base);
+  // The chunk's first token id. Ids lie below 2^31 (checked on the host), so that
+  // a negative one's distance from it, taken without sign, is past any chunk.
+  const uint32_t first = (uint32_t)a.vocab_start + (uint32_t)base;
+  int row = (int)(blockIdx.x / a.chunks) * a.group_rows;
+  const int row_end = min(a.rows, row + a.group_rows);
+
+  // The rows of one request at a time.
+  while (row < row_end) {
     const int req = a.token_to_req ? load_uniform(a.token_to_req + row) : row;
-    const bool live = req >= 0 && req < a.requests;  // a padding row: no penalties, no biases
-    if (live && req != held && (penalise || biased)) {
-      __syncthreads();
-      for (int i = threadIdx.x; i < kChunk; i += kThreads) {
-        if (penalise) counts[i] = 0;
-        if (biased) bias[i] = kNoBias;
+    int rows = 1;
+    if (a.token_to_req)
+      while (row + rows < row_end && load_uniform(a.token_to_req + row + rows) == req) ++rows;
+    // A thread's next vectors of the rows, and their grammar bits. The first are
+    // asked for before the table is built.
+    constexpr int V = kVec<TYPE>;
+    const int vec_end = VEC ? size / V * V : 0;
+    const int per_row = vec_end / V, items = rows * per_row;
+    const uint32_t* const allowed = reinterpret_cast<const uint32_t*>(a.allowed) + base / 32;
+    auto bits_at = [&](int m, int i) -> uint32_t {
+      return a.allowed ? allowed[m * a.allowed_row + i / 32] >> (i & 31) : ~0u;
+    };
+    u32x4 x[kBatch];
+    uint32_t bits[kBatch];
+    int m[kBatch], i[kBatch];
+    auto fetch = [&](int k) {
+#pragma unroll
+      for (int b = 0; b < kBatch; ++b) {
+        const int item = min(k + b * kThreads, items - 1);
+        m[b] = row + (rows > 1 ? item / per_row : 0);
+        i[b] = V * (item - (m[b] - row) * per_row);
+        x[b] = load_16(static_cast<const char*>(a.logits) +
+                       (m[b] * a.in_row + base + i[b]) * (TYPE == kFp32 ? 4 : 2));
+        bits[b] = bits_at(m[b], i[b]);
       }
+    };
+    if (items > 0) fetch(threadIdx.x);
+
+    const bool live = ruled && req >= 0 && req < a.requests;  // else the grammar mask alone
+    int specials = 0, nodes = 0;
+    if (live) {
+      // The first drafted tokens and biases: asked for before the rest.
+      int node0 = 0, all_nodes = 0;
+      if (penalise && a.ancestors) {
+        node0 = max(load_uniform(a.query_start_loc + req), 0);
+        const int end = min(load_uniform(a.query_start_loc + req + 1), a.rows);
+        all_nodes = min(end - node0, 32 * a.words);
+      }
+      auto draft = [&](int j) {
+        return j < all_nodes ? (uint32_t)a.draft_tokens[node0 + j] - first : ~0u;
+      };
+      auto bias_id = [&](int j) {
+        return j < a.biases ? (uint32_t)a.bias_ids[req * a.bias_id_row + j] - first : ~0u;
+      };
+      const uint32_t draft0 = draft(threadIdx.x);
+      const uint32_t id0 = bias_id(threadIdx.x);
+
+      __syncthreads();  // the last request's table has been read
+      for (int w = threadIdx.x; w < (Table<WIDE>::words(a.chunk) + 3) / 4; w += kThreads)
+        reinterpret_cast<u32x4*>(lds)[w] = u32x4{0, 0, 0, 0};
       __syncthreads();
       if (penalise && a.history) {
         const int len = min(max(load_uniform(a.history_lens + req), 0), a.history_width);
         const int prompt = a.prompt_lens ? load_uniform(a.prompt_lens + req) : 0;
         const int32_t* const h = a.history + req * a.history_row;
-        for (int i = threadIdx.x; i < len; i += kThreads) {
-          const int64_t at = h[i] - first;
-          if (at >= 0 && at < size) {
-            if (i < prompt) atomicOr(&counts[at], kPrompt);
-            else atomicAdd(&counts[at], 1u);
+        // Prompt tokens set a bit, the later ones add up.
+        auto see = [&](int token) {
+          const uint32_t at = (uint32_t)token - first;
+          if (at < (uint32_t)size) table.see(at);
+        };
+        auto say = [&](int token) {
+          const uint32_t at = (uint32_t)token - first;
+          if (at < (uint32_t)size) table.say(at);
+        };
+        int done = 0;
+        if (((uintptr_t)h & 15u) == 0) {
+          done = len & ~3;
+          for (int i = 4 * threadIdx.x; i < done; i += 4 * kBatch * kThreads) {
+            i32x4 t[kBatch];
+#pragma unroll
+            for (int b = 0; b < kBatch; ++b)
+              t[b] = *reinterpret_cast<const i32x4*>(h + min(i + 4 * b * kThreads, done - 4));
+#pragma unroll
+            for (int b = 0; b < kBatch; ++b) {
+              const int j = i + 4 * b * kThreads;
+              if (j >= done) break;
+              if (j >= prompt) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) say(t[b][e]);
+              } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  if (j + e < prompt) see(t[b][e]);
+                  else say(t[b][e]);
+                }
+              }
+            }
+          }
+        }
+        for (int i = done + threadIdx.x; i < len; i += kThreads) {
+          if (i < prompt) see(h[i]);
+          else say(h[i]);
+        }
+      }
+      for (int j = 0; j < all_nodes; j += kThreads)
+        specials = append(list, specials, j ? draft(j + threadIdx.x) : draft0, size, j + threadIdx.x);
+      nodes = specials;
+      for (int j = 0; j < a.biases; j += kThreads)
+        specials = append(list, specials, j ? bias_id(j + threadIdx.x) : id0, size, j + threadIdx.x);
+      for (int e = threadIdx.x; e < specials; e += kThreads) table.mark(list.column[e]);
+      __syncthreads();
+    }
+
+    RowRules r = {1.0f, 0.0f, 0.0f};
+    if (live && a.repetition) r.repetition = load_uniform(a.repetition + req);
+    if (live && a.frequency) r.frequency = load_uniform(a.frequency + req);
+    if (live && a.presence) r.presence = load_uniform(a.presence + req);
+    // The ordinary columns.
+    if constexpr (VEC) {
+      for (int k = threadIdx.x; k < items; k += kBatch * kThreads) {
+        if (k >= kBatch * kThreads) fetch(k);
+#pragma unroll
+        for (int b = 0; b < kBatch; ++b) {
+          if (k + b * kThreads >= items) break;
+          float* const out = a.out + m[b] * a.out_row + base + i[b];
+#pragma unroll
+          for (int h = 0; h < V; h += 4) {
+            f32x4 y;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) y[e] = logit_of<TYPE>(x[b], h + e);
+            const int at = i[b] + h;
+            uint32_t skip = 0;
+            if (live) {
+              const u32x4 c = table.said4(at);
+              const uint32_t seen = table.prompt[at / 32] >> (at & 31) & 15u;
+              skip = table.special[at / 32] >> (at & 31) & 15u;
+              if (c[0] | c[1] | c[2] | c[3] | seen) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) y[e] = penalised(y[e], c[e] || seen >> e & 1u, c[e], r);
+              }
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (!((bits[b] >> (h + e)) & 1u)) y[e] = kNegInf;
+            if (skip) {
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                if (!(skip >> e & 1u)) out[h + e] = y[e];
+            } else {
+              *reinterpret_cast<f32x4*>(out + h) = y;
+            }
           }
         }
       }
-      if (biased) {
-        const int32_t* const ids = a.bias_ids + req * a.bias_id_row;
-        const float* const values = a.bias_values + req * a.bias_value_row;
-        auto slot = [&](int i) -> int64_t { return ids[i] - first; };
-        // The first entry of an id owns its slot and adds up the later ones.
-        // Bit k of `owned`: the thread's k-th entry does.
-        uint64_t owned = 0;
-        for (int i = threadIdx.x; i < a.biases; i += kThreads) {
-          const int64_t at = slot(i);
-          if (at >= 0 && at < size) atomicMin(&bias[at], (uint32_t)i);
-        }
-        __syncthreads();
-        for (int i = threadIdx.x; i < a.biases; i += kThreads) {
-          const int64_t at = slot(i);
-          if (at < 0 || at >= size) continue;
-          if ((bias[at] & ~kTwice) == (uint32_t)i) owned |= 1ull << (i / kThreads);
-          else atomicOr(&bias[at], kTwice);
-        }
-        __syncthreads();
-        for (int i = threadIdx.x; i < a.biases; i += kThreads) {
-          if (!((owned >> (i / kThreads)) & 1)) continue;
-          const int64_t at = slot(i);
-          float sum = values[i];
-          if (bias[at] & kTwice)
-            for (int j = i + 1; j < a.biases; ++j)
-              if (slot(j) == at) sum += values[j];
-          if (sum != sum) sum = __builtin_nanf("");  // no NaN with the bits of kNoBias
-          bias[at] = __builtin_bit_cast(uint32_t, sum);
-        }
-      }
-      __syncthreads();
-      held = req;
     }
+    for (int m = row; m < row + rows; ++m)
+      for (int i = vec_end + threadIdx.x; i < size; i += kThreads) {
+        float y = load_logit<TYPE>(a.logits, m * a.in_row + base + i);
+        if (live) {
+          if (table.special[i / 32] >> (i & 31) & 1u) continue;
+          const uint32_t c = table.said(i);
+          y = penalised(y, c || table.prompt[i / 32] >> (i & 31) & 1u, c, r);
+        }
+        if (!(bits_at(m, i) & 1u)) y = kNegInf;
+        a.out[m * a.out_row + base + i] = y;
+      }
 
-    // A drafted node's own path: its visible ancestors' tokens.
-    int node0 = 0, nodes = 0;
-    if (live && penalise && a.ancestors) {
-      node0 = max(load_uniform(a.query_start_loc + req), 0);
-      nodes = min(min(load_uniform(a.query_start_loc + req + 1), a.rows) - node0, 32 * a.words);
-    }
-    auto path = [&](uint32_t step) {
-      for (int j = threadIdx.x; j < nodes; j += kThreads) {
-        const uint32_t word = (uint32_t)a.ancestors[row * a.ancestor_row + (j >> 5)];
-        const int64_t at = a.draft_tokens[node0 + j] - first;
-        if ((word >> (j & 31)) & 1u && at >= 0 && at < size) atomicAdd(&counts[at], step);
-      }
-    };
-    if (nodes > 0) {
-      path(1u);
-      __syncthreads();
-    }
-
-    RowRules r;
-    r.count = live && penalise;
-    r.bias = live && biased;
-    r.repetition = live && a.repetition ? load_uniform(a.repetition + req) : 1.0f;
-    r.frequency = live && a.frequency ? load_uniform(a.frequency + req) : 0.0f;
-    r.presence = live && a.presence ? load_uniform(a.presence + req) : 0.0f;
-    const uint32_t* const allowed =
-        a.allowed ? reinterpret_cast<const uint32_t*>(a.allowed) + row * a.allowed_row + base / 32
-                  : nullptr;
-    const int64_t in = row * a.in_row + base;
-    float* const out = a.out + row * a.out_row + base;
-    const int vec_end = VEC ? size & ~3 : 0;
-    if constexpr (VEC) {
-      for (int i = 4 * threadIdx.x; i < vec_end; i += 4 * kThreads) {
-        f32x4 y = load_logit4<TYPE>(a.logits, in + i);
-        const uint32_t bits = allowed ? allowed[i / 32] >> (i & 31) : 15u;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          y[e] = apply(y[e], r.count ? counts[i + e] : 0, r.bias ? bias[i + e] : kNoBias, r);
-          if (!((bits >> e) & 1u)) y[e] = kNegInf;
+    // The special ones: entry e stands for its column if no earlier entry does.
+    for (int k = threadIdx.x; k < rows * specials; k += kThreads) {
+      const int m = row + k / specials, e = k % specials;
+      const int column = list.column[e];
+      const float x = load_logit<TYPE>(a.logits, m * a.in_row + base + column);
+      const uint32_t bits = bits_at(m, column);
+      uint32_t spoken = table.said(column);
+      float bias = 0.0f;
+      bool mine = true, biased = false;
+      for (int j = 0; j < specials && mine; ++j) {
+        if (list.column[j] != column) continue;
+        const int source = list.source[j];
+        if (j < e) {
+          mine = false;
+        } else if (j < nodes) {
+          const uint32_t word = (uint32_t)a.ancestors[m * a.ancestor_row + (source >> 5)];
+          spoken += (word >> (source & 31)) & 1u;
+        } else {
+          const float value = a.bias_values[req * a.bias_value_row + source];
+          bias = biased ? bias + value : value;
+          biased = true;
         }
-        *reinterpret_cast<f32x4*>(out + i) = y;
       }
+      if (!mine) continue;
+      float y = penalised(x, spoken || table.prompt[column / 32] >> (column & 31) & 1u, spoken, r);
+      if (biased) y += bias;
+      a.out[m * a.out_row + base + column] = bits & 1u ? y : kNegInf;
     }
-    for (int i = vec_end + threadIdx.x; i < size; i += kThreads) {
-      float y = apply(load_logit<TYPE>(a.logits, in + i), r.count ? counts[i] : 0,
-                      r.bias ? bias[i] : kNoBias, r);
-      if (allowed && !((allowed[i / 32] >> (i & 31)) & 1u)) y = kNegInf;
-      out[i] = y;
-    }
-    if (nodes > 0) {
-      __syncthreads();
-      path(~0u);  // - 1
-      __syncthreads();
-    }
+    row += rows;
   }
 }
 
-template <int TYPE>
-void launch(const LogitsArgs& a, bool vec, unsigned grid, size_t lds, hipStream_t stream) {
+template <int TYPE, bool WIDE>
+void launch_table(const LogitsArgs& a, bool vec, unsigned grid, size_t lds, hipStream_t stream) {
   if (vec)
-    hipLaunchKernelGGL((logits_kernel<TYPE, true>), dim3(grid), dim3(kThreads), lds, stream, a);
+    hipLaunchKernelGGL((logits_kernel<TYPE, true, WIDE>), dim3(grid), dim3(kThreads), lds, stream, a);
   else
-    hipLaunchKernelGGL((logits_kernel<TYPE, false>), dim3(grid), dim3(kThreads), lds, stream, a);
+    hipLaunchKernelGGL((logits_kernel<TYPE, false, WIDE>), dim3(grid), dim3(kThreads), lds, stream, a);
+}
+
+template <int TYPE>
+void launch(const LogitsArgs& a, bool vec, bool wide, unsigned grid, bool ruled, hipStream_t stream) {
+  const size_t words = wide ? Table<true>::words(a.chunk) : Table<false>::words(a.chunk);
+  const size_t lds = ruled ? (words + 3) / 4 * 16 : 0;
+  if (wide) launch_table<TYPE, true>(a, vec, grid, lds, stream);
+  else launch_table<TYPE, false>(a, vec, grid, lds, stream);
 }
 
 }  // namespace
@@ -261,6 +425,8 @@ extern "C" int qsa_process_logits(
     return fail(QSA_ERR_INVALID, name + ": negative size");
   if (logits_type != kFp32 && logits_type != kBf16 && logits_type != kFp16)
     return fail(QSA_ERR_UNSUPPORTED, name + ": logits must be fp32, bf16 or fp16");
+  if (vocab_start > INT_MAX - vocab)
+    return fail(QSA_ERR_INVALID, name + ": token ids must lie below 2^31");
   if (rows == 0 || vocab == 0) return QSA_OK;
   if (!logits || !out) return fail(QSA_ERR_INVALID, name + ": null tensor pointer");
   if (history && !history_lens)
@@ -270,6 +436,10 @@ extern "C" int qsa_process_logits(
   if (num_biases > kMaxBiases)
     return fail(QSA_ERR_UNSUPPORTED,
                 name + ": at most " + std::to_string(kMaxBiases) + " biases a request");
+  if (ancestors && ancestor_words > kMaxNodes / 32)
+    return fail(QSA_ERR_UNSUPPORTED, name + ": at most " + std::to_string(kMaxNodes) +
+                                         " nodes a request (" + std::to_string(kMaxNodes / 32) +
+                                         " ancestor words)");
   if (ancestors && (!draft_tokens || !query_start_loc))
     return fail(QSA_ERR_INVALID, name + ": ancestors need draft tokens and query_start_loc");
   const size_t item = logits_type == kFp32 ? 4 : 2;
@@ -305,17 +475,22 @@ extern "C" int qsa_process_logits(
   a.ancestor_row = ancestor_row_stride;
   a.words = ancestor_words;
   a.query_start_loc = query_start_loc;
-  a.chunks = (vocab - 1) / kChunk + 1;
   a.group_rows = ancestors ? kTreeRows : 1;
-  const int64_t grid = (int64_t)a.chunks * ((rows - 1) / a.group_rows + 1);
+  const bool ruled = repetition || frequency || presence || num_biases > 0;
+  const bool wide = history_width > kMaxNarrow;
+  const int64_t groups = (rows - 1) / a.group_rows + 1;
+  const int64_t most = (vocab - 1) / kMinChunk + 1;
+  const int64_t least = (vocab - 1) / (wide ? kMaxChunkWide : kMaxChunk) + 1;
+  const int64_t chunks = std::max(least, std::min(most, kRounds * kCUs / groups));
+  a.chunk = (int)(((vocab + chunks - 1) / chunks + 31) / 32 * 32);  // whole mask words
+  a.chunks = (vocab - 1) / a.chunk + 1;
+  const int64_t grid = (int64_t)a.chunks * groups;
   if (grid > INT_MAX) return fail(QSA_ERR_UNSUPPORTED, name + ": too many rows");
-  const bool vec = ((uintptr_t)logits % (4 * item)) == 0 && logits_row_stride % 4 == 0 &&
+  const bool vec = ((uintptr_t)logits & 3u) == 0 && logits_row_stride * item % 4 == 0 &&
                    ((uintptr_t)out & 15u) == 0 && out_row_stride % 4 == 0;
-  const bool penalise = repetition || frequency || presence;
-  const size_t lds = ((penalise ? 1 : 0) + (num_biases > 0 ? 1 : 0)) * kChunk * sizeof(uint32_t);
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (logits_type == kFp32) launch<kFp32>(a, vec, (unsigned)grid, lds, s);
-  else if (logits_type == kBf16) launch<kBf16>(a, vec, (unsigned)grid, lds, s);
-  else launch<kFp16>(a, vec, (unsigned)grid, lds, s);
+  if (logits_type == kFp32) launch<kFp32>(a, vec, wide, (unsigned)grid, ruled, s);
+  else if (logits_type == kBf16) launch<kBf16>(a, vec, wide, (unsigned)grid, ruled, s);
+  else launch<kFp16>(a, vec, wide, (unsigned)grid, ruled, s);
   return check_launch(name.c_str());
 }

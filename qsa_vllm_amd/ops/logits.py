@@ -70,7 +70,9 @@ def process_logits(
       outside the shard, such as -1, are passed over; an id listed twice gets both,
       in list order).
     * ``allowed`` int32 ``[rows, ceil(vocab / 32)]``: columns whose bit ``v % 32`` of
-      word ``v // 32`` is 0 become -inf, whatever they held."""
+      word ``v // 32`` is 0 become -inf, whatever they held.
+
+    At most 1024 biases and 1024 nodes (32 ancestor words) a request."""
     if out is None:
         out = torch.empty(logits.shape, dtype=torch.float32, device=logits.device)
     per_request = (history_lens, history, prompt_lens, repetition, frequency, presence, bias_ids)

@@ -140,9 +140,9 @@ def test_listed_twice_adds_in_order():
     got = _run(torch.zeros(1, 10), dict(bias_ids=ids, bias_values=values))
     # in fp32 and list order: (1e8 + 1) - 1e8 = 0
     assert got[0].tolist() == [0, 0, 0, 0, -math.inf, 0.0, 0, 0.75, 0, 0]
-    many = torch.randint(0, 40, (2, 1500), dtype=torch.int32,
+    many = torch.randint(0, 40, (2, 1024), dtype=torch.int32,
                          generator=torch.Generator().manual_seed(3))
-    vals = torch.randint(-8, 9, (2, 1500), generator=torch.Generator().manual_seed(4)).float()
+    vals = torch.randint(-8, 9, (2, 1024), generator=torch.Generator().manual_seed(4)).float()
     want = torch.zeros(2, 50).scatter_add_(1, many.long(), vals)     # whole numbers: any order
     assert torch.equal(_run(torch.zeros(2, 50), dict(bias_ids=many, bias_values=vals)).cpu(), want)
     nan = torch.tensor([[0xFFFFFFFF - (1 << 32)]], dtype=torch.int32).view(torch.float32)
@@ -283,6 +283,11 @@ def test_refusals():
                       (dict(out=f32(1, 100).expand(3, 100)), "overlapping")):
         with pytest.raises(RuntimeError, match=match):
             process_logits(x, **kw)
+    with pytest.raises(RuntimeError, match="1024 biases"):
+        process_logits(x, bias_ids=i32(3, 1025), bias_values=f32(3, 1025))
+    with pytest.raises(RuntimeError, match="1024 nodes"):
+        process_logits(x, frequency=f32(3), ancestors=i32(3, 33), draft_tokens=i32(3),
+                       query_start_loc=i32(4))
     with pytest.raises(RuntimeError, match="fp32, bf16 or fp16"):
         process_logits(x.double())
     with pytest.raises(RuntimeError, match="unit column"):
