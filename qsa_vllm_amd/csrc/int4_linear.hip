@@ -101,12 +101,17 @@ __device__ __forceinline__ uint16_t scale_of(const u32x2& v, int q) {
   return (uint16_t)(v[q >> 1] >> (16 * (q & 1)));
 }
 
-// (w & 0x000F000F) | c in one instruction (the compiler makes two of it: a VOP3
-// instruction takes no literal, and at most one scalar).
-__device__ __forceinline__ uint32_t nibbles_or(uint32_t w, uint32_t c) {
-  uint32_t r;
-  asm("v_and_or_b32 %0, %1, %2, %3" : "=v"(r) : "v"(w), "s"(0x000F000Fu), "v"(c));
-  return r;
+// The mask of a word's lowest codes, as a value the compiler cannot see: with
+// two known constants it splits (w & mask) | c into two instructions (a VOP3
+// instruction takes no literal, and one scalar), with unknown ones it is one.
+__device__ __forceinline__ uint32_t code_mask() {
+  uint32_t m = 0x000F000Fu;
+  asm("" : "+s"(m));
+  return m;
+}
+__device__ __forceinline__ uint32_t hidden(uint32_t c) {
+  asm("" : "+v"(c));
+  return c;
 }
 
 // A type's matrix operand: unpacking a word of codes with a zero point's
@@ -120,14 +125,15 @@ struct Bf16 {
   }
   // 192 - z in both halves (128, to which a code is or-ed, without zero points).
   static __device__ __forceinline__ uint32_t zero_word(int z) {
-    return ZEROS ? 0x43404340u - (uint32_t)z * 0x10001u : 0x43004300u;
+    return ZEROS ? 0x43404340u - (uint32_t)z * 0x10001u : hidden(0x43004300u);
   }
   static __device__ __forceinline__ frag unpack(uint32_t w, uint32_t zero) {
     u32x4 r;
+    const uint32_t mask = code_mask();
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       if constexpr (ZEROS) r[i] = ((w >> (4 * i)) & 0x000F000Fu) + zero;
-      else r[i] = nibbles_or(w >> (4 * i), zero);
+      else r[i] = ((w >> (4 * i)) & mask) | zero;
     }
     return __builtin_bit_cast(frag, r);
   }
@@ -162,11 +168,11 @@ struct Fp16 {
       f16x2 p[4];
       frag f;
     } r;
-    const uint32_t v = w >> 8;
-    r.p[0] = __builtin_bit_cast(f16x2, nibbles_or(w, 0x64006400u)) + low;
+    const uint32_t v = w >> 8, mask = code_mask(), magic = hidden(0x64006400u);
+    r.p[0] = __builtin_bit_cast(f16x2, (w & mask) | magic) + low;
     r.p[1] = __builtin_elementwise_fma(
         __builtin_bit_cast(f16x2, (w & 0x00F000F0u) | 0x64006400u), sixteenth, high);
-    r.p[2] = __builtin_bit_cast(f16x2, nibbles_or(v, 0x64006400u)) + low;
+    r.p[2] = __builtin_bit_cast(f16x2, (v & mask) | magic) + low;
     r.p[3] = __builtin_elementwise_fma(
         __builtin_bit_cast(f16x2, (v & 0x00F000F0u) | 0x64006400u), sixteenth, high);
     return r.f;

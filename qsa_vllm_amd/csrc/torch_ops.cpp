@@ -897,8 +897,7 @@ void tree_attention_impl(const Tensor& q, const Tensor& k_cache, const Tensor& v
 }
 
 void process_logits_impl(const Tensor& logits, const Tensor& out, const OptTensor& token_to_req,
-                         int64_t num_requests, const OptTensor& history,
-                         const OptTensor& history_lens, const OptTensor& prompt_lens,
+                         const OptTensor& history, const OptTensor& history_lens, const OptTensor& prompt_lens,
                          const OptTensor& repetition, const OptTensor& frequency,
                          const OptTensor& presence, const OptTensor& bias_ids,
                          const OptTensor& bias_values, const OptTensor& allowed,
@@ -918,6 +917,19 @@ void process_logits_impl(const Tensor& logits, const Tensor& out, const OptTenso
   own_rows(out, "out");
   QSA_REQUIRE(out.size(0) == rows && out.size(1) == vocab, "out must have the shape of logits");
   QSA_REQUIRE(vocab_start >= 0 && vocab_start <= INT32_MAX, "vocab_start is out of range");
+  // The requests: as many as the shortest of the tensors that have one each.
+  int64_t num_requests = -1;
+  auto shortest = [&](const OptTensor& t, int64_t less) {
+    if (!t || t->dim() == 0) return;
+    const int64_t n = t->size(0) - less;
+    num_requests = num_requests < 0 ? n : std::min(num_requests, n);
+  };
+  for (const OptTensor* t : {&history, &history_lens, &prompt_lens, &repetition, &frequency,
+                             &presence, &bias_ids, &bias_values})
+    shortest(*t, 0);
+  if (query_start_loc) QSA_REQUIRE(query_start_loc->numel() >= 1, "query_start_loc is empty");
+  shortest(query_start_loc, 1);
+  if (num_requests < 0) num_requests = rows;
   if (token_to_req) vec(*token_to_req, at::kInt, "token_to_req", rows);
   else QSA_REQUIRE(num_requests >= rows, "without token_to_req every row is a request: ", rows,
                    " rows, ", num_requests, " requests");
@@ -1048,7 +1060,7 @@ TORCH_LIBRARY_FRAGMENT(yulan_qsa_kernels, m) {
       "Tensor context_lens, Tensor query_start_loc, Tensor ancestors, Tensor(a!) out, "
       "Tensor? output_gate, int max_query_len, int max_context_len) -> ()");
   m.def(
-      "process_logits(Tensor logits, Tensor(a!) out, Tensor? token_to_req, int num_requests, "
+      "process_logits(Tensor logits, Tensor(a!) out, Tensor? token_to_req, "
       "Tensor? history, Tensor? history_lens, Tensor? prompt_lens, Tensor? repetition, "
       "Tensor? frequency, Tensor? presence, Tensor? bias_ids, Tensor? bias_values, "
       "Tensor? allowed, int vocab_start, Tensor? draft_tokens, Tensor? ancestors, "
@@ -1130,7 +1142,7 @@ TORCH_LIBRARY_IMPL(yulan_qsa_kernels, Meta, m) {
                               const Tensor&, const Tensor&, const Tensor&, const Tensor&,
                               const OptTensor&, int64_t, int64_t) {});
   m.impl("process_logits",
-         [](const Tensor&, const Tensor&, const OptTensor&, int64_t, const OptTensor&,
+         [](const Tensor&, const Tensor&, const OptTensor&, const OptTensor&,
             const OptTensor&, const OptTensor&, const OptTensor&, const OptTensor&,
             const OptTensor&, const OptTensor&, const OptTensor&, const OptTensor&, int64_t,
             const OptTensor&, const OptTensor&, const OptTensor&) {});

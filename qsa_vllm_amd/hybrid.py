@@ -35,6 +35,10 @@ slice), the core output gated by ``sigmoid(gate)`` inside the attention kernel.
 GDN projection layout: ``in_proj_qkvz`` grouped per key head as
 ``[q (dk), k (dk), v (r*dv), z (r*dv)]`` and ``in_proj_ba`` as ``[b (r), a (r)]``
 (the grouped layout vLLM selects with ``gqa_interleaved_layout=True``).
+
+With ``weight_bits=4`` the projections, the MLPs and the LM head hold 4-bit
+codes with group scales (``ops/int4.py``) instead of bf16 and multiply by
+``int4_linear``: for steps of few tokens, which only stream the weights.
 """
 
 from __future__ import annotations
@@ -51,6 +55,8 @@ from .layer_step import qsa_layer_step
 from .metadata import QSABatch, QSAMetadataBuilder
 from .ops.hybrid_layers import (gated_norm, gdn_conv_state, gdn_gated_norm, gdn_prep,
                                 gdn_recurrence, silu_mul)
+from .ops.int4 import Int4Weight, int4_linear, int4_quantize
+from .ops.logits import LogitsRules, process_logits
 
 __all__ = ["HybridConfig", "HybridBatch", "HybridBatchBuilder", "HybridDecoder",
            "HybridDecodeGraph", "HybridWorkload", "make_hybrid_workload",
@@ -86,6 +92,12 @@ class HybridConfig:
     page_size: int = 16
     comp_page_size: int = 16
     init_std: float = 0.02
+    weight_bits: int = 16        # of the projections, MLPs and LM head: 16 (bf16) or 4
+    weight_group: int = 128      # inputs of a 4-bit weight's scale
+
+    def __post_init__(self):
+        if self.weight_bits not in (4, 16):
+            raise ValueError(f"weight_bits must be 4 or 16, got {self.weight_bits}")
 
     def layer_types(self) -> list[str]:
         return ["full_attention" if (i + 1) % self.full_attention_every == 0
@@ -146,6 +158,19 @@ class _Init:
         return torch.rand(shape, generator=self.gen, device=self.device) * (high - low) + low
 
 
+def _stored(cfg: HybridConfig, weight: torch.Tensor) -> torch.Tensor | Int4Weight:
+    """A projection's weight as the model holds it."""
+    if cfg.weight_bits == 16:
+        return weight
+    return int4_quantize(weight, group_size=cfg.weight_group)
+
+
+def _linear(x, weight, bias=None):
+    if isinstance(weight, Int4Weight):
+        return int4_linear(x, weight, bias)
+    return F.linear(x, weight, bias)
+
+
 class GatedNorm:
     """``YuLanGatedNorm`` (``model.py:60-98``) with vLLM's fused residual add:
     ``norm(x, residual)`` adds ``x`` into ``residual`` in place."""
@@ -168,11 +193,11 @@ class SwiGLU:
     """``Qwen2MoeMLP`` with ``hidden_act="silu"``: ``down(silu(gate) * up)``."""
 
     def __init__(self, cfg: HybridConfig, init: _Init):
-        self.gate_up_proj = init.normal(2 * cfg.intermediate, cfg.hidden_size)
-        self.down_proj = init.normal(cfg.hidden_size, cfg.intermediate)
+        self.gate_up_proj = _stored(cfg, init.normal(2 * cfg.intermediate, cfg.hidden_size))
+        self.down_proj = _stored(cfg, init.normal(cfg.hidden_size, cfg.intermediate))
 
     def __call__(self, x):
-        return F.linear(silu_mul(F.linear(x, self.gate_up_proj)), self.down_proj)
+        return _linear(silu_mul(_linear(x, self.gate_up_proj)), self.down_proj)
 
 
 class QSAAttention:
@@ -186,10 +211,10 @@ class QSAAttention:
         self.kv_size = self.kv_heads * d
         self.index_size = (cfg.indexer_heads + 1) * cfg.indexer_head_dim
         rows = self.q_size + 2 * self.kv_size + self.index_size
-        self.qkv_weight = init.normal(rows, cfg.hidden_size)
+        self.qkv_weight = _stored(cfg, init.normal(rows, cfg.hidden_size))
         self.qkv_bias = init.normal(rows)
         self.qkv_bias[-self.index_size:] = 0
-        self.o_proj = init.normal(cfg.hidden_size, self.heads * d)
+        self.o_proj = _stored(cfg, init.normal(cfg.hidden_size, self.heads * d))
         self.indexer = YuLanQSAIndexer(cfg.indexer_heads, cfg.indexer_head_dim, cfg.compress_ratio,
                                        cfg.token_topk, cfg.rope_dim, cfg.rope_theta,
                                        cfg.rms_norm_eps, max_position, ring_cache, comp_cache)
@@ -207,12 +232,12 @@ class QSAAttention:
 
     def __call__(self, x, batch: "HybridBatch"):
         t = x.shape[0]
-        qkv = F.linear(x, self.qkv_weight, self.qkv_bias)
+        qkv = _linear(x, self.qkv_weight, self.qkv_bias)
         query, gate, key, value, index_qk = self.split(qkv)
         core = torch.empty(t, self.heads, self.head_dim, dtype=torch.bfloat16, device=x.device)
         qsa_layer_step(self.indexer, self.impl, self.layer, batch.qsa, index_qk, key, value, query,
                        core, gate)
-        return F.linear(core.view(t, -1), self.o_proj)
+        return _linear(core.view(t, -1), self.o_proj)
 
 
 class GatedDeltaNet:
@@ -237,19 +262,21 @@ class GatedDeltaNet:
         del qkvz_w, ba_w
         if self.in_proj.shape[0] % 8:
             raise ValueError("GDN projection rows must pad to a multiple of 8")
-        self.in_proj_qkvz = self.in_proj[:self.n_qkvz]
-        self.in_proj_ba = self.in_proj[self.n_qkvz:self.n_qkvz + 2 * hv]
+        if cfg.weight_bits == 16:
+            self.in_proj_qkvz = self.in_proj[:self.n_qkvz]
+            self.in_proj_ba = self.in_proj[self.n_qkvz:self.n_qkvz + 2 * hv]
+        self.in_proj = _stored(cfg, self.in_proj)
         self.conv_weight = init.normal(cfg.conv_dim, cfg.conv_kernel, std=0.5)
         self.A_log = init.uniform(hv, low=1.0, high=16.0).log()
         self.dt_bias = torch.ones(hv, dtype=torch.float32, device=init.device)
         self.norm_weight = torch.ones(dv, dtype=torch.bfloat16, device=init.device)
-        self.out_proj = init.normal(cfg.hidden_size, hv * dv)
+        self.out_proj = _stored(cfg, init.normal(cfg.hidden_size, hv * dv))
         self.conv_state = init.normal(num_slots, cfg.conv_kernel - 1, cfg.conv_dim, std=1.0)
         self.ssm_state = init.normal(num_slots, hv, dk, dv, std=state_std, dtype=torch.float32)
 
     def __call__(self, x, batch: "HybridBatch"):
         t = x.shape[0]
-        proj = F.linear(x, self.in_proj)
+        proj = _linear(x, self.in_proj)
         qkvz, ba = proj[:, :self.n_qkvz], proj[:, self.n_qkvz:self.n_qkvz + 2 * self.hv]
         q, k, v, g, beta = gdn_prep(qkvz, ba, self.conv_weight, self.conv_state,
                                     batch.query_start_loc, batch.token_to_seq, batch.state_slots,
@@ -260,7 +287,7 @@ class GatedDeltaNet:
                            batch.state_slots, self.hk, self.hv,
                            max_query_len=batch.qsa.main.max_query_len)
         y = gdn_gated_norm(o, qkvz, self.norm_weight, self.eps, self.hk, self.hv)
-        return F.linear(y.view(t, -1), self.out_proj)
+        return _linear(y.view(t, -1), self.out_proj)
 
 
 class DecoderLayer:
@@ -366,21 +393,24 @@ class HybridDecoder:
                 mixer = GatedDeltaNet(cfg, init, state_slots, state_std)
             self.layers.append(DecoderLayer(kind, mixer, cfg, init))
         self.norm = GatedNorm(cfg, init)
-        self.lm_head = init.normal(cfg.vocab_shard, cfg.hidden_size)
+        self.lm_head = _stored(cfg, init.normal(cfg.vocab_shard, cfg.hidden_size))
 
     def embed(self, token_ids):
         return F.embedding(token_ids, self.embed_tokens)
 
-    def logits(self, hidden, residual, batch):
+    def logits(self, hidden, residual, batch, rules: LogitsRules | None = None):
         normalized, _ = self.norm(hidden, residual)
-        return F.linear(normalized[batch.logits_rows], self.lm_head).float()
+        logits = _linear(normalized[batch.logits_rows], self.lm_head)
+        return logits.float() if rules is None else process_logits(logits, **vars(rules))
 
-    def forward(self, batch: HybridBatch) -> torch.Tensor:
-        """One step: fp32 logits [requests, vocab shard] of each request's last token."""
+    def forward(self, batch: HybridBatch, rules: LogitsRules | None = None) -> torch.Tensor:
+        """One step: fp32 logits [requests, vocab shard] of each request's last
+        token, with the requests' ``rules`` (penalties, biases, grammar masks)
+        applied if given."""
         hidden, residual = self.embed(batch.token_ids), None
         for layer in self.layers:
             hidden, residual = layer(hidden, residual, batch)
-        return self.logits(hidden, residual, batch)
+        return self.logits(hidden, residual, batch, rules)
 
 
 class HybridDecodeGraph:
@@ -388,9 +418,11 @@ class HybridDecodeGraph:
     per request) of one size, replayed after the builder refreshes its
     buffers. ``columns`` pins the decode logits-width class during capture (0:
     the compressed page table's capacity). Capture runs the step once as a
-    warm-up, which advances the caches and states like any step."""
+    warm-up, which advances the caches and states like any step. ``rules``'
+    tensors are read anew on every replay."""
 
-    def __init__(self, model: "HybridDecoder", batch: HybridBatch, columns: int = 0):
+    def __init__(self, model: "HybridDecoder", batch: HybridBatch, columns: int = 0,
+                 rules: LogitsRules | None = None):
         if batch.qsa.main.max_query_len != 1:
             raise ValueError("graphs are captured for uniform decode batches only")
         self.num_tokens = batch.num_tokens
@@ -399,12 +431,12 @@ class HybridDecodeGraph:
         side = torch.cuda.Stream()
         side.wait_stream(torch.cuda.current_stream())
         with capture_column_scope(columns), torch.cuda.stream(side):
-            model.forward(batch)
+            model.forward(batch, rules)
         torch.cuda.current_stream().wait_stream(side)
         torch.cuda.synchronize()
         self.graph = torch.cuda.CUDAGraph()
         with capture_column_scope(columns), torch.cuda.graph(self.graph):
-            self.logits = model.forward(batch)
+            self.logits = model.forward(batch, rules)
 
     def replay(self, batch: HybridBatch | None = None) -> torch.Tensor:
         """Replay on the builder's current buffers; returns the logits buffer."""

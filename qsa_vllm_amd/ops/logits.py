@@ -8,7 +8,6 @@ from dataclasses import dataclass
 import torch
 
 from . import _torch_ops  # noqa: F401  (registers torch.ops.yulan_qsa_kernels)
-from ._torch_ops import _require
 
 __all__ = ["LogitsRules", "process_logits"]
 
@@ -75,16 +74,8 @@ def process_logits(
     At most 1024 biases and 1024 nodes (32 ancestor words) a request."""
     if out is None:
         out = torch.empty(logits.shape, dtype=torch.float32, device=logits.device)
-    per_request = (history_lens, history, prompt_lens, repetition, frequency, presence, bias_ids)
-    requests = min((t.shape[0] for t in per_request if t is not None), default=None)
-    if query_start_loc is not None:
-        starts = query_start_loc.shape[0] - 1
-        requests = starts if requests is None else min(requests, starts)
-    if requests is None:
-        requests = logits.shape[0]
-    _require(requests >= 0, "query_start_loc must have an entry for each request and the end")
     torch.ops.yulan_qsa_kernels.process_logits(
-        logits, out, token_to_req, requests, history, history_lens, prompt_lens, repetition,
+        logits, out, token_to_req, history, history_lens, prompt_lens, repetition,
         frequency, presence, bias_ids, bias_values, allowed, int(vocab_start), draft_tokens,
         ancestors, query_start_loc)
     return out

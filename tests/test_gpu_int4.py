@@ -85,6 +85,32 @@ def test_whole_numbers_are_exact(rows, k, group, dtype):
     assert torch.equal(got.cpu(), exact.float().to(dtype))
 
 
+# Every block shape of the kernel for more than 16 rows, by what is least of
+# rows and outputs: 32 x 32, 32 x 64, 32 x 96, 64 x 128 and 64 x 192, each with odd ends.
+BLOCKS = [(40, 500), (100, 2100), (204, 1544), (64, 9000), (50, 49500), (250, 22500)]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("rows,n", BLOCKS)
+def test_block_shapes_are_exact_on_whole_numbers(rows, n, group, zeros, dtype):
+    """Fewer k tiles than the waves share, and a short last one: 128 to 1288 inputs."""
+    gen = torch.Generator(device=DEV).manual_seed(rows + n)
+    for k in (128, 520, 1288):
+        codes = torch.randint(0, 16, (n, k), generator=gen, device=DEV, dtype=torch.uint8)
+        groups = -(-k // group)
+        scales = (2.0 ** torch.randint(-3, 1, (n, groups), generator=gen, device=DEV).float()).to(dtype)
+        z = torch.randint(0, 16, (n, groups), generator=gen, device=DEV, dtype=torch.uint8) if zeros else None
+        x = torch.randint(-2, 3, (rows, k), generator=gen, device=DEV).to(dtype)
+        got = int4_linear(x, int4_pack(codes, scales, z, group_size=group))
+        s = scales.float().repeat_interleave(group, 1)[:, :k]
+        shift = z.float().repeat_interleave(group, 1)[:, :k] if zeros else 8.0
+        # whole multiples of 2^-3 below 2^17: exact in fp32 in any order
+        exact = x.float() @ ((codes.float() - shift) * s).t()
+        assert torch.equal(got, exact.to(dtype)), k
+
+
 def test_strides_alignment_and_out():
     gen = torch.Generator().manual_seed(3)
     n, k, group, dtype = 50, 256, 64, torch.bfloat16
