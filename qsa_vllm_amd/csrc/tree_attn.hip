@@ -103,7 +103,7 @@ __device__ __forceinline__ Request load_request(const TreeArgs& a, int b) {
 }
 
 __device__ __forceinline__ float gate_factor(uint16_t g) {
-  return 1.0f / (1.0f + __expf(-__builtin_bit_cast(float, (uint32_t)g << 16)));
+  return __builtin_amdgcn_rcpf(1.0f + __expf(-__builtin_bit_cast(float, (uint32_t)g << 16)));
 }
 
 // Byte offset of 16-byte unit `unit` of token `tok`'s row in a K stage: units
