@@ -28,8 +28,14 @@
 // each wave has its own 16 NB rows and all tokens of a stage, with few rows the
 // waves take different tokens and merge (max, sum, O) through LDS at the end.
 //
-// A long context is cut into chunks of whole stages, a workgroup each, whose
-// normalised fp32 results and log2 sums a second kernel joins in chunk order.
+// Work is shared out by stages. A row tile's (request, kv head) units, each of its
+// request's stages, lie end to end on that tile's line, and every workgroup takes
+// an equal stretch of a line, two workgroups a CU in all. Workgroups at the same
+// place of different tiles' lines run on one XCD, whose L2 then serves the K/V to
+// all but the first. Lengths and rows are known on the device only; each
+// workgroup adds them up itself. A unit that no one stretch covers leaves
+// normalised fp32 pieces and log2 sums, which a second kernel joins in order; the
+// others are written at once.
 #include "qsa_common.h"
 #include "../../include/qsa_hip.h"
 
@@ -76,12 +82,14 @@ struct TreeArgs {
   int64_t out_row, out_head;
   const uint16_t* gate;
   int64_t g_row, g_head, g_dim;
-  float* part_out;  // [rows][q heads][splits][D]
-  float* part_lse;  // [rows][q heads][splits]
+  // Two pieces a workgroup (the end of a unit it shares with the one before, the
+  // start of one it shares with the next): [2 workgroups][slot rows][D], then sums.
+  float* part_out;
+  float* part_lse;
   int rows, num_q_heads, kv_heads, group;
   FastDiv group_div;
-  int m_tiles, splits, chunk;
-  int pair_slots;  // (request, kv head) pairs, rounded up to 8
+  int workgroups;  // 0: one for each unit (m_tiles a request and kv head)
+  int m_tiles, slot_rows, max_nodes;
   float scale_log2;
 };
 
@@ -90,16 +98,78 @@ struct TreeArgs {
 struct Request {
   int row0, nodes, context, length;
 };
-__device__ __forceinline__ Request load_request(const TreeArgs& a, int b) {
+__device__ __forceinline__ Request make_request(const TreeArgs& a, int first, int last, int context) {
   Request r;
-  const int first = load_uniform(a.query_start_loc + b);
-  const int last = load_uniform(a.query_start_loc + b + 1);
   r.row0 = min(max(first, 0), a.rows);
-  r.nodes = min(max(last, r.row0), a.rows) - r.row0;
+  r.nodes = min(min(max(last, r.row0), a.rows) - r.row0, a.max_nodes);
   const int64_t capacity = min((int64_t)a.table_width * a.page_size, (int64_t)INT_MAX / 2);
-  r.context = (int)min((int64_t)max(load_uniform(a.context_lens + b), 0), capacity);
+  r.context = (int)min((int64_t)max(context, 0), capacity);
   r.length = (int)min((int64_t)r.context + r.nodes, capacity);
   return r;
+}
+__device__ __forceinline__ Request load_request(const TreeArgs& a, int b) {  // b: a lane's own
+  return make_request(a, a.query_start_loc[b], a.query_start_loc[b + 1], a.context_lens[b]);
+}
+__device__ __forceinline__ Request uniform_request(const TreeArgs& a, int b) {  // b: the wave's
+  return make_request(a, load_uniform(a.query_start_loc + b), load_uniform(a.query_start_loc + b + 1),
+                      load_uniform(a.context_lens + b));
+}
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ int tiles_of(const TreeArgs& a, const Request& r) {
+  return (r.nodes * a.group + kTileRows - 1) / kTileRows;
+}
+__device__ __forceinline__ int stages_of(const Request& r) {
+  return max(1, (r.length + kTok - 1) / kTok);
+}
+// A request's stages on a tile's line.
+__device__ __forceinline__ int stages_on(const TreeArgs& a, const Request& r, int tile) {
+  return tile < tiles_of(a, r) ? a.kv_heads * stages_of(r) : 0;
+}
+
+// fn(request b), added up over all requests: a wave's 64 lanes take one each.
+template <typename F>
+__device__ __forceinline__ int sum_requests(const TreeArgs& a, F fn) {
+  if (a.requests == 1) return uniform(fn(0, uniform_request(a, 0)));
+  int sum = 0;
+  for (int b = threadIdx.x & 63; b < a.requests; b += 64) sum += fn(b, load_request(a, b));
+#pragma unroll
+  for (int w = 32; w > 0; w /= 2) sum += __shfl_xor(sum, w, 64);
+  return uniform(sum);
+}
+__device__ __forceinline__ int line_length(const TreeArgs& a, int tile) {
+  return sum_requests(a, [&](int, const Request& r) { return stages_on(a, r, tile); });
+}
+// Stages of a stretch.
+__device__ __forceinline__ int stretch(const TreeArgs& a) {
+  const int all = sum_requests(
+      a, [&](int, const Request& r) { return tiles_of(a, r) * a.kv_heads * stages_of(r); });
+  return max(1u, (unsigned)(all + a.workgroups - 1) / (unsigned)a.workgroups);
+}
+// Workgroups of a line, rounded up so that the next line starts at the first XCD.
+__device__ __forceinline__ int line_workgroups(int length, int mine) {
+  return ((unsigned)(length + mine - 1) / (unsigned)mine + 7) / 8 * 8;
+}
+// The request at a place on a tile's line; `place` becomes the place within it.
+__device__ __forceinline__ int locate(const TreeArgs& a, int tile, int& place) {
+  if (a.requests == 1) return 0;
+  const int lane = threadIdx.x & 63;
+  for (int b0 = 0; b0 < a.requests; b0 += 64) {
+    const int n = b0 + lane < a.requests ? stages_on(a, load_request(a, b0 + lane), tile) : 0;
+    int end = n;  // inclusive sum over the lanes
+#pragma unroll
+    for (int w = 1; w < 64; w *= 2) {
+      const int below = __shfl_up(end, w, 64);
+      end += lane >= w ? below : 0;
+    }
+    const uint64_t past = __ballot(end > place);
+    if (past) {
+      const int at = __ffsll((unsigned long long)past) - 1;
+      place = uniform(place - __shfl(end - n, at, 64));
+      return b0 + at;
+    }
+    place = uniform(place - __shfl(end, 63, 64));
+  }
+  return a.requests;
 }
 
 __device__ __forceinline__ float gate_factor(uint16_t g) {
@@ -212,16 +282,20 @@ __device__ __forceinline__ uint64_t seen_from(const TreeArgs& a, int row, int j)
   return j < 0 ? bits | ((1ull << -j) - 1) : bits;
 }
 
-// One row tile (rows m0 .. of a request's `rows`) of one chunk.
+// Tokens t_begin .. t_end of one row tile (rows m0 .. of a request's `rows`), to
+// the output or, where others take the rest of them, to piece `piece`.
 template <int D, int NB, int WM, int WT>
 __device__ __forceinline__ void attend_tile(const TreeArgs& a, const Request& rq,
                                             const int32_t* trow, int kv, int rows, int m0,
-                                            int split, int t_begin, int t_end, char* lds) {
+                                            int piece, int t_begin, int t_end, char* lds) {
   typedef Shape<D, NB, WM, WT> S;
   constexpr int U = D / 8;  // 16-byte units of a row
   constexpr int kSteps = D / 32;
   constexpr int kDims = D / 16;
-  const int lane = threadIdx.x & 63;
+  // Not to be known before the tile: what follows from it, for all four shares,
+  // would otherwise be kept in registers through the loop over tiles.
+  int lane = threadIdx.x & 63;
+  asm("" : "+v"(lane));
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n = lane & 15, g = lane >> 4;
   const int wm = wave / WT, wt = wave % WT;
@@ -511,8 +585,8 @@ __device__ __forceinline__ void attend_tile(const TreeArgs& a, const Request& rq
     if (m >= rows) continue;
     const int head = kv * a.group + m - (node[i] - rq.row0) * a.group;
     const float inv = total[i] == 0.0f ? 0.0f : 1.0f / total[i];  // a row that sees nothing: zeros
-    if (a.splits > 1) {
-      const int64_t at = ((int64_t)node[i] * a.num_q_heads + head) * a.splits + split;
+    if (piece >= 0) {
+      const int64_t at = (int64_t)piece * a.slot_rows + m - m0;
 #pragma unroll
       for (int d = 0; d < kDims; ++d)
         *reinterpret_cast<f32x4*>(a.part_out + at * D + 16 * d + 4 * g) =
@@ -540,37 +614,68 @@ template <int D>
 __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 2))) void
 tree_attn_kernel(TreeArgs a) {
   extern __shared__ __attribute__((aligned(16))) char lds[];
-  // Blocks go to the 8 XCDs in turn. Row tiles of one chunk are 8 blocks apart:
-  // the same XCD, whose L2 then serves the chunk's K/V to all but the first. A
-  // (request, kv head)'s chunks go round the XCDs, so that long and short
-  // requests spread evenly.
-  const int slot = (int)(blockIdx.x / (8 * a.m_tiles)) * 8 + (int)(blockIdx.x & 7);
-  const int m_tile = (int)(blockIdx.x >> 3) % a.m_tiles;
-  const int split = slot / a.pair_slots, place = slot % a.pair_slots;
-  const int pair = (place & ~7) | ((place - split) & 7);
-  if (pair >= a.requests * a.kv_heads) return;
-  const int kv = pair % a.kv_heads;
-  const int request = pair / a.kv_heads;
-  const Request rq = load_request(a, request);
-  const int32_t* const trow = a.table + request * a.table_row;
-  const int rows = rq.nodes * a.group;
-  const int m0 = m_tile * kTileRows;
-  const int t_begin = split * a.chunk;
-  if (m0 >= rows || (split > 0 && t_begin >= rq.length)) return;
-  // The last chunk takes whatever is left (a context longer than was said).
-  const int t_end = split + 1 == a.splits ? rq.length : min(rq.length, t_begin + a.chunk);
-  // The wave shares by the tile's own rows: requests of one batch differ.
-  const int left = rows - m0;
-  if (left > 64) attend_tile<D, 2, 4, 1>(a, rq, trow, kv, rows, m0, split, t_begin, t_end, lds);
-  else if (left > 32) attend_tile<D, 2, 2, 2>(a, rq, trow, kv, rows, m0, split, t_begin, t_end, lds);
-  else if (left > 16) attend_tile<D, 2, 1, 4>(a, rq, trow, kv, rows, m0, split, t_begin, t_end, lds);
-  else attend_tile<D, 1, 1, 4>(a, rq, trow, kv, rows, m0, split, t_begin, t_end, lds);
+  // The stretch [place, place + left) of a tile's line, place counted from the
+  // start of `request`.
+  int request, tile, place, left;
+  if (a.workgroups) {
+    const int mine = stretch(a);
+    int id = blockIdx.x, length;
+    for (tile = 0;; ++tile) {
+      length = line_length(a, tile);
+      if (length == 0) return;  // past the last line
+      const int n = line_workgroups(length, mine);
+      if (id < n) break;
+      id -= n;
+    }
+    place = id * mine;
+    left = min(mine, length - place);
+    if (left <= 0) return;
+    request = locate(a, tile, place);
+  } else {
+    const int units = a.kv_heads * a.m_tiles;
+    request = blockIdx.x / units;
+    const int unit = blockIdx.x - request * units;
+    tile = unit / a.kv_heads;
+    const Request rq = uniform_request(a, request);
+    if (tile >= tiles_of(a, rq)) return;
+    left = stages_of(rq);
+    place = (unit - tile * a.kv_heads) * left;
+  }
+  const int m0 = tile * kTileRows;
+  bool first = true;
+  while (left > 0 && request < a.requests) {
+    const Request rq = uniform_request(a, request);
+    const int stages = stages_of(rq);
+    const int units = tile < tiles_of(a, rq) ? a.kv_heads : 0;
+    for (int kv = (unsigned)place / (unsigned)stages; kv < units && left > 0; ++kv) {
+      const int s0 = place - kv * stages;
+      const int s1 = min(stages, s0 + left);
+      place += s1 - s0;
+      left -= s1 - s0;
+      const int rows = rq.nodes * a.group;
+      // A unit that starts here and goes on is the stretch's last, one that ends
+      // or goes through, its first.
+      const int piece = s0 == 0 && s1 == stages ? -1 : 2 * (int)blockIdx.x + (s0 == 0 ? 1 : 0);
+      const int t_begin = s0 * kTok, t_end = min(rq.length, s1 * kTok);
+      const int32_t* const trow = a.table + request * a.table_row;
+      if (!first) __syncthreads();  // LDS has been read by all
+      first = false;
+      // The wave shares by the tile's own rows: requests of one batch differ.
+      const int here = rows - m0;
+      if (here > 64) attend_tile<D, 2, 4, 1>(a, rq, trow, kv, rows, m0, piece, t_begin, t_end, lds);
+      else if (here > 32) attend_tile<D, 2, 2, 2>(a, rq, trow, kv, rows, m0, piece, t_begin, t_end, lds);
+      else if (here > 16) attend_tile<D, 2, 1, 4>(a, rq, trow, kv, rows, m0, piece, t_begin, t_end, lds);
+      else attend_tile<D, 1, 1, 4>(a, rq, trow, kv, rows, m0, piece, t_begin, t_end, lds);
+    }
+    ++request;
+    place = 0;
+  }
 }
 
-// Joins a row's chunks: out = sum_s 2^(lse_s - max) part_s / sum_s 2^(lse_s - max).
-// D / 4 lanes hold a (row, head)'s dims; WAYS such groups take its chunks in
+// Joins a row's pieces: out = sum_s 2^(lse_s - max) part_s / sum_s 2^(lse_s - max).
+// D / 4 lanes hold a (row, head)'s dims; WAYS such groups take its pieces in
 // turn (s mod WAYS) and add up in group order, so that a long context's many
-// partials are read side by side. Bound by reading the partials.
+// pieces are read side by side. Bound by reading them.
 template <int D, int WAYS>
 __global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs a, int row_tiles) {
   constexpr int kLanes = D / 4;
@@ -578,19 +683,45 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs a, int row_til
   constexpr int kPer = kGroups / WAYS;  // (row, head)s of a workgroup
   __shared__ f32x4 acc_lds[WAYS > 1 ? kGroups : 1][kLanes];
   __shared__ float sum_lds[WAYS > 1 ? kGroups : 1];
-  const Request rq = load_request(a, blockIdx.x / row_tiles);
+  const int request = blockIdx.x / row_tiles;
+  const Request rq = uniform_request(a, request);
+  const int64_t first_item = (int64_t)(blockIdx.x % row_tiles) * kPer;
+  if (first_item >= (int64_t)rq.nodes * a.num_q_heads) return;
   const int lane = threadIdx.x % kLanes, grp = threadIdx.x / kLanes;
   const int way = grp % WAYS;
-  const int64_t item = (int64_t)(blockIdx.x % row_tiles) * kPer + grp / WAYS;
+  const int64_t item = first_item + grp / WAYS;
   const int node = (int)(item / a.num_q_heads);
-  const bool live = node < rq.nodes;
   const int head = (int)(item - (int64_t)node * a.num_q_heads);
+  const int kv = head / a.group;
+  const int m = node * a.group + head - kv * a.group;
+  const int stages = stages_of(rq);
+  // Where the unit lies on its tile's line, and the workgroups whose stretches it
+  // meets: the first one's piece is its second, the others' their first. A
+  // workgroup's rows may be of several tiles; all lanes go through all of them.
+  const int mine = stretch(a);
+  const int my_tile = m / kTileRows;
+  int begin = 0, id0 = 0, ids = 0;
+  for (int tile = 0; tile < tiles_of(a, rq); ++tile) {
+    const int before = sum_requests(a, [&](int b, const Request& r) {
+      return b < request ? stages_on(a, r, tile) : 0;
+    });
+    if (tile == my_tile) {
+      begin = before + kv * stages;
+      id0 = ids;
+    }
+    if (tile + 1 < tiles_of(a, rq)) ids += line_workgroups(line_length(a, tile), mine);
+  }
+  const int w0 = (unsigned)begin / (unsigned)mine;
+  const int pieces = (unsigned)(begin + stages - 1) / (unsigned)mine - w0 + 1;
+  // One piece: the attention has written the row.
+  const bool live = node < rq.nodes && pieces > 1;
   const int64_t row = rq.row0 + node;
-  const int splits = live ? min(a.splits, max(1, (rq.length + a.chunk - 1) / a.chunk)) : 0;
-  const int64_t at = live ? (row * a.num_q_heads + head) * a.splits : 0;
-  const float* const lse = a.part_lse + at;
+  const int splits = live ? pieces : 0;
+  auto at = [&](int s) -> int64_t {
+    return (int64_t)(2 * (id0 + w0 + s) + (s == 0 ? 1 : 0)) * a.slot_rows + m % kTileRows;
+  };
   float top = kNegInf;
-  for (int s = lane; s < splits; s += kLanes) top = fmaxf(top, lse[s]);
+  for (int s = lane; s < splits; s += kLanes) top = fmaxf(top, a.part_lse[at(s)]);
 #pragma unroll
   for (int w = kLanes / 2; w > 0; w /= 2) top = fmaxf(top, __shfl_xor(top, w, 64));
   const float base = top == kNegInf ? 0.0f : top;
@@ -598,8 +729,8 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs a, int row_til
   f32x4 acc = {0, 0, 0, 0};
 #pragma unroll 4
   for (int s = way; s < splits; s += WAYS) {
-    const float f = fast_exp2(lse[s] - base);
-    const f32x4 part = *reinterpret_cast<const f32x4*>(a.part_out + (at + s) * D + 4 * lane);
+    const float f = fast_exp2(a.part_lse[at(s)] - base);
+    const f32x4 part = *reinterpret_cast<const f32x4*>(a.part_out + at(s) * D + 4 * lane);
     sum += f;
 #pragma unroll
     for (int r = 0; r < 4; ++r) acc[r] += f * part[r];
@@ -633,32 +764,24 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs a, int row_til
 // ---------------------------------------------------------------------------
 
 struct TreePlan {
-  int m_tiles, splits, chunk;
+  int workgroups, m_tiles, slot_rows;
 };
 
-// max_nodes and max_context bound the requests' nodes and committed tokens; the
-// results do not depend on the chunks beyond fp32 rounding, and a request longer
-// than max_context says is computed whole (its last chunk takes the rest).
+// Workgroups of a launch at most: each line's last stretch may be short, and its
+// number is rounded up to 8.
+int grid_of(const TreePlan& p) { return p.workgroups + 8 * p.m_tiles; }
+
+// max_nodes and max_context bound the requests' nodes and committed tokens. They
+// shape the launch: a longer context is computed whole all the same.
 TreePlan make_plan(int requests, int num_q_heads, int num_kv_heads, int64_t max_nodes,
                    int64_t max_context) {
   TreePlan p;
   const int64_t rows = max_nodes * (num_q_heads / num_kv_heads);
   p.m_tiles = (int)((rows + kTileRows - 1) / kTileRows);
+  p.slot_rows = (int)std::min<int64_t>(kTileRows, (rows + 15) / 16 * 16);
   const int64_t units = (int64_t)requests * num_kv_heads * p.m_tiles;
-  const int64_t length = std::min<int64_t>(max_context + max_nodes, INT_MAX / 2);
-  const int64_t stages = std::max<int64_t>(1, (length + kTok - 1) / kTok);
-  // Two workgroups fit a CU. One request's chunks are alike: one round of them
-  // (64 nodes on 131072 tokens 97 us, a round and a half 108, two 107, and each
-  // chunk's partial result is written and read again). Several requests differ
-  // in length and rows, and a chunk of the longest's share leaves CUs without
-  // work: four rounds by the longest (32 trees on 4k-32k 230 us, one round 280,
-  // eight 231; 64 single tokens on 1k-8k 73, 68 and 78).
-  const int64_t rounds = requests == 1 ? 1 : 4;
-  int64_t splits = std::min<int64_t>((rounds * 2 * kCUs + units - 1) / units, stages);
-  splits = std::max<int64_t>(1, std::min<int64_t>(splits, 256));
-  const int64_t per = (stages + splits - 1) / splits;
-  p.chunk = (int)std::min<int64_t>(per * kTok, INT_MAX / 2);
-  p.splits = (int)((stages + per - 1) / per);
+  const int64_t stages = (std::min<int64_t>(max_context + max_nodes, INT_MAX / 2) + kTok - 1) / kTok;
+  p.workgroups = stages > 1 ? (int)std::min<int64_t>(2 * kCUs, units * stages) : 0;
   return p;
 }
 
@@ -672,17 +795,19 @@ hipError_t launch_merge(const TreeArgs& a, int64_t pairs, hipStream_t stream) {
 }
 
 template <int D>
-hipError_t launch_tree(const TreeArgs& a, int max_nodes, hipStream_t stream) {
-  const unsigned grid = (unsigned)((int64_t)a.pair_slots * a.splits * a.m_tiles);
+hipError_t launch_tree(const TreeArgs& a, const TreePlan& plan, int max_nodes, hipStream_t stream) {
+  const unsigned grid =
+      a.workgroups ? grid_of(plan) : a.requests * a.kv_heads * a.m_tiles;
   constexpr size_t kLds = std::max({Shape<D, 2, 4, 1>::kLds, Shape<D, 2, 2, 2>::kLds,
                                     Shape<D, 2, 1, 4>::kLds, Shape<D, 1, 1, 4>::kLds});
   static_assert(kLds <= 65536, "two workgroups a CU, and no attribute to set");
   hipLaunchKernelGGL((tree_attn_kernel<D>), dim3(grid), dim3(64 * kWaves), kLds, stream, a);
   const hipError_t err = hipGetLastError();
-  if (err != hipSuccess || a.splits == 1) return err;
+  if (err != hipSuccess || !a.workgroups) return err;
+  // Many (row, head)s have few pieces each.
   const int64_t pairs = (int64_t)max_nodes * a.num_q_heads;
-  if (a.splits >= 8) return launch_merge<D, 8>(a, pairs, stream);
-  return launch_merge<D, 2>(a, pairs, stream);
+  return pairs * a.requests <= 4096 ? launch_merge<D, 8>(a, pairs, stream)
+                                    : launch_merge<D, 2>(a, pairs, stream);
 }
 
 // Elements from a cache's first token row to its last, -1 if a stride is negative
@@ -709,8 +834,8 @@ extern "C" size_t qsa_tree_attention_workspace_bytes(int rows, int requests, int
     return 0;
   const TreePlan p = make_plan(requests, num_q_heads, num_kv_heads, std::min(max_query_len, rows),
                                max_context_len);
-  if (p.splits == 1) return 0;
-  return (size_t)rows * num_q_heads * p.splits * (head_dim + 1) * sizeof(float);
+  if (!p.workgroups) return 0;
+  return (size_t)2 * grid_of(p) * p.slot_rows * (head_dim + 1) * sizeof(float);
 }
 
 extern "C" int qsa_tree_attention(
@@ -752,20 +877,22 @@ extern "C" int qsa_tree_attention(
   max_query_len = std::min(max_query_len, rows);
   const TreePlan plan =
       make_plan(num_requests, num_q_heads, num_kv_heads, max_query_len, max_context_len);
-  const int64_t pair_slots = ((int64_t)num_requests * num_kv_heads + 7) / 8 * 8;
-  const int64_t grid = pair_slots * plan.splits * plan.m_tiles;
+  const int64_t units = (int64_t)num_requests * num_kv_heads * plan.m_tiles;
   const int64_t merge = (int64_t)num_requests * max_query_len * num_q_heads;
-  if (grid > INT_MAX || merge > INT_MAX || (int64_t)max_query_len * num_q_heads > INT_MAX / 2)
-    return fail(QSA_ERR_UNSUPPORTED, name + ": too many requests, rows or heads");
+  const int64_t capacity = (int64_t)table_width * page_size / kTok + 1;
+  if (units > INT_MAX / 2 / capacity || merge > INT_MAX ||
+      (int64_t)max_query_len * num_q_heads > INT_MAX / 2)
+    return fail(QSA_ERR_UNSUPPORTED, name + ": too many requests, rows or heads for the page table");
   TreeArgs a = {};
-  if (plan.splits > 1) {
+  if (plan.workgroups) {
     const size_t need = qsa_tree_attention_workspace_bytes(
         rows, num_requests, num_q_heads, num_kv_heads, head_dim, max_query_len, max_context_len);
     if (!workspace || workspace_bytes < need || !aligned16(workspace))
       return fail(QSA_ERR_WORKSPACE, name + ": needs a 16-byte aligned workspace of " +
                                          std::to_string(need) + " bytes");
     a.part_out = static_cast<float*>(workspace);
-    a.part_lse = a.part_out + (size_t)rows * num_q_heads * plan.splits * head_dim;
+    a.part_lse = a.part_out +
+                 (size_t)2 * grid_of(plan) * plan.slot_rows * head_dim;
   }
   a.q = static_cast<const uint16_t*>(q);
   a.q_row = q_row_stride;
@@ -803,13 +930,13 @@ extern "C" int qsa_tree_attention(
   a.group = num_q_heads / num_kv_heads;
   a.group_div = FastDiv::make(a.group);
   a.m_tiles = plan.m_tiles;
-  a.splits = plan.splits;
-  a.pair_slots = (int)pair_slots;
-  a.chunk = plan.chunk;
+  a.workgroups = plan.workgroups;
+  a.slot_rows = plan.slot_rows;
+  a.max_nodes = max_query_len;
   a.scale_log2 = 1.4426950408889634f / sqrtf((float)head_dim);
   hipStream_t s = static_cast<hipStream_t>(stream);
-  const hipError_t err = head_dim == 128 ? launch_tree<128>(a, max_query_len, s)
-                                         : launch_tree<64>(a, max_query_len, s);
+  const hipError_t err = head_dim == 128 ? launch_tree<128>(a, plan, max_query_len, s)
+                                         : launch_tree<64>(a, plan, max_query_len, s);
   if (err != hipSuccess)
     return fail(QSA_ERR_HIP, name + " launch: " + hipGetErrorString(err));
   return QSA_OK;

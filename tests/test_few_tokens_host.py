@@ -162,11 +162,13 @@ def test_tree_attention_refuses():
 
 
 def test_tree_attention_workspace_stays_in_proportion():
-    """Partial results: at most 256 of every row, whatever the context."""
+    """Two pieces of at most 128 rows for each of at most 512 workgroups (and 8 for
+    each 128 rows of a request and kv head), whatever the context and the batch."""
     f = _lib.load().qsa_tree_attention_workspace_bytes
     for rows, nreq, most, ctx in ((1, 1, 1, 2**30), (64, 1, 64, 131072), (64, 64, 1, 131072),
                                   (4096, 64, 64, 524288)):
-        assert f(rows, nreq, 16, 2, 128, most, ctx) <= rows * 16 * 256 * 129 * 4
+        assert 0 < f(rows, nreq, 16, 2, 128, most, ctx) <= (
+            2 * (512 + 8 * -(-most * 8 // 128)) * min(128, max(16, most * 8)) * 129 * 4)
     assert f(0, 1, 16, 2, 128, 1, 1000) == 0 and f(4, 1, 16, 0, 128, 1, 1000) == 0
 
 

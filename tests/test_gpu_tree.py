@@ -139,6 +139,21 @@ def test_long_contexts_split(nodes, max_context_len):
     c.check(c.run(max_context_len=max_context_len))
 
 
+@pytest.mark.parametrize("requests,most,longest,heads,kv_heads,dim", [
+    (150, 3, 200, 4, 2, 64),        # more requests than a wave has lanes
+    (70, 40, 130, 8, 1, 64),        # row tiles of their own number in each request
+    (65, 1, 700, 2, 1, 128), (3, 64, 1500, 16, 1, 64), (130, 2, 1, 2, 2, 64)])
+def test_ragged_batches(requests, most, longest, heads, kv_heads, dim):
+    """Stretches of the work that start and end anywhere: in requests without
+    nodes or context, between kv heads, in the middle of a request."""
+    gen = torch.Generator().manual_seed(requests)
+    ctx = torch.randint(0, longest + 1, (requests,), generator=gen).tolist()
+    nodes = torch.randint(0, most + 1, (requests,), generator=gen).tolist()
+    nodes[0], nodes[-1], nodes[1] = 0, 0, most
+    c = Case(ctx, nodes, heads, kv_heads, dim, seed=requests)
+    c.check(c.run())
+
+
 def test_layouts_and_strides():
     c = Case([50, 200], [6, 3], heads=8, kv_heads=2, dim=64, layout="head_major", seed=8)
     c.check(c.run())
