@@ -377,8 +377,8 @@ __device__ __forceinline__ void attend_tile(const TreeArgs& a, const Request& rq
     page_next = load_page(t + 2 * kTok);
     if (t + kTok > rq.context) {
       // A drafted token's V may hold infinities or NaN that a row outside its
-      // branch must not see (0 times them is NaN). They are taken as 0 here,
-      // and rows that see them get NaN at the end.
+      // branch must not see (0 times them is NaN). The whole stage's are taken
+      // as 0 here, and rows that see them get NaN at the end.
       u32x4* const v = reinterpret_cast<u32x4*>(stage + S::kStage);
       bool bad = false;
       for (int i = lane; i < kTok * U; i += 64) bad |= not_finite(v[i]) != 0;
@@ -560,7 +560,8 @@ __device__ __forceinline__ void attend_tile(const TreeArgs& a, const Request& rq
   }
 
   if (poisoned) {
-    for (int pos = max(t_begin, rq.context); pos < t_end; ++pos) {
+    // From the first stage with a drafted token (stages start at multiples of 64).
+    for (int pos = max(t_begin, rq.context / kTok * kTok); pos < t_end; ++pos) {
       const int page = trow[a.page_div.div(pos)];
       if (page < 0 || page >= a.num_blocks) continue;
       const char* const v = a.v + kv * a.vh + ((uint64_t)page * a.vb << 4) +
@@ -870,9 +871,9 @@ extern "C" int qsa_tree_attention(
     return fail(QSA_ERR_INVALID, name + ": q and the caches need 16-byte alignment and strides of "
                                         "multiples of 8 elements, out 4-byte alignment");
   // The kernel's offsets are 32-bit counts of 16 bytes.
-  const int64_t span = std::max(cache_span(num_blocks, k_block_stride, page_size, k_token_stride),
-                                cache_span(num_blocks, v_block_stride, page_size, v_token_stride));
-  if (span < 0 || span / 8 >= kNoToken)
+  const int64_t k_span = cache_span(num_blocks, k_block_stride, page_size, k_token_stride);
+  const int64_t v_span = cache_span(num_blocks, v_block_stride, page_size, v_token_stride);
+  if (k_span < 0 || v_span < 0 || std::max(k_span, v_span) / 8 >= kNoToken)
     return fail(QSA_ERR_UNSUPPORTED, name + ": the cache must span under 64 GiB");
   max_query_len = std::min(max_query_len, rows);
   const TreePlan plan =

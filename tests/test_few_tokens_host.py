@@ -155,6 +155,13 @@ def test_tree_attention_refuses():
         assert f(*_tree_args(**{name: None})) == -1, name
     need = lib.qsa_tree_attention_workspace_bytes(8, 2, 16, 2, 128, 4, 60000)
     assert need > 0
+    # 64 GiB of cache from the first row to the last is too far apart, a page
+    # table and a batch whose stages pass 31 bits too much
+    assert f(*_tree_args(kb=2**32, blocks=10)) == -2 and b"64 GiB" in lib.qsa_last_error()
+    assert f(*_tree_args(vt=2**40)) == -2 and f(*_tree_args(vb=-8192)) == -2
+    assert f(*_tree_args(kt=2**62)) == -2
+    assert f(*_tree_args(nreq=1 << 20, tw=1 << 20, rows=1 << 20, mq=1)) == -2
+    assert f(*_tree_args(nreq=1, rows=2**31 - 1, mq=2**31 - 1)) == -2
     assert f(*_tree_args(mc=60000)) == -4 and b"workspace" in lib.qsa_last_error()
     assert f(*_tree_args(mc=60000, ws=1 << 28, wsb=need - 1)) == -4
     assert f(*_tree_args(mc=60000, ws=(1 << 28) + 4, wsb=need)) == -4

@@ -214,6 +214,26 @@ def test_unseen_nodes_may_hold_anything(bad, ctx, nodes):
     assert off.max() <= 2 * tol[~sees].max()
 
 
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+@pytest.mark.parametrize("at", [0, 63, 64, 69])
+@pytest.mark.parametrize("ctx,nodes,heads", [([70], [5], 16), ([70, 130], [1, 20], 4),
+                                             ([128, 70], [2, 2], 8), ([700, 70], [1, 3], 4)])
+def test_committed_values_that_are_not_finite_reach_every_row(bad, ctx, nodes, heads, at):
+    """Wherever the committed token lies: in a stage of its own kind or in one
+    that the drafted tokens share. Only its dimension is lost."""
+    case = Case(ctx, nodes, heads=heads, kv_heads=2, seed=at)
+    b = len(ctx) - 1
+    case.kv[case.table[b, at // 16], at % 16, 0, case.dim + 3] = bad
+    got = case.run().cpu()
+    hit = torch.zeros(got.shape, dtype=torch.bool)
+    if at < ctx[b]:
+        hit[case.starts[b]:case.starts[b + 1], :heads // 2, 3] = True
+    assert torch.equal(~torch.isfinite(got), hit)
+    case.kv[case.table[b, at // 16], at % 16, 0, case.dim + 3] = 0.0
+    want, tol = case.want()
+    assert ((got.double() - want).abs() <= tol)[~hit].all()
+
+
 def test_positions_without_a_page_are_not_seen():
     c = Case([100, 70], [3, 2], heads=4, kv_heads=1, seed=12)
     table = c.table.clone()
