@@ -36,6 +36,8 @@
 #include "../../include/qsa_hip.h"
 
 #include <algorithm>
+#include <climits>
+#include <type_traits>
 
 namespace qsa {
 namespace {
@@ -298,10 +300,15 @@ __global__ __launch_bounds__(512) void int4_linear_kernel(Int4Args a) {
   // Rows past the last repeat it (their results are not stored), and inputs past
   // the width the row's first ones (their codes are the zero point): no load
   // depends on a condition, which would make it wait for the ones before it.
-  uint32_t at[MT];  // the lane's byte offset in the block
+  // The lane's byte offset in the block: rows taken element by element may be any
+  // distance apart.
+  typename std::conditional<VEC, uint32_t, int64_t>::type at[MT];
 #pragma unroll
-  for (int i = 0; i < MT; ++i)
-    at[i] = (uint32_t)min(16 * i + n, a.rows - 1 - row0) * (uint32_t)(2 * a.x_row);
+  for (int i = 0; i < MT; ++i) {
+    const int row = min(16 * i + n, a.rows - 1 - row0);
+    if constexpr (VEC) at[i] = (uint32_t)row * (uint32_t)(2 * a.x_row);
+    else at[i] = row * (2 * a.x_row);
+  }
   auto load_rows = [&](int t, u32x4 (&x)[MT][4]) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -610,8 +617,11 @@ extern "C" int qsa_int4_linear(const void* x, int64_t x_row_stride, const void* 
   a.k = in_features;
   a.n_tiles = (int)(((int64_t)out_features + kTileN - 1) / kTileN);
   a.k_tiles = (int)(((int64_t)in_features + kTileK - 1) / kTileK);
-  if ((int64_t)a.n_tiles * ((rows + 15) / 16) > 0x7fffffffLL / 2)
-    return fail(QSA_ERR_UNSUPPORTED, std::string(name) + ": too many output tiles");
+  // A launch holds at most 2^32 - 1 threads, 512 for 16 rows x 16 outputs at most.
+  if ((int64_t)a.n_tiles * (((int64_t)rows + 15) / 16) > UINT_MAX / 512 - 8)
+    return fail(QSA_ERR_UNSUPPORTED, std::string(name) + ": too many rows and outputs");
+  if (in_features > (1 << 30) || x_row_stride > INT64_MAX / 4 / rows)
+    return fail(QSA_ERR_UNSUPPORTED, std::string(name) + ": at most 2^30 inputs, rows within 2^62");
   // 16-byte loads of whole rows, whose offsets within a block fit 32 bits.
   const bool vec = aligned(x, 16) && x_row_stride % 8 == 0 && in_features % 8 == 0 &&
                    x_row_stride < (1 << 24);

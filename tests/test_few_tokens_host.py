@@ -128,6 +128,10 @@ def test_int4_linear_refuses():
     assert f(*_int4_args(x=(1 << 20) + 1)) == -1
     assert f(*_int4_args(ys=32)) == -1 and b"overlap" in lib.qsa_last_error()
     assert f(*_int4_args(rows=1 << 30, n=1 << 24, ys=1 << 24)) == -2
+    assert f(*_int4_args(rows=2**31 - 1, n=64)) == -2
+    # more threads than a launch holds, offsets past 64 bits, a width past 2^30
+    assert f(*_int4_args(rows=1 << 27, n=16, xs=256)) == -2
+    assert f(*_int4_args(xs=2**61)) == -2 and f(*_int4_args(k=2**30 + 1)) == -2
 
 
 def _tree_args(**over):

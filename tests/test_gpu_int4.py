@@ -138,6 +138,25 @@ def test_strides_alignment_and_out():
     assert int4_linear(x3[:, :0].to(DEV), w).shape == (2, 0, n)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_rows_far_apart(dtype):
+    """Offsets of a block's rows past 32 bits, taken element by element (an odd
+    distance) or not (a distance that 32 bits do not hold)."""
+    if torch.cuda.mem_get_info()[0] < (30 << 30):
+        pytest.skip("needs 30 GiB")
+    gen = torch.Generator().manual_seed(12)
+    codes, scales, z = _weight(gen, 40, 200, 64, dtype, True)
+    w = int4_pack(codes.to(DEV), scales.to(DEV), z.to(DEV), group_size=64)
+    x = torch.randn(20, 200, generator=gen).to(dtype)
+    for far in ((1 << 29) + 1, 1 << 29):
+        store = torch.empty(19 * far + 200, dtype=dtype, device=DEV)
+        view = store.as_strided((20, 200), (far, 1))
+        view.copy_(x)
+        for rows in (1, 16, 20):
+            _check(int4_linear(view[:rows], w), _want(x[:rows], codes, scales, z, 64))
+        del store, view
+
+
 def test_rows_do_not_touch_each_other():
     """A row of NaN or infinities leaves the others' bits alone, and a row's bits
     do not depend on its place or on what is past the last row."""
