@@ -234,7 +234,7 @@ __global__ __launch_bounds__(kThreads) void logits_kernel(LogitsArgs a) {
       int node0 = 0, all_nodes = 0;
       if (penalise && a.ancestors) {
         node0 = max(load_uniform(a.query_start_loc + req), 0);
-        const int end = min(load_uniform(a.query_start_loc + req + 1), a.rows);
+        const int end = max(min(load_uniform(a.query_start_loc + req + 1), a.rows), 0);
         all_nodes = min(end - node0, 32 * a.words);
       }
       auto draft = [&](int j) {
@@ -485,7 +485,8 @@ extern "C" int qsa_process_logits(
   a.chunk = (int)(((vocab + chunks - 1) / chunks + 31) / 32 * 32);  // whole mask words
   a.chunks = (vocab - 1) / a.chunk + 1;
   const int64_t grid = (int64_t)a.chunks * groups;
-  if (grid > INT_MAX) return fail(QSA_ERR_UNSUPPORTED, name + ": too many rows");
+  if (grid > UINT_MAX / kThreads)  // what a launch holds
+    return fail(QSA_ERR_UNSUPPORTED, name + ": too many rows");
   const bool vec = ((uintptr_t)logits & 3u) == 0 && logits_row_stride * item % 4 == 0 &&
                    ((uintptr_t)out & 15u) == 0 && out_row_stride % 4 == 0;
   hipStream_t s = static_cast<hipStream_t>(stream);

@@ -917,18 +917,23 @@ void process_logits_impl(const Tensor& logits, const Tensor& out, const OptTenso
   own_rows(out, "out");
   QSA_REQUIRE(out.size(0) == rows && out.size(1) == vocab, "out must have the shape of logits");
   QSA_REQUIRE(vocab_start >= 0 && vocab_start <= INT32_MAX, "vocab_start is out of range");
-  // The requests: as many as the shortest of the tensors that have one each.
+  // The requests: as many as the rules have (one number for all of them), or as
+  // query_start_loc counts if that is fewer.
   int64_t num_requests = -1;
-  auto shortest = [&](const OptTensor& t, int64_t less) {
-    if (!t || t->dim() == 0) return;
-    const int64_t n = t->size(0) - less;
-    num_requests = num_requests < 0 ? n : std::min(num_requests, n);
-  };
   for (const OptTensor* t : {&history, &history_lens, &prompt_lens, &repetition, &frequency,
-                             &presence, &bias_ids, &bias_values})
-    shortest(*t, 0);
-  if (query_start_loc) QSA_REQUIRE(query_start_loc->numel() >= 1, "query_start_loc is empty");
-  shortest(query_start_loc, 1);
+                             &presence, &bias_ids, &bias_values}) {
+    if (!*t) continue;
+    const int64_t n = (*t)->dim() ? (*t)->size(0) : 0;
+    QSA_REQUIRE(num_requests < 0 || n == num_requests,
+                "the rules must have one entry a request, all of them as many: ", n, " and ",
+                num_requests);
+    num_requests = n;
+  }
+  if (query_start_loc) {
+    QSA_REQUIRE(query_start_loc->numel() >= 1, "query_start_loc is empty");
+    const int64_t n = query_start_loc->numel() - 1;
+    num_requests = num_requests < 0 ? n : std::min(num_requests, n);
+  }
   if (num_requests < 0) num_requests = rows;
   if (token_to_req) vec(*token_to_req, at::kInt, "token_to_req", rows);
   else QSA_REQUIRE(num_requests >= rows, "without token_to_req every row is a request: ", rows,

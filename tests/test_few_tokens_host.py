@@ -155,10 +155,6 @@ def test_tree_attention_refuses():
     assert f(*_tree_args(rows=-1)) == -1 and f(*_tree_args(mc=-1)) == -1
     assert f(*_tree_args(q=(1 << 20) + 8)) == -1 and f(*_tree_args(kt=516)) == -1
     assert f(*_tree_args(outr=2047)) == -1
-    for name in ("q", "k", "v", "table", "ctx", "qsl", "anc", "out"):
-        assert f(*_tree_args(**{name: None})) == -1, name
-    need = lib.qsa_tree_attention_workspace_bytes(8, 2, 16, 2, 128, 4, 60000)
-    assert need > 0
     # 64 GiB of cache from the first row to the last is too far apart, a page
     # table and a batch whose stages pass 31 bits too much
     assert f(*_tree_args(kb=2**32, blocks=10)) == -2 and b"64 GiB" in lib.qsa_last_error()
@@ -166,6 +162,10 @@ def test_tree_attention_refuses():
     assert f(*_tree_args(kt=2**62)) == -2
     assert f(*_tree_args(nreq=1 << 20, tw=1 << 20, rows=1 << 20, mq=1)) == -2
     assert f(*_tree_args(nreq=1, rows=2**31 - 1, mq=2**31 - 1)) == -2
+    for name in ("q", "k", "v", "table", "ctx", "qsl", "anc", "out"):
+        assert f(*_tree_args(**{name: None})) == -1, name
+    need = lib.qsa_tree_attention_workspace_bytes(8, 2, 16, 2, 128, 4, 60000)
+    assert need > 0
     assert f(*_tree_args(mc=60000)) == -4 and b"workspace" in lib.qsa_last_error()
     assert f(*_tree_args(mc=60000, ws=1 << 28, wsb=need - 1)) == -4
     assert f(*_tree_args(mc=60000, ws=(1 << 28) + 4, wsb=need)) == -4
@@ -203,6 +203,10 @@ def test_process_logits_refuses():
     assert f(*_logits_args(nb=3)) == -1
     assert f(*_logits_args(nb=1 << 20, bids=1 << 23, bvals=1 << 24)) == -2
     assert f(*_logits_args(anc=1 << 23)) == -1
+    assert f(*_logits_args(anc=1 << 23, words=33, draft=1 << 24, qsl=1 << 25)) == -2
+    assert f(*_logits_args(nb=1025, bids=1 << 23, bvals=1 << 24)) == -2
+    assert f(*_logits_args(first=2**31 - 1000, vocab=1000)) == -1
+    assert f(*_logits_args(rows=2**31 - 1)) == -2 and f(*_logits_args(rows=1 << 24, vocab=1)) == -2
     assert f(*_logits_args(x=(1 << 20) + 1)) == -1 and f(*_logits_args(out=(1 << 22) + 2)) == -1
 
 

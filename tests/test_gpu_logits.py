@@ -189,6 +189,61 @@ def test_lengths_out_of_range_are_kept_inside():
     _check(_run(logits, rules), _want(logits, rules))
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_histories_past_16_bits(dtype):
+    """A token said more often than 16 bits count, beside ordinary ones, in the
+    first, a middle and the last chunk of a vocabulary."""
+    gen = torch.Generator().manual_seed(8)
+    vocab, width = 45001, 70000
+    rules = _rules(gen, 3, vocab, width, 5)
+    rules["history_lens"] = torch.tensor([width, 66001, 300], dtype=torch.int32)
+    rules["prompt_lens"] = torch.tensor([0, 1, 400], dtype=torch.int32)
+    rules["history"][0, :65537] = vocab - 1
+    rules["history"][1, :66000] = 20000
+    rules["frequency"] = torch.tensor([2.0 ** -10, 0.5, 1.0])
+    logits = (torch.randn(3, vocab, generator=gen) * 4).to(dtype)
+    got = _run(logits, rules)
+    _check(got, _want(logits, rules))
+    narrow = {**rules, "history": rules["history"][:, :65535].contiguous()}
+    _check(_run(logits, narrow), _want(logits, narrow))
+
+
+def test_the_most_nodes_and_biases():
+    """1024 of each on a request, many of them on the same few tokens."""
+    gen = torch.Generator().manual_seed(9)
+    nodes, vocab = [1024, 700], 500
+    qsl = torch.tensor([0, 1024, 1724], dtype=torch.int32)
+    parents = torch.tensor([j - 1 - int(torch.randint(0, 3, (1,), generator=gen)) for t in nodes
+                            for j in range(t)])
+    anc = tree_ancestors(parents, qsl, 1024)
+    rows = torch.tensor([0, 5, 511, 512, 1023, 1024, 1024 + 513, 1723])
+    rules = _rules(gen, 2, vocab, 40, 1024)
+    draft = torch.randint(-3, vocab + 3, (1724,), generator=gen).to(torch.int32)
+    req = torch.repeat_interleave(torch.arange(2, dtype=torch.int32), torch.tensor(nodes))
+    logits = torch.randn(1724, vocab, generator=gen)
+    got = _run(logits, rules, token_to_req=req, draft_tokens=draft, ancestors=anc,
+               query_start_loc=qsl)
+    y, tol = _want(logits[rows], rules, req[rows], None, draft, anc[rows], qsl)
+    assert ((got.cpu()[rows].double() - y).abs() <= tol).all()
+
+
+def test_query_starts_out_of_range_are_kept_inside():
+    gen = torch.Generator().manual_seed(10)
+    rules = _rules(gen, 2, 90, 10, 0)
+    logits = torch.randn(4, 90, generator=gen)
+    kw = dict(token_to_req=torch.tensor([0, 0, 1, 1], dtype=torch.int32),
+              draft_tokens=torch.arange(4, dtype=torch.int32),
+              ancestors=torch.full((4, 2), -1, dtype=torch.int32))
+    for qsl in ([-2**31, 2, 2**31 - 1], [4, -2**31, 4], [2**31 - 1, 2, -2**31], [0, 2, 100]):
+        got = _run(logits, rules, query_start_loc=torch.tensor(qsl).to(torch.int32), **kw)
+        for b in range(2):   # each request by its own two entries
+            s, e = max(qsl[b], 0), max(min(qsl[b + 1], 4), 0)
+            mine = torch.tensor([s, max(e, s)] if b == 0 else [0, s, max(e, s)])
+            y, tol = _want(logits[2 * b:2 * b + 2], rules, kw["token_to_req"][2 * b:2 * b + 2],
+                           None, kw["draft_tokens"], kw["ancestors"], mine)
+            assert ((got.cpu()[2 * b:2 * b + 2].double() - y).abs() <= tol).all()
+
+
 @pytest.mark.parametrize("nodes", [[1], [5, 0, 9], [33, 64, 2], [70]])
 def test_drafted_nodes_count_their_ancestors(nodes):
     gen = torch.Generator().manual_seed(sum(nodes))
@@ -277,6 +332,8 @@ def test_refusals():
                       (dict(allowed=i32(3, 3)), "allowed"), (dict(allowed=i32(2, 4)), "allowed"),
                       (dict(ancestors=i32(3, 1)), "go together"),
                       (dict(token_to_req=i32(2)), "token_to_req"),
+                      (dict(frequency=f32(3), presence=f32(4)), "as many"),
+                      (dict(history=i32(4, 5), history_lens=i32(3)), "as many"),
                       (dict(vocab_start=-1), "vocab_start"),
                       (dict(out=f32(3, 99)), "shape of logits"),
                       (dict(out=f32(3, 100).half()), "out"),
