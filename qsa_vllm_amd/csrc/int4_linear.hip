@@ -49,21 +49,8 @@ constexpr int kTileN = 16;
 constexpr int kTileK = 128;
 constexpr int kCUs = 256;  // compute units of an MI355X
 
-// s_waitcnt immediate (gfx9 encoding): at most n vector-memory operations in
-// flight, no LDS operation.
-constexpr int loads_left(int n) { return (n & 15) | (7 << 4) | ((n >> 4) << 14); }
-
-// Barrier after the wave's LDS reads and all but its last N loads. (A fence
-// would wait for those too.)
-template <int N>
-__device__ __forceinline__ void stage_barrier() {
-  asm volatile("" ::: "memory");
-  __builtin_amdgcn_sched_barrier(0);
-  __builtin_amdgcn_s_waitcnt(loads_left(N));
-  __builtin_amdgcn_s_barrier();
-  __builtin_amdgcn_sched_barrier(0);
-  asm volatile("" ::: "memory");
-}
+// s_waitcnt immediate (gfx9 encoding): no vector-memory, no LDS operation in flight.
+constexpr int kMemoryDone = 7 << 4;
 
 struct Int4Args {
   const uint16_t* x;
@@ -362,11 +349,11 @@ __global__ __launch_bounds__(512) void int4_linear_kernel(Int4Args a) {
 
 // More than 16 rows: a workgroup of WN x WK waves takes 16 MT rows and 16 NT WN
 // outputs, wave (wn, wk) NT n tiles and one of every WK k tiles. A step's
-// activations (WK tiles of 16 MT rows x 256 bytes) go straight into LDS, AHEAD
-// steps before they are used, in a ring of AHEAD + 1 buffers; weights as far
-// ahead in registers. Unit u (16 bytes) of a row sits at place u ^ (row mod 16),
+// activations (WK tiles of 16 MT rows x 256 bytes) go straight into LDS one step
+// before they are used, into the other of two buffers; its weights into registers
+// (two and three steps ahead measured the same). Unit u (16 bytes) of a row sits at place u ^ (row mod 16),
 // so that the A operand's reads (16 rows' same unit) lie in different banks.
-template <typename T, int GROUP, bool ZEROS, int MT, int NT, int WN, int WK, int AHEAD>
+template <typename T, int GROUP, bool ZEROS, int MT, int NT, int WN, int WK>
 __global__ __launch_bounds__(64 * WN * WK) __attribute__((amdgpu_waves_per_eu(MT > 2 ? 2 : 4))) void
 int4_rows_kernel(Int4Args a) {
   typedef Tiles<GROUP, ZEROS, NT> Weights;
@@ -374,8 +361,7 @@ int4_rows_kernel(Int4Args a) {
   constexpr int kTileBytes = 16 * MT * 256;
   constexpr int kStageBytes = WK * kTileBytes;
   constexpr int kBlocks = WK * 16 * MT / 4;  // 4 rows of 256 bytes an instruction
-  constexpr int kOps = kBlocks / kWaves + NT * (ZEROS ? 3 : 2);  // a step's loads of a wave
-  static_assert(kBlocks % kWaves == 0 && (AHEAD - 1) * kOps < 64, "");
+  static_assert(kBlocks % kWaves == 0, "");
   extern __shared__ __attribute__((aligned(16))) char lds[];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -401,7 +387,7 @@ int4_rows_kernel(Int4Args a) {
     at[i] = (uint32_t)min(row, a.rows - 1 - row0) * (uint32_t)(2 * a.x_row) +
             (uint32_t)(n ^ (row & 15)) * 16;
   }
-  // Loads past the last step repeat it: the number of loads in flight is fixed.
+  // Loads past the last step repeat it: none depends on a condition.
   auto load_step = [&](int step, char* stage, Weights& b) {
     const int s = min(step, steps - 1);
     auto move = [&](int i, const char* src) {
@@ -426,18 +412,17 @@ int4_rows_kernel(Int4Args a) {
   };
 
   f32x4 acc[MT][NT] = {};
-  Weights b[AHEAD + 1];
+  Weights b[2];
+  load_step(0, lds, b[0]);
+  for (int step = 0;; step += 2) {
 #pragma unroll
-  for (int i = 0; i < AHEAD; ++i) load_step(i, lds + i * kStageBytes, b[i]);
-  for (int step = 0;; step += AHEAD + 1) {
-#pragma unroll
-    for (int i = 0; i <= AHEAD; ++i) {
+    for (int i = 0; i < 2; ++i) {
       if (step + i >= steps) goto done;
       // This step's loads are done, and the buffer that the next loads go to
       // has been read by all.
-      stage_barrier<(AHEAD - 1) * kOps>();
-      load_step(step + i + AHEAD, lds + (i + AHEAD) % (AHEAD + 1) * kStageBytes,
-                b[(i + AHEAD) % (AHEAD + 1)]);
+      __builtin_amdgcn_s_waitcnt(kMemoryDone);
+      __syncthreads();
+      load_step(step + i + 1, lds + (1 - i) * kStageBytes, b[1 - i]);
       if ((step + i) * WK + wk >= a.k_tiles) continue;
       const char* const tile = lds + i * kStageBytes + wk * kTileBytes;
       u32x4 x[MT][4];
@@ -450,7 +435,7 @@ int4_rows_kernel(Int4Args a) {
     }
   }
 done:
-  __builtin_amdgcn_s_waitcnt(loads_left(0));  // no load into LDS outlives the wave
+  __builtin_amdgcn_s_waitcnt(kMemoryDone);  // no load into LDS outlives the wave
 
   if constexpr (WK > 1) {
     f32x4* const part = reinterpret_cast<f32x4*>(lds);  // [WK][WN][MT * NT][64]
@@ -491,16 +476,12 @@ hipError_t launch_few(Int4Args a, int waves, hipStream_t stream) {
   return hipGetLastError();
 }
 
-template <typename T, int GROUP, bool ZEROS, int MT, int NT, int WN, int WK, int AHEAD>
+template <typename T, int GROUP, bool ZEROS, int MT, int NT, int WN, int WK>
 hipError_t launch_many(Int4Args a, hipStream_t stream) {
-  constexpr size_t kLds = std::max<size_t>((size_t)(AHEAD + 1) * WK * 16 * MT * 256,
+  constexpr size_t kLds = std::max<size_t>((size_t)2 * WK * 16 * MT * 256,
                                            WK > 1 ? (size_t)WK * WN * MT * NT * 1024 : 0);
-  auto* kernel = &int4_rows_kernel<T, GROUP, ZEROS, MT, NT, WN, WK, AHEAD>;
-  if (kLds > 65536) {
-    const hipError_t err = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
-                                               hipFuncAttributeMaxDynamicSharedMemorySize, (int)kLds);
-    if (err != hipSuccess) return err;
-  }
+  static_assert(kLds <= 65536, "two workgroups a CU, and no attribute to set");
+  auto* kernel = &int4_rows_kernel<T, GROUP, ZEROS, MT, NT, WN, WK>;
   a.row_blocks = (a.rows + 16 * MT - 1) / (16 * MT);
   const int64_t n_blocks = (a.n_tiles + NT * WN - 1) / (NT * WN);
   hipLaunchKernelGGL(kernel, dim3((unsigned)((n_blocks + 7) / 8 * 8 * a.row_blocks)),
@@ -556,11 +537,11 @@ hipError_t launch_rows(const Int4Args& a, bool vec, hipStream_t stream) {
     return a.n_tiles < 384 ? launch_few<T, GROUP, ZEROS, 1, 1, true>(a, 8, stream)
                            : launch_few<T, GROUP, ZEROS, 1, 4, true>(a, 4, stream);
   switch (pick_rows_shape(a.rows, a.n_tiles)) {
-    case k32x32: return launch_many<T, GROUP, ZEROS, 2, 1, 2, 4, 1>(a, stream);
-    case k32x64: return launch_many<T, GROUP, ZEROS, 2, 2, 2, 4, 1>(a, stream);
-    case k32x96: return launch_many<T, GROUP, ZEROS, 2, 3, 2, 4, 1>(a, stream);
-    case k64x128: return launch_many<T, GROUP, ZEROS, 4, 2, 4, 1, 1>(a, stream);
-    default: return launch_many<T, GROUP, ZEROS, 4, 3, 4, 1, 1>(a, stream);
+    case k32x32: return launch_many<T, GROUP, ZEROS, 2, 1, 2, 4>(a, stream);
+    case k32x64: return launch_many<T, GROUP, ZEROS, 2, 2, 2, 4>(a, stream);
+    case k32x96: return launch_many<T, GROUP, ZEROS, 2, 3, 2, 4>(a, stream);
+    case k64x128: return launch_many<T, GROUP, ZEROS, 4, 2, 4, 1>(a, stream);
+    default: return launch_many<T, GROUP, ZEROS, 4, 3, 4, 1>(a, stream);
   }
 }
 
