@@ -139,11 +139,29 @@ __device__ __forceinline__ int sum_requests(const TreeArgs& a, F fn) {
 __device__ __forceinline__ int line_length(const TreeArgs& a, int tile) {
   return sum_requests(a, [&](int, const Request& r) { return stages_on(a, r, tile); });
 }
-// Stages of a stretch.
+// Stages of a stretch: as few as keep all workgroups on the card at once. A
+// workgroup beyond the 64 that an XCD's CUs hold would run after all the others, so
+// the lines' numbers, rounded up to 8, must add up to no more than 512. (One too
+// many on one XCD: 24 trees of 1 - 40 nodes on 2048 - 30000 tokens 249 us, else 192.)
 __device__ __forceinline__ int stretch(const TreeArgs& a) {
-  const int all = sum_requests(
-      a, [&](int, const Request& r) { return tiles_of(a, r) * a.kv_heads * stages_of(r); });
-  return max(1u, (unsigned)(all + a.workgroups - 1) / (unsigned)a.workgroups);
+  int lines = 0;
+  const int all = sum_requests(a, [&](int, const Request& r) {
+    lines = max(lines, tiles_of(a, r));
+    return tiles_of(a, r) * a.kv_heads * stages_of(r);
+  });
+  unsigned n = a.workgroups;
+  if (n == 2 * kCUs) {
+    if (a.requests == 1) {  // lines of one length
+      lines = uniform(lines);
+      if (lines <= n / 8) n = lines * (n / (unsigned)max(lines, 1) / 8 * 8);
+    } else {
+#pragma unroll
+      for (int w = 32; w > 0; w /= 2) lines = max(lines, __shfl_xor(lines, w, 64));
+      lines = uniform(lines);
+      if (lines <= 8) n -= 8 * (max(lines, 1) - 1);
+    }
+  }
+  return max(1u, (all + n - 1) / max(n, 1u));
 }
 // Workgroups of a line, rounded up so that the next line starts at the first XCD.
 __device__ __forceinline__ int line_workgroups(int length, int mine) {
