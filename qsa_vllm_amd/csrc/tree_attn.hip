@@ -12,17 +12,19 @@
 //
 // Unlike the sparse attention, where each row gathers its own slots, the rows
 // of a request share their K/V: a workgroup takes a tile of (node, head) rows
-// of one kv head and streams a chunk of the request's tokens through LDS once
-// for all of them.
+// of one kv head and streams a stretch of the request's tokens through LDS once
+// for all of them, 64 a stage.
 //
 //   S^T[token][row] = K (A, 16 tokens x 32 dims) Q^T (B, 32 dims x 16 rows)
 //   O^T[dim][row]  += V^T (A, 16 dims x 32 tokens) P^T (B, 32 tokens x 16 rows)
 //
-// on mfma_f32_16x16x32_bf16. P^T is the lane's own exponentials (rounded to
-// bf16, the matrix cores' type, as in the sparse attention: 2^-9 of a weight at
-// most, of random sign; their sum is taken in fp32 before rounding), so
-// it never leaves registers; V^T comes from row-major V rows in LDS by the
-// transposing LDS read.
+// on mfma_f32_16x16x32_bf16. P^T is the lane's own exponentials, so it never
+// leaves registers; V^T comes from row-major V rows in LDS by the transposing LDS
+// read. The exponentials are rounded to bf16, the matrix cores' type (2^-8 of a
+// weight at most), and the row's sum is the product of the rounded ones with 1s,
+// in fp32: the weights that meet V add up to 1. They are taken from a base that
+// follows the row's maximum only when that has passed it by 2^8, so that most
+// stages rescale nothing.
 //
 // Rows and tokens are shared out over the four waves as WM x WT: with many rows
 // each wave has its own 16 NB rows and all tokens of a stage, with few rows the
@@ -32,10 +34,20 @@
 // request's stages, lie end to end on that tile's line, and every workgroup takes
 // an equal stretch of a line, two workgroups a CU in all. Workgroups at the same
 // place of different tiles' lines run on one XCD, whose L2 then serves the K/V to
-// all but the first. Lengths and rows are known on the device only; each
+// all but the first. (Splits of the context by a rule on the launch's sizes, one
+// workgroup each, took 234 us where the stretches take 177: 32 trees of 5 - 24
+// nodes on 4096 - 32768 tokens, at the time.) Lengths and rows are known on the device only; each
 // workgroup adds them up itself. A unit that no one stretch covers leaves
 // normalised fp32 pieces and log2 sums, which a second kernel joins in order; the
 // others are written at once.
+//
+// What bounds it (16 query and 2 kv heads of 128, pages of 16): single tokens and
+// small trees read HBM (64 single tokens on 1024 - 8192 tokens 69 us, 4.3 TB/s of
+// K/V; a large copy 4.8); 32 trees of 5 - 24 nodes on 4096 - 32768 tokens, 172 us,
+// HBM and their second tiles' passes over the same K/V (requests past 16 nodes);
+// 64 nodes on 131072 tokens, 102 us, the matrix cores with the softmax between
+// them (0.67 PFLOP/s; 1.4 in a large library product). One request of 8 nodes on
+// 500 tokens, 14.5 us, is two launches' chains of loads.
 #include "qsa_common.h"
 #include "../../include/qsa_hip.h"
 
@@ -694,7 +706,8 @@ tree_attn_kernel(TreeArgs a) {
 // Joins a row's pieces: out = sum_s 2^(lse_s - max) part_s / sum_s 2^(lse_s - max).
 // D / 4 lanes hold a (row, head)'s dims; WAYS such groups take its pieces in
 // turn (s mod WAYS) and add up in group order, so that a long context's many
-// pieces are read side by side. Bound by reading them.
+// pieces are read side by side. Bound by reading them: 33 MB in 10 us (64 nodes on
+// 131072 tokens).
 template <int D, int WAYS>
 __global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs a, int row_tiles) {
   constexpr int kLanes = D / 4;
@@ -706,30 +719,44 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs a, int row_til
   const Request rq = uniform_request(a, request);
   const int64_t first_item = (int64_t)(blockIdx.x % row_tiles) * kPer;
   if (first_item >= (int64_t)rq.nodes * a.num_q_heads) return;
+  const int stages = stages_of(rq);
+  // Where the rows' units lie on their tiles' lines, and the first workgroup of each
+  // line: found by one wave for all (the sums over the requests by every wave are
+  // most of the launch's instructions). Lane i takes (row, head) i mod kPer.
+  __shared__ int begin_lds[kPer], id0_lds[kPer], mine_lds;
+  if (threadIdx.x < 64) {
+    const int64_t item = first_item + threadIdx.x % kPer;
+    const int node = (int)(item / a.num_q_heads);
+    const int head = (int)(item - (int64_t)node * a.num_q_heads);
+    const int kv = head / a.group, my_tile = (node * a.group + head - kv * a.group) / kTileRows;
+    const int mine = stretch(a);
+    int begin = 0, id0 = 0, ids = 0;
+    for (int tile = 0; tile < tiles_of(a, rq); ++tile) {
+      const int before = sum_requests(a, [&](int b, const Request& r) {
+        return b < request ? stages_on(a, r, tile) : 0;
+      });
+      if (tile == my_tile) {
+        begin = before + kv * stages;
+        id0 = ids;
+      }
+      if (tile + 1 < tiles_of(a, rq)) ids += line_workgroups(line_length(a, tile), mine);
+    }
+    if (threadIdx.x < kPer) {
+      begin_lds[threadIdx.x] = begin;
+      id0_lds[threadIdx.x] = id0;
+    }
+    if (threadIdx.x == 0) mine_lds = mine;
+  }
+  __syncthreads();
   const int lane = threadIdx.x % kLanes, grp = threadIdx.x / kLanes;
   const int way = grp % WAYS;
   const int64_t item = first_item + grp / WAYS;
   const int node = (int)(item / a.num_q_heads);
   const int head = (int)(item - (int64_t)node * a.num_q_heads);
-  const int kv = head / a.group;
-  const int m = node * a.group + head - kv * a.group;
-  const int stages = stages_of(rq);
-  // Where the unit lies on its tile's line, and the workgroups whose stretches it
-  // meets: the first one's piece is its second, the others' their first. A
-  // workgroup's rows may be of several tiles; all lanes go through all of them.
-  const int mine = stretch(a);
-  const int my_tile = m / kTileRows;
-  int begin = 0, id0 = 0, ids = 0;
-  for (int tile = 0; tile < tiles_of(a, rq); ++tile) {
-    const int before = sum_requests(a, [&](int b, const Request& r) {
-      return b < request ? stages_on(a, r, tile) : 0;
-    });
-    if (tile == my_tile) {
-      begin = before + kv * stages;
-      id0 = ids;
-    }
-    if (tile + 1 < tiles_of(a, rq)) ids += line_workgroups(line_length(a, tile), mine);
-  }
+  const int m = node * a.group + head - head / a.group * a.group;
+  // The workgroups whose stretches the unit meets: the first one's piece is its
+  // second, the others' their first.
+  const int mine = mine_lds, begin = begin_lds[grp / WAYS], id0 = id0_lds[grp / WAYS];
   const int w0 = (unsigned)begin / (unsigned)mine;
   const int pieces = (unsigned)(begin + stages - 1) / (unsigned)mine - w0 + 1;
   // One piece: the attention has written the row.
@@ -823,10 +850,12 @@ hipError_t launch_tree(const TreeArgs& a, const TreePlan& plan, int max_nodes, h
   hipLaunchKernelGGL((tree_attn_kernel<D>), dim3(grid), dim3(64 * kWaves), kLds, stream, a);
   const hipError_t err = hipGetLastError();
   if (err != hipSuccess || !a.workgroups) return err;
-  // Many (row, head)s have few pieces each.
+  // Many (row, head)s have few pieces each and need no more workgroups. (WAYS 8 / 4
+  // / 2 / 1: 32 trees of 5 - 24 nodes 191 / 182 / 181 / 173 us in all, 64 nodes on
+  // 131072 tokens 101 / 103 / 103 / 106.)
   const int64_t pairs = (int64_t)max_nodes * a.num_q_heads;
   return pairs * a.requests <= 4096 ? launch_merge<D, 8>(a, pairs, stream)
-                                    : launch_merge<D, 2>(a, pairs, stream);
+                                    : launch_merge<D, 1>(a, pairs, stream);
 }
 
 // Elements from a cache's first token row to its last, -1 if a stride is negative

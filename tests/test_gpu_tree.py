@@ -1,7 +1,8 @@
 """Tree attention on the GPU against a 64-bit statement of it, row by row.
 
-Tolerance. Each weight is rounded to bf16 (2^-8 of it at most) before it meets V,
-so a result is off by at most 2^-8 sum p |v|; a score's fp32 sum of D products
+Tolerance. Each weight is rounded to bf16, p (1 + e) with |e| <= 2^-8, before it
+meets V, and the rounded weights are what is summed: the weighted mean o moves by
+sum p e (v - o) / sum p (1 + e), at most 2^-8 (1 + 2^-7) sum p |v - o|; a score's fp32 sum of D products
 passes at most 36 roundings of 2^-24 on sum |q k|, scaled by D^-0.5, which moves
 a weight by as much (numerator and sum: twice); the fp32 exponentials and sums
 stay under 2^-19 of a weight. The gate's factor is at most 1 and off by 2^-20.
@@ -95,13 +96,15 @@ class Case:
                     score = k @ q / math.sqrt(self.dim)
                     p = torch.softmax(score, 0)
                     spread = (k.abs() @ q.abs()).max().item() / math.sqrt(self.dim)
-                    rel = 2 ** -8 + 2 * 36 * 2 ** -24 * spread + 2 ** -18
-                    o, mass = p @ v, p @ v.abs()
+                    o = p @ v
+                    off = (2 ** -8 * (1 + 2 ** -7) * (p @ (v - o).abs()) +
+                           (2 * 36 * 2 ** -24 * spread + 2 ** -18) * (p @ v.abs()))
                     if self.gate is not None:
                         s = torch.sigmoid(self.gate[r, h].double())
-                        o, mass = o * s, mass * s
+                        off = off * s + 2 ** -20 * (o * s).abs()
+                        o = o * s
                     out[r, h] = o
-                    tol[r, h] = rel * mass + 2 ** -8 * (o.abs() + rel * mass) + 2 ** -100
+                    tol[r, h] = off + 2 ** -8 * (o.abs() + off) + 2 ** -100
         return out, tol
 
     def check(self, got, **kw):
