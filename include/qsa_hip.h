@@ -502,8 +502,8 @@ int qsa_gdn_gated_norm(const void* o, const void* qkvz, int64_t qkvz_stride, con
  *          inputs past in_features hold their zero point.
  * group_size 32, 64 or 128. bias may be null. A row of x that holds an infinity
  * or NaN (or, in bf16, values past 2^112) has no defined result; other rows are
- * not touched by it. Any alignment and row stride; 16-byte aligned rows and
- * in_features a multiple of 8 are fastest. */
+ * not touched by it. Any alignment and row stride of x and y; 16-byte aligned rows
+ * of x and in_features a multiple of 8 are fastest. At most 2^30 inputs. */
 int qsa_int4_linear(const void* x, int64_t x_row_stride, const void* codes, const void* scales,
                     const void* zeros, const void* bias, void* y, int64_t y_row_stride, int rows,
                     int out_features, int in_features, int group_size, int is_fp16, void* stream);
@@ -518,8 +518,11 @@ int qsa_int4_linear(const void* x, int64_t x_row_stride, const void* codes, cons
  * are not seen, nor are positions without a page in the cache. out = softmax of
  * the scaled scores times V, times sigmoid(gate) if gate is given, rounded once
  * to bf16; zeros for a row that sees nothing. Rows of no request are not written.
+ * K or V that is not finite makes what sees it NaN (or infinite) and nothing else.
  * max_query_len bounds a request's nodes (further ones are not computed);
- * max_context_len should bound context_lens: it shapes the launch only.
+ * max_context_len should bound context_lens: it shapes the launch only. q and the
+ * caches are 16-byte aligned with strides of multiples of 8 elements; a cache
+ * spans less than 64 GiB from its first row to its last.
  * head_dim 64 or 128. The workspace (0 bytes: none) holds the call's partial
  * results until its work is done: calls that may overlap need one each. */
 size_t qsa_tree_attention_workspace_bytes(int rows, int requests, int num_q_heads,

@@ -32,6 +32,11 @@
 //    that take different outputs (int4_rows_kernel).
 // Waves that share the inputs add their sums through LDS in wave order: no
 // atomics, the same bits every time.
+//
+// Measured (bf16, groups of 128 unless said): 1 row x 49536 x 4096 21.6 us, 4.85 TB/s
+// (a large copy 4.8); 61 rows x 11264 x 4096 12.5 us, bound by its few steps in
+// series; 250 rows x 22528 x 4096, groups of 64 with zero points, 65 us, 0.71
+// PFLOP/s: vector issue, unpacking for each block of 64 rows.
 #include "qsa_common.h"
 #include "../../include/qsa_hip.h"
 

@@ -72,8 +72,9 @@ def qsa_tree_paged_attention(
     at rows ``query_start_loc[b] ..``) over ``context_lens[b]`` committed tokens
     and the nodes that ``ancestors`` shows each row. Row order, caches, table and
     gate as in ``qsa_sparse_paged_attention``; the gated result is rounded once.
-    A row that sees nothing gets zeros; rows of no request (past
-    ``query_start_loc[-1]``) are not written. ``max_query_len`` must be at least
+    A row that sees nothing gets zeros, one that sees K or V that are not finite NaN
+    (or an infinity) there; rows of no request (past ``query_start_loc[-1]``) are
+    not written. The caches must span less than 64 GiB each. ``max_query_len`` must be at least
     every request's node count (further nodes are not computed);
     ``max_context_len`` should be at least every context length: it shapes the
     launch, not the result. Captured into a graph, both hold for its replays."""
