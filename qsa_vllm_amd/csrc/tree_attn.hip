@@ -35,16 +35,17 @@
 // an equal stretch of a line, two workgroups a CU in all. Workgroups at the same
 // place of different tiles' lines run on one XCD, whose L2 then serves the K/V to
 // all but the first. (Splits of the context by a rule on the launch's sizes, one
-// workgroup each, took 234 us where the stretches take 177: 32 trees of 5 - 24
-// nodes on 4096 - 32768 tokens, at the time.) Lengths and rows are known on the device only; each
+// workgroup each, took 234 us when the stretches took 177: 32 trees of 5 - 24 nodes
+// on 4096 - 32768 tokens.) Lengths and rows are known on the device only; each
 // workgroup adds them up itself. A unit that no one stretch covers leaves
 // normalised fp32 pieces and log2 sums, which a second kernel joins in order; the
 // others are written at once.
 //
 // What bounds it (16 query and 2 kv heads of 128, pages of 16): single tokens and
 // small trees read HBM (64 single tokens on 1024 - 8192 tokens 69 us, 4.3 TB/s of
-// K/V; a large copy 4.8); 32 trees of 5 - 24 nodes on 4096 - 32768 tokens, 172 us,
-// HBM and their second tiles' passes over the same K/V (requests past 16 nodes);
+// K/V; a large copy 4.8); 32 trees of 5 - 24 nodes on 4096 - 32768 tokens, 174 us,
+// a workgroup's stages in series (2.9 us each; the second tiles of requests past
+// 16 nodes add to them, though reading K/V once for both measured no faster);
 // 64 nodes on 131072 tokens, 102 us, the matrix cores with the softmax between
 // them (0.67 PFLOP/s; 1.4 in a large library product). One request of 8 nodes on
 // 500 tokens, 14.5 us, is two launches' chains of loads.
@@ -170,6 +171,7 @@ __device__ __forceinline__ int stretch(const TreeArgs& a) {
 #pragma unroll
       for (int w = 32; w > 0; w /= 2) lines = max(lines, __shfl_xor(lines, w, 64));
       lines = uniform(lines);
+      // (lines of unequal lengths; of more than 8 the rounding would cost too much)
       if (lines <= 8) n -= 8 * (max(lines, 1) - 1);
     }
   }
