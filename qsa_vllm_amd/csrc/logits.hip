@@ -28,8 +28,8 @@
 // A history is scanned once per chunk, so chunks are as large as LDS allows for
 // two workgroups a CU, unless there would be too few workgroups.
 //
-// Measured: 128 rows x 99072 fp32, histories of 512 - 32768 tokens, 37 us (3.0 TB/s
-// of the logits, results and masks); 8 x 61 drafted nodes x 49536 bf16 50 us (3.0
+// Measured: 128 rows x 99072 fp32, histories of 512 - 32768 tokens, 38 us (2.9 TB/s
+// of the logits, results and masks); 8 x 61 drafted nodes x 49536 bf16 51 us (2.9
 // TB/s); one row of 49536 6.5 us, the chain of loads before the stream. A history of
 // one repeated token serialises its LDS atomics: 128 such rows take 92 us.
 #include "qsa_common.h"

@@ -43,10 +43,10 @@
 //
 // What bounds it (16 query and 2 kv heads of 128, pages of 16): single tokens and
 // small trees read HBM (64 single tokens on 1024 - 8192 tokens 69 us, 4.3 TB/s of
-// K/V; a large copy 4.8); 32 trees of 5 - 24 nodes on 4096 - 32768 tokens, 174 us,
+// K/V; a large copy 4.8); 32 trees of 5 - 24 nodes on 4096 - 32768 tokens, 176 us,
 // a workgroup's stages in series (2.9 us each; the second tiles of requests past
 // 16 nodes add to them, though reading K/V once for both measured no faster);
-// 64 nodes on 131072 tokens, 102 us, the matrix cores with the softmax between
+// 64 nodes on 131072 tokens, 103 us, the matrix cores with the softmax between
 // them (0.67 PFLOP/s; 1.4 in a large library product). One request of 8 nodes on
 // 500 tokens, 14.5 us, is two launches' chains of loads.
 #include "qsa_common.h"
