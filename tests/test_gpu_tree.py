@@ -157,6 +157,16 @@ def test_ragged_batches(requests, most, longest, heads, kv_heads, dim):
     c.check(c.run())
 
 
+@pytest.mark.parametrize("ctx,nodes", [
+    ([2000], [150]),           # one request of 19 row tiles: lines of one length
+    ([300], [530]),            # of 67: more lines than workgroups in blocks of 8 hold
+    ([700, 1500, 90], [90, 20, 130]),   # lines of 17 lengths
+])
+def test_many_row_tiles(ctx, nodes):
+    c = Case(ctx, nodes, heads=16, kv_heads=1, dim=64, seed=sum(nodes))
+    c.check(c.run())
+
+
 def test_layouts_and_strides():
     c = Case([50, 200], [6, 3], heads=8, kv_heads=2, dim=64, layout="head_major", seed=8)
     c.check(c.run())
