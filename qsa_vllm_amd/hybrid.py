@@ -43,7 +43,7 @@ codes with group scales (``ops/int4.py``) instead of bf16 and multiply by
 
 from __future__ import annotations
 
-from dataclasses import dataclass, field
+from dataclasses import dataclass, field, replace
 
 import numpy as np
 import torch
@@ -419,7 +419,8 @@ class HybridDecodeGraph:
     buffers. ``columns`` pins the decode logits-width class during capture (0:
     the compressed page table's capacity). Capture runs the step once as a
     warm-up, which advances the caches and states like any step. ``rules``'
-    tensors are read anew on every replay."""
+    tensors are read anew on every replay: the graph keeps them, and what is
+    written into them counts. Tensors put in their place later do not."""
 
     def __init__(self, model: "HybridDecoder", batch: HybridBatch, columns: int = 0,
                  rules: LogitsRules | None = None):
@@ -428,6 +429,8 @@ class HybridDecodeGraph:
         self.num_tokens = batch.num_tokens
         self.columns = columns
         self.compress_ratio = model.cfg.compress_ratio
+        # The captured kernels hold the tensors' addresses only.
+        self.rules = rules = None if rules is None else replace(rules)
         side = torch.cuda.Stream()
         side.wait_stream(torch.cuda.current_stream())
         with capture_column_scope(columns), torch.cuda.stream(side):

@@ -2,12 +2,18 @@
 layout and rounding, ancestor bits against a walk up the tree, and what the C
 entry points refuse (no launch)."""
 
+import contextlib
+import gc
+import types
+import weakref
+
 import numpy as np
 import pytest
 import torch
 
 from qsa_vllm_amd import _lib
-from qsa_vllm_amd.ops import (int4_linear, int4_pack, int4_quantize, process_logits,
+from qsa_vllm_amd.hybrid import HybridDecodeGraph
+from qsa_vllm_amd.ops import (LogitsRules, int4_linear, int4_pack, int4_quantize, process_logits,
                               qsa_tree_paged_attention, tree_ancestors)
 
 
@@ -242,3 +248,32 @@ def test_python_layer_refuses():
         tree_ancestors(i32, i32, 0)
     with pytest.raises(RuntimeError, match="parents"):
         tree_ancestors(i32.float(), i32, 1)
+
+
+# --- a captured step keeps what its kernels read ---------------------------------
+
+def test_a_captured_step_keeps_its_rules(monkeypatch):
+    """The kernels of a graph hold addresses, not tensors: the rules' tensors
+    must live as long as the graph, also where the caller's object is dropped or
+    its fields get other tensors."""
+    stream = types.SimpleNamespace(wait_stream=lambda other: None)
+    for name, value in (("Stream", lambda: stream), ("current_stream", lambda: stream),
+                        ("stream", lambda s: contextlib.nullcontext()),
+                        ("synchronize", lambda: None), ("CUDAGraph", lambda: None),
+                        ("graph", lambda g: contextlib.nullcontext())):
+        monkeypatch.setattr(torch.cuda, name, value)
+    batch = types.SimpleNamespace(
+        num_tokens=2, qsa=types.SimpleNamespace(main=types.SimpleNamespace(max_query_len=1)))
+    model = types.SimpleNamespace(cfg=types.SimpleNamespace(compress_ratio=4),
+                                  forward=lambda batch, rules: torch.zeros(2, 8))
+    rules = LogitsRules(frequency=torch.ones(2), presence=torch.ones(2), vocab_start=8)
+    alive = [weakref.ref(rules.frequency), weakref.ref(rules.presence)]
+    graph = HybridDecodeGraph(model, batch, rules=rules)
+    rules.frequency = torch.zeros(2)
+    del rules
+    gc.collect()
+    assert all(ref() is not None for ref in alive)
+    del graph
+    gc.collect()
+    assert all(ref() is None for ref in alive)
+    assert HybridDecodeGraph(model, batch).rules is None

@@ -291,3 +291,26 @@ def test_decoder_applies_the_rules(bits):
 def test_weight_bits_are_checked():
     with pytest.raises(ValueError, match="weight_bits"):
         HybridConfig(weight_bits=8)
+
+
+def test_a_graph_of_passing_rules():
+    """The caller's rules are dropped after the capture and memory of their sizes
+    is allocated and filled anew: the replays apply the rules all the same."""
+    wl = _workload(weight_bits=4)
+    batch = wl.build_decode()
+    states = [t.clone() for t in wl.layer_states()]
+
+    def reset():
+        for t, s in zip(wl.layer_states(), states):
+            t.copy_(s)
+    want = wl.model.forward(batch, _rules(4, wl.cfg.vocab_shard)).clone()
+    reset()
+    graph = HybridDecodeGraph(wl.model, batch, rules=_rules(4, wl.cfg.vocab_shard))
+    over = [torch.zeros_like(t) for _ in range(8) for t in vars(_rules(4, wl.cfg.vocab_shard)).values()
+            if isinstance(t, torch.Tensor)]
+    for step in range(3):
+        reset()
+        got = graph.replay().clone()
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)
+    del over
