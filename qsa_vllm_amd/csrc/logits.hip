@@ -18,8 +18,8 @@
 //   1. it counts the request's history within the chunk in LDS, with LDS atomics
 //      (whole numbers: any order gives the same counts);
 //   2. it lists the chunk's special columns, those of biases and of drafted
-//      tokens, whose values differ by row or need a sum, and marks them in the
-//      table;
+//      tokens, whose values differ by row or need a sum, sorts the list by column
+//      and marks them in the table;
 //   3. it streams its rows, four vectors of a thread in flight, each logit by its
 //      count alone, and leaves the special columns;
 //   4. it computes those, one (row, column) a thread: the visible nodes' tokens
@@ -28,7 +28,7 @@
 // A history is scanned once per chunk, so chunks are as large as LDS allows for
 // two workgroups a CU, unless there would be too few workgroups.
 //
-// Measured: 128 rows x 99072 fp32, histories of 512 - 32768 tokens, 38 us (2.9 TB/s
+// Measured: 128 rows x 99072 fp32, histories of 512 - 32768 tokens, 35 us (2.9 TB/s
 // of the logits, results and masks); 8 x 61 drafted nodes x 49536 bf16 51 us (2.9
 // TB/s); one row of 49536 6.5 us, the chain of loads before the stream. A history of
 // one repeated token serialises its LDS atomics: 128 such rows take 92 us.
@@ -125,17 +125,20 @@ __device__ __forceinline__ float penalised(float x, bool seen, uint32_t spoken, 
   return x;
 }
 
-// Special columns of a chunk: entry e < nodes is drafted node `source`'s token,
-// the others are biases, in list order.
+// Special columns of a chunk. An entry is a column, whether it is a bias (else a
+// drafted node's token), and which of the request's. Sorted, a column's entries
+// lie side by side, its nodes first, then its biases in list order.
+constexpr int kMaxSpecials = kMaxNodes + kMaxBiases;
+constexpr uint32_t kBias = 0x8000u;
+static_assert(kMaxNodes <= kBias && kMaxBiases <= kBias && kMaxChunk <= 65536, "16 bits each");
 struct Specials {
-  uint16_t column[kMaxNodes + kMaxBiases];
-  uint16_t source[kMaxNodes + kMaxBiases];
+  __attribute__((aligned(16))) uint32_t entry[kMaxSpecials];
   int wave[kThreads / 64];
 };
 
 // Appends the threads' entries in thread order; returns the list's new length.
 __device__ __forceinline__ int append(Specials& list, int length, uint32_t column, uint32_t size,
-                                      int source) {
+                                      uint32_t source) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const bool take = column < size;
   const uint64_t mask = __ballot(take);
@@ -150,11 +153,48 @@ __device__ __forceinline__ int append(Specials& list, int length, uint32_t colum
   }
   if (take) {
     at += __popcll(mask & ((1ull << lane) - 1));
-    list.column[at] = (uint16_t)column;
-    list.source[at] = (uint16_t)source;
+    list.entry[at] = column << 16 | source;
   }
   __syncthreads();
   return length;
+}
+
+// Sorts the list: no two entries are alike, so an entry's place is how many are
+// smaller. Every thread compares its entries with all, 16 at a time from one
+// address for the whole wave. (A list of 300 entries takes about 1 us, of 1000
+// 18. 8 x 64 rows, 2000 columns, 1024 biases a request: 63 us in all; 2.2 ms with a
+// pass over the list for every row and entry instead. One column listed 1024 times
+// is added up by one thread a row: 200 us.)
+__device__ __forceinline__ void sort(Specials& list, int length) {
+  constexpr int kOwn = kMaxSpecials / kThreads, kStep = 16;
+  const int padded = (length + kStep - 1) / kStep * kStep;
+  if ((int)threadIdx.x < padded - length) list.entry[length + threadIdx.x] = ~0u;
+  uint32_t mine[kOwn];
+  int place[kOwn];
+#pragma unroll
+  for (int o = 0; o < kOwn; ++o) {
+    const int e = threadIdx.x + o * kThreads;
+    mine[o] = e < length ? list.entry[e] : 0u;
+    place[o] = 0;
+  }
+  __syncthreads();
+  for (int j = 0; j < padded; j += kStep) {
+    u32x4 other[kStep / 4];
+#pragma unroll
+    for (int i = 0; i < kStep / 4; ++i)
+      other[i] = *reinterpret_cast<const u32x4*>(list.entry + j + 4 * i);
+#pragma unroll
+    for (int o = 0; o < kOwn; ++o) {
+      if (o * kThreads >= length) break;
+#pragma unroll
+      for (int i = 0; i < kStep; ++i) place[o] += other[i / 4][i % 4] < mine[o];
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int o = 0; o < kOwn; ++o)
+    if ((int)threadIdx.x + o * kThreads < length) list.entry[place[o]] = mine[o];
+  __syncthreads();
 }
 
 // The chunk's table in LDS: how often each token was said (WIDE: 32 bits, else
@@ -233,7 +273,7 @@ __global__ __launch_bounds__(kThreads) void logits_kernel(LogitsArgs a) {
     if (items > 0) fetch(threadIdx.x);
 
     const bool live = ruled && req >= 0 && req < a.requests;  // else the grammar mask alone
-    int specials = 0, nodes = 0;
+    int specials = 0;
     if (live) {
       // The first drafted tokens and biases: asked for before the rest.
       int node0 = 0, all_nodes = 0;
@@ -300,11 +340,12 @@ __global__ __launch_bounds__(kThreads) void logits_kernel(LogitsArgs a) {
       }
       for (int j = 0; j < all_nodes; j += kThreads)
         specials = append(list, specials, j ? draft(j + threadIdx.x) : draft0, size, j + threadIdx.x);
-      nodes = specials;
       for (int j = 0; j < a.biases; j += kThreads)
-        specials = append(list, specials, j ? bias_id(j + threadIdx.x) : id0, size, j + threadIdx.x);
-      for (int e = threadIdx.x; e < specials; e += kThreads) table.mark(list.column[e]);
-      __syncthreads();
+        specials = append(list, specials, j ? bias_id(j + threadIdx.x) : id0, size,
+                          kBias | (j + threadIdx.x));
+      for (int e = threadIdx.x; e < specials; e += kThreads) table.mark(list.entry[e] >> 16);
+      if (specials > 1) sort(list, specials);
+      else __syncthreads();
     }
 
     RowRules r = {1.0f, 0.0f, 0.0f};
@@ -361,30 +402,29 @@ __global__ __launch_bounds__(kThreads) void logits_kernel(LogitsArgs a) {
         a.out[m * a.out_row + base + i] = y;
       }
 
-    // The special ones: entry e stands for its column if no earlier entry does.
+    // The special ones, each by its column's first entry.
     for (int k = threadIdx.x; k < rows * specials; k += kThreads) {
       const int m = row + k / specials, e = k % specials;
-      const int column = list.column[e];
+      const int column = list.entry[e] >> 16;
+      if (e > 0 && (int)(list.entry[e - 1] >> 16) == column) continue;
       const float x = load_logit<TYPE>(a.logits, m * a.in_row + base + column);
       const uint32_t bits = bits_at(m, column);
       uint32_t spoken = table.said(column);
       float bias = 0.0f;
-      bool mine = true, biased = false;
-      for (int j = 0; j < specials && mine; ++j) {
-        if (list.column[j] != column) continue;
-        const int source = list.source[j];
-        if (j < e) {
-          mine = false;
-        } else if (j < nodes) {
-          const uint32_t word = (uint32_t)a.ancestors[m * a.ancestor_row + (source >> 5)];
-          spoken += (word >> (source & 31)) & 1u;
-        } else {
+      bool biased = false;
+      for (int j = e; j < specials; ++j) {
+        const uint32_t entry = list.entry[j];
+        if ((int)(entry >> 16) != column) break;
+        const int source = entry & (kBias - 1);
+        if (entry & kBias) {
           const float value = a.bias_values[req * a.bias_value_row + source];
           bias = biased ? bias + value : value;
           biased = true;
+        } else {
+          const uint32_t word = (uint32_t)a.ancestors[m * a.ancestor_row + (source >> 5)];
+          spoken += (word >> (source & 31)) & 1u;
         }
       }
-      if (!mine) continue;
       float y = penalised(x, spoken || table.prompt[column / 32] >> (column & 31) & 1u, spoken, r);
       if (biased) y += bias;
       a.out[m * a.out_row + base + column] = bits & 1u ? y : kNegInf;

@@ -349,3 +349,64 @@ def test_refusals():
         process_logits(x.double())
     with pytest.raises(RuntimeError, match="unit column"):
         process_logits(x.t())
+
+
+@pytest.mark.parametrize("nb", [1, 15, 16, 17, 511, 513, 1024])
+@pytest.mark.parametrize("tokens", [1, 3, 400, 6000])
+def test_lists_of_any_length(nb, tokens):
+    """Biases and drafted nodes on the same columns, from one column for all to
+    mostly one each, in place: nodes count, biases add in list order (large ones
+    cancel, so that another order would show)."""
+    gen = torch.Generator().manual_seed(nb + tokens)
+    nodes, vocab = [70, 1, 13], 7001
+    qsl = torch.tensor([0, 70, 71, 84], dtype=torch.int32)
+    parents = torch.tensor([int(torch.randint(-1, j, (1,), generator=gen)) if j else -1
+                            for t in nodes for j in range(t)])
+    anc = tree_ancestors(parents, qsl, 70)
+    rules = _rules(gen, 3, vocab, 50, nb)
+    rules["bias_ids"] = torch.randint(0, tokens, (3, nb), generator=gen, dtype=torch.int32)
+    rules["bias_values"] = (torch.randn(3, nb, generator=gen) *
+                            10.0 ** torch.randint(0, 8, (3, nb), generator=gen)).round()
+    draft = torch.randint(0, tokens, (84,), generator=gen).to(torch.int32)
+    req = torch.repeat_interleave(torch.arange(3, dtype=torch.int32), torch.tensor(nodes))
+    # a bias's sum in fp32 in list order, the rest in 64 bits
+    sums = torch.zeros(3, vocab)
+    for i in range(nb):
+        at = rules["bias_ids"][:, i].long()
+        sums[torch.arange(3), at] += rules["bias_values"][:, i]
+    logits = torch.randn(84, vocab, generator=gen)
+    kw = dict(token_to_req=req, draft_tokens=draft, ancestors=anc, query_start_loc=qsl)
+    y, tol = _want(logits, {k: v for k, v in rules.items() if "bias" not in k}, **kw)
+    want = y + sums[req.long()].double()
+    tol = tol + 2.0 ** -24 * (want.abs() + tol)
+    buf = logits.to(DEV)
+    got = process_logits(buf, buf, **{k: v.to(DEV) if isinstance(v, torch.Tensor) else v
+                                      for k, v in {**rules, **kw}.items()})
+    assert got.data_ptr() == buf.data_ptr()
+    assert ((got.cpu().double() - want).abs() <= tol).all()
+
+
+def test_long_lists_are_no_slower_than_the_plain_form():
+    """Eight requests of 64 drafted nodes with 1024 biases each on 2000 columns,
+    against the time of the same rules as scatter operations of torch, about 500 us
+    here (with a pass over the list for every row and entry it was 2.2 ms)."""
+    gen = torch.Generator().manual_seed(77)
+    vocab, nreq, t = 2000, 8, 64
+    rows = nreq * t
+    rules = {k: v.to(DEV) if isinstance(v, torch.Tensor) else v
+             for k, v in _rules(gen, nreq, vocab, 500, 1024).items()}
+    kw = dict(token_to_req=torch.arange(nreq, dtype=torch.int32, device=DEV).repeat_interleave(t),
+              draft_tokens=torch.randint(0, vocab, (rows,), generator=gen).to(torch.int32).to(DEV),
+              ancestors=torch.full((rows, 2), -1, dtype=torch.int32, device=DEV),
+              query_start_loc=torch.arange(nreq + 1, dtype=torch.int32, device=DEV) * t)
+    logits = torch.randn(rows, vocab, generator=gen).to(DEV)
+    out = torch.empty_like(logits)
+    times = []
+    for _ in range(8):
+        a, b = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+        a.record()
+        process_logits(logits, out, **rules, **kw)
+        b.record()
+        b.synchronize()
+        times.append(a.elapsed_time(b) * 1e3)
+    assert min(times) < 500, times
