@@ -471,12 +471,17 @@ done:
 // Host side
 // ---------------------------------------------------------------------------
 
+// What a launch of more than 2^32 - 1 threads is refused with.
+constexpr hipError_t kTooLarge = hipErrorInvalidConfiguration;
+bool fits(int64_t blocks, int threads) { return blocks <= UINT_MAX / (unsigned)threads; }
+
 template <typename T, int GROUP, bool ZEROS, int MT, int NT, bool VEC>
 hipError_t launch_few(Int4Args a, int waves, hipStream_t stream) {
   waves = std::min(waves, a.k_tiles);
-  a.row_blocks = (a.rows + 16 * MT - 1) / (16 * MT);
-  const unsigned grid = (unsigned)((int64_t)a.row_blocks * ((a.n_tiles + NT - 1) / NT));
-  hipLaunchKernelGGL((int4_linear_kernel<T, GROUP, ZEROS, MT, NT, VEC>), dim3(grid),
+  a.row_blocks = (a.rows - 1) / (16 * MT) + 1;
+  const int64_t grid = (int64_t)a.row_blocks * ((a.n_tiles - 1) / NT + 1);
+  if (!fits(grid, 64 * waves)) return kTooLarge;
+  hipLaunchKernelGGL((int4_linear_kernel<T, GROUP, ZEROS, MT, NT, VEC>), dim3((unsigned)grid),
                      dim3(64 * waves), (size_t)waves * MT * NT * 64 * sizeof(f32x4), stream, a);
   return hipGetLastError();
 }
@@ -487,10 +492,11 @@ hipError_t launch_many(Int4Args a, hipStream_t stream) {
                                            WK > 1 ? (size_t)WK * WN * MT * NT * 1024 : 0);
   static_assert(kLds <= 65536, "two workgroups a CU, and no attribute to set");
   auto* kernel = &int4_rows_kernel<T, GROUP, ZEROS, MT, NT, WN, WK>;
-  a.row_blocks = (a.rows + 16 * MT - 1) / (16 * MT);
-  const int64_t n_blocks = (a.n_tiles + NT * WN - 1) / (NT * WN);
-  hipLaunchKernelGGL(kernel, dim3((unsigned)((n_blocks + 7) / 8 * 8 * a.row_blocks)),
-                     dim3(64 * WN * WK), kLds, stream, a);
+  a.row_blocks = (a.rows - 1) / (16 * MT) + 1;
+  const int64_t n_blocks = (a.n_tiles - 1) / (NT * WN) + 1;
+  const int64_t grid = (n_blocks + 7) / 8 * 8 * a.row_blocks;
+  if (!fits(grid, 64 * WN * WK)) return kTooLarge;
+  hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(64 * WN * WK), kLds, stream, a);
   return hipGetLastError();
 }
 
@@ -603,9 +609,9 @@ extern "C" int qsa_int4_linear(const void* x, int64_t x_row_stride, const void* 
   a.k = in_features;
   a.n_tiles = (int)(((int64_t)out_features + kTileN - 1) / kTileN);
   a.k_tiles = (int)(((int64_t)in_features + kTileK - 1) / kTileK);
-  // A launch holds at most 2^32 - 1 threads, 512 for 16 rows x 16 outputs at most.
-  if ((int64_t)a.n_tiles * (((int64_t)rows + 15) / 16) > UINT_MAX / 512 - 8)
-    return fail(QSA_ERR_UNSUPPORTED, std::string(name) + ": too many rows and outputs");
+  // The kernels count rows and outputs in 32 bits, to the end of the last block.
+  if (rows > INT_MAX - 64 || out_features > INT_MAX - 256)
+    return fail(QSA_ERR_UNSUPPORTED, std::string(name) + ": too many rows or outputs");
   if (in_features > (1 << 30) || x_row_stride > INT64_MAX / 4 / rows)
     return fail(QSA_ERR_UNSUPPORTED, std::string(name) + ": at most 2^30 inputs, rows within 2^62");
   // 16-byte loads of whole rows, whose offsets within a block fit 32 bits.
@@ -614,6 +620,8 @@ extern "C" int qsa_int4_linear(const void* x, int64_t x_row_stride, const void* 
   hipStream_t s = static_cast<hipStream_t>(stream);
   const hipError_t err = is_fp16 ? launch<Fp16>(a, group_size, vec, s)
                                  : launch<Bf16>(a, group_size, vec, s);
+  if (err == kTooLarge)
+    return fail(QSA_ERR_UNSUPPORTED, std::string(name) + ": too many rows and outputs");
   if (err != hipSuccess)
     return fail(QSA_ERR_HIP, std::string(name) + " launch: " + hipGetErrorString(err));
   return QSA_OK;

@@ -140,6 +140,19 @@ def test_int4_linear_refuses():
     assert f(*_int4_args(xs=2**61)) == -2 and f(*_int4_args(k=2**30 + 1)) == -2
 
 
+@pytest.mark.parametrize("rows,n,k,x", [
+    (1 << 26, 16, 256, 1 << 20), ((1 << 25) - 31, 16, 256, 1 << 20), (1 << 24, 1 << 20, 256, 1 << 20),
+    (1 << 28, 16, 2048, (1 << 20) + 2), (2**31 - 1, 1, 64, (1 << 20) + 2), (2**31 - 64, 1, 8, 1 << 20),
+    (1, 2**31 - 1, 256, 1 << 20), (5, (1 << 31) - 512, 1024, 1 << 20)])
+def test_int4_linear_refuses_more_threads_than_a_launch_holds(rows, n, k, x):
+    """By the blocks of the very launch, whatever they are rounded up to: a
+    refusal, not a launch that fails. (32 rows x 8 blocks of 512 threads: 2^25 - 31
+    rows are one block too many.)"""
+    lib = _lib.load()
+    assert lib.qsa_int4_linear(*_int4_args(rows=rows, n=n, k=k, x=x, ys=2**31)) == -2
+    assert b"too many rows" in lib.qsa_last_error()
+
+
 def _tree_args(**over):
     a = dict(q=1 << 20, qr=2048, qh=128, rows=8, hq=16, d=128, k=1 << 21, kb=8192, kt=512, kh=256,
              v=(1 << 21) + 256, vb=8192, vt=512, vh=256, blocks=64, page=16, hkv=2, table=1 << 23,
