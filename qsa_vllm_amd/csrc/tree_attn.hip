@@ -833,29 +833,41 @@ TreePlan make_plan(int requests, int num_q_heads, int num_kv_heads, int64_t max_
   return p;
 }
 
+// What a launch of more than 2^32 - 1 threads (256 a workgroup) is refused with.
+constexpr hipError_t kTooLarge = hipErrorInvalidConfiguration;
+bool fits(int64_t blocks) { return blocks <= UINT_MAX / 256; }
+
+// Workgroups of the joining launch for each request.
+template <int D, int WAYS>
+int64_t merge_tiles(int64_t pairs) {
+  constexpr int kPer = 256 / (D / 4) / WAYS;
+  return (pairs + kPer - 1) / kPer;
+}
 template <int D, int WAYS>
 hipError_t launch_merge(const TreeArgs& a, int64_t pairs, hipStream_t stream) {
-  constexpr int kPer = 256 / (D / 4) / WAYS;
-  const int row_tiles = (int)((pairs + kPer - 1) / kPer);
+  const int64_t row_tiles = merge_tiles<D, WAYS>(pairs);
   hipLaunchKernelGGL((tree_merge_kernel<D, WAYS>), dim3((unsigned)(a.requests * row_tiles)),
-                     dim3(256), 0, stream, a, row_tiles);
+                     dim3(256), 0, stream, a, (int)row_tiles);
   return hipGetLastError();
 }
 
 template <int D>
 hipError_t launch_tree(const TreeArgs& a, const TreePlan& plan, int max_nodes, hipStream_t stream) {
-  const unsigned grid =
-      a.workgroups ? grid_of(plan) : a.requests * a.kv_heads * a.m_tiles;
+  const int64_t grid =
+      a.workgroups ? grid_of(plan) : (int64_t)a.requests * a.kv_heads * a.m_tiles;
+  // Both launches' sizes before the first: a call that is refused has written nothing.
+  // (Only few (row, head)s are joined 8 ways.)
+  const int64_t pairs = (int64_t)max_nodes * a.num_q_heads;
+  if (!fits(grid) || (a.workgroups && !fits(a.requests * merge_tiles<D, 1>(pairs)))) return kTooLarge;
   constexpr size_t kLds = std::max({Shape<D, 2, 4, 1>::kLds, Shape<D, 2, 2, 2>::kLds,
                                     Shape<D, 2, 1, 4>::kLds, Shape<D, 1, 1, 4>::kLds});
   static_assert(kLds <= 65536, "two workgroups a CU, and no attribute to set");
-  hipLaunchKernelGGL((tree_attn_kernel<D>), dim3(grid), dim3(64 * kWaves), kLds, stream, a);
+  hipLaunchKernelGGL((tree_attn_kernel<D>), dim3((unsigned)grid), dim3(64 * kWaves), kLds, stream, a);
   const hipError_t err = hipGetLastError();
   if (err != hipSuccess || !a.workgroups) return err;
   // Many (row, head)s have few pieces each and need no more workgroups. (WAYS 8 / 4
   // / 2 / 1: 32 trees of 5 - 24 nodes 191 / 182 / 181 / 173 us in all, 64 nodes on
   // 131072 tokens 101 / 103 / 103 / 106.)
-  const int64_t pairs = (int64_t)max_nodes * a.num_q_heads;
   return pairs * a.requests <= 4096 ? launch_merge<D, 8>(a, pairs, stream)
                                     : launch_merge<D, 1>(a, pairs, stream);
 }
@@ -987,6 +999,8 @@ extern "C" int qsa_tree_attention(
   hipStream_t s = static_cast<hipStream_t>(stream);
   const hipError_t err = head_dim == 128 ? launch_tree<128>(a, plan, max_query_len, s)
                                          : launch_tree<64>(a, plan, max_query_len, s);
+  if (err == kTooLarge)
+    return fail(QSA_ERR_UNSUPPORTED, name + ": too many requests, rows or heads");
   if (err != hipSuccess)
     return fail(QSA_ERR_HIP, name + " launch: " + hipGetErrorString(err));
   return QSA_OK;

@@ -191,6 +191,21 @@ def test_tree_attention_refuses():
     assert lib.qsa_tree_attention_workspace_bytes(8, 2, 16, 2, 128, 4, 60) == 0
 
 
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("nreq,mq,hq,mc", [
+    (1 << 24, 1, 16, 60000),        # joining: 2^24 requests of at least one workgroup each
+    (1 << 18, 64, 32, 60000),       # 2^18 x 64 x 32 (row, head)s, 8 or 16 a workgroup
+    (1 << 24, 1, 2, 0),             # attention: a workgroup for each request and kv head
+])
+def test_tree_attention_refuses_more_threads_than_a_launch_holds(d, nreq, mq, hq, mc):
+    """Either launch's, before the first: a refused call writes nothing."""
+    lib = _lib.load()
+    args = dict(rows=min(nreq * mq, 2**31 - 1), hq=hq, hkv=2, d=d, tw=1, nreq=nreq, mq=mq, mc=mc,
+                ws=1 << 30, wsb=1 << 40)
+    assert lib.qsa_tree_attention(*_tree_args(**args)) == -2
+    assert b"too many" in lib.qsa_last_error()
+
+
 def test_tree_attention_workspace_stays_in_proportion():
     """Two pieces of at most 128 rows for each of at most 512 workgroups (and 8 for
     each 128 rows of a request and kv head), whatever the context and the batch."""
