@@ -490,7 +490,10 @@ __device__ __forceinline__ void attend_tile(const TreeArgs& a, const Request& rq
         top = fmaxf(fmaxf(top, sc[i][u][2]), sc[i][u][3]);
       }
       if (__any(top > base[i] + slack)) {
-        const float m = fmaxf(base[i], max_over_groups(top));
+        // Only the rows that passed it: a row's bits are its own. (A row that has
+        // seen nothing yet has -inf, and so has one whose scores are NaN.)
+        const float row_top = max_over_groups(top);
+        const float m = row_top > base[i] + slack ? row_top : base[i];
         const float shrink =
             m == kNegInf ? 1.0f : fast_exp2((base[i] - m) * a.scale_log2);
         base[i] = m;

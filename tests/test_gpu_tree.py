@@ -405,3 +405,33 @@ def test_refusals():
                         (dict(a6=args[6].cpu()), "GPU")):
         with pytest.raises(RuntimeError, match=match):
             call(**over)
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+@pytest.mark.parametrize("scale", [1.0, 5.0])
+@pytest.mark.parametrize("longest", [None, 0])
+@pytest.mark.parametrize("ctx,nodes,heads", [([100], [6], 8), ([0], [60], 8), ([61, 300], [9, 30], 16),
+                                             ([1500], [20], 4)])
+def test_a_row_has_its_own_bits(bad, ctx, nodes, heads, longest, scale):
+    """Neither nodes that it does not see nor the other rows' queries reach a
+    row's result: the same bits whatever those hold. A stage for each workgroup and
+    (no context announced) all stages in one, with maxima that keep rising."""
+    c = Case(ctx, nodes, heads=heads, kv_heads=2, seed=21, scale=scale)
+    clean = c.run(max_context_len=longest)
+    b, node = len(ctx) - 1, 1
+    first, pos = c.starts[b], ctx[b] + node
+    sees = torch.zeros(clean.shape[0], dtype=torch.bool)
+    sees[first:] = (c.anc[first:, 0] >> node) & 1 != 0
+    assert sees.any() and not sees.all()
+    keep = c.kv[c.table[b, pos // 16], pos % 16].clone()
+    for what in (slice(None), slice(0, c.dim), slice(c.dim, None)):      # K and V, K, V
+        c.kv[c.table[b, pos // 16], pos % 16, :, what] = bad
+        got = c.run(max_context_len=longest)
+        assert torch.equal(got[~sees], clean[~sees])
+        assert not torch.isfinite(got[sees]).any()
+        c.kv[c.table[b, pos // 16], pos % 16] = keep
+    one = torch.arange(clean.shape[0]) % 3 == 0
+    q = torch.where(one[:, None, None], c.q, (c.q.float() * 9).bfloat16()).to(DEV)
+    assert torch.equal(c.run(q=q, max_context_len=longest)[one], clean[one])
+    q[~one.to(DEV)] = bad
+    assert torch.equal(c.run(q=q, max_context_len=longest)[one], clean[one])
