@@ -410,7 +410,7 @@ __device__ __forceinline__ void attend_tile(const TreeArgs& a, const Request& rq
     if (t + kTok > rq.context) {
       // A drafted token's V may hold infinities or NaN that a row outside its
       // branch must not see (0 times them is NaN). The whole stage's are taken
-      // as 0 here, and rows that see them get NaN at the end.
+      // as 0 here, and added at the end to the rows that see them.
       u32x4* const v = reinterpret_cast<u32x4*>(stage + S::kStage);
       bool bad = false;
       for (int i = lane; i < kTok * U; i += 64) bad |= not_finite(v[i]) != 0;
@@ -608,8 +608,11 @@ __device__ __forceinline__ void attend_tile(const TreeArgs& a, const Request& rq
         for (int d = 0; d < kDims; ++d) {
           const u32x2 x = load_u32x2(v + (16 * d + 4 * g) * 2);
 #pragma unroll
-          for (int r = 0; r < 4; ++r)
-            if ((x[r >> 1] >> (16 * (r & 1)) & 0x7F80u) == 0x7F80u) o[i][d][r] = __builtin_nanf("");
+          for (int r = 0; r < 4; ++r) {
+            // (a positive weight times an infinity or NaN is the same)
+            const uint32_t bits = r & 1 ? x[r >> 1] & 0xFFFF0000u : x[r >> 1] << 16;
+            if ((bits & 0x7F800000u) == 0x7F800000u) o[i][d][r] += __builtin_bit_cast(float, bits);
+          }
         }
       }
     }

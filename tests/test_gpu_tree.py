@@ -435,3 +435,39 @@ def test_a_row_has_its_own_bits(bad, ctx, nodes, heads, longest, scale):
     assert torch.equal(c.run(q=q, max_context_len=longest)[one], clean[one])
     q[~one.to(DEV)] = bad
     assert torch.equal(c.run(q=q, max_context_len=longest)[one], clean[one])
+
+
+def _softmax(case, row, head, b):
+    """A row's result in 64 bits by IEEE arithmetic, but for a score of -inf, whose
+    weight is 0: zeros if there is no other."""
+    h = head // (case.heads // case.kv_heads)
+    seen = list(range(case.ctx[b])) + [case.ctx[b] + j for j in range(case.nodes[b])
+                                       if (int(case.anc[row, j // 32]) >> (j % 32)) & 1]
+    kv = torch.stack([case.kv[case.table[b, p // case.page], p % case.page, h] for p in seen]).double()
+    s = kv[:, :case.dim] @ case.q[row, head].double() / math.sqrt(case.dim)
+    live = s != -math.inf
+    if not live.any():
+        return torch.zeros(case.dim, dtype=torch.float64)
+    p = torch.exp(s[live] - s[live].max())
+    return (p / p.sum()) @ kv[live, case.dim:]
+
+
+@pytest.mark.parametrize("ctx,at", [(100, 101), (100, 60), (64, 65), (700, 702), (700, 3)])
+@pytest.mark.parametrize("heads", [2, 16])
+def test_infinite_values_give_what_their_sum_gives(ctx, at, heads):
+    """One infinity in a dimension: an infinity of its sign. Two of unlike signs, or
+    a NaN: NaN. The same for committed tokens and drafted ones."""
+    inf, nan = math.inf, math.nan
+    c = Case([ctx], [8], heads=heads, kv_heads=2, seed=22, chain=True)
+    near = at + 1 if at + 1 != ctx else at - 1
+    for pos, dim, value in ((at, 0, inf), (at, 17, -inf), (at, 40, nan), (at, 63, inf),
+                            (near, 63, -inf), (near, 100, -inf), (at, 100, -inf)):
+        c.kv[c.table[0, pos // 16], pos % 16, :, c.dim + dim] = value
+    for longest in (None, 0):
+        got = c.run(max_context_len=longest).cpu().double()
+        for row in (0, 1, 2, 4, 7):
+            want = _softmax(c, row, 0, 0)
+            fine = torch.isfinite(want)
+            assert torch.equal(torch.nan_to_num(got[row, 0, ~fine], nan=7.0),
+                               torch.nan_to_num(want[~fine], nan=7.0)), (row, longest)
+            assert torch.isfinite(got[row, 0, fine]).all()
