@@ -518,7 +518,9 @@ int qsa_int4_linear(const void* x, int64_t x_row_stride, const void* codes, cons
  * are not seen, nor are positions without a page in the cache. out = softmax of
  * the scaled scores times V, times sigmoid(gate) if gate is given, rounded once
  * to bf16; zeros for a row that sees nothing. Rows of no request are not written.
- * K or V that is not finite makes what sees it NaN (or infinite) and nothing else.
+ * Infinities and NaN in K or V reach the rows that see them, as arithmetic has it
+ * (an infinite score gives NaN, an infinite value an infinity), and nothing else. A
+ * score of minus infinity weighs nothing; a row that has no other gets zeros.
  * max_query_len bounds a request's nodes (further ones are not computed);
  * max_context_len should bound context_lens: it shapes the launch only. q and the
  * caches are 16-byte aligned with strides of multiples of 8 elements; a cache

@@ -72,12 +72,14 @@ def qsa_tree_paged_attention(
     at rows ``query_start_loc[b] ..``) over ``context_lens[b]`` committed tokens
     and the nodes that ``ancestors`` shows each row. Row order, caches, table and
     gate as in ``qsa_sparse_paged_attention``; the gated result is rounded once.
-    A row that sees nothing gets zeros, one that sees K or V that are not finite NaN
-    (or an infinity) there; rows of no request (past ``query_start_loc[-1]``) are
-    not written. The caches must span less than 64 GiB each. ``max_query_len`` must be at least
-    every request's node count (further nodes are not computed);
-    ``max_context_len`` should be at least every context length: it shapes the
-    launch, not the result. Captured into a graph, both hold for its replays."""
+    A row that sees nothing gets zeros. Infinities and NaN in K or V reach the rows
+    that see them, as arithmetic has it, and no others; a score of minus infinity
+    weighs nothing, and a row that has no other gets zeros. Rows of no request
+    (past ``query_start_loc[-1]``) are not written. The caches must span less than
+    64 GiB each. ``max_query_len`` must be at least every request's node count
+    (further nodes are not computed); ``max_context_len`` should be at least every
+    context length: it shapes the launch, not the result. Captured into a graph,
+    both hold for its replays."""
     if out is None:
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
     torch.ops.yulan_qsa_kernels.tree_attention(

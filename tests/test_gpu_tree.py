@@ -471,3 +471,26 @@ def test_infinite_values_give_what_their_sum_gives(ctx, at, heads):
             assert torch.equal(torch.nan_to_num(got[row, 0, ~fine], nan=7.0),
                                torch.nan_to_num(want[~fine], nan=7.0)), (row, longest)
             assert torch.isfinite(got[row, 0, fine]).all()
+
+
+@pytest.mark.parametrize("ctx,at", [(100, 20), (100, 102), (3, 0), (900, 640)])
+def test_infinite_keys_follow_their_scores(ctx, at):
+    """One infinite element of K: the score is an infinity of its product's sign.
+    Infinity gives NaN, minus infinity no weight; a row that has no other score
+    gets zeros like one that sees nothing."""
+    c = Case([ctx], [5], heads=4, kv_heads=2, seed=23, chain=True)
+    for sign in (1.0, -1.0):
+        c.kv[c.table[0, at // 16], at % 16, :, 5] = sign * math.inf
+        for longest in (None, 0):
+            got = c.run(max_context_len=longest).cpu().double()
+            for row in range(5):
+                for head in range(4):
+                    want = _softmax(c, row, head, 0)
+                    assert torch.equal(want.isnan(), got[row, head].isnan())
+                    if not want.isnan().any():       # values of about 1, weights off by 2^-8
+                        assert (got[row, head] - want).abs().max() < 0.1
+    c = Case([40], [3], heads=2, kv_heads=1, seed=24, chain=True)
+    for pos in range(43):
+        c.kv[c.table[0, pos // 16], pos % 16, :, 5] = math.inf
+    c.q[:, :, 5] = -c.q[:, :, 5].abs() - 1
+    assert (c.run() == 0).all() and (c.run(max_context_len=0) == 0).all()
