@@ -410,3 +410,42 @@ def test_long_lists_are_no_slower_than_the_plain_form():
         b.synchronize()
         times.append(a.elapsed_time(b) * 1e3)
     assert min(times) < 500, times
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_served_sizes(dtype):
+    """128 rows of 99072 words (four chunks a row) with histories to 32768 tokens:
+    the counts and biases as scatter operations of torch in 64 bits."""
+    rows, vocab, width, nb = 128, 99072, 32768, 64
+    gen = torch.Generator(device=DEV).manual_seed(31)
+    rand = lambda *shape: torch.rand(*shape, generator=gen, device=DEV)
+    history = (rand(rows, width) ** 3 * (vocab + 100)).to(torch.int32)
+    lens = (rand(rows) * (width + 1)).to(torch.int32)
+    lens[3], lens[4] = width, 0
+    prompt = (lens * rand(rows)).to(torch.int32)
+    rep, freq, pres = rand(rows) + 0.7, rand(rows), rand(rows)
+    ids = torch.stack([torch.randperm(vocab + 50, generator=gen, device=DEV)[:nb] for _ in range(rows)])
+    values = torch.randn(rows, nb, generator=gen, device=DEV)
+    allowed = torch.randint(-2**31, 2**31, (rows, vocab // 32), generator=gen, device=DEV).to(torch.int32)
+    x = (torch.randn(rows, vocab, generator=gen, device=DEV) * 3).to(dtype)
+    got = process_logits(x, history=history, history_lens=lens, prompt_lens=prompt, repetition=rep,
+                         frequency=freq, presence=pres, bias_ids=ids.to(torch.int32),
+                         bias_values=values, allowed=allowed)
+    at = torch.arange(width, device=DEV)
+    counts = []
+    for live in (at < lens[:, None], (at < lens[:, None]) & (at >= prompt[:, None])):
+        n = torch.zeros(rows, vocab + 100, dtype=torch.int64, device=DEV)
+        n.scatter_add_(1, history.long(), live.long())
+        counts.append(n[:, :vocab])
+    ever, said = counts
+    y = x.double()
+    r, f, p = (t.double()[:, None] for t in (rep, freq, pres))
+    m = y.abs() * torch.maximum(r, 1 / r) + f * said + p
+    y = torch.where(ever > 0, torch.where(y > 0, y / r, y * r), y) - f * said - p * (said > 0)
+    bias = torch.zeros(rows, vocab + 50, dtype=torch.float64, device=DEV)
+    bias = bias.scatter_(1, ids, values.double())[:, :vocab]     # no id twice
+    y, m = y + bias, m + bias.abs()
+    free = (allowed[:, :, None] >> torch.arange(32, device=DEV, dtype=torch.int32)) & 1 != 0
+    free = free.view(rows, vocab)
+    assert (got[~free] == -math.inf).all()
+    assert ((got.double() - y).abs() <= 7 * 2.0 ** -24 * m)[free].all()

@@ -494,3 +494,67 @@ def test_infinite_keys_follow_their_scores(ctx, at):
         c.kv[c.table[0, pos // 16], pos % 16, :, 5] = math.inf
     c.q[:, :, 5] = -c.q[:, :, 5].abs() - 1
     assert (c.run() == 0).all() and (c.run(max_context_len=0) == 0).all()
+
+
+@pytest.mark.parametrize("ctx,nodes,heads,longest", [([30], [20], 2, None), ([700, 90], [20, 13], 16, None),
+                                                     ([90, 2500, 64], [9, 40, 8], 8, None),
+                                                     ([700, 90], [20, 13], 16, 0)])
+def test_rows_past_the_announced_nodes_are_not_written(ctx, nodes, heads, longest):
+    """Requests of more nodes than ``max_query_len``, in one stage and over several
+    workgroups and the joining launch: the first ones are right, the rest left."""
+    c = Case(ctx, nodes, heads=heads, kv_heads=2 if heads > 2 else 1, seed=25)
+    out = torch.full((sum(nodes), heads, 128), 5.0, dtype=torch.bfloat16, device=DEV)
+    c.run(out=out, max_query_len=8, max_context_len=longest)
+    want, tol = c.want()
+    done = torch.zeros(sum(nodes), dtype=torch.bool)
+    for start, n in zip(c.starts, nodes):
+        done[start:start + min(n, 8)] = True
+    got = out.cpu().double()
+    assert ((got - want).abs() <= tol)[done].all()
+    assert (got[~done] == 5).all()
+
+
+@pytest.mark.parametrize("ctx,nodes,heads,kv_heads,dim,page", [
+    ([131072], [1], 16, 2, 128, 16), ([131072], [64], 16, 2, 128, 16), ([65537], [33], 8, 1, 64, 272),
+    ([32768, 4096, 20000, 1, 9999], [24, 5, 1, 16, 17], 16, 2, 128, 16)])
+def test_served_lengths(ctx, nodes, heads, kv_heads, dim, page):
+    """Contexts as long as they are served, against 64 bits on the GPU. The
+    tolerance is the 64-bit statement's of the other tests, one row at a time."""
+    gen = torch.Generator(device=DEV).manual_seed(sum(ctx))
+    cpu = torch.Generator().manual_seed(sum(ctx))
+    pages = [-(-(c + t) // page) for c, t in zip(ctx, nodes)]
+    order = torch.randperm(sum(pages), generator=cpu).to(torch.int32)
+    table = torch.full((len(ctx), max(pages)), -1, dtype=torch.int32)
+    at = 0
+    for b, p in enumerate(pages):
+        table[b, :p] = order[at:at + p]
+        at += p
+    table = table.to(DEV)
+    kv = torch.randn(len(order), page, kv_heads, 2 * dim, generator=gen, device=DEV).bfloat16()
+    rows, group = sum(nodes), heads // kv_heads
+    q = torch.randn(rows, heads, dim, generator=gen, device=DEV).bfloat16()
+    starts = torch.tensor([0] + nodes).cumsum(0)
+    parents = torch.cat([torch.arange(t) - 1 - torch.randint(0, 4, (t,), generator=cpu) for t in nodes])
+    anc = tree_ancestors(parents, starts, max(nodes))
+    got = qsa_tree_paged_attention(
+        q, kv[..., :dim], kv[..., dim:], table, torch.tensor(ctx, dtype=torch.int32, device=DEV),
+        starts.to(torch.int32).to(DEV), anc.to(DEV), max_query_len=max(nodes),
+        max_context_len=max(ctx)).double()
+    for b, (c, t) in enumerate(zip(ctx, nodes)):
+        pos = torch.arange(c + t, device=DEV)
+        of = kv[table[b].long()[pos // page], pos % page].double()
+        for j in {0, t // 2, t - 1}:
+            row = int(starts[b]) + j
+            seen = torch.ones(c + t, dtype=torch.bool)
+            seen[c:] = torch.tensor([(int(anc[row, i // 32]) >> (i % 32)) & 1 != 0 for i in range(t)])
+            mine = of[seen.to(DEV)]
+            for h in range(heads):
+                k, v = mine[:, h // group, :dim], mine[:, h // group, dim:]
+                x = q[row, h].double()
+                p = torch.softmax((k * x).sum(1) / math.sqrt(dim), 0)
+                o = (p[:, None] * v).sum(0)
+                spread = (k * x).abs().sum(1).max() / math.sqrt(dim)
+                off = (2 ** -8 * (1 + 2 ** -7) * (p[:, None] * (v - o).abs()).sum(0)
+                       + (2 * 36 * 2 ** -24 * spread + 2 ** -18) * (p[:, None] * v.abs()).sum(0))
+                tol = off + 2 ** -8 * (o.abs() + off)
+                assert ((got[row, h] - o).abs() <= tol).all(), (b, j, h)
