@@ -13,7 +13,8 @@
 //   sum x (q - z) = sum x (c0 + q - z) - c0 sum x,
 // and the last term, the same for every output, is the accumulator's start: the
 // product of x with a constant. Both are summed in fp32, whose step is 2^-16 of
-// bf16's. With fp16 the code becomes 1024 + q (or 1024 + 16 q) and one packed
+// bf16's; where that gives no finite sum, it is taken again without the constant
+// (plain_sum). With fp16 the code becomes 1024 + q (or 1024 + 16 q) and one packed
 // add (or fma) gives q - z exactly.
 //
 // Layout. Weights are stored in tiles of 16 outputs x 128 inputs, 1 KiB each:
@@ -252,17 +253,65 @@ __device__ __forceinline__ void multiply(const u32x4 (&x)[MT][4], const Tiles<GR
   }
 }
 
-// A tile's sums (a lane: rows 4 g + r of output n) to y.
+// A tile's sums (a lane: rows 4 g + r of output n) to y. Returns which of the four
+// are not finite, as bits.
 template <typename T>
-__device__ __forceinline__ void store(const Int4Args& a, int m0, int tile, int lane,
-                                      const f32x4& sum) {
+__device__ __forceinline__ uint32_t store(const Int4Args& a, int m0, int tile, int lane,
+                                          const f32x4& sum) {
   const int col = tile * kTileN + (lane & 15);
-  if (col >= a.n) return;
+  uint32_t bad = 0;
+  if (col >= a.n) return bad;
   const float b = a.bias ? T::to_float(a.bias[col]) : 0.0f;
 #pragma unroll
   for (int r = 0; r < 4; ++r) {
     const int m = m0 + 4 * (lane >> 4) + r;
-    if (m < a.rows) a.y[m * a.y_row + col] = T::from_float(sum[r] + b);
+    if (m >= a.rows) continue;
+    const float v = sum[r];
+    a.y[m * a.y_row + col] = T::from_float(v + b);
+    bad |= (uint32_t)((__builtin_bit_cast(uint32_t, v) & 0x7F800000u) == 0x7F800000u) << r;
+  }
+  return bad;
+}
+
+// One result as its formula has it, term by term. Infinities in x, or bf16 values
+// past 2^112, make the offset's product and the codes' cancel to NaN, and padded
+// inputs repeat the row's first ones, which may be infinite: a sum that is not
+// finite is taken again here. (A NaN in x ends it at once.)
+template <typename T, int GROUP, bool ZEROS>
+__device__ __forceinline__ float plain_sum(const Int4Args& a, int m, int col) {
+  constexpr int kGroups = kTileK / GROUP;
+  const int tile = col / kTileN, n = col % kTileN;
+  const uint16_t* const x = a.x + m * a.x_row;
+  const uint32_t* const words = reinterpret_cast<const uint32_t*>(a.codes);
+  float sum = 0.0f;
+  for (int k = 0; k < a.k && sum == sum; k += 8) {
+    const int in = k % kTileK, j = in / 32, g = in % 32 / 8;
+    const int64_t at = (int64_t)tile * a.k_tiles + k / kTileK;
+    const int64_t group = (at * kTileN + n) * kGroups + in / GROUP;
+    const uint32_t w = words[(at * 64 + 16 * g + n) * 4 + j];
+    const float scale = T::to_float(reinterpret_cast<const uint16_t*>(a.scales)[group]);
+    const int zero = ZEROS ? reinterpret_cast<const uint8_t*>(a.zeros)[group] : 8;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (k + i < a.k) {
+        const int code = (int)(w >> (4 * (i / 2) + 16 * (i % 2))) & 15;
+        sum = __builtin_fmaf(T::to_float(x[k + i]), (float)(code - zero) * scale, sum);
+      }
+  }
+  return sum;
+}
+
+// Results of a wave's tiles whose sums were not finite: bit 4 u + r of `bad` for row
+// 4 g + r of tile u (row block u / NT, output tile u % NT).
+template <typename T, int GROUP, bool ZEROS, int NT>
+__device__ __forceinline__ void repair(const Int4Args& a, uint64_t bad, int row0, int tile0, int lane) {
+  while (bad) {
+    const int at = __ffsll((unsigned long long)bad) - 1;
+    bad &= bad - 1;
+    const int m = row0 + 16 * (at / 4 / NT) + 4 * (lane >> 4) + at % 4;
+    const int col = (tile0 + at / 4 % NT) * kTileN + (lane & 15);
+    const float b = a.bias ? T::to_float(a.bias[col]) : 0.0f;
+    a.y[m * a.y_row + col] = T::from_float(plain_sum<T, GROUP, ZEROS>(a, m, col) + b);
   }
 }
 
@@ -345,11 +394,13 @@ __global__ __launch_bounds__(512) void int4_linear_kernel(Int4Args a) {
 #pragma unroll
     for (int v = 0; v < NT; ++v) part[(wave * MT * NT + i * NT + v) * 64 + lane] = acc[i][v];
   __syncthreads();
+  uint64_t bad = 0;
   for (int u = wave; u < MT * NT; u += waves) {
     f32x4 sum = part[u * 64 + lane];
     for (int o = 1; o < waves; ++o) sum += part[(o * MT * NT + u) * 64 + lane];
-    store<T>(a, row0 + 16 * (u / NT), tile0 + u % NT, lane, sum);
+    bad |= (uint64_t)store<T>(a, row0 + 16 * (u / NT), tile0 + u % NT, lane, sum) << (4 * u);
   }
+  repair<T, GROUP, ZEROS, NT>(a, bad, row0, tile0, lane);
 }
 
 // More than 16 rows: a workgroup of WN x WK waves takes 16 MT rows and 16 NT WN
@@ -442,6 +493,8 @@ int4_rows_kernel(Int4Args a) {
 done:
   __builtin_amdgcn_s_waitcnt(kMemoryDone);  // no load into LDS outlives the wave
 
+  static_assert(4 * MT * NT <= 64, "a bit for each of a lane's results");
+  uint64_t bad = 0;
   if constexpr (WK > 1) {
     f32x4* const part = reinterpret_cast<f32x4*>(lds);  // [WK][WN][MT * NT][64]
     __syncthreads();
@@ -456,15 +509,18 @@ done:
 #pragma unroll
       for (int o = 1; o < WK; ++o) sum += part[((o * WN + wn) * MT * NT + u) * 64 + lane];
       if (tile0 + u % NT < a.n_tiles)
-        store<T>(a, row0 + 16 * (u / NT), tile0 + u % NT, lane, sum);
+        bad |= (uint64_t)store<T>(a, row0 + 16 * (u / NT), tile0 + u % NT, lane, sum) << (4 * u);
     }
   } else {
 #pragma unroll
     for (int i = 0; i < MT; ++i)
 #pragma unroll
       for (int v = 0; v < NT; ++v)
-        if (tile0 + v < a.n_tiles) store<T>(a, row0 + 16 * i, tile0 + v, lane, acc[i][v]);
+        if (tile0 + v < a.n_tiles)
+          bad |= (uint64_t)store<T>(a, row0 + 16 * i, tile0 + v, lane, acc[i][v])
+                 << (4 * (i * NT + v));
   }
+  repair<T, GROUP, ZEROS, NT>(a, bad, row0, tile0, lane);
 }
 
 // ---------------------------------------------------------------------------

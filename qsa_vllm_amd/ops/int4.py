@@ -150,8 +150,9 @@ def int4_linear(x: torch.Tensor, weight: Int4Weight, bias: torch.Tensor | None =
     """``x @ weight.T + bias`` for ``x`` ``[..., in_features]`` of the weight's
     type (bf16 or fp16), summed in fp32 and rounded once. ``out`` (only for a
     two-dimensional ``x``) receives the result. Made for few rows, where it
-    streams the 4-bit weight once (per 64 rows); it is right for any number. A
-    row with an infinity or NaN (or bf16 values past 2^112) has no defined result."""
+    streams the 4-bit weight once (per 64 rows); it is right for any number, and
+    for any values: results that are not finite at first (infinities in a row, or
+    bf16 values past 2^112) are taken again term by term, which is slow."""
     rows = x
     if x.dim() != 2:
         _require(x.dim() >= 1 and out is None, "x must be [..., in_features]; out needs a 2-D x")

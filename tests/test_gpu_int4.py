@@ -251,3 +251,68 @@ def test_refusals():
         with pytest.raises(RuntimeError, match=match):
             bad()
     assert int4_linear(x[:0], w).shape == (0, 32)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("zeros,group", [(True, 32), (False, 128), (True, 64)])
+@pytest.mark.parametrize("rows,k,offset", [(1, 512, 0), (3, 200, 0), (7, 264, 0), (16, 1023, 0), (20, 200, 0),
+                                           (61, 520, 0), (250, 392, 0), (5, 200, 1), (40, 72, 1)])
+def test_infinite_and_huge_activations(rows, k, offset, zeros, group, dtype):
+    """What x times the dequantized weight gives in any order: an infinity where
+    one is met by weights of one sign, NaN by 0 or by unlike signs, and finite sums of
+    bf16 values whose product with the codes alone would overflow. In rows of
+    every kind: sixteen bytes at a time or not, a width that is no whole tile."""
+    gen = torch.Generator().manual_seed(rows + k)
+    n = 4200 if rows in (7, 250) else 70
+    codes, scales, z = _weight(gen, n, k, group, dtype, zeros)
+    x = torch.randn(rows, k, generator=gen).to(dtype)
+    special = {0: [(0, "inf")], 2: [(k - 1, "-inf")], 3: [(5, "inf"), (k // 2, "inf")],
+               4: [(1, "inf"), (9, "-inf")], 6: [(k - 2, "nan")], 17: [(3, "-inf")], 19: [(k // 3, "nan")],
+               33: [(k - 9, "inf")], 60: [(0, "inf")], 200: [(63, "-inf")], 249: [(k - 1, "inf")]}
+    for row, places in special.items():
+        if row < rows:
+            for at, value in places:
+                x[row, at] = float(value)
+    huge = [r for r in range(rows) if r % 5 == 1] if dtype == torch.bfloat16 else []
+    for r in huge:
+        x[r] = (x[r].float() * 2.0 ** 119).bfloat16()
+    w = int4_pack(codes.to(DEV), scales.to(DEV), z.to(DEV) if zeros else None, group_size=group)
+    store = torch.zeros(rows * (k + 8) + 8, dtype=dtype, device=DEV)
+    view = store.as_strided((rows, k), (k + 8 - k % 8, 1), offset)
+    view.copy_(x)
+    got = int4_linear(view, w).cpu().double()
+    wd = w.dequantize().cpu().double()
+    for r in range(rows):
+        terms = x[r].double() * wd
+        want = terms.sum(1)
+        if r in special:
+            assert not torch.isfinite(want).all()
+            assert torch.equal(torch.nan_to_num(got[r], nan=7.0), torch.nan_to_num(want, nan=7.0)), r
+        else:
+            s = scales.double().repeat_interleave(group, 1)[:, :k]
+            sums = U * (36 * 2 * 143 * (x[r].double().abs() * s).sum(1) + (k + 12) * terms.abs().sum(1))
+            tol = sums + torch.finfo(dtype).eps / 2 * (want.abs() + sums) + 2.0 ** -25
+            assert ((got[r] - want).abs() <= tol).all(), r
+
+
+def test_a_nan_row_ends_at_once():
+    """Rows of NaN, as padding may hold them, cost little more than others."""
+    gen = torch.Generator(device=DEV).manual_seed(40)
+    weight = (torch.randn(11264, 4096, generator=gen, device=DEV) * 0.02).bfloat16()
+    w = int4_quantize(weight)
+    x = torch.randn(61, 4096, generator=gen, device=DEV).bfloat16()
+    dirty = x.clone()
+    dirty[20:] = float("nan")
+    out = torch.empty(61, 11264, dtype=torch.bfloat16, device=DEV)
+    times = {}
+    for name, rows in (("clean", x), ("dirty", dirty)):
+        for _ in range(8):
+            a, b = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+            a.record()
+            for _ in range(10):
+                int4_linear(rows, w, out=out)
+            b.record()
+            b.synchronize()
+            times[name] = min(times.get(name, 1e9), a.elapsed_time(b))
+    assert out[20:].isnan().all() and torch.isfinite(out[:20]).all()
+    assert times["dirty"] < 4 * times["clean"], times
