@@ -114,7 +114,8 @@ def int4_quantize(weight: torch.Tensor, *, group_size: int = 128,
     """Round a bf16 or fp16 weight ``[out, in]`` to 4 bits: per group the scale
     ``max |w| / 7`` about code 8, or with ``zero_points`` ``(max - min) / 15``
     over a range that holds 0. Scales are rounded to the weight's type first, so
-    each code is the nearest to ``w / scale``."""
+    each code is the nearest to ``w / scale``. Infinities, NaN and
+    values from 2^127 on are refused."""
     _check_group(group_size)
     _require(weight.dim() == 2 and weight.dtype in (torch.bfloat16, torch.float16),
              "weight must be bf16 or fp16 [out, in]")
@@ -127,6 +128,8 @@ def int4_quantize(weight: torch.Tensor, *, group_size: int = 128,
     step = max(1, _PACK_CODES // max(k, 1))
     for r in range(0, n, step):
         w = weight[r:r + step].float()
+        # (past 2^127 a group's range, or its dequantized ends, pass fp32's)
+        _require(bool((w.abs() < 2.0 ** 127).all()), "weight must be finite and below 2^127")
         w = torch.nn.functional.pad(w, (0, groups * group_size - k)).view(-1, groups, group_size)
         if zero_points:
             low, high = w.amin(-1).clamp(max=0), w.amax(-1).clamp(min=0)

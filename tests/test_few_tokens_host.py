@@ -75,6 +75,32 @@ def test_quantized_weight_is_the_nearest_code(dtype, zero_points, group):
     assert (q.dequantize()[3, :group] == 0).all()
 
 
+@pytest.mark.parametrize("zero_points", [False, True])
+def test_quantizing_takes_finite_weights_and_no_others(zero_points):
+    """Large values of both signs have a range past the type's; an infinity or NaN has
+    no code, nor bf16 values whose range passes 32 bits."""
+    for dtype, top in ((torch.bfloat16, 2.0 ** 127 - 2.0 ** 119), (torch.float16, 65504.0),
+                       (torch.bfloat16, torch.finfo(torch.bfloat16).max)):
+        w = torch.zeros(3, 130, dtype=dtype)
+        w[0, 0], w[0, 1], w[1, 129] = top, -top, -top
+        if top > 2.0 ** 127:
+            with pytest.raises(RuntimeError, match="finite"):
+                int4_quantize(w, group_size=64, zero_points=zero_points)
+            continue
+        q = int4_quantize(w, group_size=64, zero_points=zero_points)
+        got = q.dequantize().double()
+        step = top / (7.5 if zero_points else 7)
+        # half a step, as much again for the zero point's own rounding, and what the
+        # scale's rounding moves the range's end by
+        off = step * ((1.0 if zero_points else 0.5) + 15 * torch.finfo(dtype).eps / 2)
+        assert (got - w.double()).abs().max() <= off
+        for bad in (float("nan"), float("inf"), -float("inf")):
+            broken = w.clone()
+            broken[2, 70] = bad
+            with pytest.raises(RuntimeError, match="finite"):
+                int4_quantize(broken, group_size=64, zero_points=zero_points)
+
+
 def _walk(parents, starts, words):
     bits = np.zeros((len(parents), words), dtype=np.uint32)
     for b in range(len(starts) - 1):
