@@ -871,10 +871,16 @@ hipError_t launch_tree(const TreeArgs& a, const TreePlan& plan, int max_nodes, h
   hipLaunchKernelGGL((tree_attn_kernel<D>), dim3((unsigned)grid), dim3(64 * kWaves), kLds, stream, a);
   const hipError_t err = hipGetLastError();
   if (err != hipSuccess || !a.workgroups) return err;
-  // Many (row, head)s have few pieces each and need no more workgroups. (WAYS 8 / 4
-  // / 2 / 1: 32 trees of 5 - 24 nodes 191 / 182 / 181 / 173 us in all, 64 nodes on
-  // 131072 tokens 101 / 103 / 103 / 106.)
-  return pairs * a.requests <= 4096 ? launch_merge<D, 8>(a, pairs, stream)
+  // Many (row, head)s have few pieces each and need no more workgroups. In all, us,
+  // WAYS 8 / 4 / 2 / 1, by (row, head)s at most:
+  //   1024   64 nodes on 131072 tokens          100.3 / 100.0 / 100.5 / 103.0
+  //   1024   8 trees of 8 nodes on 8000          33.1 / 33.0 / 33.5 / 33.7
+  //   2048   2 trees of 64 nodes on 65536       109.9 / 109.0 / 109.2 / 109.8
+  //   4096   4 trees of 64 nodes on 32768       118.4 / 110.0 / 109.3 / 108.4
+  //   4096   256 single tokens on 1024 - 4096   146.4 / 140.6 / 138.8 / 138.7
+  //   8192   8 trees of 64 nodes on 16384       135.5 / 117.9 / 110.7 / 109.7
+  //   12288  32 trees of 5 - 24 nodes           186.9 / 177.6 / 175.7 / 172.3
+  return pairs * a.requests <= 2048 ? launch_merge<D, 8>(a, pairs, stream)
                                     : launch_merge<D, 1>(a, pairs, stream);
 }
 
