@@ -14,8 +14,9 @@
 // and the last term, the same for every output, is the accumulator's start: the
 // product of x with a constant. Both are summed in fp32, whose step is 2^-16 of
 // bf16's; where that gives no finite sum, it is taken again without the constant
-// (plain_sum). With fp16 the code becomes 1024 + q (or 1024 + 16 q) and one packed
-// add (or fma) gives q - z exactly.
+// (plain_sum). With fp16 the code becomes 1024 + q (or 1024 + 16 q), a number below
+// 2^10 or-ed into the mantissa of 1024 (a common way to make fp16 of small whole
+// numbers), and one packed add (or fma) gives q - z exactly.
 //
 // Layout. Weights are stored in tiles of 16 outputs x 128 inputs, 1 KiB each:
 // lane (n, g) of a wave holds output n's codes of inputs 32 j + 8 g .. + 7 as
@@ -35,8 +36,8 @@
 // atomics, the same bits every time.
 //
 // Measured (bf16, groups of 128 unless said): 1 row x 49536 x 4096 21.6 us, 4.85 TB/s
-// (a large copy 4.8); 61 rows x 11264 x 4096 12.5 us, bound by its few steps in
-// series; 250 rows x 22528 x 4096, groups of 64 with zero points, 65 us, 0.71
+// (a large copy 4.8); 61 rows x 11264 x 4096 12.7 us, bound by its few steps in
+// series; 250 rows x 22528 x 4096, groups of 64 with zero points, 66 us, 0.70
 // PFLOP/s: vector issue, unpacking for each block of 64 rows.
 #include "qsa_common.h"
 #include "../../include/qsa_hip.h"
@@ -564,6 +565,11 @@ hipError_t launch_many(Int4Args a, hipStream_t stream) {
 //   one / two a CU    8.3/12.5   10.1/16  12.3/20.5  28.5/45     35/58
 // A larger block unpacks each weight for more rows and loads less, a smaller
 // one fills the card sooner: the least max(one, two ceil(blocks / CUs) / 2).
+// Groups of 128 in fp16 take about the same times. Zero points cost the 32 x 96 blocks
+// more than the others (us, 32 x 64 / 32 x 96 / 64 x 128 at 4096 inputs, groups of
+// 64: 61 rows x 11264 18.0 / 20.8 / 31.7, 61 x 22528 26.9 / 30.6 / 32.1, 17 x 49536
+// 37.3 / 54.4 / 48.6; groups of 32: 61 x 22528 29.3 / 32.0 / 35.9), which this rule
+// does not know: it takes 32 x 96 in these four.
 enum RowsShape { k32x32, k32x64, k32x96, k64x128, k64x192, kRowsShapes };
 RowsShape pick_rows_shape(int rows, int n_tiles) {
   static constexpr struct {
@@ -589,14 +595,17 @@ RowsShape pick_rows_shape(int rows, int n_tiles) {
 
 template <typename T, int GROUP, bool ZEROS>
 hipError_t launch_rows(const Int4Args& a, bool vec, hipStream_t stream) {
-  if (!vec)  // rows that no 16-byte load can take
+  // Rows that no 16-byte load can take, element by element (11264 x 4095 at 1 / 16 /
+  // 61 / 250 rows 21 / 60 / 215 / 829 us; 11264 x 4096 7.5 / 9.9 / 13.7 / 38).
+  if (!vec)
     return a.rows <= 16 ? launch_few<T, GROUP, ZEROS, 1, 1, false>(a, 8, stream)
                         : launch_few<T, GROUP, ZEROS, 2, 1, false>(a, 8, stream);
   // To 16 rows: more outputs a wave (and fewer waves) share the activations'
   // loads and the closing sum, once there are enough of them for every CU
   // (K = 4096, us for 1 / 2 / 4 n tiles a wave. 1 row: 11264 outputs 7.1 / 8.0 /
   // 8.4, 22528 11.8 / 10.8 / 12.0, 49536 28.4 / 21.9 / 22.5; 16 rows: 2048
-  // 6.7 / 7.0 / 8.3, 8832 14.5 / 11.2 / 9.2, 49536 52 / 35 / 28).
+  // 6.7 / 7.0 / 8.3, 8832 14.5 / 11.2 / 9.2, 49536 52 / 35 / 28. In between, groups
+  // of 32 with zero points: 7 rows x 11264 11.1 / 10.9 / 12.1, x 22528 18.2 / 14.1 / 16.5).
   if (a.rows <= 4)
     return a.n_tiles < 1024 ? launch_few<T, GROUP, ZEROS, 1, 1, true>(a, 8, stream)
                             : launch_few<T, GROUP, ZEROS, 1, 2, true>(a, 4, stream);

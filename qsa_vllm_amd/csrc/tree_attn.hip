@@ -42,8 +42,8 @@
 // others are written at once.
 //
 // What bounds it (16 query and 2 kv heads of 128, pages of 16): single tokens and
-// small trees read HBM (64 single tokens on 1024 - 8192 tokens 69 us, 4.3 TB/s of
-// K/V; a large copy 4.8); 32 trees of 5 - 24 nodes on 4096 - 32768 tokens, 176 us,
+// small trees read HBM (64 single tokens on 1024 - 8192 tokens 69 us, 4.4 TB/s of
+// K/V; a large copy 4.8); 32 trees of 5 - 24 nodes on 4096 - 32768 tokens, 174 us,
 // a workgroup's stages in series (2.9 us each; the second tiles of requests past
 // 16 nodes add to them, though reading K/V once for both measured no faster);
 // 64 nodes on 131072 tokens, 103 us, the matrix cores with the softmax between
@@ -204,6 +204,8 @@ __device__ __forceinline__ int locate(const TreeArgs& a, int tile, int& place) {
   return a.requests;
 }
 
+// sigmoid(g), 0 and 1 at the infinities. The hardware's exponential and reciprocal:
+// off by 2^-20 for gates to 10, by 2^-17 for the least: far inside the output's 2^-8.
 __device__ __forceinline__ float gate_factor(uint16_t g) {
   return __builtin_amdgcn_rcpf(1.0f + __expf(-__builtin_bit_cast(float, (uint32_t)g << 16)));
 }

@@ -56,7 +56,9 @@ def process_logits(
     Row r belongs to request ``token_to_req[r]`` (int32; without it, to request
     r); rows of no request (negative or too large) get their grammar mask alone.
     All of the requests' tensors must have as many entries (rows).
-    In this order, each rule left out where its tensors are None:
+    In this order (penalties before biases: an engine that adds biases first gives
+    other logits to tokens that have both), each rule left out where its tensors
+    are None:
 
     * ``history`` int32 ``[requests, width]`` holds a request's tokens, the first
       ``history_lens`` of them valid and the first ``prompt_lens`` of those (0

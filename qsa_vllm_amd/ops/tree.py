@@ -8,6 +8,8 @@ order. Which nodes a row sees is a bit row (``ancestors``), made from parent
 indices by ``tree_ancestors``; a chain of drafted tokens, or a single token, is
 a tree too. Unlike ``qsa_sparse_paged_attention`` nothing is selected: rows
 attend over the whole committed context, whose K/V are read once for all nodes.
+So past the number of tokens that a sparse layer selects, the result is not that
+layer's.
 """
 
 from __future__ import annotations
