@@ -502,8 +502,9 @@ int qsa_gdn_gated_norm(const void* o, const void* qkvz, int64_t qkvz_stride, con
  *          inputs past in_features hold their zero point.
  * group_size 32, 64 or 128. bias may be null. Infinities and NaN in a row of x
  * give what the sum gives, for that row alone; such results (and those of bf16
- * values past 2^112) are computed apart and slowly. Any alignment and row stride of x and y; 16-byte aligned rows
- * of x and in_features a multiple of 8 are fastest. At most 2^30 inputs. */
+ * values past 2^112) are computed apart and slowly. Any alignment and row stride of
+ * x and y; 16-byte aligned rows of x and in_features a multiple of 8 are fastest. At
+ * most 2^30 inputs. */
 int qsa_int4_linear(const void* x, int64_t x_row_stride, const void* codes, const void* scales,
                     const void* zeros, const void* bias, void* y, int64_t y_row_stride, int rows,
                     int out_features, int in_features, int group_size, int is_fp16, void* stream);

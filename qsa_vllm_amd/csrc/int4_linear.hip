@@ -277,7 +277,8 @@ __device__ __forceinline__ uint32_t store(const Int4Args& a, int m0, int tile, i
 // One result as its formula has it, term by term. Infinities in x, or bf16 values
 // past 2^112, make the offset's product and the codes' cancel to NaN, and padded
 // inputs repeat the row's first ones, which may be infinite: a sum that is not
-// finite is taken again here. (A NaN in x ends it at once.)
+// finite is taken again here, a result a lane. A NaN in x ends it at once; an infinity
+// at the end of one row, or of each, of 61 rows x 11264 x 4096 takes 0.4 or 2.6 ms.
 template <typename T, int GROUP, bool ZEROS>
 __device__ __forceinline__ float plain_sum(const Int4Args& a, int m, int col) {
   constexpr int kGroups = kTileK / GROUP;

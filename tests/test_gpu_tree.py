@@ -558,3 +558,41 @@ def test_served_lengths(ctx, nodes, heads, kv_heads, dim, page):
                        + (2 * 36 * 2 ** -24 * spread + 2 ** -18) * (p[:, None] * v.abs()).sum(0))
                 tol = off + 2 ** -8 * (o.abs() + off)
                 assert ((got[row, h] - o).abs() <= tol).all(), (b, j, h)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("longest", [None, 0])
+def test_keys_and_values_in_caches_of_their_own(dim, longest):
+    """K and V of unlike strides: tokens before heads in one, heads before tokens
+    with a margin around each row in the other; a gate of any strides."""
+    c = Case([333, 64, 5], [7, 20, 1], heads=8, kv_heads=2, dim=dim, gate=True, seed=27)
+    k = c.kv[..., :dim].contiguous().to(DEV)
+    blocks, page = c.kv.shape[:2]
+    wide = torch.full((blocks, 2, page, dim + 24), float("nan"), dtype=torch.bfloat16, device=DEV)
+    v = wide.permute(0, 2, 1, 3)[..., 8:8 + dim]
+    v.copy_(c.kv[..., dim:])
+    gate = c.gate.permute(2, 0, 1).contiguous().to(DEV).permute(1, 2, 0)
+    got = qsa_tree_paged_attention(
+        c.q.to(DEV), k, v, c.table.to(DEV), torch.tensor(c.ctx, dtype=torch.int32, device=DEV),
+        c.qsl.to(DEV), c.anc.to(DEV), output_gate=gate, max_query_len=20,
+        max_context_len=max(c.ctx) if longest is None else longest)
+    c.check(got)
+
+
+def test_a_padded_batch():
+    """Requests behind the last one (no rows, whatever their lengths and pages) and
+    rows behind the last request: the others are right, those rows left."""
+    c = Case([500, 90], [9, 4], heads=8, kv_heads=2, seed=28)
+    k, v = c.device_cache()
+    i32 = dict(dtype=torch.int32, device=DEV)
+    table = torch.cat([c.table, torch.full((3, c.table.shape[1]), 2**31 - 1, dtype=torch.int32)]).to(DEV)
+    ctx = torch.tensor(c.ctx + [2**31 - 1, -5, 7], **i32)
+    qsl = torch.tensor([0, 9, 13, 13, 13, 13], **i32)
+    q = torch.cat([c.q, torch.full((6, 8, 128), float("nan"), dtype=torch.bfloat16)]).to(DEV)
+    anc = torch.nn.functional.pad(c.anc, (0, 0, 0, 6), value=-1).to(DEV)
+    out = torch.full_like(q, 5.0)
+    for longest in (500, 0):
+        qsa_tree_paged_attention(q, k, v, table, ctx, qsl, anc, out, max_query_len=9,
+                                 max_context_len=longest)
+        c.check(out[:13])
+        assert (out[13:] == 5).all()
