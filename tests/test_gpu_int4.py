@@ -316,3 +316,21 @@ def test_a_nan_row_ends_at_once():
             times[name] = min(times.get(name, 1e9), a.elapsed_time(b))
     assert out[20:].isnan().all() and torch.isfinite(out[:20]).all()
     assert times["dirty"] < 4 * times["clean"], times
+
+
+@pytest.mark.parametrize("rows,n,dtype", [(1 << 20, 4096, torch.bfloat16), (150000, 99072, torch.float16)])
+def test_millions_of_blocks(rows, n, dtype):
+    """Launches of many blocks, to the last row and output."""
+    k = 128
+    if torch.cuda.mem_get_info()[0] < (64 << 30):
+        pytest.skip("needs 64 GiB of free GPU memory")
+    gen = torch.Generator(device=DEV).manual_seed(rows)
+    codes = torch.randint(0, 16, (n, k), generator=gen, device=DEV, dtype=torch.uint8)
+    scales = torch.full((n, 1), 0.125, dtype=dtype, device=DEV)
+    w = int4_pack(codes, scales)
+    x = torch.randint(-2, 3, (rows, k), generator=gen, device=DEV, dtype=torch.int8).to(dtype)
+    got = int4_linear(x, w)
+    weight = w.dequantize()
+    for part in (slice(0, 70), slice(rows // 2, rows // 2 + 70), slice(rows - 70, rows)):
+        # multiples of 2^-3 below 2^12: exact in fp32 in any order
+        assert torch.equal(got[part], (x[part].float() @ weight.t()).to(dtype))
