@@ -572,6 +572,98 @@ int qsa_process_logits(const void* logits, int logits_type, int64_t logits_row_s
                        const int32_t* ancestors, int64_t ancestor_row_stride, int ancestor_words,
                        const int32_t* query_start_loc, void* stream);
 
+/* ------------------------------------------------------------------------ */
+/* Attention layers over the whole context or a window: no counterpart in the */
+/* reference                                                                  */
+/* ------------------------------------------------------------------------ */
+
+/* A KV cache held in 4 bits: data [blocks, kv_heads, page bytes], any block and
+ * head strides of multiples of 16 bytes. A page of one kv head holds, for its
+ * page_size tokens, the K codes (head_dim / 2 bytes a token), the V codes, the K
+ * words and the V words (a 16-bit word for each group of 32 dims, little end
+ * first), both word blocks filled up to 16 bytes. A group's word: zero point z in
+ * the low four bits, the others a bf16 scale s of four significant bits; the values
+ * are (code - z) * s, bf16 values exactly. Code words of 8 dims, 32 bits: V's word w
+ * holds dims 8 w .., 4 bits a dim in order; K's word b * head_dim / 32 + a holds dims
+ * 32 a + 8 b .., dim 2 i in bits 4 i .., dim 2 i + 1 in bits 16 + 4 i ...
+ * qsa_kv4_page_bytes: the bytes of such a page (0 for head dims but 64 and 128). */
+int64_t qsa_kv4_page_bytes(int page_size, int head_dim);
+
+/* Norm and rotation of query and key heads, K and V into the paged cache, in one
+ * launch: per (token, head) row, in fp32 and rounded once, x / sqrt(mean(x^2) + eps)
+ * * weight (no norm where the weight is null), then dims i and i + rotary_dim / 2
+ * rotated by the position's row of cos_sin [max_positions, rotary_dim] (cosines, then
+ * sines; fp32 or bf16; rotary_dim 0: no rotation; positions outside the table give
+ * zeros in those dims). Values are taken as they are. query may be null (no query
+ * heads), value too (without a cache). q_out, k_out and v_out [tokens, heads, dim]
+ * receive the rows (k_out and v_out may be null; an output may be its input). With a
+ * cache, K and V go to slot_mapping's slots (block * page_size + place; others than
+ * the cache's are passed over; one slot twice is undefined): cache_bits 16, k_cache
+ * and v_cache [blocks, page, kv_heads, dim] bf16; or cache_bits 4, k_cache the data
+ * above with k_block_stride and k_cache_head_stride in bytes (the other cache
+ * arguments are not read), and k_out and v_out then receive the values that the cache
+ * holds. Codes: s = (max(x, 0) - min(x, 0)) / 15 of the group, raised to four
+ * significant bits (2^-100 at least); z = round(-min(x, 0) / s); round(x / s) + z within
+ * 0 .. 15. A group with an infinity, a NaN or a value from 2^126 on reads as NaN.
+ * Rows, weights, table and caches 16-byte aligned, strides multiples of 8 elements.
+ * head_dim 64 or 128; rotary_dim a multiple of 16. */
+int qsa_qk_norm_rope(const void* query, int64_t q_token_stride, int64_t q_head_stride,
+                     int num_q_heads, const void* key, int64_t k_token_stride,
+                     int64_t k_head_stride, const void* value, int64_t v_token_stride,
+                     int64_t v_head_stride, int num_kv_heads, int head_dim, int tokens,
+                     const void* q_weight, const void* k_weight, float eps,
+                     const int64_t* positions, const void* cos_sin, int cos_sin_fp32,
+                     int max_positions, int rotary_dim, void* q_out, int64_t q_out_token_stride,
+                     int64_t q_out_head_stride, void* k_out, int64_t k_out_token_stride,
+                     int64_t k_out_head_stride, void* v_out, int64_t v_out_token_stride,
+                     int64_t v_out_head_stride, int cache_bits, const int64_t* slot_mapping,
+                     void* k_cache, int64_t k_block_stride, int64_t k_cache_token_stride,
+                     int64_t k_cache_head_stride, void* v_cache, int64_t v_block_stride,
+                     int64_t v_cache_token_stride, int64_t v_cache_head_stride, int num_blocks,
+                     int page_size, void* stream);
+
+/* Causal attention over the paged cache. Request b owns rows query_start_loc[b] ..
+ * query_start_loc[b + 1] - 1 of q [rows, num_q_heads, head_dim] bf16, the last tokens
+ * of its seq_lens[b]: row i of n is at position p = seq_lens[b] - n + i and sees the
+ * cached positions j <= p with j > p - window or j < sink_tokens (window 0: all of
+ * them) that have a page in the cache. out = softmax of the scaled scores times V,
+ * times sigmoid(gate) if gate is given, rounded once to bf16; zeros for a row that sees
+ * nothing. Rows of no request are not written. Infinities and NaN in K or V reach the
+ * rows that see them, as arithmetic has it (an infinite score gives NaN, an infinite
+ * value an infinity or NaN), and no others. A score of minus infinity weighs nothing; a
+ * row that has no other gets zeros. max_query_len bounds a request's rows (further
+ * ones are not computed); max_seq_len should bound seq_lens: it shapes the launch only.
+ * q and the caches are 16-byte aligned with strides of multiples of 8 elements; a cache
+ * spans less than 64 GiB from its first row to its last. head_dim 64 or 128. The
+ * workspace (0 bytes: none) holds the call's partial results until its work is done:
+ * calls that may overlap need one each. qsa_int4_kv_attention: the same over a 4-bit
+ * cache (block and head strides in bytes). */
+size_t qsa_paged_attention_workspace_bytes(int rows, int requests, int num_q_heads,
+                                           int num_kv_heads, int head_dim, int window,
+                                           int sink_tokens, int max_query_len, int max_seq_len);
+int qsa_window_attention(const void* q, int64_t q_row_stride, int64_t q_head_stride, int rows,
+                         int num_q_heads, int head_dim, const void* k_cache,
+                         int64_t k_block_stride, int64_t k_token_stride, int64_t k_head_stride,
+                         const void* v_cache, int64_t v_block_stride, int64_t v_token_stride,
+                         int64_t v_head_stride, int num_blocks, int page_size, int num_kv_heads,
+                         const int32_t* block_table, int64_t table_row_stride, int table_width,
+                         int num_requests, const int32_t* seq_lens,
+                         const int32_t* query_start_loc, int window, int sink_tokens, void* out,
+                         int64_t out_row_stride, int64_t out_head_stride, const void* gate,
+                         int64_t gate_row_stride, int64_t gate_head_stride,
+                         int64_t gate_dim_stride, int max_query_len, int max_seq_len,
+                         void* workspace, size_t workspace_bytes, void* stream);
+int qsa_int4_kv_attention(const void* q, int64_t q_row_stride, int64_t q_head_stride, int rows,
+                          int num_q_heads, int head_dim, const void* cache, int64_t block_stride,
+                          int64_t head_stride, int num_blocks, int page_size, int num_kv_heads,
+                          const int32_t* block_table, int64_t table_row_stride, int table_width,
+                          int num_requests, const int32_t* seq_lens,
+                          const int32_t* query_start_loc, int window, int sink_tokens, void* out,
+                          int64_t out_row_stride, int64_t out_head_stride, const void* gate,
+                          int64_t gate_row_stride, int64_t gate_head_stride,
+                          int64_t gate_dim_stride, int max_query_len, int max_seq_len,
+                          void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

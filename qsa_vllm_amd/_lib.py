@@ -192,6 +192,23 @@ SIGNATURES = {
         c_ptr, c_i64, c_i32, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_i64,
         c_ptr, c_i64, c_i32, c_ptr, c_i64, c_ptr, c_ptr, c_i64, c_i32, c_ptr,
         c_ptr]),
+    "qsa_kv4_page_bytes": (c_i64, [
+        c_i32, c_i32]),
+    "qsa_qk_norm_rope": (c_i32, [
+        c_ptr, c_i64, c_i64, c_i32, c_ptr, c_i64, c_i64, c_ptr, c_i64, c_i64, c_i32, c_i32,
+        c_i32, c_ptr, c_ptr, ctypes.c_float, c_ptr, c_ptr, c_i32, c_i32, c_i32, c_ptr, c_i64,
+        c_i64, c_ptr, c_i64, c_i64, c_ptr, c_i64, c_i64, c_i32, c_ptr, c_ptr, c_i64, c_i64,
+        c_i64, c_ptr, c_i64, c_i64, c_i64, c_i32, c_i32, c_ptr]),
+    "qsa_paged_attention_workspace_bytes": (c_size, [
+        c_i32, c_i32, c_i32, c_i32, c_i32, c_i32, c_i32, c_i32, c_i32]),
+    "qsa_window_attention": (c_i32, [
+        c_ptr, c_i64, c_i64, c_i32, c_i32, c_i32, c_ptr, c_i64, c_i64, c_i64, c_ptr, c_i64,
+        c_i64, c_i64, c_i32, c_i32, c_i32, c_ptr, c_i64, c_i32, c_i32, c_ptr, c_ptr, c_i32,
+        c_i32, c_ptr, c_i64, c_i64, c_ptr, c_i64, c_i64, c_i64, c_i32, c_i32, c_ptr, c_size, c_ptr]),
+    "qsa_int4_kv_attention": (c_i32, [
+        c_ptr, c_i64, c_i64, c_i32, c_i32, c_i32, c_ptr, c_i64, c_i64, c_i32, c_i32, c_i32,
+        c_ptr, c_i64, c_i32, c_i32, c_ptr, c_ptr, c_i32, c_i32, c_ptr, c_i64, c_i64, c_ptr,
+        c_i64, c_i64, c_i64, c_i32, c_i32, c_ptr, c_size, c_ptr]),
 }
 
 

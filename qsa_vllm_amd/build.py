@@ -26,7 +26,7 @@ OBJ_DIR = PACKAGE_DIR / "_build"
 
 SOURCES = ["qsa_errors.hip", "prepare.hip", "topk.hip", "indexer.hip", "sparse_attn.hip",
            "sparse_attn_wide.hip", "hybrid.hip", "gdn_scan.hip", "int4_linear.hip",
-           "tree_attn.hip", "logits.hip"]
+           "tree_attn.hip", "logits.hip", "head_rope.hip", "paged_attn.hip"]
 
 # Packed fp32 VALU ops are disabled: the kernels get no benefit from them and
 # some of their forms are not trusted on this hardware.

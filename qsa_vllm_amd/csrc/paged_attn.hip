@@ -1,0 +1,884 @@
+// Causal attention over the paged cache, whole or windowed, bf16 or 4 bits, gfx950.
+//
+// Request b's rows of this step are its last tokens: row i of n has position
+// p = length - n + i, and attends over the positions j <= p with j > p - window or
+// j < sinks (all of them without a window):
+//
+//   o = sum_j e^{s_j - m} v_j / sum_j e^{s_j - m},   s_j = q . k_j / sqrt(D)
+//
+// in one pass with a running maximum and sum, then sigmoid(gate) if given. A row
+// that sees nothing gets zeros.
+//
+// A workgroup takes a tile of 32 W (token, head) rows of one kv head, 32 a wave, and
+// streams the positions that any of them sees through LDS, 64 a stage:
+//
+//   S^T[token][row] = K (A, 32 tokens x 16 dims) Q^T (B, 16 dims x 32 rows)
+//   O^T[dim][row]  += V^T (A, 32 dims x 16 tokens) P^T (B, 16 tokens x 32 rows)
+//
+// on mfma_f32_32x32x16_bf16. P^T is the lane's own exponentials, so it never leaves
+// registers; V^T comes from row-major V rows in LDS by the transposing LDS read. The
+// exponentials are rounded to bf16, the matrix cores' type (2^-8 of a weight at
+// most), and the rounded ones are what is summed, in fp32: the weights that meet V
+// add up to 1. They are taken from a base that follows the row's maximum only when
+// that has passed it by 2^8, so that most stages rescale nothing.
+//
+// A 4-bit cache (kv4.h) is taken apart on the way into LDS: its values are bf16
+// values, exactly, and the rest is the same.
+#include "qsa_common.h"
+#include "../../include/qsa_hip.h"
+#include "kv4.h"
+
+#include <algorithm>
+#include <climits>
+
+namespace qsa {
+namespace {
+
+constexpr float kNegInf = -__builtin_huge_valf();
+constexpr int kCUs = 256;
+constexpr int kTok = 64;  // tokens of a stage
+constexpr uint32_t kNoToken = 0xFFFFFFFFu;
+constexpr int kNoWindow = INT_MAX / 2;  // past every position
+constexpr float kSlack = 8.0f;  // log2: how far scores may pass the exponents' base
+// s_waitcnt for the vector-memory counter alone (gfx9 encoding), at 0.
+constexpr int kLoadsDone = (7 << 4) | (15 << 8);
+
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+
+struct PagedArgs {
+  const uint16_t* q;
+  int64_t q_row, q_head;  // elements
+  // bf16: both caches, strides in units of 16 bytes, heads in bytes. 4 bits: k is the
+  // data, kb its block stride in units of 16 bytes and kh its head stride.
+  const char* k;
+  const char* v;
+  uint32_t kb, kt, vb, vt;
+  int64_t kh, vh;
+  int num_blocks, page_size;
+  FastDiv page_div;
+  const int32_t* table;
+  int64_t table_row;
+  int table_width;
+  int requests;
+  const int32_t* seq_lens;
+  const int32_t* query_start_loc;
+  int window, sinks;  // window: kNoWindow for none
+  uint16_t* out;
+  int64_t out_row, out_head;
+  const uint16_t* gate;
+  int64_t g_row, g_head, g_dim;
+  float* part_out;  // [pieces][tile rows][D], normalised
+  float* part_lse;  // [pieces][tile rows], log2
+  int rows, num_q_heads, kv_heads, group;
+  FastDiv group_div;
+  int max_rows;   // a request's rows at most
+  int splits;     // pieces of a tile's positions
+  int tiles;      // of the launch
+  float scale_log2;
+};
+
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+
+// One request's rows and tokens, kept within the query tensor and the page table
+// whatever the device arrays say.
+struct Request {
+  int row0, rows;   // rows that are computed
+  int first;        // position of row 0, negative where the length is too short
+  int length;       // tokens within the table
+};
+__device__ __forceinline__ Request make_request(const PagedArgs& a, int first, int last, int length) {
+  Request r;
+  r.row0 = min(max(first, 0), a.rows);
+  const int rows = min(max(last, r.row0), a.rows) - r.row0;
+  r.rows = min(rows, a.max_rows);
+  const int len = min(max(length, 0), kNoWindow);
+  r.first = len - rows;
+  r.length = (int)min((int64_t)len, (int64_t)a.table_width * a.page_size);
+  return r;
+}
+__device__ __forceinline__ Request load_request(const PagedArgs& a, int b) {  // b: a lane's own
+  return make_request(a, a.query_start_loc[b], a.query_start_loc[b + 1], a.seq_lens[b]);
+}
+__device__ __forceinline__ Request uniform_request(const PagedArgs& a, int b) {  // b: the wave's
+  return make_request(a, load_uniform(a.query_start_loc + b), load_uniform(a.query_start_loc + b + 1),
+                      load_uniform(a.seq_lens + b));
+}
+template <int R>
+__device__ __forceinline__ int tiles_of(const PagedArgs& a, const Request& r) {
+  return (r.rows * a.group + R - 1) / R;
+}
+
+// The request that holds item `place` where request b has count(b) of them; `place`
+// becomes the place within it. a.requests if there are fewer.
+template <typename F>
+__device__ __forceinline__ int locate(const PagedArgs& a, int& place, F count) {
+  const int lane = threadIdx.x & 63;
+  for (int b0 = 0; b0 < a.requests; b0 += 64) {
+    const int n = b0 + lane < a.requests ? count(load_request(a, b0 + lane)) : 0;
+    int end = n;  // inclusive sum over the lanes
+#pragma unroll
+    for (int w = 1; w < 64; w *= 2) {
+      const int below = __shfl_up(end, w, 64);
+      end += lane >= w ? below : 0;
+    }
+    const uint64_t past = __ballot(end > place);
+    if (past) {
+      const int at = __ffsll((unsigned long long)past) - 1;
+      place = uniform(place - __shfl(end - n, at, 64));
+      return b0 + at;
+    }
+    place = uniform(place - __shfl(end, 63, 64));
+  }
+  return a.requests;
+}
+
+// The positions that rows at p_lo .. p_hi see, as stages of 64.
+struct Span {
+  int p_lo, p_hi, end;           // end: past the last position that a row may see
+  int sink_stages, main, count;  // main: the first stage of the window
+  __device__ __forceinline__ int base(int stage) const {
+    return (stage < sink_stages ? stage : main + stage - sink_stages) * kTok;
+  }
+};
+__device__ __forceinline__ Span make_span(const PagedArgs& a, const Request& r, int i_lo, int i_hi) {
+  Span s;
+  s.p_lo = r.first + i_lo;
+  s.p_hi = r.first + i_hi;
+  s.end = max(0, min(s.p_hi + 1, r.length));
+  const int begin = max(0, min(s.p_lo - a.window + 1, s.end));
+  s.main = begin / kTok;
+  const int sink_end = min(a.sinks, s.end);
+  s.sink_stages = min((sink_end + kTok - 1) / kTok, s.main);
+  s.count = s.sink_stages + max(0, (s.end + kTok - 1) / kTok - s.main);
+  return s;
+}
+// Bits 0 .. n - 1.
+__device__ __forceinline__ uint64_t below(int n) {
+  return n <= 0 ? 0 : n >= 64 ? ~0ull : (1ull << n) - 1;
+}
+// What the row at position p sees of base .. base + 63.
+__device__ __forceinline__ uint64_t seen_from(const PagedArgs& a, int p, int base) {
+  return below(p + 1 - base) & (~below(p - a.window + 1 - base) | below(a.sinks - base));
+}
+// Whether the rows of a span see the stage differently.
+__device__ __forceinline__ bool is_mixed(const PagedArgs& a, const Span& s, int base) {
+  return base + kTok - 1 > s.p_lo || (base <= s.p_hi - a.window && base + kTok > a.sinks);
+}
+
+// sigmoid(g), 0 and 1 at the infinities. The hardware's exponential and reciprocal:
+// off by 2^-20 for gates to 10, by 2^-17 for the least: far inside the output's 2^-8.
+__device__ __forceinline__ float gate_factor(uint16_t g) {
+  return __builtin_amdgcn_rcpf(1.0f + __expf(-bf16_lo(g)));
+}
+
+// Byte offset of 16-byte unit `unit` of token `tok`'s row in a K stage: units are
+// permuted by the token so that 8 tokens' same unit (what one pass of the A
+// operand's read takes) lie in different banks.
+template <int D>
+__device__ __forceinline__ int k_swizzle(int tok) {
+  return D == 128 ? tok & 15 : (tok >> 1) & 7;
+}
+template <int D>
+__device__ __forceinline__ int k_at(int tok, int unit) {
+  return (tok * (D / 8) + (unit ^ k_swizzle<D>(tok))) * 16;
+}
+// The same for V, permuted in 32-byte units (what the transposing read takes).
+template <int D>
+__device__ __forceinline__ int v_swizzle(int tok) {
+  return D == 128 ? (tok & 7) << 1 : ((tok >> 1) & 3) << 1;
+}
+template <int D>
+__device__ __forceinline__ int v_at(int tok, int unit) {
+  return (tok * (D / 8) + (unit ^ v_swizzle<D>(tok))) * 16;
+}
+
+// Lane i of 16 passes the address of 4 dims of token i / 4 and gets dim i of the four.
+__device__ __forceinline__ s16x4 read_transposed(const char* p) {
+  return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p);
+}
+__device__ __forceinline__ void load_to_lds(const char* src, char* dst) {  // 16 bytes a lane
+  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src,
+                                   (__attribute__((address_space(3))) void*)dst, 16, 0, 0);
+}
+
+// Whether any of eight bf16 values is an infinity or NaN; and 0 in their place.
+__device__ __forceinline__ bool not_finite(const u32x4& v) {
+  bool bad = false;
+#pragma unroll
+  for (int w = 0; w < 4; ++w)
+    bad |= (v[w] & 0x7F80u) == 0x7F80u || (v[w] & 0x7F800000u) == 0x7F800000u;
+  return bad;
+}
+__device__ __forceinline__ u32x4 finite_or_zero(u32x4 v) {
+#pragma unroll
+  for (int w = 0; w < 4; ++w)
+    v[w] &= ((v[w] & 0x7F80u) == 0x7F80u ? 0u : 0xFFFFu) |
+            ((v[w] & 0x7F800000u) == 0x7F800000u ? 0u : 0xFFFF0000u);
+  return v;
+}
+
+// max over the two lanes of a query row.
+__device__ __forceinline__ float max_over_halves(float v) {
+  const uint32_t b = __builtin_bit_cast(uint32_t, v);
+  const auto r = __builtin_amdgcn_permlane32_swap(b, b, false, false);
+  return fmaxf(__builtin_bit_cast(float, (uint32_t)r[0]), __builtin_bit_cast(float, (uint32_t)r[1]));
+}
+// c + both halves of a pair of bf16 values.
+__device__ __forceinline__ float add_pair(uint32_t pair, float c) {
+  typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+  return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, pair),
+                                         __builtin_bit_cast(bf16x2, 0x3F803F80u), c, false);
+}
+
+// 8 codes (a word of kv4.h) as bf16 values in dim order.
+template <bool K>
+__device__ __forceinline__ u32x4 values4(uint32_t codes, uint32_t word) {
+  const float s = __builtin_bit_cast(float, (word & 0xFFF0u) << 16);
+  const float z = (float)(word & 15u);
+  u32x4 r;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float c0 = (float)(codes >> (K ? 4 * i : 8 * i) & 15u);
+    const float c1 = (float)(codes >> (K ? 4 * i + 16 : 8 * i + 4) & 15u);
+    // (exact in bf16, so the packing truncates nothing)
+    r[i] = perm_b32(__builtin_bit_cast(uint32_t, (c1 - z) * s),
+                    __builtin_bit_cast(uint32_t, (c0 - z) * s), 0x07060302u);
+  }
+  return r;
+}
+
+template <int D, int W, bool KV4>
+__global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(2, 2))) void
+paged_tile_kernel(PagedArgs a) {
+  constexpr int R = 32 * W;          // rows of the tile
+  constexpr int U = D / 8;           // 16-byte units of a row
+  constexpr int kSteps = D / 16;     // products of a score
+  constexpr int kDims = D / 32;
+  constexpr int kStage = kTok * D * 2;                    // bytes of K or V of a stage
+  constexpr int kLoads = 2 * kTok * U / (64 * W);         // 16-byte loads of a lane, K then V
+  constexpr int kCodes = kLoads / 2;                      // pairs of code words of a lane, K then V
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+
+  const int lane = threadIdx.x & 63;
+  const int wave = uniform(threadIdx.x >> 6);
+  const int n = lane & 31, h = lane >> 5;
+
+  // Which tile: kv heads innermost, then the pieces, then the tiles.
+  const int kv = blockIdx.x % a.kv_heads;
+  const int split = blockIdx.x / a.kv_heads % a.splits;
+  const int tile_id = blockIdx.x / a.kv_heads / a.splits;
+  int tile = tile_id;
+  const int b = locate(a, tile, [&](const Request& r) { return tiles_of<R>(a, r); });
+  if (b >= a.requests) return;
+  const Request rq = uniform_request(a, b);
+  // The last rows see most: they come first.
+  tile = tiles_of<R>(a, rq) - 1 - tile;
+  const int rows = rq.rows * a.group, m0 = tile * R;
+  const Span span = make_span(a, rq, a.group_div.div(m0), a.group_div.div(min(m0 + R, rows) - 1));
+  const int s_begin = (int)((int64_t)span.count * split / a.splits);
+  const int s_end = (int)((int64_t)span.count * (split + 1) / a.splits);
+  const int32_t* const trow = a.table + b * a.table_row;
+
+  // The lane's query row, dims 16 s + 8 h .. + 7.
+  const int m = min(m0 + wave * 32 + n, rows - 1);
+  const int node = a.group_div.div(m);
+  const int head = kv * a.group + m - node * a.group;
+  const int pos = rq.first + node;
+  bf16x8 q[kSteps];
+  {
+    const uint16_t* src = a.q + (int64_t)(rq.row0 + node) * a.q_row + head * a.q_head;
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s)
+      q[s] = __builtin_bit_cast(bf16x8, load_u32x4(src + 16 * s + 8 * h));
+  }
+
+  // Page of token base + lane, -1 past the end or where the table has none.
+  auto load_page = [&](int stage) {
+    const int at = stage < s_end ? span.base(stage) + lane : INT_MAX;
+    return *(at < span.end ? trow + a.page_div.div(at) : g_qsa_no_page);
+  };
+  // Offsets (16-byte units) of token base + lane.
+  struct Places {
+    uint32_t k, v;
+    int at;
+    uint64_t valid;
+  };
+  auto places = [&](int stage, int page) {
+    Places p;
+    const int t = span.base(stage) + lane;
+    const bool ok = page >= 0 && page < a.num_blocks;
+    p.at = t - a.page_div.div(t) * a.page_size;
+    p.k = !ok ? kNoToken : page * a.kb + (KV4 ? 0 : p.at * a.kt);
+    p.v = page * a.vb + p.at * a.vt;
+    p.valid = __ballot(ok);
+    return p;
+  };
+  const char* const zero = reinterpret_cast<const char*>(g_qsa_zero_rows);
+
+  // bf16: straight into LDS. Block i of a stage (64 units) is moved by wave i mod W, and
+  // a lane's unit of a row is the same in all its blocks of K (or V).
+  auto start_loads = [&](const Places& p, char* stage) {
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      const bool is_v = i >= kLoads / 2;
+      const int block = (i % (kLoads / 2)) * W + wave;
+      const int tok = block * (64 / U) + lane / U;
+      const int unit = lane % U ^ (is_v ? v_swizzle<D>(tok) : k_swizzle<D>(tok));
+      const uint32_t ko = __builtin_amdgcn_ds_bpermute(4 * tok, p.k);
+      const uint32_t o = is_v ? __builtin_amdgcn_ds_bpermute(4 * tok, p.v) : ko;
+      const char* src = (is_v ? a.v + kv * a.vh : a.k + kv * a.kh) + ((uint64_t)o << 4);
+      src = (ko != kNoToken ? src : zero) + unit * 16;
+      load_to_lds(src, stage + (is_v ? kStage : 0) + block * 1024);
+    }
+  };
+  // 4 bits: codes and words into registers, values into LDS a stage later. Pair i of a
+  // lane is two words of a token's K (first half of the pairs) or V codes.
+  u32x2 codes[KV4 ? kCodes : 1];
+  uint32_t words[KV4 ? kCodes : 1];
+  const Kv4Page lay{a.page_size, D};
+  constexpr int kPairs = kTok * (D / 16);  // of K, and of V
+  auto load_codes = [&](const Places& p) {
+#pragma unroll
+    for (int i = 0; i < kCodes; ++i) {
+      const int pair = i * 64 * W + threadIdx.x;
+      const bool is_v = pair >= kPairs;
+      const int at = pair % kPairs, tok = at / (D / 16), part = at % (D / 16);
+      const uint32_t o = __builtin_amdgcn_ds_bpermute(4 * tok, p.k);
+      const int place = __builtin_amdgcn_ds_bpermute(4 * tok, p.at);
+      const char* const src = a.k + kv * a.kh + ((uint64_t)o << 4);
+      const char* c = src + (is_v ? lay.v_codes() : 0) + (int64_t)place * lay.row() + part * 8;
+      // K: words of groups 2 (part % (D / 64)) and the next. V: both of one group.
+      const char* w = src + (is_v ? lay.v_words() : lay.k_words()) + (int64_t)place * lay.words() +
+                      (is_v ? part / 2 * 2 : part % (D / 64) * 4);
+      const bool ok = o != kNoToken;
+      codes[i] = load_u32x2(ok ? c : zero);
+      const uint16_t* w16 = reinterpret_cast<const uint16_t*>(ok ? w : zero);
+      words[i] = w16[0] | (uint32_t)w16[is_v ? 0 : 1] << 16;
+    }
+  };
+  auto store_values = [&](char* stage) {
+#pragma unroll
+    for (int i = 0; i < kCodes; ++i) {
+      const int pair = i * 64 * W + threadIdx.x;
+      const bool is_v = pair >= kPairs;
+      const int at = pair % kPairs, tok = at / (D / 16), part = at % (D / 16);
+      if (!is_v) {
+        // word 2 part of b D / 32 + a: group a, dims 8 b ..
+        const int first = 2 * part % (D / 32), b8 = 2 * part / (D / 32);
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          *reinterpret_cast<u32x4*>(stage + k_at<D>(tok, 4 * (first + e) + b8)) =
+              values4<true>(codes[i][e], words[i] >> (16 * e));
+      } else {
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          *reinterpret_cast<u32x4*>(stage + kStage + v_at<D>(tok, 2 * part + e)) =
+              values4<false>(codes[i][e], words[i] >> (16 * e));
+      }
+    }
+  };
+
+  f32x16 o[kDims];
+#pragma unroll
+  for (int d = 0; d < kDims; ++d)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) o[d][r] = 0.0f;
+  float sum = 0.0f, base = kNegInf;  // base: what the exponents are taken from
+  const float slack = kSlack / a.scale_log2;
+  bool poisoned = false;
+
+  int buffer = 0;
+  uint64_t valid = 0, valid_next = 0;
+  if (s_begin < s_end) {
+    const Places p = places(s_begin, load_page(s_begin));
+    valid_next = p.valid;
+    if constexpr (KV4) {
+      load_codes(p);
+      store_values(lds);
+    } else {
+      start_loads(p, lds);
+    }
+  }
+  int page_next = load_page(s_begin + 1);
+
+  for (int stage = s_begin; stage < s_end; ++stage) {
+    char* const here = lds + buffer * 2 * kStage;
+    char* const next = lds + (buffer ^ 1) * 2 * kStage;
+    buffer ^= 1;
+    __builtin_amdgcn_s_waitcnt(kLoadsDone);
+    __syncthreads();  // the stage is in LDS, and the one before has been read by all
+    valid = valid_next;
+    if (stage + 1 < s_end) {
+      const Places p = places(stage + 1, page_next);
+      valid_next = p.valid;
+      if constexpr (KV4) load_codes(p);
+      else start_loads(p, next);
+    }
+    page_next = load_page(stage + 2);
+    const int t0 = span.base(stage);
+    const bool mixed = valid != ~0ull || is_mixed(a, span, t0);
+    if (mixed) {
+      // V may hold infinities or NaN that a row must not see (0 times them is NaN). The
+      // whole stage's are taken as 0 here, and added at the end to the rows that see them.
+      u32x4* const v = reinterpret_cast<u32x4*>(here + kStage);
+      bool bad = false;
+      for (int i = lane; i < kTok * U; i += 64) bad |= not_finite(v[i]);
+      if (__any(bad)) {  // every wave has looked at the whole stage
+        __syncthreads();
+        for (int i = threadIdx.x; i < kTok * U; i += 64 * W) v[i] = finite_or_zero(v[i]);
+        __syncthreads();
+        poisoned = true;
+      }
+    }
+
+    f32x16 sc[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) sc[u][r] = 0.0f;
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s) {
+        const bf16x8 kf =
+            __builtin_bit_cast(bf16x8, load_u32x4(here + k_at<D>(32 * u + n, 2 * s + h)));
+        sc[u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, q[s], sc[u], 0, 0, 0);
+      }
+    }
+    if (mixed) {
+      // bit 8 (r / 4) + r % 4 of each subtile's: the lane's token 8 (r / 4) + 4 h + r % 4
+      const uint64_t seen = (valid & seen_from(a, pos, t0)) >> (4 * h);
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          sc[u][r] = (seen >> (32 * u + 8 * (r / 4) + r % 4)) & 1 ? sc[u][r] : kNegInf;
+    }
+
+    float top = kNegInf;
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) top = fmaxf(top, sc[u][r]);
+    if (__any(top > base + slack)) {
+      // Only the rows that passed it: a row's bits are its own. (A row that has seen
+      // nothing yet has -inf, and so has one whose scores are NaN.)
+      const float row_top = max_over_halves(top);
+      const float to = row_top > base + slack ? row_top : base;
+      const float shrink = to == kNegInf ? 1.0f : fast_exp2((base - to) * a.scale_log2);
+      base = to;
+      sum *= shrink;
+#pragma unroll
+      for (int d = 0; d < kDims; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[d][r] *= shrink;
+    }
+
+    const float from = base == kNegInf ? 0.0f : -base * a.scale_log2;
+    const int vt = 4 * h + (lane & 15) / 4;  // the lane's token of a transposing read
+    const char* const v_lane = here + kStage + vt * D * 2 + (lane & 1) * 8;
+    const int v_unit = (lane >> 4 & 1) * 2 + (lane >> 1 & 1), v_swz = v_swizzle<D>(vt);
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      uint32_t p[8];  // weights of tokens 8 (i / 2) + 4 h + 2 (i % 2) .., bf16 pairs
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        p[i] = pack_bf16x2(fast_exp2(__builtin_fmaf(sc[u][2 * i], a.scale_log2, from)),
+                           fast_exp2(__builtin_fmaf(sc[u][2 * i + 1], a.scale_log2, from)));
+        sum = add_pair(p[i], sum);
+      }
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const bf16x8 pb = __builtin_bit_cast(
+            bf16x8, (u32x4{p[4 * half], p[4 * half + 1], p[4 * half + 2], p[4 * half + 3]}));
+#pragma unroll
+        for (int d = 0; d < kDims; ++d) {
+          const char* const src =
+              v_lane + (32 * u + 16 * half) * D * 2 + ((4 * d + v_unit) ^ v_swz) * 16;
+          const s16x4 v0 = read_transposed(src);
+          const s16x4 v1 = read_transposed(src + 8 * D * 2);
+          const s16x8 vf = __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7);
+          o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, vf), pb, o[d],
+                                                         0, 0, 0);
+        }
+      }
+    }
+    if constexpr (KV4) {
+      if (stage + 1 < s_end) store_values(next);
+    }
+  }
+  sum = sum_wave_halves(sum);
+
+  if (poisoned) {
+    for (int stage = s_begin; stage < s_end; ++stage) {
+      const int t0 = span.base(stage);
+      for (int i = 0; i < kTok && t0 + i < span.end; ++i) {
+        const int page = trow[a.page_div.div(t0 + i)];
+        if (page < 0 || page >= a.num_blocks) continue;
+        const int at = t0 + i - a.page_div.div(t0 + i) * a.page_size;
+        // A stage with a page missing is one that was looked at, as all mixed ones are.
+        if (!(is_mixed(a, span, t0) || t0 + kTok > span.end)) {
+          bool whole = true;
+          for (int k = 0; k < kTok; ++k) {
+            const int other = trow[a.page_div.div(t0 + k)];
+            whole &= other >= 0 && other < a.num_blocks;
+          }
+          if (whole) break;
+        }
+        if (!(seen_from(a, pos, t0) >> i & 1)) continue;
+#pragma unroll
+        for (int d = 0; d < kDims; ++d)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int dim = 32 * d + 8 * j + 4 * h;
+            if constexpr (KV4) {
+              const char* const src = a.k + kv * a.kh + ((uint64_t)((uint32_t)page * a.kb) << 4);
+              const uint32_t word = *reinterpret_cast<const uint16_t*>(
+                  src + lay.v_words() + (int64_t)at * lay.words() + d * 2);
+              if ((word & 0x7F80u) == 0x7F80u)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) o[d][4 * j + r] = __builtin_nanf("");
+            } else {
+              const char* const src = a.v + kv * a.vh +
+                                      ((uint64_t)((uint32_t)page * a.vb + (uint32_t)at * a.vt) << 4);
+              const u32x2 x = load_u32x2(src + dim * 2);
+#pragma unroll
+              for (int r = 0; r < 4; ++r) {
+                // (a positive weight times an infinity or NaN is the same)
+                const uint32_t bits = r & 1 ? x[r >> 1] & 0xFFFF0000u : x[r >> 1] << 16;
+                if ((bits & 0x7F800000u) == 0x7F800000u)
+                  o[d][4 * j + r] += __builtin_bit_cast(float, bits);
+              }
+            }
+          }
+      }
+    }
+  }
+
+  if (m0 + wave * 32 + n >= rows) return;
+  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;  // a row that sees nothing: zeros
+  if (a.splits > 1) {
+    const int64_t at =
+        (((int64_t)tile_id * a.kv_heads + kv) * a.splits + split) * R + wave * 32 + n;
+#pragma unroll
+    for (int d = 0; d < kDims; ++d)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        *reinterpret_cast<f32x4*>(a.part_out + at * D + 32 * d + 8 * j + 4 * h) =
+            f32x4{o[d][4 * j] * inv, o[d][4 * j + 1] * inv, o[d][4 * j + 2] * inv,
+                  o[d][4 * j + 3] * inv};
+    if (h == 0)
+      a.part_lse[at] = sum == 0.0f ? kNegInf : base * a.scale_log2 + __log2f(sum);
+    return;
+  }
+  uint16_t* const dst = a.out + (int64_t)(rq.row0 + node) * a.out_row + head * a.out_head;
+  const uint16_t* const gate =
+      a.gate ? a.gate + (int64_t)(rq.row0 + node) * a.g_row + head * a.g_head : nullptr;
+#pragma unroll
+  for (int d = 0; d < kDims; ++d)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      float y[4];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        y[r] = o[d][4 * j + r] * inv;
+        if (gate) y[r] *= gate_factor(gate[(32 * d + 8 * j + 4 * h + r) * a.g_dim]);
+      }
+      u32x2 w = {pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3])};
+      __builtin_memcpy(dst + 32 * d + 8 * j + 4 * h, &w, 8);
+    }
+}
+
+// Joins a tile's pieces in order: a workgroup for a row, D / 4 lanes a head.
+template <int D, int W>
+__global__ __launch_bounds__(256) void paged_merge_kernel(PagedArgs a) {
+  constexpr int R = 32 * W, kLanes = D / 4;
+  // The row's request: rows past the last one are of none.
+  const int row = blockIdx.x, wave_lane = threadIdx.x & 63;
+  int tiles = 0, b = -1;
+  for (int b0 = 0; b0 < a.requests; b0 += 64) {
+    Request r = {0, 0, 0, 0};
+    if (b0 + wave_lane < a.requests) r = load_request(a, b0 + wave_lane);
+    const uint64_t mine = __ballot(row >= r.row0 && row < r.row0 + r.rows);
+    const int at = mine ? __ffsll((unsigned long long)mine) - 1 : 64;
+    int before = wave_lane < at ? tiles_of<R>(a, r) : 0;
+#pragma unroll
+    for (int w = 32; w > 0; w /= 2) before += __shfl_xor(before, w, 64);
+    tiles += uniform(before);
+    if (mine) {
+      b = b0 + at;
+      break;
+    }
+  }
+  if (b < 0) return;
+  const Request rq = uniform_request(a, b);
+  for (int head = threadIdx.x / kLanes; head < a.num_q_heads; head += 256 / kLanes) {
+    const int lane = threadIdx.x % kLanes;
+    const int kv = a.group_div.div(head);
+    const int m = (row - rq.row0) * a.group + head - kv * a.group;
+    const int tile = tiles + tiles_of<R>(a, rq) - 1 - m / R;
+    if (tile >= a.tiles) return;  // (requests whose rows overlap)
+    const int64_t first = ((int64_t)tile * a.kv_heads + kv) * a.splits * R + m % R;
+    float top = kNegInf;
+    for (int s = 0; s < a.splits; ++s) top = fmaxf(top, a.part_lse[first + (int64_t)s * R]);
+    const float base = top == kNegInf ? 0.0f : top;
+    float sum = 0.0f;
+    f32x4 acc = {0, 0, 0, 0};
+    for (int s = 0; s < a.splits; ++s) {
+      const int64_t at = first + (int64_t)s * R;
+      const float f = fast_exp2(a.part_lse[at] - base);
+      const f32x4 part = *reinterpret_cast<const f32x4*>(a.part_out + at * D + 4 * lane);
+      sum += f;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) acc[r] += f * part[r];
+    }
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    float y[4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      y[r] = acc[r] * inv;
+      if (a.gate) y[r] *= gate_factor(a.gate[row * a.g_row + head * a.g_head + (4 * lane + r) * a.g_dim]);
+    }
+    u32x2 w = {pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3])};
+    __builtin_memcpy(a.out + row * a.out_row + head * a.out_head + 4 * lane, &w, 8);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Host side
+// ---------------------------------------------------------------------------
+
+struct PagedPlan {
+  int waves, splits;
+  int64_t tiles;  // of all requests, at most
+};
+
+// The bounds shape the launch: a longer context is computed whole all the same.
+PagedPlan make_plan(int rows, int requests, int num_q_heads, int num_kv_heads, int max_query_len,
+                    int max_seq_len, int window, int sinks) {
+  PagedPlan p;
+  const int64_t group = num_q_heads / num_kv_heads;
+  const int64_t most = std::min(max_query_len, rows) * group;
+  p.waves = most <= 64 ? 2 : most <= 128 ? 4 : 8;
+  const int64_t tile_rows = 32 * p.waves;
+  p.tiles = std::min<int64_t>((rows * group) / tile_rows + std::min(requests, rows),
+                              (int64_t)requests * ((most + tile_rows - 1) / tile_rows));
+  int64_t seen = std::min<int64_t>(max_seq_len, (int64_t)window + tile_rows / group + 1);
+  if (window < max_seq_len) seen += std::min(sinks, max_seq_len) + 2 * kTok;
+  const int64_t stages = (seen + kTok - 1) / kTok;
+  const int64_t units = std::max<int64_t>(p.tiles * num_kv_heads, 1);
+  p.splits = (int)std::max<int64_t>(1, std::min(2 * kCUs / units, stages / 4));
+  return p;
+}
+
+size_t workspace_of(const PagedPlan& p, int num_kv_heads, int head_dim) {
+  if (p.splits <= 1) return 0;
+  return (size_t)p.tiles * num_kv_heads * p.splits * 32 * p.waves * (head_dim + 1) * sizeof(float);
+}
+
+template <int D, int W, bool KV4>
+hipError_t launch_paged(const PagedArgs& a, int64_t tiles, hipStream_t stream) {
+  constexpr int kLds = 4 * kTok * D * 2;
+  static_assert(kLds <= 65536, "no attribute to set");
+  const int64_t grid = tiles * a.splits * a.kv_heads;
+  if (grid > UINT_MAX / (64 * W) || a.rows > (int)(UINT_MAX / 256)) return hipErrorInvalidConfiguration;
+  hipLaunchKernelGGL((paged_tile_kernel<D, W, KV4>), dim3((unsigned)grid), dim3(64 * W), kLds, stream, a);
+  const hipError_t err = hipGetLastError();
+  if (err != hipSuccess || a.splits <= 1) return err;
+  hipLaunchKernelGGL((paged_merge_kernel<D, W>), dim3((unsigned)a.rows), dim3(256), 0, stream, a);
+  return hipGetLastError();
+}
+template <int D, bool KV4>
+hipError_t launch_waves(const PagedArgs& a, const PagedPlan& p, hipStream_t stream) {
+  return p.waves == 2   ? launch_paged<D, 2, KV4>(a, p.tiles, stream)
+         : p.waves == 4 ? launch_paged<D, 4, KV4>(a, p.tiles, stream)
+                        : launch_paged<D, 8, KV4>(a, p.tiles, stream);
+}
+
+bool aligned16(const void* p) { return ((uintptr_t)p & 15u) == 0; }
+
+// Elements from a cache's first token row to its last, -1 if a stride is negative or
+// the span past 2^62.
+int64_t cache_span(int64_t blocks, int64_t block_stride, int64_t page, int64_t token_stride) {
+  if (block_stride < 0 || token_stride < 0 || block_stride >= INT64_MAX / 4 / (blocks + 1) ||
+      token_stride >= INT64_MAX / 4 / page)
+    return -1;
+  return blocks > 0 ? (blocks - 1) * block_stride + (page - 1) * token_stride : 0;
+}
+
+// What both entry points check and set; the caches are theirs.
+int run_paged(const std::string& name, PagedArgs a, bool kv4, const void* q, int64_t q_row_stride,
+              int64_t q_head_stride, int rows, int num_q_heads, int head_dim, int num_blocks,
+              int page_size, int num_kv_heads, const int32_t* block_table, int64_t table_row_stride,
+              int table_width, int num_requests, const int32_t* seq_lens,
+              const int32_t* query_start_loc, int window, int sink_tokens, void* out,
+              int64_t out_row_stride, int64_t out_head_stride, const void* gate,
+              int64_t gate_row_stride, int64_t gate_head_stride, int64_t gate_dim_stride,
+              int max_query_len, int max_seq_len, void* workspace, size_t workspace_bytes,
+              void* stream) {
+  if ((!block_table && table_width > 0) || !q || !seq_lens || !query_start_loc || !out)
+    return fail(QSA_ERR_INVALID, name + ": null tensor pointer");
+  if (!aligned16(q) || ((uintptr_t)out & 3u) || ((q_row_stride | q_head_stride) & 7) ||
+      ((out_row_stride | out_head_stride) & 1))
+    return fail(QSA_ERR_INVALID, name + ": q needs 16-byte alignment and strides of multiples of 8 "
+                                        "elements, out 4-byte alignment");
+  max_query_len = std::min(max_query_len, rows);
+  a.window = window > 0 ? std::min(window, kNoWindow) : kNoWindow;
+  if ((int64_t)rows * num_q_heads > INT_MAX / 2)
+    return fail(QSA_ERR_UNSUPPORTED, name + ": too many rows or heads");
+  const PagedPlan plan = make_plan(rows, num_requests, num_q_heads, num_kv_heads, max_query_len,
+                                   max_seq_len, a.window, sink_tokens);
+  const size_t need = workspace_of(plan, num_kv_heads, head_dim);
+  if (need && (!workspace || workspace_bytes < need || !aligned16(workspace)))
+    return fail(QSA_ERR_WORKSPACE, name + ": needs a 16-byte aligned workspace of " +
+                                       std::to_string(need) + " bytes");
+  if (need) {
+    a.part_out = static_cast<float*>(workspace);
+    a.part_lse = a.part_out + need / sizeof(float) / (head_dim + 1) * head_dim;
+  }
+  a.q = static_cast<const uint16_t*>(q);
+  a.q_row = q_row_stride;
+  a.q_head = q_head_stride;
+  a.num_blocks = num_blocks;
+  a.page_size = page_size;
+  a.page_div = FastDiv::make(page_size);
+  a.table = block_table;
+  a.table_row = table_row_stride;
+  a.table_width = table_width;
+  a.requests = num_requests;
+  a.seq_lens = seq_lens;
+  a.query_start_loc = query_start_loc;
+  a.sinks = sink_tokens;
+  a.out = static_cast<uint16_t*>(out);
+  a.out_row = out_row_stride;
+  a.out_head = out_head_stride;
+  a.gate = static_cast<const uint16_t*>(gate);
+  a.g_row = gate_row_stride;
+  a.g_head = gate_head_stride;
+  a.g_dim = gate_dim_stride;
+  a.rows = rows;
+  a.num_q_heads = num_q_heads;
+  a.kv_heads = num_kv_heads;
+  a.group = num_q_heads / num_kv_heads;
+  a.group_div = FastDiv::make(a.group);
+  a.max_rows = max_query_len;
+  a.splits = plan.splits;
+  a.tiles = (int)plan.tiles;
+  a.scale_log2 = 1.4426950408889634f / sqrtf((float)head_dim);
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  const hipError_t err = head_dim == 128 ? (kv4 ? launch_waves<128, true>(a, plan, s)
+                                                : launch_waves<128, false>(a, plan, s))
+                                         : (kv4 ? launch_waves<64, true>(a, plan, s)
+                                                : launch_waves<64, false>(a, plan, s));
+  if (err == hipErrorInvalidConfiguration)
+    return fail(QSA_ERR_UNSUPPORTED, name + ": too many requests, rows or heads");
+  if (err != hipSuccess) return fail(QSA_ERR_HIP, name + " launch: " + hipGetErrorString(err));
+  return QSA_OK;
+}
+
+// QSA_OK: go on; 1: nothing to do.
+int check_sizes(const std::string& name, int rows, int num_q_heads, int num_kv_heads, int head_dim,
+                int num_blocks, int page_size, int table_width, int num_requests, int window,
+                int sink_tokens, int max_query_len, int max_seq_len) {
+  if (rows < 0 || num_requests < 0 || num_blocks < 0 || table_width < 0 || max_query_len < 0 ||
+      max_seq_len < 0 || window < 0 || sink_tokens < 0)
+    return fail(QSA_ERR_INVALID, name + ": negative size");
+  if (rows == 0 || num_requests == 0 || max_query_len == 0) return 1;
+  if (head_dim != 64 && head_dim != 128)
+    return fail(QSA_ERR_UNSUPPORTED, name + ": head_dim must be 64 or 128");
+  if (num_kv_heads <= 0 || num_q_heads <= 0 || num_q_heads % num_kv_heads)
+    return fail(QSA_ERR_UNSUPPORTED, name + ": query heads must be a multiple of kv heads");
+  if (page_size <= 0) return fail(QSA_ERR_INVALID, name + ": page size must be positive");
+  return QSA_OK;
+}
+
+}  // namespace
+}  // namespace qsa
+
+using namespace qsa;
+
+extern "C" size_t qsa_paged_attention_workspace_bytes(int rows, int requests, int num_q_heads,
+                                                      int num_kv_heads, int head_dim, int window,
+                                                      int sink_tokens, int max_query_len,
+                                                      int max_seq_len) {
+  if (rows <= 0 || requests <= 0 || num_kv_heads <= 0 || num_q_heads < num_kv_heads ||
+      head_dim <= 0 || max_query_len <= 0 || max_seq_len < 0 || window < 0 || sink_tokens < 0)
+    return 0;
+  return workspace_of(make_plan(rows, requests, num_q_heads, num_kv_heads,
+                                std::min(max_query_len, rows), max_seq_len,
+                                window > 0 ? std::min(window, kNoWindow) : kNoWindow, sink_tokens),
+                      num_kv_heads, head_dim);
+}
+
+extern "C" int qsa_window_attention(
+    const void* q, int64_t q_row_stride, int64_t q_head_stride, int rows, int num_q_heads,
+    int head_dim, const void* k_cache, int64_t k_block_stride, int64_t k_token_stride,
+    int64_t k_head_stride, const void* v_cache, int64_t v_block_stride, int64_t v_token_stride,
+    int64_t v_head_stride, int num_blocks, int page_size, int num_kv_heads,
+    const int32_t* block_table, int64_t table_row_stride, int table_width, int num_requests,
+    const int32_t* seq_lens, const int32_t* query_start_loc, int window, int sink_tokens, void* out,
+    int64_t out_row_stride, int64_t out_head_stride, const void* gate, int64_t gate_row_stride,
+    int64_t gate_head_stride, int64_t gate_dim_stride, int max_query_len, int max_seq_len,
+    void* workspace, size_t workspace_bytes, void* stream) {
+  const std::string name = "qsa_window_attention";
+  const int st = check_sizes(name, rows, num_q_heads, num_kv_heads, head_dim, num_blocks, page_size,
+                             table_width, num_requests, window, sink_tokens, max_query_len,
+                             max_seq_len);
+  if (st) return st > 0 ? QSA_OK : st;
+  // (an empty cache has no address and is not read)
+  if ((!k_cache || !v_cache) && num_blocks > 0)
+    return fail(QSA_ERR_INVALID, name + ": null tensor pointer");
+  if (!aligned16(k_cache) || !aligned16(v_cache) ||
+      ((k_block_stride | k_token_stride | k_head_stride | v_block_stride | v_token_stride |
+        v_head_stride) & 7))
+    return fail(QSA_ERR_INVALID, name + ": the caches need 16-byte alignment and strides of "
+                                        "multiples of 8 elements");
+  // The kernel's offsets are 32-bit counts of 16 bytes.
+  const int64_t k_span = cache_span(num_blocks, k_block_stride, page_size, k_token_stride);
+  const int64_t v_span = cache_span(num_blocks, v_block_stride, page_size, v_token_stride);
+  if (k_span < 0 || v_span < 0 || std::max(k_span, v_span) / 8 >= kNoToken)
+    return fail(QSA_ERR_UNSUPPORTED, name + ": the cache must span under 64 GiB");
+  PagedArgs a = {};
+  a.k = static_cast<const char*>(k_cache);
+  a.v = static_cast<const char*>(v_cache);
+  a.kb = (uint32_t)(k_block_stride / 8);
+  a.kt = (uint32_t)(k_token_stride / 8);
+  a.kh = 2 * k_head_stride;
+  a.vb = (uint32_t)(v_block_stride / 8);
+  a.vt = (uint32_t)(v_token_stride / 8);
+  a.vh = 2 * v_head_stride;
+  return run_paged(name, a, false, q, q_row_stride, q_head_stride, rows, num_q_heads, head_dim,
+                   num_blocks, page_size, num_kv_heads, block_table, table_row_stride, table_width,
+                   num_requests, seq_lens, query_start_loc, window, sink_tokens, out,
+                   out_row_stride, out_head_stride, gate, gate_row_stride, gate_head_stride,
+                   gate_dim_stride, max_query_len, max_seq_len, workspace, workspace_bytes, stream);
+}
+
+extern "C" int qsa_int4_kv_attention(
+    const void* q, int64_t q_row_stride, int64_t q_head_stride, int rows, int num_q_heads,
+    int head_dim, const void* cache, int64_t block_stride, int64_t head_stride, int num_blocks,
+    int page_size, int num_kv_heads, const int32_t* block_table, int64_t table_row_stride,
+    int table_width, int num_requests, const int32_t* seq_lens, const int32_t* query_start_loc,
+    int window, int sink_tokens, void* out, int64_t out_row_stride, int64_t out_head_stride,
+    const void* gate, int64_t gate_row_stride, int64_t gate_head_stride, int64_t gate_dim_stride,
+    int max_query_len, int max_seq_len, void* workspace, size_t workspace_bytes, void* stream) {
+  const std::string name = "qsa_int4_kv_attention";
+  const int st = check_sizes(name, rows, num_q_heads, num_kv_heads, head_dim, num_blocks, page_size,
+                             table_width, num_requests, window, sink_tokens, max_query_len,
+                             max_seq_len);
+  if (st) return st > 0 ? QSA_OK : st;
+  if (!cache && num_blocks > 0) return fail(QSA_ERR_INVALID, name + ": null tensor pointer");
+  if (!aligned16(cache) || block_stride < 0 || head_stride < 0 || ((block_stride | head_stride) & 15))
+    return fail(QSA_ERR_INVALID, name + ": the cache needs 16-byte alignment and strides of "
+                                        "multiples of 16 bytes");
+  if (block_stride / 16 >= kNoToken || (int64_t)num_blocks * (block_stride / 16) >= kNoToken)
+    return fail(QSA_ERR_UNSUPPORTED, name + ": the cache must span under 64 GiB");
+  PagedArgs a = {};
+  a.k = static_cast<const char*>(cache);
+  a.kb = (uint32_t)(block_stride / 16);
+  a.kh = head_stride;
+  return run_paged(name, a, true, q, q_row_stride, q_head_stride, rows, num_q_heads, head_dim,
+                   num_blocks, page_size, num_kv_heads, block_table, table_row_stride, table_width,
+                   num_requests, seq_lens, query_start_loc, window, sink_tokens, out,
+                   out_row_stride, out_head_stride, gate, gate_row_stride, gate_head_stride,
+                   gate_dim_stride, max_query_len, max_seq_len, workspace, workspace_bytes, stream);
+}

@@ -992,6 +992,217 @@ void process_logits_impl(const Tensor& logits, const Tensor& out, const OptTenso
         "qsa_process_logits");
 }
 
+// --- attention layers over the whole context or a window ------------------------
+
+// [tokens, heads, dim] bf16 rows with unit dim stride.
+void head_rows(const Tensor& t, int64_t tokens, int64_t heads, int64_t dim, const char* name) {
+  dtype(t, at::kBFloat16, name);
+  QSA_REQUIRE(t.dim() == 3 && t.size(0) == tokens && t.size(1) == heads && t.size(2) == dim &&
+                  t.stride(2) == 1,
+              name, " must be [", tokens, ", ", heads, ", ", dim, "] with unit dim stride");
+}
+
+// A tensor that is written: no two elements at one address.
+void own_rows3(const Tensor& t, const char* name) {
+  if (t.numel() == 0) return;
+  const int64_t dim = t.size(2), row = sdim(t, 0), head = sdim(t, 1);
+  QSA_REQUIRE((t.size(1) == 1 || head >= dim) &&
+                  (t.size(0) == 1 || row >= (t.size(1) - 1) * head + dim ||
+                   (row >= dim && (t.size(1) == 1 || head >= (t.size(0) - 1) * row + dim))),
+              name, "'s rows must not overlap");
+}
+
+// A 4-bit cache's data [blocks, kv_heads, page bytes].
+void kv4_data(const Tensor& t, int64_t page_size, int64_t dim) {
+  dtype(t, at::kByte, "4-bit cache");
+  QSA_REQUIRE(page_size > 0 && page_size <= INT32_MAX, "page size is out of range: ", page_size);
+  QSA_REQUIRE(dim == 64 || dim == 128, "a 4-bit cache's head dim must be 64 or 128, got ", dim);
+  QSA_REQUIRE(t.dim() == 3 && t.stride(2) == 1 &&
+                  t.size(2) == qsa_kv4_page_bytes((int)page_size, (int)dim),
+              "a 4-bit cache must be [blocks, kv_heads, ",
+              qsa_kv4_page_bytes((int)page_size, (int)dim), "] with unit byte stride");
+}
+
+// Cache: none, k_cache and v_cache (page_size 0), or k_cache alone, the 4-bit data of
+// pages of page_size tokens.
+void qk_norm_rope_impl(const OptTensor& query, const Tensor& key, const OptTensor& value,
+                       const OptTensor& q_weight, const OptTensor& k_weight, double eps,
+                       const OptTensor& pos, const OptTensor& cos_sin, const OptTensor& q_out,
+                       const OptTensor& k_out, const OptTensor& v_out,
+                       const OptTensor& slot_mapping, const OptTensor& k_cache,
+                       const OptTensor& v_cache, int64_t page_size) {
+  const auto dev = on_gpu({&key, opt(query), opt(value), opt(q_weight), opt(k_weight), opt(pos),
+                           opt(cos_sin), opt(q_out), opt(k_out), opt(v_out), opt(slot_mapping),
+                           opt(k_cache), opt(v_cache)});
+  QSA_REQUIRE(key.dim() == 3, "key must be [tokens, kv_heads, dim]");
+  const int64_t tokens = key.size(0), hkv = key.size(1), dim = key.size(2);
+  head_rows(key, tokens, hkv, dim, "key");
+  if (value) head_rows(*value, tokens, hkv, dim, "value");
+  int64_t hq = 0;
+  QSA_REQUIRE(!query == !q_out, "query and q_out go together");
+  if (query) {
+    QSA_REQUIRE(query->dim() == 3, "query must be [tokens, heads, dim]");
+    hq = query->size(1);
+    head_rows(*query, tokens, hq, dim, "query");
+    head_rows(*q_out, tokens, hq, dim, "q_out");
+    own_rows3(*q_out, "q_out");
+  }
+  if (k_out) head_rows(*k_out, tokens, hkv, dim, "k_out");
+  if (v_out) head_rows(*v_out, tokens, hkv, dim, "v_out");
+  if (k_out) own_rows3(*k_out, "k_out");
+  if (v_out) own_rows3(*v_out, "v_out");
+  QSA_REQUIRE(!v_out || value, "v_out needs values");
+  if (q_weight) bf16_vec(*q_weight, dim, "q_weight");
+  if (k_weight) bf16_vec(*k_weight, dim, "k_weight");
+  int64_t rotary = 0, max_positions = 0;
+  if (cos_sin) {
+    QSA_REQUIRE(cos_sin->scalar_type() == at::kFloat || cos_sin->scalar_type() == at::kBFloat16,
+                "cos_sin must be fp32 or bf16, got ", cos_sin->scalar_type());
+    QSA_REQUIRE(cos_sin->dim() == 2 && cos_sin->is_contiguous(),
+                "cos_sin must be a contiguous [positions, rotary_dim] tensor");
+    QSA_REQUIRE(pos.has_value(), "a rotation needs positions");
+    positions(*pos, tokens, "positions");
+    max_positions = cos_sin->size(0);
+    rotary = cos_sin->size(1);
+  }
+  const int bits = !k_cache ? 0 : v_cache ? 16 : 4;
+  QSA_REQUIRE(k_cache || !v_cache, "v_cache without k_cache");
+  int64_t blocks = 0, page = page_size;
+  if (bits) {
+    QSA_REQUIRE(value && slot_mapping, "a cache needs values and a slot mapping");
+    positions(*slot_mapping, tokens, "slot_mapping");
+    blocks = k_cache->size(0);
+    if (bits == 16) {
+      dtype(*k_cache, at::kBFloat16, "k_cache");
+      dtype(*v_cache, at::kBFloat16, "v_cache");
+      QSA_REQUIRE(k_cache->dim() == 4 && k_cache->sizes() == v_cache->sizes() &&
+                      k_cache->size(2) == hkv && k_cache->size(3) == dim &&
+                      k_cache->stride(3) == 1 && v_cache->stride(3) == 1,
+                  "caches must be [blocks, page, kv_heads, dim] with unit dim stride");
+      page = k_cache->size(1);
+    } else {
+      kv4_data(*k_cache, page_size, dim);
+      QSA_REQUIRE(k_cache->size(1) == hkv, "the cache must have the kv heads of key");
+    }
+  }
+  if (tokens == 0 || (hq == 0 && hkv == 0)) return;
+  c10::hip::HIPGuard guard(dev.index());
+  auto ptr = [](const OptTensor& t) { return t ? t->data_ptr() : nullptr; };
+  auto stride = [](const OptTensor& t, int64_t d) { return t ? sdim(*t, d) : (int64_t)0; };
+  const bool wide = bits == 16;
+  check(qsa_qk_norm_rope(
+            ptr(query), stride(query, 0), stride(query, 1), as_int(hq, "query heads"),
+            key.data_ptr(), sdim(key, 0), sdim(key, 1), ptr(value), stride(value, 0),
+            stride(value, 1), as_int(hkv, "kv heads"), as_int(dim, "head dim"),
+            as_int(tokens, "tokens"), ptr(q_weight), ptr(k_weight), (float)eps,
+            pos ? at_elem<int64_t>(*pos) : nullptr, rotary ? ptr(cos_sin) : nullptr,
+            cos_sin && cos_sin->scalar_type() == at::kFloat ? 1 : 0,
+            as_int(max_positions, "positions of cos_sin"), as_int(rotary, "rotary dim"), ptr(q_out),
+            stride(q_out, 0), stride(q_out, 1), ptr(k_out), stride(k_out, 0), stride(k_out, 1),
+            ptr(v_out), stride(v_out, 0), stride(v_out, 1), bits,
+            slot_mapping ? at_elem<int64_t>(*slot_mapping) : nullptr, ptr(k_cache),
+            stride(k_cache, 0), wide ? stride(k_cache, 1) : 0, stride(k_cache, wide ? 2 : 1),
+            ptr(v_cache), stride(v_cache, 0), wide ? stride(v_cache, 1) : 0,
+            wide ? stride(v_cache, 2) : 0, as_int(blocks, "blocks"), as_int(page, "page size"),
+            stream_of(dev)),
+        "qsa_qk_norm_rope");
+}
+
+// What both caches' attention checks; returns whether there is anything to do.
+struct PagedCall {
+  int64_t rows, heads, dim, requests;
+  GateStrides gate;
+  int most, longest, window, sinks;
+};
+PagedCall paged_call(const Tensor& q, const Tensor& block_table, const Tensor& seq_lens,
+                     const Tensor& query_start_loc, const Tensor& out, const OptTensor& output_gate,
+                     int64_t window, int64_t sink_tokens, int64_t max_query_len,
+                     int64_t max_seq_len) {
+  PagedCall c;
+  dtype(q, at::kBFloat16, "q");
+  QSA_REQUIRE(q.dim() == 3 && q.stride(2) == 1, "q must be [rows, heads, dim] with unit dim stride");
+  c.rows = q.size(0);
+  c.heads = q.size(1);
+  c.dim = q.size(2);
+  check_out(out, c.rows, c.heads, c.dim);
+  own_rows3(out, "out");
+  table2d(block_table, "block_table");
+  c.requests = block_table.size(0);
+  vec(seq_lens, at::kInt, "seq_lens", c.requests);
+  vec(query_start_loc, at::kInt, "query_start_loc", c.requests + 1);
+  c.gate = gate_strides(output_gate, c.rows, c.heads, c.dim);
+  c.window = as_int(window, "window");
+  c.sinks = as_int(sink_tokens, "sink_tokens");
+  c.most = as_int(max_query_len, "max_query_len");
+  c.longest = as_int(max_seq_len, "max_seq_len");
+  return c;
+}
+
+void window_attention_impl(const Tensor& q, const Tensor& k_cache, const Tensor& v_cache,
+                           const Tensor& block_table, const Tensor& seq_lens,
+                           const Tensor& query_start_loc, const Tensor& out,
+                           const OptTensor& output_gate, int64_t window, int64_t sink_tokens,
+                           int64_t max_query_len, int64_t max_seq_len) {
+  const auto dev = on_gpu({&q, &k_cache, &v_cache, &block_table, &seq_lens, &query_start_loc, &out,
+                           opt(output_gate)});
+  const PagedCall c = paged_call(q, block_table, seq_lens, query_start_loc, out, output_gate, window,
+                                 sink_tokens, max_query_len, max_seq_len);
+  dtype(k_cache, at::kBFloat16, "k_cache");
+  dtype(v_cache, at::kBFloat16, "v_cache");
+  QSA_REQUIRE(k_cache.dim() == 4 && v_cache.dim() == 4 && k_cache.sizes() == v_cache.sizes(),
+              "k_cache/v_cache must be [blocks, page, kv_heads, dim] of one shape");
+  QSA_REQUIRE(k_cache.stride(3) == 1 && v_cache.stride(3) == 1, "k/v caches need a unit dim stride");
+  QSA_REQUIRE(k_cache.size(3) == c.dim, "cache head dim must match q");
+  if (c.rows == 0 || c.requests == 0) return;
+  c10::hip::HIPGuard guard(dev.index());
+  const int kv_heads = as_int(k_cache.size(2), "kv heads");
+  const size_t ws_bytes = qsa_paged_attention_workspace_bytes(
+      as_int(c.rows, "rows"), as_int(c.requests, "requests"), as_int(c.heads, "heads"), kv_heads,
+      (int)c.dim, c.window, c.sinks, c.most, c.longest);
+  Tensor ws = ws_bytes ? workspace(ws_bytes, dev) : Tensor();
+  check(qsa_window_attention(
+            q.data_ptr(), sdim(q, 0), sdim(q, 1), (int)c.rows, (int)c.heads, (int)c.dim,
+            k_cache.data_ptr(), sdim(k_cache, 0), sdim(k_cache, 1), sdim(k_cache, 2),
+            v_cache.data_ptr(), sdim(v_cache, 0), sdim(v_cache, 1), sdim(v_cache, 2),
+            as_int(k_cache.size(0), "blocks"), as_int(k_cache.size(1), "page size"), kv_heads,
+            at_elem<int32_t>(block_table), block_table.stride(0),
+            as_int(block_table.size(1), "table width"), (int)c.requests,
+            at_elem<int32_t>(seq_lens), at_elem<int32_t>(query_start_loc), c.window, c.sinks,
+            out.data_ptr(), sdim(out, 0), sdim(out, 1), ptr_or_null(opt(output_gate)), c.gate.row,
+            c.gate.head, c.gate.dim, c.most, c.longest, ws_bytes ? ws.data_ptr() : nullptr,
+            ws_bytes, stream_of(dev)),
+        "qsa_window_attention");
+}
+
+void int4_kv_attention_impl(const Tensor& q, const Tensor& cache, int64_t page_size,
+                            const Tensor& block_table, const Tensor& seq_lens,
+                            const Tensor& query_start_loc, const Tensor& out,
+                            const OptTensor& output_gate, int64_t window, int64_t sink_tokens,
+                            int64_t max_query_len, int64_t max_seq_len) {
+  const auto dev = on_gpu({&q, &cache, &block_table, &seq_lens, &query_start_loc, &out,
+                           opt(output_gate)});
+  const PagedCall c = paged_call(q, block_table, seq_lens, query_start_loc, out, output_gate, window,
+                                 sink_tokens, max_query_len, max_seq_len);
+  kv4_data(cache, page_size, c.dim);
+  if (c.rows == 0 || c.requests == 0) return;
+  c10::hip::HIPGuard guard(dev.index());
+  const int kv_heads = as_int(cache.size(1), "kv heads");
+  const size_t ws_bytes = qsa_paged_attention_workspace_bytes(
+      as_int(c.rows, "rows"), as_int(c.requests, "requests"), as_int(c.heads, "heads"), kv_heads,
+      (int)c.dim, c.window, c.sinks, c.most, c.longest);
+  Tensor ws = ws_bytes ? workspace(ws_bytes, dev) : Tensor();
+  check(qsa_int4_kv_attention(
+            q.data_ptr(), sdim(q, 0), sdim(q, 1), (int)c.rows, (int)c.heads, (int)c.dim,
+            cache.data_ptr(), sdim(cache, 0), sdim(cache, 1), as_int(cache.size(0), "blocks"),
+            (int)page_size, kv_heads, at_elem<int32_t>(block_table), block_table.stride(0),
+            as_int(block_table.size(1), "table width"), (int)c.requests,
+            at_elem<int32_t>(seq_lens), at_elem<int32_t>(query_start_loc), c.window, c.sinks,
+            out.data_ptr(), sdim(out, 0), sdim(out, 1), ptr_or_null(opt(output_gate)), c.gate.row,
+            c.gate.head, c.gate.dim, c.most, c.longest, ws_bytes ? ws.data_ptr() : nullptr,
+            ws_bytes, stream_of(dev)),
+        "qsa_int4_kv_attention");
+}
+
 }  // namespace
 
 TORCH_LIBRARY_FRAGMENT(yulan_qsa_kernels, m) {
@@ -1070,6 +1281,19 @@ TORCH_LIBRARY_FRAGMENT(yulan_qsa_kernels, m) {
       "Tensor? frequency, Tensor? presence, Tensor? bias_ids, Tensor? bias_values, "
       "Tensor? allowed, int vocab_start, Tensor? draft_tokens, Tensor? ancestors, "
       "Tensor? query_start_loc) -> ()");
+  m.def(
+      "qk_norm_rope(Tensor? query, Tensor key, Tensor? value, Tensor? q_weight, "
+      "Tensor? k_weight, float eps, Tensor? positions, Tensor? cos_sin, Tensor(a!)? q_out, "
+      "Tensor(b!)? k_out, Tensor(c!)? v_out, Tensor? slot_mapping, Tensor(d!)? k_cache, "
+      "Tensor(e!)? v_cache, int page_size) -> ()");
+  m.def(
+      "window_attention(Tensor q, Tensor k_cache, Tensor v_cache, Tensor block_table, "
+      "Tensor seq_lens, Tensor query_start_loc, Tensor(a!) out, Tensor? output_gate, int window, "
+      "int sink_tokens, int max_query_len, int max_seq_len) -> ()");
+  m.def(
+      "int4_kv_attention(Tensor q, Tensor cache, int page_size, Tensor block_table, "
+      "Tensor seq_lens, Tensor query_start_loc, Tensor(a!) out, Tensor? output_gate, int window, "
+      "int sink_tokens, int max_query_len, int max_seq_len) -> ()");
 }
 
 TORCH_LIBRARY_IMPL(yulan_qsa_kernels, CUDA, m) {
@@ -1091,6 +1315,9 @@ TORCH_LIBRARY_IMPL(yulan_qsa_kernels, CUDA, m) {
   m.impl("int4_linear", &int4_linear_impl);
   m.impl("tree_attention", &tree_attention_impl);
   m.impl("process_logits", &process_logits_impl);
+  m.impl("qk_norm_rope", &qk_norm_rope_impl);
+  m.impl("window_attention", &window_attention_impl);
+  m.impl("int4_kv_attention", &int4_kv_attention_impl);
 }
 
 // Shape-only tracing (fake / meta tensors): the ops mutate their outputs in
@@ -1151,4 +1378,14 @@ TORCH_LIBRARY_IMPL(yulan_qsa_kernels, Meta, m) {
             const OptTensor&, const OptTensor&, const OptTensor&, const OptTensor&,
             const OptTensor&, const OptTensor&, const OptTensor&, const OptTensor&, int64_t,
             const OptTensor&, const OptTensor&, const OptTensor&) {});
+  m.impl("qk_norm_rope",
+         [](const OptTensor&, const Tensor&, const OptTensor&, const OptTensor&, const OptTensor&,
+            double, const OptTensor&, const OptTensor&, const OptTensor&, const OptTensor&,
+            const OptTensor&, const OptTensor&, const OptTensor&, const OptTensor&, int64_t) {});
+  m.impl("window_attention", [](const Tensor&, const Tensor&, const Tensor&, const Tensor&,
+                                const Tensor&, const Tensor&, const Tensor&, const OptTensor&,
+                                int64_t, int64_t, int64_t, int64_t) {});
+  m.impl("int4_kv_attention", [](const Tensor&, const Tensor&, int64_t, const Tensor&,
+                                 const Tensor&, const Tensor&, const Tensor&, const OptTensor&,
+                                 int64_t, int64_t, int64_t, int64_t) {});
 }
