@@ -68,13 +68,17 @@ struct PagedArgs {
   int64_t out_row, out_head;
   const uint16_t* gate;
   int64_t g_row, g_head, g_dim;
-  float* part_out;  // [pieces][tile rows][D], normalised
+  float* part_out;  // tiles' pieces [pieces][tile rows][D], normalised
   float* part_lse;  // [pieces][tile rows], log2
+  float* row_out;   // the same of requests of few rows, [pieces][16][D]
+  float* row_lse;
   int rows, num_q_heads, kv_heads, group;
   FastDiv group_div;
   int max_rows;   // a request's rows at most
   int splits;     // pieces of a tile's positions
   int tiles;      // of the launch
+  int few;        // (row, head)s of a kv head up to which a request is one of few rows; 0: none is
+  int few_groups;  // workgroups of the launch for those, 0: one for each request and kv head
   float scale_log2;
 };
 
@@ -104,9 +108,12 @@ __device__ __forceinline__ Request uniform_request(const PagedArgs& a, int b) { 
   return make_request(a, load_uniform(a.query_start_loc + b), load_uniform(a.query_start_loc + b + 1),
                       load_uniform(a.seq_lens + b));
 }
+__device__ __forceinline__ bool is_few(const PagedArgs& a, const Request& r) {
+  return r.rows * a.group <= a.few;
+}
 template <int R>
 __device__ __forceinline__ int tiles_of(const PagedArgs& a, const Request& r) {
-  return (r.rows * a.group + R - 1) / R;
+  return is_few(a, r) ? 0 : (r.rows * a.group + R - 1) / R;
 }
 
 // The request that holds item `place` where request b has count(b) of them; `place`
@@ -133,24 +140,30 @@ __device__ __forceinline__ int locate(const PagedArgs& a, int& place, F count) {
   return a.requests;
 }
 
-// The positions that rows at p_lo .. p_hi see, as stages of 64.
+// The positions that rows at p_lo .. p_hi see, as stages of T.
+template <int T>
 struct Span {
   int p_lo, p_hi, end;           // end: past the last position that a row may see
   int sink_stages, main, count;  // main: the first stage of the window
   __device__ __forceinline__ int base(int stage) const {
-    return (stage < sink_stages ? stage : main + stage - sink_stages) * kTok;
+    return (stage < sink_stages ? stage : main + stage - sink_stages) * T;
+  }
+  // Whether the rows see the stage differently.
+  __device__ __forceinline__ bool mixed(const PagedArgs& a, int base) const {
+    return base + T - 1 > p_lo || (base <= p_hi - a.window && base + T > a.sinks);
   }
 };
-__device__ __forceinline__ Span make_span(const PagedArgs& a, const Request& r, int i_lo, int i_hi) {
-  Span s;
+template <int T>
+__device__ __forceinline__ Span<T> make_span(const PagedArgs& a, const Request& r, int i_lo, int i_hi) {
+  Span<T> s;
   s.p_lo = r.first + i_lo;
   s.p_hi = r.first + i_hi;
   s.end = max(0, min(s.p_hi + 1, r.length));
   const int begin = max(0, min(s.p_lo - a.window + 1, s.end));
-  s.main = begin / kTok;
+  s.main = begin / T;
   const int sink_end = min(a.sinks, s.end);
-  s.sink_stages = min((sink_end + kTok - 1) / kTok, s.main);
-  s.count = s.sink_stages + max(0, (s.end + kTok - 1) / kTok - s.main);
+  s.sink_stages = min((sink_end + T - 1) / T, s.main);
+  s.count = s.sink_stages + max(0, (s.end + T - 1) / T - s.main);
   return s;
 }
 // Bits 0 .. n - 1.
@@ -161,11 +174,6 @@ __device__ __forceinline__ uint64_t below(int n) {
 __device__ __forceinline__ uint64_t seen_from(const PagedArgs& a, int p, int base) {
   return below(p + 1 - base) & (~below(p - a.window + 1 - base) | below(a.sinks - base));
 }
-// Whether the rows of a span see the stage differently.
-__device__ __forceinline__ bool is_mixed(const PagedArgs& a, const Span& s, int base) {
-  return base + kTok - 1 > s.p_lo || (base <= s.p_hi - a.window && base + kTok > a.sinks);
-}
-
 // sigmoid(g), 0 and 1 at the infinities. The hardware's exponential and reciprocal:
 // off by 2^-20 for gates to 10, by 2^-17 for the least: far inside the output's 2^-8.
 __device__ __forceinline__ float gate_factor(uint16_t g) {
@@ -275,7 +283,7 @@ paged_tile_kernel(PagedArgs a) {
   // The last rows see most: they come first.
   tile = tiles_of<R>(a, rq) - 1 - tile;
   const int rows = rq.rows * a.group, m0 = tile * R;
-  const Span span = make_span(a, rq, a.group_div.div(m0), a.group_div.div(min(m0 + R, rows) - 1));
+  const Span<kTok> span = make_span<kTok>(a, rq, a.group_div.div(m0), a.group_div.div(min(m0 + R, rows) - 1));
   const int s_begin = (int)((int64_t)span.count * split / a.splits);
   const int s_end = (int)((int64_t)span.count * (split + 1) / a.splits);
   const int32_t* const trow = a.table + b * a.table_row;
@@ -402,10 +410,9 @@ paged_tile_kernel(PagedArgs a) {
   }
   int page_next = load_page(s_begin + 1);
 
-  for (int stage = s_begin; stage < s_end; ++stage) {
-    char* const here = lds + buffer * 2 * kStage;
-    char* const next = lds + (buffer ^ 1) * 2 * kStage;
-    buffer ^= 1;
+  // (The pointers are said to be apart: the compiler would otherwise wait for the loads
+  // into `next` before it reads V from `here`.)
+  auto step = [&](int stage, char* __restrict here, char* __restrict next) {
     __builtin_amdgcn_s_waitcnt(kLoadsDone);
     __syncthreads();  // the stage is in LDS, and the one before has been read by all
     valid = valid_next;
@@ -417,7 +424,7 @@ paged_tile_kernel(PagedArgs a) {
     }
     page_next = load_page(stage + 2);
     const int t0 = span.base(stage);
-    const bool mixed = valid != ~0ull || is_mixed(a, span, t0);
+    const bool mixed = valid != ~0ull || span.mixed(a, t0);
     if (mixed) {
       // V may hold infinities or NaN that a row must not see (0 times them is NaN). The
       // whole stage's are taken as 0 here, and added at the end to the rows that see them.
@@ -505,6 +512,10 @@ paged_tile_kernel(PagedArgs a) {
     if constexpr (KV4) {
       if (stage + 1 < s_end) store_values(next);
     }
+  };
+  for (int stage = s_begin; stage < s_end; ++stage) {
+    step(stage, lds + buffer * 2 * kStage, lds + (buffer ^ 1) * 2 * kStage);
+    buffer ^= 1;
   }
   sum = sum_wave_halves(sum);
 
@@ -516,7 +527,7 @@ paged_tile_kernel(PagedArgs a) {
         if (page < 0 || page >= a.num_blocks) continue;
         const int at = t0 + i - a.page_div.div(t0 + i) * a.page_size;
         // A stage with a page missing is one that was looked at, as all mixed ones are.
-        if (!(is_mixed(a, span, t0) || t0 + kTok > span.end)) {
+        if (!(span.mixed(a, t0) || t0 + kTok > span.end)) {
           bool whole = true;
           for (int k = 0; k < kTok; ++k) {
             const int other = trow[a.page_div.div(t0 + k)];
@@ -611,6 +622,7 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedArgs a) {
   }
   if (b < 0) return;
   const Request rq = uniform_request(a, b);
+  if (is_few(a, rq)) return;
   for (int head = threadIdx.x / kLanes; head < a.num_q_heads; head += 256 / kLanes) {
     const int lane = threadIdx.x % kLanes;
     const int kv = a.group_div.div(head);
@@ -644,43 +656,618 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedArgs a) {
 }
 
 // ---------------------------------------------------------------------------
+// Few rows
+// ---------------------------------------------------------------------------
+//
+// A request of at most 16 (row, head)s a kv head (single tokens, a few drafted ones)
+// is bound by its K/V, which one workgroup reads for all of its rows. The four waves
+// of a workgroup take blocks of positions in turn, each on its own: K goes from memory
+// into the matrix cores' operand registers, V through the wave's own LDS, so that no
+// wave waits for another until they join their results at the end. The scores are the
+// transposed products of 16 rows, mfma_f32_16x16x32_bf16, weights and sums as above.
+//
+// Work is shared out by blocks: requests of more blocks than an equal share of the
+// whole launch are cut into pieces, found on the device, which a second kernel joins.
+//
+// From a 4-bit cache the codes themselves are the matrix cores' operands, as the bf16
+// numbers 16 + c (a code's bits in the fraction of 16.0), and the groups' scales and
+// zero points come in afterwards, by 32 dims (one product):
+//
+//   s_t  = sum_G s_tG [ sum_d (16 + c_td) q_d  -  (16 + z_tG) sum_d q_d ]
+//   o_d += sum_t (p_t s_tG) (16 + c_td)  -  sum_t (p_t s_tG) (16 + z_tG)
+//
+// the last sum once a group, by one more product. p_t s_tG is rounded to bf16 for both.
+
+constexpr int kFew = 16;
+constexpr int kRowWaves = 4;
+constexpr int kMinBlocks = 8;  // of a piece
+
+template <int D, bool KV4>
+struct RowShape {
+  static constexpr int kBlock = KV4 ? 64 : 32;    // positions of a wave's block
+  static constexpr int kSub = kBlock / 16;
+  static constexpr int kGroups = D / 32;
+  static constexpr int kVRow = KV4 ? D / 2 : 2 * D;  // bytes of a V row in LDS
+  static constexpr int kV = kBlock * kVRow;
+  // 4 bits: K's scales, K's scales times 16 + z, V's scales (fp32), V's 16 + z (bf16)
+  static constexpr int kWords = KV4 ? kGroups * kBlock * 14 : 0;
+  static constexpr int kWave = 2 * kV + kWords;
+  static constexpr int kMerge = 16 * (D + 2) * 4;  // a wave's result
+  static constexpr int kLds = kRowWaves * (kWave > kMerge ? kWave : kMerge);
+};
+
+template <int T>
+__device__ __forceinline__ int blocks_of(const PagedArgs& a, const Request& r) {
+  return r.rows > 0 && is_few(a, r) ? make_span<T>(a, r, 0, r.rows - 1).count : 0;
+}
+// Blocks of a piece, such that all pieces are at most a.few_groups.
+template <int T>
+__device__ __forceinline__ int blocks_of_piece(const PagedArgs& a) {
+  if (!a.few_groups) return INT_MAX;
+  const int lane = threadIdx.x & 63;
+  int blocks = 0, units = 0;
+  for (int b = lane; b < a.requests; b += 64) {
+    const Request r = load_request(a, b);
+    blocks += blocks_of<T>(a, r);
+    units += r.rows > 0 && is_few(a, r);
+  }
+#pragma unroll
+  for (int w = 32; w > 0; w /= 2) {
+    blocks += __shfl_xor(blocks, w, 64);
+    units += __shfl_xor(units, w, 64);
+  }
+  // A request's last piece may be short: the pieces are at most total / per + units.
+  const unsigned total = uniform(blocks), spare = a.few_groups / a.kv_heads - uniform(units);
+  return max(kMinBlocks, (int)((total + spare - 1) / max(spare, 1u)));
+}
+template <int T>
+__device__ __forceinline__ int pieces_of(const PagedArgs& a, const Request& r, int per) {
+  if (r.rows <= 0 || !is_few(a, r)) return 0;
+  return max(1, (int)(((unsigned)blocks_of<T>(a, r) + (unsigned)per - 1u) / (unsigned)per));
+}
+
+// max over the four lanes of a query row.
+__device__ __forceinline__ float max_over_quarters(float v) {
+  v = max_over_halves(v);
+  const uint32_t b = __builtin_bit_cast(uint32_t, v);
+  const auto r = __builtin_amdgcn_permlane16_swap(b, b, false, false);
+  return fmaxf(__builtin_bit_cast(float, (uint32_t)r[0]), __builtin_bit_cast(float, (uint32_t)r[1]));
+}
+__device__ __forceinline__ float sum_over_quarters(float v) {
+  v = sum_wave_halves(v);
+  const uint32_t b = __builtin_bit_cast(uint32_t, v);
+  const auto r = __builtin_amdgcn_permlane16_swap(b, b, false, false);
+  return __builtin_bit_cast(float, (uint32_t)r[0]) + __builtin_bit_cast(float, (uint32_t)r[1]);
+}
+
+// Codes of nibbles i and i + 4 of a word, i = 0 .. 3, as bf16 pairs of 16 + c.
+__device__ __forceinline__ u32x4 codes_of(uint32_t w) {
+  u32x4 r;
+  r[0] = ((w << 3) & 0x00780078u) | 0x41804180u;
+  r[1] = ((w >> 1) & 0x00780078u) | 0x41804180u;
+  r[2] = ((w >> 5) & 0x00780078u) | 0x41804180u;
+  r[3] = ((w >> 9) & 0x00780078u) | 0x41804180u;
+  return r;
+}
+__device__ __forceinline__ f32x4 product(u32x4 a, u32x4 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a),
+                                                 __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+// Lane i of 16 passes the address of 16 codes (8 bytes) and gets code i of all 16.
+__device__ __forceinline__ u32x2 read_transposed4(const char* p) {
+  typedef int v2i __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(
+      u32x2, __builtin_amdgcn_ds_read_tr4_b64_v2i32((__attribute__((address_space(3))) v2i*)p));
+}
+// Where 16-byte unit `unit` of a token's V codes lies: the units of 64 tokens' same
+// place are spread over the banks.
+template <int D>
+__device__ __forceinline__ int v4_at(int tok, int unit) {
+  return tok * (D / 2) + (unit ^ (D == 128 ? tok >> 2 & 3 : tok >> 3 & 1)) * 16;
+}
+
+template <int D, bool KV4>
+__global__ __launch_bounds__(64 * kRowWaves) __attribute__((amdgpu_waves_per_eu(2, 3))) void
+paged_rows_kernel(PagedArgs a) {
+  typedef RowShape<D, KV4> S;
+  constexpr int T = S::kBlock;
+  constexpr int U = D / 8;
+  constexpr int kGroups = S::kGroups;  // of 32 dims: products of a score
+  constexpr int kDims = D / 16;
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  const int lane = threadIdx.x & 63;
+  const int wave = uniform(threadIdx.x >> 6);
+  const int n = lane & 15, g = lane >> 4;
+
+  const int per = blocks_of_piece<T>(a);
+  int place = blockIdx.x;
+  const int b = locate(a, place, [&](const Request& r) { return pieces_of<T>(a, r, per) * a.kv_heads; });
+  if (b >= a.requests) return;
+  const Request rq = uniform_request(a, b);
+  const int pieces = pieces_of<T>(a, rq, per);
+  const int kv = place / pieces, piece = place - kv * pieces;
+  const int rows = rq.rows * a.group;
+  const Span<T> span = make_span<T>(a, rq, 0, rq.rows - 1);
+  const int s_begin = (int)((int64_t)span.count * piece / pieces);
+  const int s_end = (int)((int64_t)span.count * (piece + 1) / pieces);
+  const int32_t* const trow = a.table + b * a.table_row;
+
+  // The lane's query row, dims 32 s + 8 g .. + 7.
+  const int m = min(n, rows - 1);
+  const int node = a.group_div.div(m);
+  const int head = kv * a.group + m - node * a.group;
+  const int pos = rq.first + node;
+  u32x4 q[kGroups];
+  {
+    const uint16_t* src = a.q + (int64_t)(rq.row0 + node) * a.q_row + head * a.q_head;
+#pragma unroll
+    for (int s = 0; s < kGroups; ++s) q[s] = load_u32x4(src + 32 * s + 8 * g);
+  }
+  float q_sum[kGroups];
+  if constexpr (KV4) {
+#pragma unroll
+    for (int s = 0; s < kGroups; ++s) {
+      float v = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v += bf16_lo(q[s][i]) + bf16_hi(q[s][i]);
+      q_sum[s] = sum_over_quarters(v);
+    }
+  }
+
+  char* const mine = lds + wave * S::kWave;
+  char* const words = mine + 2 * S::kV;
+  const char* const zero = reinterpret_cast<const char*>(g_qsa_zero_rows);
+  const Kv4Page lay{a.page_size, D};
+
+  auto load_page = [&](int block) {
+    const int at = block < s_end ? span.base(block) + lane % T : INT_MAX;
+    return *(at < span.end ? trow + a.page_div.div(at) : g_qsa_no_page);
+  };
+  // A block on its way: K in registers, V on its way into LDS.
+  struct Block {
+    u32x4 k[S::kSub][KV4 ? 1 : kGroups];
+    u32x2 kw, vw;  // 4 bits: the lane's token's words
+    uint64_t valid;
+  };
+  auto start = [&](int block, int page, char* v_lds) {
+    Block r;
+    const int t = span.base(block) + lane % T;
+    const bool ok = page >= 0 && page < a.num_blocks;
+    const int at = t - a.page_div.div(t) * a.page_size;
+    r.valid = __ballot(ok);
+    if constexpr (KV4) {
+      const uint32_t block_at = ok ? page * a.kb : kNoToken;
+      const char* const own = a.k + kv * a.kh + ((uint64_t)block_at << 4);
+#pragma unroll
+      for (int u = 0; u < S::kSub; ++u) {
+        const uint32_t o = __builtin_amdgcn_ds_bpermute(4 * (16 * u + n), block_at);
+        const int p = __builtin_amdgcn_ds_bpermute(4 * (16 * u + n), at);
+        const char* src = a.k + kv * a.kh + ((uint64_t)o << 4) + (int64_t)p * lay.row() + g * (D / 8);
+        src = o != kNoToken ? src : zero;
+        if constexpr (D == 128) {
+          r.k[u][0] = load_u32x4(src);
+        } else {
+          const u32x2 x = load_u32x2(src);
+          r.k[u][0] = u32x4{x[0], x[1], 0, 0};
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < S::kV / 1024; ++i) {
+        constexpr int kParts = D / 32;  // 16-byte units of a row
+        const int tok = i * (64 / kParts) + lane / kParts;
+        const int unit = (v4_at<D>(tok, lane % kParts) - tok * (D / 2)) / 16;
+        const uint32_t o = __builtin_amdgcn_ds_bpermute(4 * tok, block_at);
+        const int p = __builtin_amdgcn_ds_bpermute(4 * tok, at);
+        const char* src = a.k + kv * a.kh + ((uint64_t)o << 4) + lay.v_codes() +
+                          (int64_t)p * lay.row() + unit * 16;
+        load_to_lds(o != kNoToken ? src : zero, v_lds + i * 1024);
+      }
+      const char* kw = own + lay.k_words() + (int64_t)at * lay.words();
+      const char* vw = own + lay.v_words() + (int64_t)at * lay.words();
+      kw = ok ? kw : zero;
+      vw = ok ? vw : zero;
+      if constexpr (D == 128) {
+        r.kw = load_u32x2(kw);
+        r.vw = load_u32x2(vw);
+      } else {
+        r.kw = u32x2{*reinterpret_cast<const uint32_t*>(kw), 0};
+        r.vw = u32x2{*reinterpret_cast<const uint32_t*>(vw), 0};
+      }
+    } else {
+      const uint32_t k_at = ok ? page * a.kb + at * a.kt : kNoToken;
+      const uint32_t v_off = page * a.vb + at * a.vt;
+#pragma unroll
+      for (int u = 0; u < S::kSub; ++u) {
+        const uint32_t o = __builtin_amdgcn_ds_bpermute(4 * (16 * u + n), k_at);
+        const char* src = a.k + kv * a.kh + ((uint64_t)o << 4);
+        src = (o != kNoToken ? src : zero) + 16 * g;
+#pragma unroll
+        for (int s = 0; s < kGroups; ++s) r.k[u][s] = load_u32x4(src + 64 * s);
+      }
+#pragma unroll
+      for (int i = 0; i < S::kV / 1024; ++i) {
+        const int tok = i * (64 / U) + lane / U;
+        const int unit = lane % U ^ v_swizzle<D>(tok);
+        const uint32_t o = __builtin_amdgcn_ds_bpermute(4 * tok, v_off);
+        const uint32_t ko = __builtin_amdgcn_ds_bpermute(4 * tok, k_at);
+        const char* src = a.v + kv * a.vh + ((uint64_t)o << 4);
+        load_to_lds((ko != kNoToken ? src : zero) + unit * 16, v_lds + i * 1024);
+      }
+    }
+    return r;
+  };
+
+  f32x4 o[kDims], oz[KV4 ? kGroups : 1];
+#pragma unroll
+  for (int d = 0; d < kDims; ++d) o[d] = f32x4{0, 0, 0, 0};
+#pragma unroll
+  for (int s = 0; s < (KV4 ? kGroups : 1); ++s) oz[s] = f32x4{0, 0, 0, 0};
+  float sum = 0.0f, base = kNegInf;
+  const float slack = kSlack / a.scale_log2;
+  bool poisoned = false;
+
+  Block next = {};
+  int page_next = -1;
+  if (s_begin + wave < s_end) next = start(s_begin + wave, load_page(s_begin + wave), mine);
+  page_next = load_page(s_begin + wave + kRowWaves);
+
+  // (The pointers are said to be apart: the compiler would otherwise wait for the loads
+  // into `v_next` before it reads V.)
+  auto step = [&](int block, char* __restrict v_lds, char* __restrict v_next) {
+    __builtin_amdgcn_s_waitcnt(kLoadsDone);
+    asm volatile("" ::: "memory");  // nothing is read from LDS before
+    const Block now = next;
+    if (block + kRowWaves < s_end) next = start(block + kRowWaves, page_next, v_next);
+    page_next = load_page(block + 2 * kRowWaves);
+    const int t0 = span.base(block);
+    constexpr uint64_t kAll = T == 64 ? ~0ull : (1ull << (T % 64)) - 1;
+    const bool mixed = (now.valid & kAll) != kAll || span.mixed(a, t0);
+    const uint64_t seen = mixed ? now.valid & seen_from(a, pos, t0) : 0;  // of the lane's row
+
+    f32x4 sc[S::kSub];
+    if constexpr (KV4) {
+      // The lane's token's words, taken apart for all.
+      float* const ks = reinterpret_cast<float*>(words);
+      float* const kz = ks + kGroups * T;
+      float* const vs = kz + kGroups * T;
+      uint16_t* const vz = reinterpret_cast<uint16_t*>(vs + kGroups * T);
+#pragma unroll
+      for (int s = 0; s < kGroups; ++s) {
+        const uint32_t kw = now.kw[s / 2] >> (16 * (s % 2)), vw = now.vw[s / 2] >> (16 * (s % 2));
+        const float scale = __builtin_bit_cast(float, (kw & 0xFFF0u) << 16);
+        ks[s * T + lane] = scale;
+        kz[s * T + lane] = scale * (float)(16 + (kw & 15u));
+        vs[s * T + lane] = __builtin_bit_cast(float, (vw & 0xFFF0u) << 16);
+        // Token 16 u + 4 g' + r at the place of its code in the other operand.
+        const int u = lane >> 4, gt = lane >> 2 & 3, r = lane & 3;
+        vz[((s * 2 + u / 2) * 4 + gt) * 8 + r * 2 + u % 2] = (uint16_t)(0x4180u | (vw & 15u) << 3);
+      }
+#pragma unroll
+      for (int u = 0; u < S::kSub; ++u) {
+        sc[u] = f32x4{0, 0, 0, 0};
+#pragma unroll
+        for (int s = 0; s < kGroups; ++s) {
+          const f32x4 x = product(codes_of(now.k[u][0][s]), q[s], f32x4{0, 0, 0, 0});
+          const f32x4 scale = *reinterpret_cast<const f32x4*>(ks + s * T + 16 * u + 4 * g);
+          const f32x4 zero_at = *reinterpret_cast<const f32x4*>(kz + s * T + 16 * u + 4 * g);
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            sc[u][r] = __builtin_fmaf(scale[r], x[r], __builtin_fmaf(-zero_at[r], q_sum[s], sc[u][r]));
+        }
+      }
+    } else {
+      if (mixed) {
+        // V may hold infinities or NaN that a row must not see: as in the tiles' kernel.
+        u32x4* const v = reinterpret_cast<u32x4*>(v_lds);
+        bool bad = false;
+        for (int i = lane; i < T * U; i += 64) bad |= not_finite(v[i]);
+        if (__any(bad)) {
+          for (int i = lane; i < T * U; i += 64) v[i] = finite_or_zero(v[i]);
+          poisoned = true;
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < S::kSub; ++u) {
+        sc[u] = f32x4{0, 0, 0, 0};
+#pragma unroll
+        for (int s = 0; s < kGroups; ++s) sc[u] = product(now.k[u][s], q[s], sc[u]);
+      }
+    }
+    if (mixed) {
+#pragma unroll
+      for (int u = 0; u < S::kSub; ++u)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          sc[u][r] = seen >> (16 * u + 4 * g + r) & 1 ? sc[u][r] : kNegInf;
+    }
+
+    float top = kNegInf;
+#pragma unroll
+    for (int u = 0; u < S::kSub; ++u)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) top = fmaxf(top, sc[u][r]);
+    if (__any(top > base + slack)) {
+      const float row_top = max_over_quarters(top);
+      const float to = row_top > base + slack ? row_top : base;
+      const float shrink = to == kNegInf ? 1.0f : fast_exp2((base - to) * a.scale_log2);
+      base = to;
+      sum *= shrink;
+#pragma unroll
+      for (int d = 0; d < kDims; ++d)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) o[d][r] *= shrink;
+      if constexpr (KV4)
+#pragma unroll
+        for (int s = 0; s < kGroups; ++s)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) oz[s][r] *= shrink;
+    }
+    const float from = base == kNegInf ? 0.0f : -base * a.scale_log2;
+#pragma unroll
+    for (int u = 0; u < S::kSub; ++u)
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        sc[u][r] = fast_exp2(__builtin_fmaf(sc[u][r], a.scale_log2, from));
+
+    if constexpr (KV4) {
+      const float* const vs = reinterpret_cast<const float*>(words) + 2 * kGroups * T;
+      const uint16_t* const vz = reinterpret_cast<const uint16_t*>(vs + kGroups * T);
+#pragma unroll
+      for (int u = 0; u < S::kSub; ++u)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) sum += sc[u][r];
+      // The lane's V row of a transposing read: code i of its token, in the weights' order.
+      const int tok = 16 * (n >> 2) + 4 * g + (n & 3);
+#pragma unroll
+      for (int s = 0; s < kGroups; ++s) {
+        u32x4 p[2];  // weights times scales of subtiles 2 i and 2 i + 1, pairs by token
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          f32x4 w[2];
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int u = 2 * i + e;
+            w[e] = *reinterpret_cast<const f32x4*>(vs + s * T + 16 * u + 4 * g);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              // (a scale may be NaN: not in a place that the row does not see)
+              if (mixed) w[e][r] = seen >> (16 * u + 4 * g + r) & 1 ? w[e][r] : 0.0f;
+              w[e][r] *= sc[u][r];
+            }
+          }
+#pragma unroll
+          for (int r = 0; r < 4; ++r) p[i][r] = pack_bf16x2(w[0][r], w[1][r]);
+          oz[s] = product(load_u32x4(vz + ((s * 2 + i) * 4 + g) * 8), p[i], oz[s]);
+        }
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int d = 2 * s + e;
+          const u32x2 c = read_transposed4(v_lds + v4_at<D>(tok, d / 2) + d % 2 * 8);
+          o[d] = product(codes_of(c[0]), p[0], o[d]);
+          o[d] = product(codes_of(c[1]), p[1], o[d]);
+        }
+      }
+    } else {
+      u32x4 p;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        p[i] = pack_bf16x2(sc[i / 2][2 * (i % 2)], sc[i / 2][2 * (i % 2) + 1]);
+        sum = add_pair(p[i], sum);
+      }
+      const int vt = 4 * g + (n >> 2);
+      const char* const v_lane = v_lds + vt * D * 2 + (n & 1) * 8;
+      const int v_unit = (n & 3) >> 1, v_swz = v_swizzle<D>(vt);
+#pragma unroll
+      for (int d = 0; d < kDims; ++d) {
+        const char* const src = v_lane + ((2 * d + v_unit) ^ v_swz) * 16;
+        const s16x4 v0 = read_transposed(src), v1 = read_transposed(src + 16 * D * 2);
+        o[d] = product(__builtin_bit_cast(
+                           u32x4, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7)),
+                       p, o[d]);
+      }
+    }
+  };
+  int buffer = 0;
+  for (int block = s_begin + wave; block < s_end; block += kRowWaves) {
+    step(block, mine + buffer * S::kV, mine + (buffer ^ 1) * S::kV);
+    buffer ^= 1;
+  }
+  sum = sum_over_quarters(sum);
+  if constexpr (KV4) {
+#pragma unroll
+    for (int d = 0; d < kDims; ++d) o[d] -= oz[d / 2];
+  }
+
+  if (!KV4 && poisoned) {
+    for (int block = s_begin + wave; block < s_end; block += kRowWaves) {
+      const int t0 = span.base(block);
+      bool whole = t0 + T <= span.end;  // a page missing: a block that was looked at
+      for (int i = 0; i < T && t0 + i < span.end; ++i) {
+        const int page = trow[a.page_div.div(t0 + i)];
+        whole &= page >= 0 && page < a.num_blocks;
+      }
+      if (whole && !span.mixed(a, t0)) continue;
+      for (int i = 0; i < T && t0 + i < span.end; ++i) {
+        const int page = trow[a.page_div.div(t0 + i)];
+        if (page < 0 || page >= a.num_blocks || !(seen_from(a, pos, t0) >> i & 1)) continue;
+        const int at = t0 + i - a.page_div.div(t0 + i) * a.page_size;
+        const char* const v = a.v + kv * a.vh +
+                              ((uint64_t)((uint32_t)page * a.vb + (uint32_t)at * a.vt) << 4);
+#pragma unroll
+        for (int d = 0; d < kDims; ++d) {
+          const u32x2 x = load_u32x2(v + (16 * d + 4 * g) * 2);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const uint32_t bits = r & 1 ? x[r >> 1] & 0xFFFF0000u : x[r >> 1] << 16;
+            if ((bits & 0x7F800000u) == 0x7F800000u) o[d][r] += __builtin_bit_cast(float, bits);
+          }
+        }
+      }
+    }
+  }
+
+  // The waves' shares, joined in wave order by D / 4 lanes a row.
+  __syncthreads();  // (all have read their V)
+  float* const merge = reinterpret_cast<float*>(lds);
+  {
+    float* const to = merge + wave * (S::kMerge / 4);
+#pragma unroll
+    for (int d = 0; d < kDims; ++d)
+      *reinterpret_cast<f32x4*>(to + n * D + ((16 * d + 4 * g) ^ ((n & 7) << 2))) = o[d];
+    if (g == 0) {
+      to[16 * D + n] = base == kNegInf ? kNegInf : base * a.scale_log2;
+      to[16 * D + 16 + n] = sum;
+    }
+  }
+  __syncthreads();
+  constexpr int kLanes = D / 4;
+  const int at = threadIdx.x % kLanes;
+  for (int row = threadIdx.x / kLanes; row < rows; row += 64 * kRowWaves / kLanes) {
+    float top = kNegInf;
+#pragma unroll
+    for (int w = 0; w < kRowWaves; ++w) top = fmaxf(top, merge[w * (S::kMerge / 4) + 16 * D + row]);
+    const float from = top == kNegInf ? 0.0f : top;
+    f32x4 acc = {0, 0, 0, 0};
+    float total = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kRowWaves; ++w) {
+      const float* const part = merge + w * (S::kMerge / 4);
+      const float f = fast_exp2(part[16 * D + row] - from);
+      total += f * part[16 * D + 16 + row];
+      const f32x4 x = *reinterpret_cast<const f32x4*>(part + row * D + ((4 * at) ^ ((row & 7) << 2)));
+#pragma unroll
+      for (int r = 0; r < 4; ++r) acc[r] += f * x[r];
+    }
+    const float inv = total == 0.0f ? 0.0f : 1.0f / total;  // a row that sees nothing: zeros
+#pragma unroll
+    for (int r = 0; r < 4; ++r) acc[r] *= inv;
+    if (pieces > 1) {
+      const int64_t slot = (int64_t)blockIdx.x * kFew + row;
+      *reinterpret_cast<f32x4*>(a.row_out + slot * D + 4 * at) = acc;
+      if (at == 0) a.row_lse[slot] = total == 0.0f ? kNegInf : top + __log2f(total);
+      continue;
+    }
+    const int own = a.group_div.div(row);
+    const int h = kv * a.group + row - own * a.group;
+    const int64_t r0 = rq.row0 + own;
+    if (a.gate)
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        acc[r] *= gate_factor(a.gate[r0 * a.g_row + h * a.g_head + (4 * at + r) * a.g_dim]);
+    u32x2 w = {pack_bf16x2(acc[0], acc[1]), pack_bf16x2(acc[2], acc[3])};
+    __builtin_memcpy(a.out + r0 * a.out_row + h * a.out_head + 4 * at, &w, 8);
+  }
+}
+
+// Joins the pieces of requests of few rows in order: a workgroup for a request's row,
+// D / 4 lanes a head.
+template <int D, bool KV4>
+__global__ __launch_bounds__(256) void paged_rows_merge_kernel(PagedArgs a, int rows_each) {
+  constexpr int T = RowShape<D, KV4>::kBlock, kLanes = D / 4;
+  const int b = blockIdx.x / rows_each, i = blockIdx.x % rows_each;
+  const Request rq = uniform_request(a, b);
+  if (i >= rq.rows || !is_few(a, rq)) return;
+  const int per = blocks_of_piece<T>(a);
+  const int pieces = pieces_of<T>(a, rq, per);
+  if (pieces <= 1) return;
+  int before = 0;
+  for (int o = threadIdx.x & 63; o < b; o += 64)
+    before += pieces_of<T>(a, load_request(a, o), per);
+#pragma unroll
+  for (int w = 32; w > 0; w /= 2) before += __shfl_xor(before, w, 64);
+  before = uniform(before);
+  if ((before + pieces) * a.kv_heads > a.few_groups) return;  // (requests whose rows overlap)
+  const int row = rq.row0 + i, lane = threadIdx.x % kLanes;
+  for (int head = threadIdx.x / kLanes; head < a.num_q_heads; head += 256 / kLanes) {
+    const int kv = a.group_div.div(head);
+    const int m = i * a.group + head - kv * a.group;
+    const int64_t first = ((int64_t)before * a.kv_heads + (int64_t)kv * pieces) * kFew + m;
+    float top = kNegInf;
+    for (int s = 0; s < pieces; ++s) top = fmaxf(top, a.row_lse[first + (int64_t)s * kFew]);
+    const float base = top == kNegInf ? 0.0f : top;
+    float sum = 0.0f;
+    f32x4 acc = {0, 0, 0, 0};
+#pragma unroll 4
+    for (int s = 0; s < pieces; ++s) {
+      const int64_t at = first + (int64_t)s * kFew;
+      const float f = fast_exp2(a.row_lse[at] - base);
+      const f32x4 part = *reinterpret_cast<const f32x4*>(a.row_out + at * D + 4 * lane);
+      sum += f;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) acc[r] += f * part[r];
+    }
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    float y[4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      y[r] = acc[r] * inv;
+      if (a.gate) y[r] *= gate_factor(a.gate[row * a.g_row + head * a.g_head + (4 * lane + r) * a.g_dim]);
+    }
+    u32x2 w = {pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3])};
+    __builtin_memcpy(a.out + row * a.out_row + head * a.out_head + 4 * lane, &w, 8);
+  }
+}
+
+// ---------------------------------------------------------------------------
 // Host side
 // ---------------------------------------------------------------------------
 
 struct PagedPlan {
-  int waves, splits;
-  int64_t tiles;  // of all requests, at most
+  int waves, splits;   // of the tiles
+  int64_t tiles;       // of all requests, at most; 0: no launch
+  int few, few_groups;
+  int64_t few_units;   // requests of few rows and kv heads, at most; 0: no launch
 };
 
 // The bounds shape the launch: a longer context is computed whole all the same.
 PagedPlan make_plan(int rows, int requests, int num_q_heads, int num_kv_heads, int max_query_len,
                     int max_seq_len, int window, int sinks) {
-  PagedPlan p;
+  PagedPlan p = {};
   const int64_t group = num_q_heads / num_kv_heads;
   const int64_t most = std::min(max_query_len, rows) * group;
-  p.waves = most <= 64 ? 2 : most <= 128 ? 4 : 8;
-  const int64_t tile_rows = 32 * p.waves;
-  p.tiles = std::min<int64_t>((rows * group) / tile_rows + std::min(requests, rows),
-                              (int64_t)requests * ((most + tile_rows - 1) / tile_rows));
-  int64_t seen = std::min<int64_t>(max_seq_len, (int64_t)window + tile_rows / group + 1);
-  if (window < max_seq_len) seen += std::min(sinks, max_seq_len) + 2 * kTok;
-  const int64_t stages = (seen + kTok - 1) / kTok;
-  const int64_t units = std::max<int64_t>(p.tiles * num_kv_heads, 1);
-  p.splits = (int)std::max<int64_t>(1, std::min(2 * kCUs / units, stages / 4));
+  requests = std::min(requests, rows);
+  // Positions that n rows see, in whole blocks.
+  auto seen = [&](int64_t n) {
+    int64_t s = std::min<int64_t>(max_seq_len, (int64_t)window + n);
+    return window < max_seq_len ? s + std::min(sinks, max_seq_len) + 2 * kTok : s;
+  };
+  // (A single request of more rows is one of the tiles, whatever its number turns out to be.)
+  if (group <= kFew && (most <= kFew || requests > 1)) {
+    p.few = kFew;
+    p.few_units = (int64_t)requests * num_kv_heads;
+    const int64_t blocks = (seen(kFew / group) + 31) / 32;
+    if (blocks > kMinBlocks && p.few_units <= 16 * kCUs)
+      p.few_groups = (int)std::max<int64_t>(2 * kCUs, 2 * p.few_units);
+  }
+  if (most > p.few) {
+    p.waves = most <= 64 ? 2 : most <= 128 ? 4 : 8;
+    const int64_t tile_rows = 32 * p.waves;
+    p.tiles = std::min<int64_t>((rows * group) / tile_rows + requests,
+                                requests * ((most + tile_rows - 1) / tile_rows));
+    const int64_t stages = (seen(tile_rows / group + 1) + kTok - 1) / kTok;
+    const int64_t units = std::max<int64_t>(p.tiles * num_kv_heads, 1);
+    p.splits = (int)std::max<int64_t>(1, std::min(2 * kCUs / units, stages / 4));
+  }
   return p;
 }
 
+// Floats of the pieces' rows: the tiles', then those of few rows.
+size_t tile_rows_of(const PagedPlan& p, int num_kv_heads) {
+  return p.splits <= 1 ? 0 : (size_t)p.tiles * num_kv_heads * p.splits * 32 * p.waves;
+}
 size_t workspace_of(const PagedPlan& p, int num_kv_heads, int head_dim) {
-  if (p.splits <= 1) return 0;
-  return (size_t)p.tiles * num_kv_heads * p.splits * 32 * p.waves * (head_dim + 1) * sizeof(float);
+  return (tile_rows_of(p, num_kv_heads) + (size_t)p.few_groups * kFew) * (head_dim + 1) * sizeof(float);
 }
 
+// A launch of more than 2^32 - 1 threads is refused.
+constexpr hipError_t kTooLarge = hipErrorInvalidConfiguration;
+bool fits(int64_t blocks, int threads) { return blocks <= UINT_MAX / threads; }
+
 template <int D, int W, bool KV4>
-hipError_t launch_paged(const PagedArgs& a, int64_t tiles, hipStream_t stream) {
+hipError_t launch_tiles(const PagedArgs& a, int64_t tiles, hipStream_t stream) {
   constexpr int kLds = 4 * kTok * D * 2;
   static_assert(kLds <= 65536, "no attribute to set");
   const int64_t grid = tiles * a.splits * a.kv_heads;
-  if (grid > UINT_MAX / (64 * W) || a.rows > (int)(UINT_MAX / 256)) return hipErrorInvalidConfiguration;
   hipLaunchKernelGGL((paged_tile_kernel<D, W, KV4>), dim3((unsigned)grid), dim3(64 * W), kLds, stream, a);
   const hipError_t err = hipGetLastError();
   if (err != hipSuccess || a.splits <= 1) return err;
@@ -688,10 +1275,29 @@ hipError_t launch_paged(const PagedArgs& a, int64_t tiles, hipStream_t stream) {
   return hipGetLastError();
 }
 template <int D, bool KV4>
-hipError_t launch_waves(const PagedArgs& a, const PagedPlan& p, hipStream_t stream) {
-  return p.waves == 2   ? launch_paged<D, 2, KV4>(a, p.tiles, stream)
-         : p.waves == 4 ? launch_paged<D, 4, KV4>(a, p.tiles, stream)
-                        : launch_paged<D, 8, KV4>(a, p.tiles, stream);
+hipError_t launch_paged(const PagedArgs& a, const PagedPlan& p, hipStream_t stream) {
+  // All launches' sizes before the first: a call that is refused has written nothing.
+  const int64_t grid = p.few_groups ? p.few_groups : p.few_units;
+  const int rows_each = std::min(a.max_rows, kFew / std::min(a.group, kFew));
+  if (!fits(p.tiles * std::max(p.splits, 1) * a.kv_heads, 64 * 8) || !fits(a.rows, 256) ||
+      !fits(grid, 256) || !fits((int64_t)a.requests * rows_each, 256))
+    return kTooLarge;
+  if (p.tiles) {
+    const hipError_t err = p.waves == 2   ? launch_tiles<D, 2, KV4>(a, p.tiles, stream)
+                           : p.waves == 4 ? launch_tiles<D, 4, KV4>(a, p.tiles, stream)
+                                          : launch_tiles<D, 8, KV4>(a, p.tiles, stream);
+    if (err != hipSuccess) return err;
+  }
+  if (!p.few_units) return hipSuccess;
+  constexpr int kLds = RowShape<D, KV4>::kLds;
+  static_assert(kLds <= 65536, "no attribute to set");
+  hipLaunchKernelGGL((paged_rows_kernel<D, KV4>), dim3((unsigned)grid), dim3(64 * kRowWaves), kLds,
+                     stream, a);
+  const hipError_t err = hipGetLastError();
+  if (err != hipSuccess || !p.few_groups) return err;
+  hipLaunchKernelGGL((paged_rows_merge_kernel<D, KV4>), dim3((unsigned)(a.requests * rows_each)),
+                     dim3(256), 0, stream, a, rows_each);
+  return hipGetLastError();
 }
 
 bool aligned16(const void* p) { return ((uintptr_t)p & 15u) == 0; }
@@ -732,8 +1338,11 @@ int run_paged(const std::string& name, PagedArgs a, bool kv4, const void* q, int
     return fail(QSA_ERR_WORKSPACE, name + ": needs a 16-byte aligned workspace of " +
                                        std::to_string(need) + " bytes");
   if (need) {
+    const size_t tile_rows = tile_rows_of(plan, num_kv_heads);
     a.part_out = static_cast<float*>(workspace);
-    a.part_lse = a.part_out + need / sizeof(float) / (head_dim + 1) * head_dim;
+    a.row_out = a.part_out + tile_rows * head_dim;
+    a.part_lse = a.row_out + (size_t)plan.few_groups * kFew * head_dim;
+    a.row_lse = a.part_lse + tile_rows;
   }
   a.q = static_cast<const uint16_t*>(q);
   a.q_row = q_row_stride;
@@ -763,13 +1372,15 @@ int run_paged(const std::string& name, PagedArgs a, bool kv4, const void* q, int
   a.max_rows = max_query_len;
   a.splits = plan.splits;
   a.tiles = (int)plan.tiles;
+  a.few = plan.few;
+  a.few_groups = plan.few_groups;
   a.scale_log2 = 1.4426950408889634f / sqrtf((float)head_dim);
   hipStream_t s = static_cast<hipStream_t>(stream);
-  const hipError_t err = head_dim == 128 ? (kv4 ? launch_waves<128, true>(a, plan, s)
-                                                : launch_waves<128, false>(a, plan, s))
-                                         : (kv4 ? launch_waves<64, true>(a, plan, s)
-                                                : launch_waves<64, false>(a, plan, s));
-  if (err == hipErrorInvalidConfiguration)
+  const hipError_t err = head_dim == 128 ? (kv4 ? launch_paged<128, true>(a, plan, s)
+                                                : launch_paged<128, false>(a, plan, s))
+                                         : (kv4 ? launch_paged<64, true>(a, plan, s)
+                                                : launch_paged<64, false>(a, plan, s));
+  if (err == kTooLarge)
     return fail(QSA_ERR_UNSUPPORTED, name + ": too many requests, rows or heads");
   if (err != hipSuccess) return fail(QSA_ERR_HIP, name + " launch: " + hipGetErrorString(err));
   return QSA_OK;
