@@ -21,12 +21,14 @@
 #include "../../include/qsa_hip.h"
 #include "kv4.h"
 
+#include <algorithm>
 #include <climits>
 
 namespace qsa {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kSmall = 4096;  // rows up to which each has its own lanes
 
 struct Rows {  // [tokens, heads, D] bf16, strides in elements
   uint16_t* p;
@@ -35,9 +37,10 @@ struct Rows {  // [tokens, heads, D] bf16, strides in elements
 
 struct HeadRopeArgs {
   Rows q, k, v, q_out, k_out, v_out;
-  int q_heads, kv_heads;  // of the rows that the launch has: 0 query heads without queries
-  FastDiv rows_div;       // rows of a token: query, key and value heads
-  int total;              // rows of the launch
+  int q_heads, kv_heads;  // 0 query heads without queries
+  int kv_parts;           // keys, and values if there are any
+  FastDiv q_div, kv_div;  // groups of lanes of a token, of one part
+  int q_items, kv_items, q_blocks;  // groups of all tokens, and the queries' workgroups
   const uint16_t* q_weight;
   const uint16_t* k_weight;
   float eps;
@@ -49,7 +52,8 @@ struct HeadRopeArgs {
   char* k_cache;  // the 4-bit cache's data, strides in bytes
   char* v_cache;
   int64_t kb, kt, kh, vb, vt, vh;  // bytes
-  int num_blocks, page;
+  int64_t num_slots;
+  FastDiv page_div;
 };
 
 __device__ __forceinline__ void unpack8(const u32x4& v, float (&f)[8]) {
@@ -66,156 +70,212 @@ __device__ __forceinline__ u32x4 pack8(const float (&f)[8]) {
   return v;
 }
 
-// Rows of 8 dims a lane: 4 lanes share a group of 32. Returns the group's word, the
-// lane's 8 codes packed (each byte of `lo`: dims 0 .. 3, `hi`: dims 4 .. 7), and puts
-// the values that they stand for into f.
-__device__ __forceinline__ uint32_t quantize4(const u32x4& x, float (&f)[8], uint32_t (&codes)[8]) {
+// x / d correctly rounded, for the rounded reciprocal r of d: the quotient's residual is
+// exact (Markstein's division step). No operand here is near the type's ends.
+__device__ __forceinline__ float divide(float x, float d, float r) {
+  const float q = x * r;
+  return __builtin_fmaf(__builtin_fmaf(-q, d, x), r, q);
+}
+
+// Rows of 8 dims a lane: 4 lanes share a group of 32. The lane's codes go to `codes`,
+// and (where `f` is wanted) the values that they stand for to f; returns the group's word.
+__device__ __forceinline__ uint32_t quantize4(const u32x4& x, bool wanted, float (&f)[8],
+                                              uint32_t (&codes)[8]) {
 #pragma clang fp contract(off)
+  typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
   unpack8(x, f);
   float low = 0.0f, high = 0.0f;
-  int bad = 0;
+  u16x2 top = {0, 0};  // largest magnitudes' bits: infinities and NaN are above all others
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    low = fminf(low, f[i]);
-    high = fmaxf(high, f[i]);
-    bad |= (__builtin_bit_cast(uint32_t, f[i]) & 0x7FFFFFFFu) >= 0x7E800000u;
+  for (int i = 0; i < 4; ++i) {
+    low = fminf(low, fminf(f[2 * i], f[2 * i + 1]));
+    high = fmaxf(high, fmaxf(f[2 * i], f[2 * i + 1]));
+    top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2, x[i] & 0x7FFF7FFFu));
   }
+  int bad = top[0] >= 0x7E80 || top[1] >= 0x7E80;
 #pragma unroll
   for (int m = 1; m < 4; m *= 2) {
     low = fminf(low, __shfl_xor(low, m, 64));
     high = fmaxf(high, __shfl_xor(high, m, 64));
     bad |= __shfl_xor(bad, m, 64);
   }
-  if (bad) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      codes[i] = 1;
-      f[i] = __builtin_nanf("");
-    }
-    return kKv4NaN;
-  }
-  const float step = fmaxf(__fdiv_rn(high - low, 15.0f), 0x1p-100f);
+  const float step = fmaxf(divide(high - low, 15.0f, 1.0f / 15.0f), 0x1p-100f);
   const uint32_t sbits = (__builtin_bit_cast(uint32_t, step) + 0xFFFFFu) & ~0xFFFFFu;
   const float s = __builtin_bit_cast(float, sbits);
-  const float z = fminf(rintf(__fdiv_rn(-low, s)), 15.0f);
+  const float r = __fdiv_rn(1.0f, s);
+  const float z = fminf(rintf(divide(-low, s, r)), 15.0f);
+  float c[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float c = fminf(fmaxf(rintf(__fdiv_rn(f[i], s)) + z, 0.0f), 15.0f);
-    codes[i] = (uint32_t)c;
-    f[i] = (c - z) * s;
+  for (int i = 0; i < 8; ++i) c[i] = fminf(fmaxf(rintf(divide(f[i], s, r)) + z, 0.0f), 15.0f);
+  if (wanted) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = bad ? __builtin_nanf("") : (c[i] - z) * s;
   }
-  return sbits >> 16 | (uint32_t)z;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) codes[i] = bad ? 1u : (uint32_t)c[i];
+  return bad ? kKv4NaN : sbits >> 16 | (uint32_t)z;
 }
 
-template <int D, int BITS>
-__global__ __launch_bounds__(kThreads) void head_rope_kernel(HeadRopeArgs a) {
+// ROWS heads of one part (0: queries, 1: keys, 2: values) of one token, from head
+// `first` on. Everything is loaded before anything is used: one chain of two loads (the
+// position, then its row of the table) is all that a call waits for.
+template <int D, int BITS, int ROWS>
+__device__ __forceinline__ void take_heads(const HeadRopeArgs& a, int part, int token, int first,
+                                           int j) {
   constexpr int kLanes = D / 8;
-  const int j = threadIdx.x % kLanes;
-  const int64_t item = (int64_t)blockIdx.x * (kThreads / kLanes) + threadIdx.x / kLanes;
-  if (item >= a.total) return;  // whole groups of lanes
-  const int token = a.rows_div.div((int)item);
-  int head = (int)item - token * a.rows_div.divisor;
-  const int part = head < a.q_heads ? 0 : head < a.q_heads + a.kv_heads ? 1 : 2;  // q, k, v
-  head -= part == 0 ? 0 : a.q_heads + (part - 1) * a.kv_heads;
   const Rows& src = part == 0 ? a.q : part == 1 ? a.k : a.v;
   const Rows& dst = part == 0 ? a.q_out : part == 1 ? a.k_out : a.v_out;
-
-  u32x4 x = load_u32x4(src.p + token * src.token + head * src.head + 8 * j);
-  const uint16_t* const weight = part == 0 ? a.q_weight : part == 1 ? a.k_weight : nullptr;
+  const int heads = part == 0 ? a.q_heads : a.kv_heads;
+  const bool store = BITS != 0 && part > 0;
   const bool turn = part < 2 && a.rotary > 0;
-  if (weight || turn) {
-    float f[8];
-    unpack8(x, f);
-    if (weight) {
-      float w[8], sum = 0.0f;
-      unpack8(load_u32x4(weight + 8 * j), w);
+  const int64_t pos = turn ? a.positions[token] : 0;
+  const int64_t slot = store ? a.slots[token] : -1;
+  u32x4 x[ROWS];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) sum += f[i] * f[i];
+  for (int r = 0; r < ROWS; ++r)
+    x[r] = load_u32x4(src.p + token * src.token + min(first + r, heads - 1) * src.head + 8 * j);
+  const uint16_t* const weight = part == 0 ? a.q_weight : part == 1 ? a.k_weight : nullptr;
+  const char* const zero = reinterpret_cast<const char*>(g_qsa_zero_rows);
+  const u32x4 wr = load_u32x4(weight ? (const char*)(weight + 8 * j) : zero);
+
+  // The table's row: zeros outside it.
+  const int half = a.rotary / 2;
+  const bool rotated = turn && 8 * j < a.rotary, lower = 8 * j < half;
+  const bool in_table = rotated && pos >= 0 && pos < a.max_positions;
+  const int64_t entry = in_table ? pos * a.rotary + (lower ? 8 * j : 8 * j - half) : 0;
+  float c[8], s[8];
+  if (a.cos_sin_fp32) {
+    const char* const t = in_table ? (const char*)a.cos_sin + 4 * entry : zero;
+    const int64_t apart = in_table ? 4 * half : 0;
 #pragma unroll
-      for (int m = 1; m < kLanes; m *= 2) sum += __shfl_xor(sum, m, 64);
-      const float inv = __fdiv_rn(1.0f, __fsqrt_rn(sum * (1.0f / D) + a.eps));
+    for (int e = 0; e < 2; ++e) {
+      const f32x4 cv = *reinterpret_cast<const f32x4*>(t + 16 * e);
+      const f32x4 sv = *reinterpret_cast<const f32x4*>(t + apart + 16 * e);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) f[i] = f[i] * inv * w[i];
-    }
-    if (turn) {
-      const int half = a.rotary / 2;
-      const int64_t pos = a.positions[token];
-      float c[8] = {}, s[8] = {};
-      if (8 * j < a.rotary && pos >= 0 && pos < a.max_positions) {
-        const int64_t at = pos * a.rotary + 8 * j % half;
-        if (a.cos_sin_fp32) {
-          const float* t = static_cast<const float*>(a.cos_sin) + at;
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            c[i] = t[i];
-            s[i] = t[half + i];
-          }
-        } else {
-          const uint16_t* t = static_cast<const uint16_t*>(a.cos_sin) + at;
-          unpack8(load_u32x4(t), c);
-          unpack8(load_u32x4(t + half), s);
-        }
-      }
-      // dims i < half turn with i + half: the lane half / 8 further.
-      const int lane = threadIdx.x & 63;
-      const bool rotated = 8 * j < a.rotary, first = 8 * j < half;
-      const int partner = rotated ? (first ? lane + half / 8 : lane - half / 8) : lane;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float other = __shfl(f[i], partner, 64);
-        f[i] = rotated ? f[i] * c[i] + (first ? -other : other) * s[i] : f[i];
+      for (int i = 0; i < 4; ++i) {
+        c[4 * e + i] = cv[i];
+        s[4 * e + i] = sv[i];
       }
     }
-    x = pack8(f);
+  } else {
+    const char* const t = in_table ? (const char*)a.cos_sin + 2 * entry : zero;
+    unpack8(load_u32x4(t), c);
+    unpack8(load_u32x4(t + (in_table ? 2 * half : 0)), s);
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) s[i] = lower ? -s[i] : s[i];
+  // dims i < half turn with i + half: the lane half / 8 further.
+  const int lane = threadIdx.x & 63;
+  const int partner = rotated ? (lower ? lane + half / 8 : lane - half / 8) : lane;
+
+  int64_t block = -1;
+  int place = 0;
+  if (slot >= 0 && slot < a.num_slots) {
+    block = a.num_slots <= INT_MAX ? a.page_div.div((int)slot) : slot / a.page_div.divisor;
+    place = (int)(slot - block * a.page_div.divisor);
   }
 
-  if (part > 0 && BITS != 0) {
-    const int64_t slot = a.slots[token];
-    const int64_t block = slot >= 0 ? slot / a.page : -1;
-    const bool live = block >= 0 && block < a.num_blocks;
-    const int place = live ? (int)(slot - block * a.page) : 0;
-    if constexpr (BITS == 16) {
-      char* const to = part == 1 ? a.k_cache + block * a.kb + place * a.kt + head * a.kh
-                                 : a.v_cache + block * a.vb + place * a.vt + head * a.vh;
-      if (live) *reinterpret_cast<u32x4*>(to + 16 * j) = x;
-    } else {
+#pragma unroll
+  for (int r = 0; r < ROWS; ++r) {
+    const int head = first + r;
+    if (head >= heads) break;
+    if (weight || turn) {
       float f[8];
-      uint32_t c[8];
-      const uint32_t word = quantize4(x, f, c);
-      const Kv4Page lay{a.page, D};
-      char* const to = a.k_cache + block * a.kb + head * a.kh;
-      uint32_t packed = 0;
-      if (live) {
-        if (part == 1) {
+      unpack8(x[r], f);
+      if (weight) {
+        float w[8], sum = 0.0f;
+        unpack8(wr, w);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) packed |= c[i] << (4 * (i / 2) + 16 * (i % 2));
-          *reinterpret_cast<uint32_t*>(to + (int64_t)place * lay.row() +
-                                       4 * (j % 4 * (D / 32) + j / 4)) = packed;
-        } else {
+        for (int i = 0; i < 8; ++i) sum += f[i] * f[i];
 #pragma unroll
-          for (int i = 0; i < 8; ++i) packed |= c[i] << (4 * i);
-          *reinterpret_cast<uint32_t*>(to + lay.v_codes() + (int64_t)place * lay.row() + 4 * j) =
-              packed;
-        }
-        if (j % 4 == 0)
-          *reinterpret_cast<uint16_t*>(to + (part == 1 ? lay.k_words() : lay.v_words()) +
-                                       place * lay.words() + j / 4 * 2) = (uint16_t)word;
+        for (int m = 1; m < kLanes; m *= 2) sum += __shfl_xor(sum, m, 64);
+        const float inv = __fdiv_rn(1.0f, __fsqrt_rn(sum * (1.0f / D) + a.eps));
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[i] = f[i] * inv * w[i];
       }
-      x = pack8(f);
+      if (turn) {
+        float other[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) other[i] = __shfl(f[i], partner, 64);
+        if (rotated) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) f[i] = f[i] * c[i] + other[i] * s[i];
+        }
+      }
+      x[r] = pack8(f);
     }
+    if (store) {
+      if constexpr (BITS == 16) {
+        char* const to = part == 1 ? a.k_cache + block * a.kb + place * a.kt + head * a.kh
+                                   : a.v_cache + block * a.vb + place * a.vt + head * a.vh;
+        if (block >= 0) *reinterpret_cast<u32x4*>(to + 16 * j) = x[r];
+      } else if constexpr (BITS == 4) {
+        float f[8];
+        uint32_t code[8];
+        const uint32_t word = quantize4(x[r], dst.p != nullptr, f, code);
+        const Kv4Page lay{a.page_div.divisor, D};
+        char* const to = a.k_cache + block * a.kb + head * a.kh;
+        if (block >= 0) {
+          uint32_t packed = 0;
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            packed |= code[i] << (part == 1 ? 4 * (i / 2) + 16 * (i % 2) : 4 * i);
+          *reinterpret_cast<uint32_t*>(
+              to + (part == 1 ? 0 : lay.v_codes()) + (int64_t)place * lay.row() +
+              4 * (part == 1 ? j % 4 * (D / 32) + j / 4 : j)) = packed;
+          if (j % 4 == 0)
+            *reinterpret_cast<uint16_t*>(to + (part == 1 ? lay.k_words() : lay.v_words()) +
+                                         place * lay.words() + j / 4 * 2) = (uint16_t)word;
+        }
+        x[r] = pack8(f);
+      }
+    }
+    if (dst.p)
+      *reinterpret_cast<u32x4*>(dst.p + token * dst.token + head * dst.head + 8 * j) = x[r];
   }
-  if (dst.p)
-    *reinterpret_cast<u32x4*>(dst.p + token * dst.token + head * dst.head + 8 * j) = x;
+}
+
+// Groups of lanes: first those of the queries (ROWS heads each), from workgroup q_blocks
+// on those of all keys, then of all values, so that a wave's groups have the same to do.
+template <int D, int BITS, int ROWS>
+__global__ __launch_bounds__(kThreads) void head_rope_kernel(HeadRopeArgs a) {
+  constexpr int kLanes = D / 8, kPer = kThreads / kLanes, kKvRows = ROWS > 2 ? 2 : ROWS;
+  const int j = threadIdx.x % kLanes, group = threadIdx.x / kLanes;
+  if ((int)blockIdx.x < a.q_blocks) {
+    const int item = blockIdx.x * kPer + group;
+    if (item >= a.q_items) return;
+    const int token = a.q_div.div(item);
+    take_heads<D, BITS, ROWS>(a, 0, token, (item - token * a.q_div.divisor) * ROWS, j);
+  } else {
+    int item = (blockIdx.x - a.q_blocks) * kPer + group;
+    if (item >= a.kv_parts * a.kv_items) return;
+    const int part = item < a.kv_items ? 1 : 2;
+    item -= (part - 1) * a.kv_items;
+    const int token = a.kv_div.div(item);
+    take_heads<D, BITS, kKvRows>(a, part, token, (item - token * a.kv_div.divisor) * kKvRows, j);
+  }
 }
 
 bool aligned16(const void* p) { return ((uintptr_t)p & 15u) == 0; }
 
+template <int D, int ROWS>
+void launch_head_rope(HeadRopeArgs& a, int tokens, int bits, hipStream_t stream) {
+  constexpr int kPer = kThreads / (D / 8), kKvRows = ROWS > 2 ? 2 : ROWS;
+  const int q = (a.q_heads + ROWS - 1) / ROWS, kv = (a.kv_heads + kKvRows - 1) / kKvRows;
+  a.q_div = FastDiv::make(std::max(q, 1));
+  a.kv_div = FastDiv::make(std::max(kv, 1));
+  a.q_items = q * tokens;
+  a.kv_items = kv * tokens;
+  a.q_blocks = (a.q_items + kPer - 1) / kPer;
+  const dim3 grid((unsigned)(a.q_blocks + (a.kv_parts * a.kv_items + kPer - 1) / kPer)), block(kThreads);
+  if (bits == 0) hipLaunchKernelGGL((head_rope_kernel<D, 0, ROWS>), grid, block, 0, stream, a);
+  else if (bits == 16) hipLaunchKernelGGL((head_rope_kernel<D, 16, ROWS>), grid, block, 0, stream, a);
+  else hipLaunchKernelGGL((head_rope_kernel<D, 4, ROWS>), grid, block, 0, stream, a);
+}
 template <int D>
-void launch_head_rope(const HeadRopeArgs& a, int bits, unsigned blocks, hipStream_t stream) {
-  const dim3 grid(blocks), block(kThreads);
-  if (bits == 0) hipLaunchKernelGGL((head_rope_kernel<D, 0>), grid, block, 0, stream, a);
-  else if (bits == 16) hipLaunchKernelGGL((head_rope_kernel<D, 16>), grid, block, 0, stream, a);
-  else hipLaunchKernelGGL((head_rope_kernel<D, 4>), grid, block, 0, stream, a);
+void launch_rows(HeadRopeArgs& a, int tokens, int bits, hipStream_t stream) {
+  if ((int64_t)(a.q_heads + a.kv_parts * a.kv_heads) * tokens <= kSmall) launch_head_rope<D, 1>(a, tokens, bits, stream);
+  else launch_head_rope<D, 4>(a, tokens, bits, stream);
 }
 
 }  // namespace
@@ -278,7 +338,7 @@ extern "C" int qsa_qk_norm_rope(
                                         "strides of multiples of 8 elements");
   const int64_t rows = (int64_t)num_q_heads + num_kv_heads * (value ? 2 : 1);
   if (rows == 0) return QSA_OK;
-  if (rows * tokens > INT_MAX) return fail(QSA_ERR_UNSUPPORTED, name + ": too many rows");
+  if (rows * tokens > INT_MAX - 4096) return fail(QSA_ERR_UNSUPPORTED, name + ": too many rows");
   HeadRopeArgs a = {};
   auto view = [](const void* p, int64_t token, int64_t head) {
     return Rows{static_cast<uint16_t*>(const_cast<void*>(p)), token, head};
@@ -291,8 +351,7 @@ extern "C" int qsa_qk_norm_rope(
   a.v_out = view(v_out, v_out_token_stride, v_out_head_stride);
   a.q_heads = num_q_heads;
   a.kv_heads = num_kv_heads;
-  a.rows_div = FastDiv::make((int)rows);
-  a.total = (int)(rows * tokens);
+  a.kv_parts = value ? 2 : 1;
   a.q_weight = static_cast<const uint16_t*>(q_weight);
   a.k_weight = static_cast<const uint16_t*>(k_weight);
   a.eps = eps;
@@ -311,13 +370,10 @@ extern "C" int qsa_qk_norm_rope(
   a.vb = unit * v_block_stride;
   a.vt = unit * v_cache_token_stride;
   a.vh = unit * v_cache_head_stride;
-  a.num_blocks = num_blocks;
-  a.page = page_size;
-  const int per = kThreads / (head_dim / 8);
-  const unsigned blocks = (unsigned)((rows * tokens + per - 1) / per);
-  if (blocks > UINT_MAX / kThreads) return fail(QSA_ERR_UNSUPPORTED, name + ": too many rows");
+  a.num_slots = (int64_t)num_blocks * page_size;
+  a.page_div = FastDiv::make(std::max(page_size, 1));
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (head_dim == 128) launch_head_rope<128>(a, cache_bits, blocks, s);
-  else launch_head_rope<64>(a, cache_bits, blocks, s);
+  if (head_dim == 128) launch_rows<128>(a, tokens, cache_bits, s);
+  else launch_rows<64>(a, tokens, cache_bits, s);
   return check_launch("qsa_qk_norm_rope launch");
 }

@@ -72,6 +72,7 @@ struct PagedArgs {
   float* part_lse;  // [pieces][tile rows], log2
   float* row_out;   // the same of requests of few rows, [pieces][16][D]
   float* row_lse;
+  int32_t* row_pieces;  // [requests]: first piece, pieces of a kv head
   int rows, num_q_heads, kv_heads, group;
   FastDiv group_div;
   int max_rows;   // a request's rows at most
@@ -700,30 +701,86 @@ template <int T>
 __device__ __forceinline__ int blocks_of(const PagedArgs& a, const Request& r) {
   return r.rows > 0 && is_few(a, r) ? make_span<T>(a, r, 0, r.rows - 1).count : 0;
 }
-// Blocks of a piece, such that all pieces are at most a.few_groups.
-template <int T>
-__device__ __forceinline__ int blocks_of_piece(const PagedArgs& a) {
-  if (!a.few_groups) return INT_MAX;
-  const int lane = threadIdx.x & 63;
-  int blocks = 0, units = 0;
-  for (int b = lane; b < a.requests; b += 64) {
-    const Request r = load_request(a, b);
-    blocks += blocks_of<T>(a, r);
-    units += r.rows > 0 && is_few(a, r);
-  }
-#pragma unroll
-  for (int w = 32; w > 0; w /= 2) {
-    blocks += __shfl_xor(blocks, w, 64);
-    units += __shfl_xor(units, w, 64);
-  }
-  // A request's last piece may be short: the pieces are at most total / per + units.
-  const unsigned total = uniform(blocks), spare = a.few_groups / a.kv_heads - uniform(units);
-  return max(kMinBlocks, (int)((total + spare - 1) / max(spare, 1u)));
+// What a workgroup of the launch takes: a piece of a request and kv head.
+struct Share {
+  Request rq;
+  int request, kv, piece, pieces;
+  int first;  // the request's first piece of the launch
+};
+__device__ __forceinline__ int pieces_of(int blocks, int per) {
+  return max(1, (int)(((unsigned)blocks + (unsigned)per - 1u) / (unsigned)per));
 }
+// Blocks of a piece, such that all pieces are at most a.few_groups: a request's last
+// piece may be short, so that there are up to blocks / per + requests for a kv head.
+__device__ __forceinline__ int piece_blocks(const PagedArgs& a, int blocks, int requests) {
+  if (!a.few_groups) return INT_MAX;
+  const unsigned spare = max(a.few_groups / a.kv_heads - requests, 1);
+  return max(kMinBlocks, (int)(((unsigned)blocks + spare - 1u) / spare));
+}
+// False where the launch has no such workgroup.
 template <int T>
-__device__ __forceinline__ int pieces_of(const PagedArgs& a, const Request& r, int per) {
-  if (r.rows <= 0 || !is_few(a, r)) return 0;
-  return max(1, (int)(((unsigned)blocks_of<T>(a, r) + (unsigned)per - 1u) / (unsigned)per));
+__device__ __forceinline__ bool find_share(const PagedArgs& a, Share& s) {
+  int place = blockIdx.x;
+  if (a.requests == 1) {
+    s.rq = uniform_request(a, 0);
+    if (s.rq.rows <= 0 || !is_few(a, s.rq)) return false;
+    const int blocks = uniform(blocks_of<T>(a, s.rq));
+    s.request = s.first = 0;
+    s.pieces = pieces_of(blocks, piece_blocks(a, blocks, 1));
+  } else {
+    // A lane for each request, the first 64 kept.
+    const int lane = threadIdx.x & 63;
+    const Request none = {0, 0, 0, 0};
+    const Request own = lane < a.requests ? load_request(a, lane) : none;
+    auto request = [&](int b0) {
+      return b0 == 0 ? own : b0 + lane < a.requests ? load_request(a, b0 + lane) : none;
+    };
+    int blocks = 0, live = 0;
+    for (int b0 = 0; b0 < a.requests; b0 += 64) {
+      const Request r = request(b0);
+      blocks += blocks_of<T>(a, r);
+      live += r.rows > 0 && is_few(a, r);
+    }
+#pragma unroll
+    for (int w = 32; w > 0; w /= 2) {
+      blocks += __shfl_xor(blocks, w, 64);
+      live += __shfl_xor(live, w, 64);
+    }
+    const int per = piece_blocks(a, uniform(blocks), uniform(live));
+    s.request = -1;
+    s.first = 0;
+    for (int b0 = 0; b0 < a.requests; b0 += 64) {
+      const Request r = request(b0);
+      const int n = r.rows > 0 && is_few(a, r) ? pieces_of(blocks_of<T>(a, r), per) * a.kv_heads : 0;
+      int end = n;  // inclusive sum over the lanes
+#pragma unroll
+      for (int w = 1; w < 64; w *= 2) {
+        const int below = __shfl_up(end, w, 64);
+        end += lane >= w ? below : 0;
+      }
+      const uint64_t past = __ballot(end > place);
+      if (past) {
+        const int at = __ffsll((unsigned long long)past) - 1;
+        const int before = __builtin_amdgcn_readlane(end - n, at);
+        s.request = b0 + at;
+        s.pieces = __builtin_amdgcn_readlane(n, at) / a.kv_heads;
+        s.rq.row0 = __builtin_amdgcn_readlane(r.row0, at);
+        s.rq.rows = __builtin_amdgcn_readlane(r.rows, at);
+        s.rq.first = __builtin_amdgcn_readlane(r.first, at);
+        s.rq.length = __builtin_amdgcn_readlane(r.length, at);
+        s.first += before;
+        place -= before;
+        break;
+      }
+      const int all = __builtin_amdgcn_readlane(end, 63);
+      s.first += all;
+      place -= all;
+    }
+    if (s.request < 0) return false;
+  }
+  s.kv = place / s.pieces;
+  s.piece = place - s.kv * s.pieces;
+  return s.kv < a.kv_heads;
 }
 
 // max over the four lanes of a query row.
@@ -779,18 +836,19 @@ paged_rows_kernel(PagedArgs a) {
   const int wave = uniform(threadIdx.x >> 6);
   const int n = lane & 15, g = lane >> 4;
 
-  const int per = blocks_of_piece<T>(a);
-  int place = blockIdx.x;
-  const int b = locate(a, place, [&](const Request& r) { return pieces_of<T>(a, r, per) * a.kv_heads; });
-  if (b >= a.requests) return;
-  const Request rq = uniform_request(a, b);
-  const int pieces = pieces_of<T>(a, rq, per);
-  const int kv = place / pieces, piece = place - kv * pieces;
+  Share share;
+  if (!find_share<T>(a, share)) return;
+  const Request rq = share.rq;
+  const int kv = share.kv, pieces = share.pieces;
+  if (a.few_groups && kv == 0 && share.piece == 0 && threadIdx.x == 0) {
+    a.row_pieces[2 * share.request] = share.first;
+    a.row_pieces[2 * share.request + 1] = pieces;
+  }
   const int rows = rq.rows * a.group;
   const Span<T> span = make_span<T>(a, rq, 0, rq.rows - 1);
-  const int s_begin = (int)((int64_t)span.count * piece / pieces);
-  const int s_end = (int)((int64_t)span.count * (piece + 1) / pieces);
-  const int32_t* const trow = a.table + b * a.table_row;
+  const int s_begin = (int)((int64_t)span.count * share.piece / pieces);
+  const int s_end = (int)((int64_t)span.count * (share.piece + 1) / pieces);
+  const int32_t* const trow = a.table + share.request * a.table_row;
 
   // The lane's query row, dims 32 s + 8 g .. + 7.
   const int m = min(n, rows - 1);
@@ -1159,53 +1217,86 @@ paged_rows_kernel(PagedArgs a) {
   }
 }
 
-// Joins the pieces of requests of few rows in order: a workgroup for a request's row,
-// D / 4 lanes a head.
-template <int D, bool KV4>
-__global__ __launch_bounds__(256) void paged_rows_merge_kernel(PagedArgs a, int rows_each) {
-  constexpr int T = RowShape<D, KV4>::kBlock, kLanes = D / 4;
-  const int b = blockIdx.x / rows_each, i = blockIdx.x % rows_each;
+// Joins the pieces of requests of few rows in order, D / 4 lanes a head and WAYS times
+// as many that take every WAYS-th piece.
+template <int D, int WAYS>
+__global__ __launch_bounds__(256) void paged_rows_merge_kernel(PagedArgs a, int rows_each,
+                                                               int head_groups) {
+  constexpr int kLanes = D / 4, kHeads = 256 / kLanes / WAYS, kAhead = 4;
+  __shared__ f32x4 acc_lds[256 / kLanes][kLanes];
+  __shared__ float top_lds[256 / kLanes], sum_lds[256 / kLanes];
+  const int hg = blockIdx.x % head_groups;
+  const int bi = blockIdx.x / head_groups, b = bi / rows_each, i = bi - b * rows_each;
+  const int first_piece = a.row_pieces[2 * b], pieces = a.row_pieces[2 * b + 1];
   const Request rq = uniform_request(a, b);
-  if (i >= rq.rows || !is_few(a, rq)) return;
-  const int per = blocks_of_piece<T>(a);
-  const int pieces = pieces_of<T>(a, rq, per);
-  if (pieces <= 1) return;
-  int before = 0;
-  for (int o = threadIdx.x & 63; o < b; o += 64)
-    before += pieces_of<T>(a, load_request(a, o), per);
-#pragma unroll
-  for (int w = 32; w > 0; w /= 2) before += __shfl_xor(before, w, 64);
-  before = uniform(before);
-  if ((before + pieces) * a.kv_heads > a.few_groups) return;  // (requests whose rows overlap)
+  // (Only requests of few rows have their pieces written.)
+  if (i >= rq.rows || !is_few(a, rq) || pieces <= 1) return;
+  if (first_piece < 0 || first_piece + (int64_t)pieces * a.kv_heads > a.few_groups)
+    return;  // (requests whose rows overlap: some have no workgroup)
   const int row = rq.row0 + i, lane = threadIdx.x % kLanes;
-  for (int head = threadIdx.x / kLanes; head < a.num_q_heads; head += 256 / kLanes) {
-    const int kv = a.group_div.div(head);
-    const int m = i * a.group + head - kv * a.group;
-    const int64_t first = ((int64_t)before * a.kv_heads + (int64_t)kv * pieces) * kFew + m;
-    float top = kNegInf;
-    for (int s = 0; s < pieces; ++s) top = fmaxf(top, a.row_lse[first + (int64_t)s * kFew]);
-    const float base = top == kNegInf ? 0.0f : top;
-    float sum = 0.0f;
-    f32x4 acc = {0, 0, 0, 0};
-#pragma unroll 4
-    for (int s = 0; s < pieces; ++s) {
-      const int64_t at = first + (int64_t)s * kFew;
-      const float f = fast_exp2(a.row_lse[at] - base);
-      const f32x4 part = *reinterpret_cast<const f32x4*>(a.row_out + at * D + 4 * lane);
-      sum += f;
+  const int grp = threadIdx.x / kLanes, way = grp % WAYS;
+  const int head = min(hg * kHeads + grp / WAYS, a.num_q_heads - 1);
+  const int kv = a.group_div.div(head);
+  const int m = i * a.group + head - kv * a.group;
+  const int64_t first = ((int64_t)first_piece + (int64_t)kv * pieces) * kFew + m;
+  // Running maximum and sum over the way's pieces, some of them in flight together.
+  float top = kNegInf, sum = 0.0f;
+  f32x4 acc = {0, 0, 0, 0};
+  for (int s = way; s < pieces; s += WAYS * kAhead) {
+    float lse[kAhead];
+    f32x4 part[kAhead];
 #pragma unroll
-      for (int r = 0; r < 4; ++r) acc[r] += f * part[r];
+    for (int e = 0; e < kAhead; ++e) {
+      const int64_t at = first + (int64_t)min(s + e * WAYS, pieces - 1) * kFew;
+      lse[e] = a.row_lse[at];
+      part[e] = *reinterpret_cast<const f32x4*>(a.row_out + at * D + 4 * lane);
     }
-    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-    float y[4];
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      y[r] = acc[r] * inv;
-      if (a.gate) y[r] *= gate_factor(a.gate[row * a.g_row + head * a.g_head + (4 * lane + r) * a.g_dim]);
+    for (int e = 0; e < kAhead; ++e) {
+      if (s + e * WAYS >= pieces) break;
+      const float to = fmaxf(top, lse[e]);
+      const float from = to == kNegInf ? 0.0f : to;
+      const float old = fast_exp2(top - from), f = fast_exp2(lse[e] - from);
+      top = to;
+      sum = sum * old + f;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) acc[r] = acc[r] * old + f * part[e][r];
     }
-    u32x2 w = {pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3])};
-    __builtin_memcpy(a.out + row * a.out_row + head * a.out_head + 4 * lane, &w, 8);
   }
+  if constexpr (WAYS > 1) {
+    acc_lds[grp][lane] = acc;
+    if (lane == 0) {
+      top_lds[grp] = top;
+      sum_lds[grp] = sum;
+    }
+    __syncthreads();
+    if (way > 0) return;
+    float all = top;
+#pragma unroll
+    for (int w = 1; w < WAYS; ++w) all = fmaxf(all, top_lds[grp + w]);
+    const float from = all == kNegInf ? 0.0f : all;
+    const float own = fast_exp2(top - from);
+    sum *= own;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) acc[r] *= own;
+#pragma unroll
+    for (int w = 1; w < WAYS; ++w) {
+      const float f = fast_exp2(top_lds[grp + w] - from);
+      sum += f * sum_lds[grp + w];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) acc[r] += f * acc_lds[grp + w][lane][r];
+    }
+  }
+  if (hg * kHeads + grp / WAYS >= a.num_q_heads) return;
+  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+  float y[4];
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    y[r] = acc[r] * inv;
+    if (a.gate) y[r] *= gate_factor(a.gate[row * a.g_row + head * a.g_head + (4 * lane + r) * a.g_dim]);
+  }
+  u32x2 w = {pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3])};
+  __builtin_memcpy(a.out + row * a.out_row + head * a.out_head + 4 * lane, &w, 8);
 }
 
 // ---------------------------------------------------------------------------
@@ -1215,7 +1306,7 @@ __global__ __launch_bounds__(256) void paged_rows_merge_kernel(PagedArgs a, int 
 struct PagedPlan {
   int waves, splits;   // of the tiles
   int64_t tiles;       // of all requests, at most; 0: no launch
-  int few, few_groups;
+  int requests, few, few_groups;
   int64_t few_units;   // requests of few rows and kv heads, at most; 0: no launch
 };
 
@@ -1225,14 +1316,17 @@ PagedPlan make_plan(int rows, int requests, int num_q_heads, int num_kv_heads, i
   PagedPlan p = {};
   const int64_t group = num_q_heads / num_kv_heads;
   const int64_t most = std::min(max_query_len, rows) * group;
+  p.requests = requests;
+  const int64_t all = (int64_t)requests * max_query_len;
   requests = std::min(requests, rows);
   // Positions that n rows see, in whole blocks.
   auto seen = [&](int64_t n) {
     int64_t s = std::min<int64_t>(max_seq_len, (int64_t)window + n);
     return window < max_seq_len ? s + std::min(sinks, max_seq_len) + 2 * kTok : s;
   };
-  // (A single request of more rows is one of the tiles, whatever its number turns out to be.)
-  if (group <= kFew && (most <= kFew || requests > 1)) {
+  // Where all requests have as many rows, more than a few, the tiles do for them all
+  // (whatever their numbers turn out to be).
+  if (group <= kFew && (most <= kFew || rows < all)) {
     p.few = kFew;
     p.few_units = (int64_t)requests * num_kv_heads;
     const int64_t blocks = (seen(kFew / group) + 31) / 32;
@@ -1256,7 +1350,8 @@ size_t tile_rows_of(const PagedPlan& p, int num_kv_heads) {
   return p.splits <= 1 ? 0 : (size_t)p.tiles * num_kv_heads * p.splits * 32 * p.waves;
 }
 size_t workspace_of(const PagedPlan& p, int num_kv_heads, int head_dim) {
-  return (tile_rows_of(p, num_kv_heads) + (size_t)p.few_groups * kFew) * (head_dim + 1) * sizeof(float);
+  const size_t rows = tile_rows_of(p, num_kv_heads) + (size_t)p.few_groups * kFew;
+  return (rows * (head_dim + 1) + (p.few_groups ? 2 * (size_t)p.requests : 0)) * sizeof(float);
 }
 
 // A launch of more than 2^32 - 1 threads is refused.
@@ -1274,13 +1369,22 @@ hipError_t launch_tiles(const PagedArgs& a, int64_t tiles, hipStream_t stream) {
   hipLaunchKernelGGL((paged_merge_kernel<D, W>), dim3((unsigned)a.rows), dim3(256), 0, stream, a);
   return hipGetLastError();
 }
+template <int D, int WAYS>
+hipError_t launch_rows_merge(const PagedArgs& a, int rows_each, hipStream_t stream) {
+  constexpr int kHeads = 256 / (D / 4) / WAYS;
+  const int head_groups = (a.num_q_heads + kHeads - 1) / kHeads;
+  hipLaunchKernelGGL((paged_rows_merge_kernel<D, WAYS>),
+                     dim3((unsigned)((int64_t)a.requests * rows_each * head_groups)), dim3(256), 0,
+                     stream, a, rows_each, head_groups);
+  return hipGetLastError();
+}
 template <int D, bool KV4>
 hipError_t launch_paged(const PagedArgs& a, const PagedPlan& p, hipStream_t stream) {
   // All launches' sizes before the first: a call that is refused has written nothing.
   const int64_t grid = p.few_groups ? p.few_groups : p.few_units;
   const int rows_each = std::min(a.max_rows, kFew / std::min(a.group, kFew));
   if (!fits(p.tiles * std::max(p.splits, 1) * a.kv_heads, 64 * 8) || !fits(a.rows, 256) ||
-      !fits(grid, 256) || !fits((int64_t)a.requests * rows_each, 256))
+      !fits(grid, 256) || !fits((int64_t)a.requests * rows_each * a.num_q_heads, 256))
     return kTooLarge;
   if (p.tiles) {
     const hipError_t err = p.waves == 2   ? launch_tiles<D, 2, KV4>(a, p.tiles, stream)
@@ -1295,9 +1399,10 @@ hipError_t launch_paged(const PagedArgs& a, const PagedPlan& p, hipStream_t stre
                      stream, a);
   const hipError_t err = hipGetLastError();
   if (err != hipSuccess || !p.few_groups) return err;
-  hipLaunchKernelGGL((paged_rows_merge_kernel<D, KV4>), dim3((unsigned)(a.requests * rows_each)),
-                     dim3(256), 0, stream, a, rows_each);
-  return hipGetLastError();
+  // Few (row, head)s are joined 8 ways.
+  return (int64_t)a.requests * rows_each * a.num_q_heads <= 2048
+             ? launch_rows_merge<D, 8>(a, rows_each, stream)
+             : launch_rows_merge<D, 1>(a, rows_each, stream);
 }
 
 bool aligned16(const void* p) { return ((uintptr_t)p & 15u) == 0; }
@@ -1343,6 +1448,7 @@ int run_paged(const std::string& name, PagedArgs a, bool kv4, const void* q, int
     a.row_out = a.part_out + tile_rows * head_dim;
     a.part_lse = a.row_out + (size_t)plan.few_groups * kFew * head_dim;
     a.row_lse = a.part_lse + tile_rows;
+    a.row_pieces = reinterpret_cast<int32_t*>(a.row_lse + (size_t)plan.few_groups * kFew);
   }
   a.q = static_cast<const uint16_t*>(q);
   a.q_row = q_row_stride;

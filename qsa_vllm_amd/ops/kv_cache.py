@@ -21,6 +21,8 @@ from ._torch_ops import _require
 __all__ = ["Int4KVCache", "qk_norm_rope", "rotary_table"]
 
 _GROUP = 32
+# (looked up once: 1 us of a call)
+_qk_norm_rope = torch.ops.yulan_qsa_kernels.qk_norm_rope.default
 
 
 @dataclass(frozen=True)
@@ -130,7 +132,7 @@ def qk_norm_rope(
         k_cache, v_cache, page = cache.data, None, cache.page_size
     else:
         k_cache, v_cache = cache
-    torch.ops.yulan_qsa_kernels.qk_norm_rope(
+    _qk_norm_rope(
         query, key, value, q_weight, k_weight, float(eps), positions, cos_sin, q_out, k_out, v_out,
         slot_mapping, k_cache, v_cache, int(page))
     return q_out, k_out
