@@ -302,43 +302,52 @@ paged_tile_kernel(PagedArgs a) {
       q[s] = __builtin_bit_cast(bf16x8, load_u32x4(src + 16 * s + 8 * h));
   }
 
-  // Page of token base + lane, -1 past the end or where the table has none.
+  // Page of token base + lane; past the end some other's. (Without a token there is no
+  // stage, and any address does.)
   auto load_page = [&](int stage) {
-    const int at = stage < s_end ? span.base(stage) + lane : INT_MAX;
-    return *(at < span.end ? trow + a.page_div.div(at) : g_qsa_no_page);
+    return *(span.end > 0 ? trow + a.page_div.div(min(span.base(stage) + lane, span.end - 1))
+                          : a.seq_lens);
   };
-  // Offsets (16-byte units) of token base + lane.
+  // Offsets (16-byte units) of token base + lane. What is no token is loaded from the
+  // cache's first rows instead, whose scores are masked.
   struct Places {
     uint32_t k, v;
     int at;
     uint64_t valid;
   };
-  auto places = [&](int stage, int page) {
+  auto places = [&](int stage, int page) __attribute__((always_inline)) {
     Places p;
     const int t = span.base(stage) + lane;
-    const bool ok = page >= 0 && page < a.num_blocks;
-    p.at = t - a.page_div.div(t) * a.page_size;
-    p.k = !ok ? kNoToken : page * a.kb + (KV4 ? 0 : p.at * a.kt);
-    p.v = page * a.vb + p.at * a.vt;
+    const bool ok = page >= 0 && page < a.num_blocks && t < span.end && stage < s_end;
+    const int live = ok ? -1 : 0;
+    p.at = (t - a.page_div.div(t) * a.page_size) & live;
+    const uint32_t block = page & live;
+    p.k = block * a.kb + (KV4 ? 0 : p.at * a.kt);
+    p.v = KV4 ? p.k : block * a.vb + p.at * a.vt;
     p.valid = __ballot(ok);
     return p;
   };
   const char* const zero = reinterpret_cast<const char*>(g_qsa_zero_rows);
+  const char* const k_rows = a.num_blocks > 0 ? a.k + kv * a.kh : zero;  // (no cache: zeros)
+  const char* const v_rows = a.num_blocks > 0 && !KV4 ? a.v + kv * a.vh : zero;
 
-  // bf16: straight into LDS. Block i of a stage (64 units) is moved by wave i mod W, and
-  // a lane's unit of a row is the same in all its blocks of K (or V).
-  auto start_loads = [&](const Places& p, char* stage) {
+  // bf16: straight into LDS. Block i of a stage (64 units) is moved by wave i mod W.
+  auto start_loads = [&](const Places& p, char* stage) __attribute__((always_inline)) {
+    uint32_t o[kLoads];
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      const bool is_v = i >= kLoads / 2;
+      const int tok = ((i % (kLoads / 2)) * W + wave) * (64 / U) + lane / U;
+      o[i] = __builtin_amdgcn_ds_bpermute(4 * tok, is_v ? p.v : p.k);
+    }
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
       const bool is_v = i >= kLoads / 2;
       const int block = (i % (kLoads / 2)) * W + wave;
       const int tok = block * (64 / U) + lane / U;
       const int unit = lane % U ^ (is_v ? v_swizzle<D>(tok) : k_swizzle<D>(tok));
-      const uint32_t ko = __builtin_amdgcn_ds_bpermute(4 * tok, p.k);
-      const uint32_t o = is_v ? __builtin_amdgcn_ds_bpermute(4 * tok, p.v) : ko;
-      const char* src = (is_v ? a.v + kv * a.vh : a.k + kv * a.kh) + ((uint64_t)o << 4);
-      src = (ko != kNoToken ? src : zero) + unit * 16;
-      load_to_lds(src, stage + (is_v ? kStage : 0) + block * 1024);
+      load_to_lds((is_v ? v_rows : k_rows) + unit * 16 + ((uint64_t)o[i] << 4),
+                  stage + (is_v ? kStage : 0) + block * 1024);
     }
   };
   // 4 bits: codes and words into registers, values into LDS a stage later. Pair i of a
@@ -346,6 +355,9 @@ paged_tile_kernel(PagedArgs a) {
   u32x2 codes[KV4 ? kCodes : 1];
   uint32_t words[KV4 ? kCodes : 1];
   const Kv4Page lay{a.page_size, D};
+  const int64_t v_codes = a.num_blocks > 0 ? lay.v_codes() : 0;
+  const int64_t k_words = a.num_blocks > 0 ? lay.k_words() : 0;
+  const int64_t v_words = a.num_blocks > 0 ? lay.v_words() : 0;
   constexpr int kPairs = kTok * (D / 16);  // of K, and of V
   auto load_codes = [&](const Places& p) {
 #pragma unroll
@@ -355,15 +367,12 @@ paged_tile_kernel(PagedArgs a) {
       const int at = pair % kPairs, tok = at / (D / 16), part = at % (D / 16);
       const uint32_t o = __builtin_amdgcn_ds_bpermute(4 * tok, p.k);
       const int place = __builtin_amdgcn_ds_bpermute(4 * tok, p.at);
-      const char* const src = a.k + kv * a.kh + ((uint64_t)o << 4);
-      const char* c = src + (is_v ? lay.v_codes() : 0) + (int64_t)place * lay.row() + part * 8;
+      const char* const src = k_rows + ((uint64_t)o << 4);
+      codes[i] = load_u32x2(src + (is_v ? v_codes : 0) + (int64_t)place * lay.row() + part * 8);
       // K: words of groups 2 (part % (D / 64)) and the next. V: both of one group.
-      const char* w = src + (is_v ? lay.v_words() : lay.k_words()) + (int64_t)place * lay.words() +
-                      (is_v ? part / 2 * 2 : part % (D / 64) * 4);
-      const bool ok = o != kNoToken;
-      codes[i] = load_u32x2(ok ? c : zero);
-      const uint16_t* w16 = reinterpret_cast<const uint16_t*>(ok ? w : zero);
-      words[i] = w16[0] | (uint32_t)w16[is_v ? 0 : 1] << 16;
+      const char* const w = src + (is_v ? v_words : k_words) + (int64_t)place * lay.words();
+      if (is_v) words[i] = reinterpret_cast<const uint16_t*>(w)[part / 2] * 0x10001u;
+      else words[i] = reinterpret_cast<const uint32_t*>(w)[part % (D / 64)];
     }
   };
   auto store_values = [&](char* stage) {
@@ -878,8 +887,8 @@ paged_rows_kernel(PagedArgs a) {
   const Kv4Page lay{a.page_size, D};
 
   auto load_page = [&](int block) {
-    const int at = block < s_end ? span.base(block) + lane % T : INT_MAX;
-    return *(at < span.end ? trow + a.page_div.div(at) : g_qsa_no_page);
+    return *(span.end > 0 ? trow + a.page_div.div(min(span.base(block) + lane % T, span.end - 1))
+                          : a.seq_lens);
   };
   // A block on its way: K in registers, V on its way into LDS.
   struct Block {
@@ -890,7 +899,7 @@ paged_rows_kernel(PagedArgs a) {
   auto start = [&](int block, int page, char* v_lds) {
     Block r;
     const int t = span.base(block) + lane % T;
-    const bool ok = page >= 0 && page < a.num_blocks;
+    const bool ok = page >= 0 && page < a.num_blocks && t < span.end;
     const int at = t - a.page_div.div(t) * a.page_size;
     r.valid = __ballot(ok);
     if constexpr (KV4) {
@@ -1311,8 +1320,8 @@ struct PagedPlan {
 };
 
 // The bounds shape the launch: a longer context is computed whole all the same.
-PagedPlan make_plan(int rows, int requests, int num_q_heads, int num_kv_heads, int max_query_len,
-                    int max_seq_len, int window, int sinks) {
+PagedPlan make_plan(bool kv4, int rows, int requests, int num_q_heads, int num_kv_heads,
+                    int max_query_len, int max_seq_len, int window, int sinks) {
   PagedPlan p = {};
   const int64_t group = num_q_heads / num_kv_heads;
   const int64_t most = std::min(max_query_len, rows) * group;
@@ -1334,7 +1343,11 @@ PagedPlan make_plan(int rows, int requests, int num_q_heads, int num_kv_heads, i
       p.few_groups = (int)std::max<int64_t>(2 * kCUs, 2 * p.few_units);
   }
   if (most > p.few) {
-    p.waves = most <= 64 ? 2 : most <= 128 ? 4 : 8;
+    // Tiles of 128 rows, two workgroups a CU; of fewer where requests have no more. Tiles
+    // of 256 read K/V half as often and wait for their longest longer: 286 us for 259 on
+    // 8192 rows of 32 heads and a window of 4096. A 4-bit cache's are 256: its values are
+    // made once a tile, 297 us for 336 on 4 x 500 rows of 32 heads on 16k.
+    p.waves = most <= 64 ? 2 : most <= 128 || !kv4 ? 4 : 8;
     const int64_t tile_rows = 32 * p.waves;
     p.tiles = std::min<int64_t>((rows * group) / tile_rows + requests,
                                 requests * ((most + tile_rows - 1) / tile_rows));
@@ -1436,8 +1449,8 @@ int run_paged(const std::string& name, PagedArgs a, bool kv4, const void* q, int
   a.window = window > 0 ? std::min(window, kNoWindow) : kNoWindow;
   if ((int64_t)rows * num_q_heads > INT_MAX / 2)
     return fail(QSA_ERR_UNSUPPORTED, name + ": too many rows or heads");
-  const PagedPlan plan = make_plan(rows, num_requests, num_q_heads, num_kv_heads, max_query_len,
-                                   max_seq_len, a.window, sink_tokens);
+  const PagedPlan plan = make_plan(kv4, rows, num_requests, num_q_heads, num_kv_heads,
+                                   max_query_len, max_seq_len, a.window, sink_tokens);
   const size_t need = workspace_of(plan, num_kv_heads, head_dim);
   if (need && (!workspace || workspace_bytes < need || !aligned16(workspace)))
     return fail(QSA_ERR_WORKSPACE, name + ": needs a 16-byte aligned workspace of " +
@@ -1520,10 +1533,14 @@ extern "C" size_t qsa_paged_attention_workspace_bytes(int rows, int requests, in
   if (rows <= 0 || requests <= 0 || num_kv_heads <= 0 || num_q_heads < num_kv_heads ||
       head_dim <= 0 || max_query_len <= 0 || max_seq_len < 0 || window < 0 || sink_tokens < 0)
     return 0;
-  return workspace_of(make_plan(rows, requests, num_q_heads, num_kv_heads,
-                                std::min(max_query_len, rows), max_seq_len,
-                                window > 0 ? std::min(window, kNoWindow) : kNoWindow, sink_tokens),
-                      num_kv_heads, head_dim);
+  size_t need = 0;  // for either cache
+  for (const bool kv4 : {false, true})
+    need = std::max(need, workspace_of(make_plan(kv4, rows, requests, num_q_heads, num_kv_heads,
+                                                 std::min(max_query_len, rows), max_seq_len,
+                                                 window > 0 ? std::min(window, kNoWindow) : kNoWindow,
+                                                 sink_tokens),
+                                       num_kv_heads, head_dim));
+  return need;
 }
 
 extern "C" int qsa_window_attention(

@@ -346,6 +346,16 @@ def test_empty_calls():
     assert (got == 0).all()
 
 
+@pytest.mark.parametrize("bits", [16, 4])
+@pytest.mark.parametrize("new", [[1], [2, 1], [40], [300]])
+def test_no_blocks(new, bits):
+    """Lengths and a table that speak of pages that the cache does not have."""
+    c = Case([100] * len(new), new, bits=bits)
+    cache = c.device_cache()
+    cache = Int4KVCache(cache.data[:0], 16, 128) if bits == 4 else (cache[0][:0], cache[1][:0])
+    assert (c.run(cache=cache) == 0).all()
+
+
 def test_refusals():
     c = Case([10], [2])
     k, v = c.device_cache()
