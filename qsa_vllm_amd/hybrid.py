@@ -36,6 +36,13 @@ GDN projection layout: ``in_proj_qkvz`` grouped per key head as
 ``[q (dk), k (dk), v (r*dv), z (r*dv)]`` and ``in_proj_ba`` as ``[b (r), a (r)]``
 (the grouped layout vLLM selects with ``gqa_interleaved_layout=True``).
 
+Layers named in ``window_layers`` are ordinary causal attention over the last
+``attention_window`` tokens and the first ``sink_tokens`` ("sliding_attention") in
+place of their mixer: the projection ``[q|gate head-interleaved, k, v]``, every head
+normed, rotated and stored by ``qk_norm_rope``, then ``qsa_window_paged_attention``
+over a bf16 cache or, with ``window_kv_bits=4``, ``qsa_int4_paged_attention`` over
+one of 4 bits. They share the QSA layers' page table. The model served here has none.
+
 With ``weight_bits=4`` the projections, the MLPs and the LM head hold 4-bit
 codes with group scales (``ops/int4.py``) instead of bf16 and multiply by
 ``int4_linear``: for steps of few tokens, which only stream the weights.
@@ -56,7 +63,9 @@ from .metadata import QSABatch, QSAMetadataBuilder
 from .ops.hybrid_layers import (gated_norm, gdn_conv_state, gdn_gated_norm, gdn_prep,
                                 gdn_recurrence, silu_mul)
 from .ops.int4 import Int4Weight, int4_linear, int4_quantize
+from .ops.kv_cache import Int4KVCache, qk_norm_rope, rotary_table
 from .ops.logits import LogitsRules, process_logits
+from .ops.paged import qsa_int4_paged_attention, qsa_window_paged_attention
 
 __all__ = ["HybridConfig", "HybridBatch", "HybridBatchBuilder", "HybridDecoder",
            "HybridDecodeGraph", "HybridWorkload", "make_hybrid_workload",
@@ -94,13 +103,23 @@ class HybridConfig:
     init_std: float = 0.02
     weight_bits: int = 16        # of the projections, MLPs and LM head: 16 (bf16) or 4
     weight_group: int = 128      # inputs of a 4-bit weight's scale
+    window_layers: tuple[int, ...] = ()   # layers of windowed attention
+    attention_window: int | None = 4096   # their window in tokens; None: the whole context
+    sink_tokens: int = 0         # first tokens that they see at any distance
+    window_kv_bits: int = 16     # of their caches: 16 (bf16) or 4
 
     def __post_init__(self):
         if self.weight_bits not in (4, 16):
             raise ValueError(f"weight_bits must be 4 or 16, got {self.weight_bits}")
+        if self.window_kv_bits not in (4, 16):
+            raise ValueError(f"window_kv_bits must be 4 or 16, got {self.window_kv_bits}")
+        if any(not 0 <= i < self.num_layers for i in self.window_layers):
+            raise ValueError(f"window_layers must be layers 0 .. {self.num_layers - 1}, "
+                             f"got {self.window_layers}")
 
     def layer_types(self) -> list[str]:
-        return ["full_attention" if (i + 1) % self.full_attention_every == 0
+        return ["sliding_attention" if i in self.window_layers
+                else "full_attention" if (i + 1) % self.full_attention_every == 0
                 else "linear_attention" for i in range(self.num_layers)]
 
     @property
@@ -237,6 +256,59 @@ class QSAAttention:
         core = torch.empty(t, self.heads, self.head_dim, dtype=torch.bfloat16, device=x.device)
         qsa_layer_step(self.indexer, self.impl, self.layer, batch.qsa, index_qk, key, value, query,
                        core, gate)
+        return _linear(core.view(t, -1), self.o_proj)
+
+
+class WindowAttention:
+    """Causal attention over a sliding window and the first tokens, gated."""
+
+    def __init__(self, cfg: HybridConfig, init: _Init, num_blocks: int, max_position: int,
+                 cache_std: float):
+        d = cfg.head_dim
+        self.heads, self.kv_heads, self.head_dim = cfg.heads, cfg.kv_heads, d
+        self.window, self.sinks, self.eps = cfg.attention_window, cfg.sink_tokens, cfg.rms_norm_eps
+        self.page_size = cfg.page_size
+        self.q_size, self.kv_size = 2 * self.heads * d, self.kv_heads * d
+        rows = self.q_size + 2 * self.kv_size
+        self.qkv_weight = _stored(cfg, init.normal(rows, cfg.hidden_size))
+        self.qkv_bias = init.normal(rows)
+        self.q_norm = torch.ones(d, dtype=torch.bfloat16, device=init.device)
+        self.k_norm = torch.ones(d, dtype=torch.bfloat16, device=init.device)
+        self.o_proj = _stored(cfg, init.normal(cfg.hidden_size, self.heads * d))
+        self.cos_sin = rotary_table(max_position, cfg.rope_dim, cfg.rope_theta, init.device)
+        kv = init.normal(num_blocks, cfg.page_size, self.kv_heads, 2 * d, std=cache_std)
+        if cfg.window_kv_bits == 16:
+            self.cache = kv[..., :d], kv[..., d:]
+            self.state = kv
+        else:
+            self.cache = Int4KVCache.allocate(num_blocks, cfg.page_size, self.kv_heads, d,
+                                              init.device)
+            self.state = self.cache.data
+            rows = kv.flatten(0, 1)
+            slots = torch.arange(rows.shape[0], device=init.device)
+            qk_norm_rope(None, rows[..., :d], None, None, None, None, self.eps, value=rows[..., d:],
+                         cache=self.cache, slot_mapping=slots)
+
+    def __call__(self, x, batch: "HybridBatch"):
+        t, d, qsa = x.shape[0], self.head_dim, batch.qsa
+        qkv = _linear(x, self.qkv_weight, self.qkv_bias)
+        qg, key, value = qkv.split((self.q_size, self.kv_size, self.kv_size), dim=-1)
+        qg = qg.view(t, self.heads, 2 * d)
+        query, _ = qk_norm_rope(qg[..., :d], key.view(t, self.kv_heads, d), self.q_norm, self.k_norm,
+                                qsa.positions, self.cos_sin, self.eps,
+                                value=value.view(t, self.kv_heads, d), cache=self.cache,
+                                slot_mapping=qsa.main.slot_mapping)
+        table = qsa.main.block_table
+        # A graph is replayed on longer contexts: its launches are shaped for all.
+        longest = (table.shape[1] * self.page_size if torch.cuda.is_current_stream_capturing()
+                   else qsa.compressed.max_seq_len)
+        args = dict(window=self.window, sink_tokens=self.sinks, output_gate=qg[..., d:],
+                    max_query_len=qsa.main.max_query_len, max_seq_len=longest)
+        where = table, qsa.compressed.seq_lens, qsa.raw.query_start_loc
+        if isinstance(self.cache, Int4KVCache):
+            core = qsa_int4_paged_attention(query, self.cache, *where, **args)
+        else:
+            core = qsa_window_paged_attention(query, *self.cache, *where, **args)
         return _linear(core.view(t, -1), self.o_proj)
 
 
@@ -389,6 +461,8 @@ class HybridDecoder:
                 comp = init.normal(comp_blocks, cfg.comp_page_size, 1, dx, std=cache_std)
                 mixer = QSAAttention(cfg, init, kv.permute(0, 2, 1, 3), ring, comp, max_tokens,
                                      max_position)
+            elif kind == "sliding_attention":
+                mixer = WindowAttention(cfg, init, num_blocks, max_position, cache_std)
             else:
                 mixer = GatedDeltaNet(cfg, init, state_slots, state_std)
             self.layers.append(DecoderLayer(kind, mixer, cfg, init))
@@ -494,6 +568,8 @@ class HybridWorkload:
             mx = layer.mixer
             if layer.kind == "full_attention":
                 out += [mx.layer.kv_cache, mx.indexer.raw_key_cache, mx.indexer.compressed_key_cache]
+            elif layer.kind == "sliding_attention":
+                out.append(mx.state)
             else:
                 out += [mx.conv_state, mx.ssm_state]
         return out

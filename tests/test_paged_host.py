@@ -135,3 +135,15 @@ def test_cpu_tensors_are_refused():
                  lambda: qk_norm_rope(q, q, None, None, None, None, 1e-6)):
         with pytest.raises((RuntimeError, NotImplementedError)):
             call()
+
+
+def test_window_layers_of_the_hybrid_decoder():
+    from qsa_vllm_amd.hybrid import HybridConfig
+
+    assert "sliding_attention" not in HybridConfig().layer_types()
+    kinds = HybridConfig(num_layers=4, window_layers=(0, 3)).layer_types()
+    assert kinds == ["sliding_attention", "linear_attention", "linear_attention", "sliding_attention"]
+    with pytest.raises(ValueError, match="window_kv_bits"):
+        HybridConfig(window_kv_bits=8)
+    with pytest.raises(ValueError, match="window_layers"):
+        HybridConfig(num_layers=4, window_layers=(4,))
