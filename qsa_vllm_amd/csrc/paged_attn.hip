@@ -80,6 +80,7 @@ struct PagedArgs {
   int tiles;      // of the launch
   int few;        // (row, head)s of a kv head up to which a request is one of few rows; 0: none is
   int few_groups;  // workgroups of the launch for those, 0: one for each request and kv head
+  int few_waves;   // of such a workgroup
   float scale_log2;
 };
 
@@ -308,8 +309,8 @@ paged_tile_kernel(PagedArgs a) {
     return *(span.end > 0 ? trow + a.page_div.div(min(span.base(stage) + lane, span.end - 1))
                           : a.seq_lens);
   };
-  // Offsets (16-byte units) of token base + lane. What is no token is loaded from the
-  // cache's first rows instead, whose scores are masked.
+  // Offsets (16-byte units) of token base + lane. In place of what is no token the last
+  // one is loaded, or the cache's first rows where a page is missing: those scores are masked.
   struct Places {
     uint32_t k, v;
     int at;
@@ -317,9 +318,10 @@ paged_tile_kernel(PagedArgs a) {
   };
   auto places = [&](int stage, int page) __attribute__((always_inline)) {
     Places p;
-    const int t = span.base(stage) + lane;
-    const bool ok = page >= 0 && page < a.num_blocks && t < span.end && stage < s_end;
-    const int live = ok ? -1 : 0;
+    const int t = min(span.base(stage) + lane, span.end - 1);
+    const bool paged = page >= 0 && page < a.num_blocks;
+    const bool ok = paged && span.base(stage) + lane < span.end && stage < s_end;
+    const int live = paged ? -1 : 0;
     p.at = (t - a.page_div.div(t) * a.page_size) & live;
     const uint32_t block = page & live;
     p.k = block * a.kb + (KV4 ? 0 : p.at * a.kt);
@@ -683,27 +685,26 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedArgs a) {
 // numbers 16 + c (a code's bits in the fraction of 16.0), and the groups' scales and
 // zero points come in afterwards, by 32 dims (one product):
 //
-//   s_t  = sum_G s_tG [ sum_d (16 + c_td) q_d  -  (16 + z_tG) sum_d q_d ]
+//   s_t  = sum_G s_tG sum_d (16 + c_td) q_d  -  sum_G (16 s_tG + s_tG z_tG) sum_d q_d
 //   o_d += sum_t (p_t s_tG) (16 + c_td)  -  sum_t (p_t s_tG) (16 + z_tG)
 //
-// the last sum once a group, by one more product. p_t s_tG is rounded to bf16 for both.
+// the last sums by one more product each: 16 s and s z are bf16 numbers (of 4 and 8
+// bits), the sums of q are split in three. p_t s_tG is rounded to bf16 for both.
 
 constexpr int kFew = 16;
-constexpr int kRowWaves = 4;
-constexpr int kMinBlocks = 8;  // of a piece
 
-template <int D, bool KV4>
+template <int D, bool KV4, int W>
 struct RowShape {
   static constexpr int kBlock = KV4 ? 64 : 32;    // positions of a wave's block
   static constexpr int kSub = kBlock / 16;
   static constexpr int kGroups = D / 32;
   static constexpr int kVRow = KV4 ? D / 2 : 2 * D;  // bytes of a V row in LDS
   static constexpr int kV = kBlock * kVRow;
-  // 4 bits: K's scales, K's scales times 16 + z, V's scales (fp32), V's 16 + z (bf16)
+  // 4 bits: K's scales (fp32), its 16 s and s z (bf16), V's scales (fp32), V's 16 + z (bf16)
   static constexpr int kWords = KV4 ? kGroups * kBlock * 14 : 0;
-  static constexpr int kWave = 2 * kV + kWords;
+  static constexpr int kWave = kV + kWords;
   static constexpr int kMerge = 16 * (D + 2) * 4;  // a wave's result
-  static constexpr int kLds = kRowWaves * (kWave > kMerge ? kWave : kMerge);
+  static constexpr int kLds = W * (kWave > kMerge ? kWave : kMerge);
 };
 
 template <int T>
@@ -724,7 +725,7 @@ __device__ __forceinline__ int pieces_of(int blocks, int per) {
 __device__ __forceinline__ int piece_blocks(const PagedArgs& a, int blocks, int requests) {
   if (!a.few_groups) return INT_MAX;
   const unsigned spare = max(a.few_groups / a.kv_heads - requests, 1);
-  return max(kMinBlocks, (int)(((unsigned)blocks + spare - 1u) / spare));
+  return max(a.few_waves, (int)(((unsigned)blocks + spare - 1u) / spare));
 }
 // False where the launch has no such workgroup.
 template <int T>
@@ -807,12 +808,13 @@ __device__ __forceinline__ float sum_over_quarters(float v) {
 }
 
 // Codes of nibbles i and i + 4 of a word, i = 0 .. 3, as bf16 pairs of 16 + c.
-__device__ __forceinline__ u32x4 codes_of(uint32_t w) {
+// `bits` is 0x00780078, in a vector register: two constants do not fit one instruction.
+__device__ __forceinline__ u32x4 codes_of(uint32_t w, uint32_t bits) {
   u32x4 r;
-  r[0] = ((w << 3) & 0x00780078u) | 0x41804180u;
-  r[1] = ((w >> 1) & 0x00780078u) | 0x41804180u;
-  r[2] = ((w >> 5) & 0x00780078u) | 0x41804180u;
-  r[3] = ((w >> 9) & 0x00780078u) | 0x41804180u;
+  r[0] = ((w << 3) & bits) | 0x41804180u;
+  r[1] = ((w >> 1) & bits) | 0x41804180u;
+  r[2] = ((w >> 5) & bits) | 0x41804180u;
+  r[3] = ((w >> 9) & bits) | 0x41804180u;
   return r;
 }
 __device__ __forceinline__ f32x4 product(u32x4 a, u32x4 b, f32x4 c) {
@@ -832,10 +834,10 @@ __device__ __forceinline__ int v4_at(int tok, int unit) {
   return tok * (D / 2) + (unit ^ (D == 128 ? tok >> 2 & 3 : tok >> 3 & 1)) * 16;
 }
 
-template <int D, bool KV4>
-__global__ __launch_bounds__(64 * kRowWaves) __attribute__((amdgpu_waves_per_eu(2, 3))) void
+template <int D, bool KV4, int W>
+__global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(2, 3))) void
 paged_rows_kernel(PagedArgs a) {
-  typedef RowShape<D, KV4> S;
+  typedef RowShape<D, KV4, W> S;
   constexpr int T = S::kBlock;
   constexpr int U = D / 8;
   constexpr int kGroups = S::kGroups;  // of 32 dims: products of a score
@@ -870,98 +872,88 @@ paged_rows_kernel(PagedArgs a) {
 #pragma unroll
     for (int s = 0; s < kGroups; ++s) q[s] = load_u32x4(src + 32 * s + 8 * g);
   }
-  float q_sum[kGroups];
+  // 4 bits: minus the sums of q over the groups, in three bf16 parts (all 24 bits), part g
+  // in quarter g, as the operand that meets 16 s and s z.
+  u32x4 q_sums = {0, 0, 0, 0};
   if constexpr (KV4) {
 #pragma unroll
     for (int s = 0; s < kGroups; ++s) {
       float v = 0.0f;
 #pragma unroll
       for (int i = 0; i < 4; ++i) v += bf16_lo(q[s][i]) + bf16_hi(q[s][i]);
-      q_sum[s] = sum_over_quarters(v);
+      float rest = -sum_over_quarters(v);
+#pragma unroll
+      for (int part = 0; part < 3; ++part) {
+        const uint32_t top = __builtin_bit_cast(uint32_t, rest) & 0xFFFF0000u;
+        q_sums[s] = g == part ? top | top >> 16 : q_sums[s];
+        rest -= __builtin_bit_cast(float, top);
+      }
     }
   }
 
-  char* const mine = lds + wave * S::kWave;
-  char* const words = mine + 2 * S::kV;
+  char* const mine = lds + wave * S::kWave;  // V, then a 4-bit cache's words
+  char* const words = mine + S::kV;
   const char* const zero = reinterpret_cast<const char*>(g_qsa_zero_rows);
   const Kv4Page lay{a.page_size, D};
+  const bool any = a.num_blocks > 0;  // (no cache: zeros)
+  const char* const k_rows = any ? a.k + kv * a.kh : zero;
+  const char* const v_rows = !any ? zero : KV4 ? k_rows + lay.v_codes() : a.v + kv * a.vh;
+  const char* const k_words = k_rows + (any ? lay.k_words() : 0);
+  const char* const v_words = k_rows + (any ? lay.v_words() : 0);
 
-  auto load_page = [&](int block) {
+  // Page of token base + lane, past the end the last one's. (Without a token any address does.)
+  auto load_page = [&](int block) __attribute__((always_inline)) {
     return *(span.end > 0 ? trow + a.page_div.div(min(span.base(block) + lane % T, span.end - 1))
                           : a.seq_lens);
   };
-  // A block on its way: K in registers, V on its way into LDS.
+  // A block on its way, all of it in registers.
   struct Block {
     u32x4 k[S::kSub][KV4 ? 1 : kGroups];
+    u32x4 v[S::kV / 1024];
     u32x2 kw, vw;  // 4 bits: the lane's token's words
     uint64_t valid;
   };
-  auto start = [&](int block, int page, char* v_lds) {
-    Block r;
-    const int t = span.base(block) + lane % T;
-    const bool ok = page >= 0 && page < a.num_blocks && t < span.end;
-    const int at = t - a.page_div.div(t) * a.page_size;
-    r.valid = __ballot(ok);
-    if constexpr (KV4) {
-      const uint32_t block_at = ok ? page * a.kb : kNoToken;
-      const char* const own = a.k + kv * a.kh + ((uint64_t)block_at << 4);
+  // In place of what is no token the last one is loaded, or the cache's first rows where
+  // a page is missing: those scores are masked.
+  auto start = [&](int block, int page, Block& r) __attribute__((always_inline)) {
+    const int own = span.base(block) + lane % T;
+    const int t = min(own, span.end - 1);
+    const bool paged = page >= 0 && page < a.num_blocks && span.end > 0;
+    const uint32_t at = paged ? t - a.page_div.div(t) * a.page_size : 0;
+    const uint32_t in = paged ? page : 0;
+    r.valid = __ballot(paged && own < span.end && block < s_end);
+    // (units of 16 bytes)
+    const uint32_t k_at = in * a.kb + at * (KV4 ? D / 32 : a.kt);
+    const uint32_t v_at = KV4 ? k_at : in * a.vb + at * a.vt;
 #pragma unroll
-      for (int u = 0; u < S::kSub; ++u) {
-        const uint32_t o = __builtin_amdgcn_ds_bpermute(4 * (16 * u + n), block_at);
-        const int p = __builtin_amdgcn_ds_bpermute(4 * (16 * u + n), at);
-        const char* src = a.k + kv * a.kh + ((uint64_t)o << 4) + (int64_t)p * lay.row() + g * (D / 8);
-        src = o != kNoToken ? src : zero;
-        if constexpr (D == 128) {
-          r.k[u][0] = load_u32x4(src);
-        } else {
-          const u32x2 x = load_u32x2(src);
-          r.k[u][0] = u32x4{x[0], x[1], 0, 0};
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < S::kV / 1024; ++i) {
-        constexpr int kParts = D / 32;  // 16-byte units of a row
-        const int tok = i * (64 / kParts) + lane / kParts;
-        const int unit = (v4_at<D>(tok, lane % kParts) - tok * (D / 2)) / 16;
-        const uint32_t o = __builtin_amdgcn_ds_bpermute(4 * tok, block_at);
-        const int p = __builtin_amdgcn_ds_bpermute(4 * tok, at);
-        const char* src = a.k + kv * a.kh + ((uint64_t)o << 4) + lay.v_codes() +
-                          (int64_t)p * lay.row() + unit * 16;
-        load_to_lds(o != kNoToken ? src : zero, v_lds + i * 1024);
-      }
-      const char* kw = own + lay.k_words() + (int64_t)at * lay.words();
-      const char* vw = own + lay.v_words() + (int64_t)at * lay.words();
-      kw = ok ? kw : zero;
-      vw = ok ? vw : zero;
-      if constexpr (D == 128) {
-        r.kw = load_u32x2(kw);
-        r.vw = load_u32x2(vw);
+    for (int u = 0; u < S::kSub; ++u) {
+      const uint32_t o = __builtin_amdgcn_ds_bpermute(4 * (16 * u + n), k_at);
+      const char* const src = k_rows + ((uint64_t)o << 4) + (KV4 ? g * (D / 8) : 16 * g);
+      if constexpr (KV4 && D == 64) {
+        const u32x2 x = load_u32x2(src);
+        r.k[u][0] = u32x4{x[0], x[1], 0, 0};
       } else {
-        r.kw = u32x2{*reinterpret_cast<const uint32_t*>(kw), 0};
-        r.vw = u32x2{*reinterpret_cast<const uint32_t*>(vw), 0};
-      }
-    } else {
-      const uint32_t k_at = ok ? page * a.kb + at * a.kt : kNoToken;
-      const uint32_t v_off = page * a.vb + at * a.vt;
 #pragma unroll
-      for (int u = 0; u < S::kSub; ++u) {
-        const uint32_t o = __builtin_amdgcn_ds_bpermute(4 * (16 * u + n), k_at);
-        const char* src = a.k + kv * a.kh + ((uint64_t)o << 4);
-        src = (o != kNoToken ? src : zero) + 16 * g;
-#pragma unroll
-        for (int s = 0; s < kGroups; ++s) r.k[u][s] = load_u32x4(src + 64 * s);
-      }
-#pragma unroll
-      for (int i = 0; i < S::kV / 1024; ++i) {
-        const int tok = i * (64 / U) + lane / U;
-        const int unit = lane % U ^ v_swizzle<D>(tok);
-        const uint32_t o = __builtin_amdgcn_ds_bpermute(4 * tok, v_off);
-        const uint32_t ko = __builtin_amdgcn_ds_bpermute(4 * tok, k_at);
-        const char* src = a.v + kv * a.vh + ((uint64_t)o << 4);
-        load_to_lds((ko != kNoToken ? src : zero) + unit * 16, v_lds + i * 1024);
+        for (int s = 0; s < (KV4 ? 1 : kGroups); ++s) r.k[u][s] = load_u32x4(src + 64 * s);
       }
     }
-    return r;
+    constexpr int kUnits = S::kVRow / 16;
+#pragma unroll
+    for (int i = 0; i < S::kV / 1024; ++i) {
+      const int tok = i * (64 / kUnits) + lane / kUnits;
+      const uint32_t o = __builtin_amdgcn_ds_bpermute(4 * tok, v_at);
+      r.v[i] = load_u32x4(v_rows + ((uint64_t)o << 4) + lane % kUnits * 16);
+    }
+    if constexpr (KV4) {
+      const uint64_t from = ((uint64_t)(in * a.kb) << 4) + at * (D / 16);
+      if constexpr (D == 128) {
+        r.kw = load_u32x2(k_words + from);
+        r.vw = load_u32x2(v_words + from);
+      } else {
+        r.kw = u32x2{*reinterpret_cast<const uint32_t*>(k_words + from), 0};
+        r.vw = u32x2{*reinterpret_cast<const uint32_t*>(v_words + from), 0};
+      }
+    }
   };
 
   f32x4 o[kDims], oz[KV4 ? kGroups : 1];
@@ -973,54 +965,78 @@ paged_rows_kernel(PagedArgs a) {
   const float slack = kSlack / a.scale_log2;
   bool poisoned = false;
 
-  Block next = {};
-  int page_next = -1;
-  if (s_begin + wave < s_end) next = start(s_begin + wave, load_page(s_begin + wave), mine);
-  page_next = load_page(s_begin + wave + kRowWaves);
+  uint32_t bits = 0x00780078u;
+  asm volatile("" : "+v"(bits));
+  Block now;  // the wave's next block
+  start(s_begin + wave, load_page(s_begin + wave), now);
+  int page = load_page(s_begin + wave + W);  // of the one behind it
 
-  // (The pointers are said to be apart: the compiler would otherwise wait for the loads
-  // into `v_next` before it reads V.)
-  auto step = [&](int block, char* __restrict v_lds, char* __restrict v_next) {
-    __builtin_amdgcn_s_waitcnt(kLoadsDone);
-    asm volatile("" ::: "memory");  // nothing is read from LDS before
-    const Block now = next;
-    if (block + kRowWaves < s_end) next = start(block + kRowWaves, page_next, v_next);
-    page_next = load_page(block + 2 * kRowWaves);
+  for (int block = s_begin + wave; block < s_end; block += W) {
+    char* const v_lds = mine;
+    const uint64_t valid = now.valid;
+#pragma unroll
+    for (int i = 0; i < S::kV / 1024; ++i) {
+      constexpr int kUnits = S::kVRow / 16;
+      const int tok = i * (64 / kUnits) + lane / kUnits, unit = lane % kUnits;
+      *reinterpret_cast<u32x4*>(mine + (KV4 ? v4_at<D>(tok, unit) : v_at<D>(tok, unit))) = now.v[i];
+    }
     const int t0 = span.base(block);
     constexpr uint64_t kAll = T == 64 ? ~0ull : (1ull << (T % 64)) - 1;
-    const bool mixed = (now.valid & kAll) != kAll || span.mixed(a, t0);
-    const uint64_t seen = mixed ? now.valid & seen_from(a, pos, t0) : 0;  // of the lane's row
+    const bool mixed = (valid & kAll) != kAll || span.mixed(a, t0);
+    const uint64_t seen = mixed ? valid & seen_from(a, pos, t0) : 0;  // of the lane's row
 
     f32x4 sc[S::kSub];
     if constexpr (KV4) {
       // The lane's token's words, taken apart for all.
       float* const ks = reinterpret_cast<float*>(words);
-      float* const kz = ks + kGroups * T;
-      float* const vs = kz + kGroups * T;
+      uint32_t* const kz = reinterpret_cast<uint32_t*>(ks + kGroups * T);
+      float* const vs = reinterpret_cast<float*>(kz + kGroups * T);
       uint16_t* const vz = reinterpret_cast<uint16_t*>(vs + kGroups * T);
+      u32x4 zero_at = {0, 0, 0, 0};
+      bool bad = false;
 #pragma unroll
       for (int s = 0; s < kGroups; ++s) {
         const uint32_t kw = now.kw[s / 2] >> (16 * (s % 2)), vw = now.vw[s / 2] >> (16 * (s % 2));
         const float scale = __builtin_bit_cast(float, (kw & 0xFFF0u) << 16);
         ks[s * T + lane] = scale;
-        kz[s * T + lane] = scale * (float)(16 + (kw & 15u));
-        vs[s * T + lane] = __builtin_bit_cast(float, (vw & 0xFFF0u) << 16);
+        zero_at[s] = perm_b32(__builtin_bit_cast(uint32_t, scale * (float)(kw & 15u)),
+                              __builtin_bit_cast(uint32_t, scale * 16.0f), 0x07060302u);
+        const uint32_t v_scale = (vw & 0xFFF0u) << 16;
+        bad |= v_scale >= 0x7F800000u;  // (NaN: the only one past the finite)
+        vs[s * T + lane] = __builtin_bit_cast(float, v_scale);
         // Token 16 u + 4 g' + r at the place of its code in the other operand.
         const int u = lane >> 4, gt = lane >> 2 & 3, r = lane & 3;
         vz[((s * 2 + u / 2) * 4 + gt) * 8 + r * 2 + u % 2] = (uint16_t)(0x4180u | (vw & 15u) << 3);
       }
+      if constexpr (D == 128)
+        *reinterpret_cast<u32x4*>(kz + 4 * lane) = zero_at;
+      else
+        *reinterpret_cast<u32x2*>(kz + 2 * lane) = u32x2{zero_at[0], zero_at[1]};
+      if (mixed && __any(bad)) {
+        // V may be NaN where a row must not see it: as in the tiles' kernel.
+#pragma unroll
+        for (int s = 0; s < kGroups; ++s)
+          if (__builtin_bit_cast(uint32_t, vs[s * T + lane]) >= 0x7F800000u) vs[s * T + lane] = 0.0f;
+        poisoned = true;
+      }
 #pragma unroll
       for (int u = 0; u < S::kSub; ++u) {
-        sc[u] = f32x4{0, 0, 0, 0};
+        if constexpr (D == 128) {
+          zero_at = load_u32x4(kz + 4 * (16 * u + n));
+        } else {
+          const u32x2 x = load_u32x2(kz + 2 * (16 * u + n));
+          zero_at = u32x4{x[0], x[1], 0, 0};
+        }
+        sc[u] = product(zero_at, q_sums, f32x4{0, 0, 0, 0});
 #pragma unroll
         for (int s = 0; s < kGroups; ++s) {
-          const f32x4 x = product(codes_of(now.k[u][0][s]), q[s], f32x4{0, 0, 0, 0});
+          const f32x4 x = product(codes_of(now.k[u][0][s], bits), q[s], f32x4{0, 0, 0, 0});
           const f32x4 scale = *reinterpret_cast<const f32x4*>(ks + s * T + 16 * u + 4 * g);
-          const f32x4 zero_at = *reinterpret_cast<const f32x4*>(kz + s * T + 16 * u + 4 * g);
 #pragma unroll
-          for (int r = 0; r < 4; ++r)
-            sc[u][r] = __builtin_fmaf(scale[r], x[r], __builtin_fmaf(-zero_at[r], q_sum[s], sc[u][r]));
+          for (int r = 0; r < 4; ++r) sc[u][r] = __builtin_fmaf(scale[r], x[r], sc[u][r]);
         }
+        // (Pinned: the compiler would move the sums behind the branch, and spill.)
+        asm volatile("" : "+v"(sc[u]));
       }
     } else {
       if (mixed) {
@@ -1040,6 +1056,8 @@ paged_rows_kernel(PagedArgs a) {
         for (int s = 0; s < kGroups; ++s) sc[u] = product(now.k[u][s], q[s], sc[u]);
       }
     }
+    start(block + W, page, now);
+    page = load_page(block + 2 * W);
     if (mixed) {
 #pragma unroll
       for (int u = 0; u < S::kSub; ++u)
@@ -1096,11 +1114,7 @@ paged_rows_kernel(PagedArgs a) {
             const int u = 2 * i + e;
             w[e] = *reinterpret_cast<const f32x4*>(vs + s * T + 16 * u + 4 * g);
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              // (a scale may be NaN: not in a place that the row does not see)
-              if (mixed) w[e][r] = seen >> (16 * u + 4 * g + r) & 1 ? w[e][r] : 0.0f;
-              w[e][r] *= sc[u][r];
-            }
+            for (int r = 0; r < 4; ++r) w[e][r] *= sc[u][r];
           }
 #pragma unroll
           for (int r = 0; r < 4; ++r) p[i][r] = pack_bf16x2(w[0][r], w[1][r]);
@@ -1110,8 +1124,8 @@ paged_rows_kernel(PagedArgs a) {
         for (int e = 0; e < 2; ++e) {
           const int d = 2 * s + e;
           const u32x2 c = read_transposed4(v_lds + v4_at<D>(tok, d / 2) + d % 2 * 8);
-          o[d] = product(codes_of(c[0]), p[0], o[d]);
-          o[d] = product(codes_of(c[1]), p[1], o[d]);
+          o[d] = product(codes_of(c[0], bits), p[0], o[d]);
+          o[d] = product(codes_of(c[1], bits), p[1], o[d]);
         }
       }
     } else {
@@ -1133,11 +1147,6 @@ paged_rows_kernel(PagedArgs a) {
                        p, o[d]);
       }
     }
-  };
-  int buffer = 0;
-  for (int block = s_begin + wave; block < s_end; block += kRowWaves) {
-    step(block, mine + buffer * S::kV, mine + (buffer ^ 1) * S::kV);
-    buffer ^= 1;
   }
   sum = sum_over_quarters(sum);
   if constexpr (KV4) {
@@ -1145,8 +1154,8 @@ paged_rows_kernel(PagedArgs a) {
     for (int d = 0; d < kDims; ++d) o[d] -= oz[d / 2];
   }
 
-  if (!KV4 && poisoned) {
-    for (int block = s_begin + wave; block < s_end; block += kRowWaves) {
+  if (poisoned) {
+    for (int block = s_begin + wave; block < s_end; block += W) {
       const int t0 = span.base(block);
       bool whole = t0 + T <= span.end;  // a page missing: a block that was looked at
       for (int i = 0; i < T && t0 + i < span.end; ++i) {
@@ -1158,6 +1167,14 @@ paged_rows_kernel(PagedArgs a) {
         const int page = trow[a.page_div.div(t0 + i)];
         if (page < 0 || page >= a.num_blocks || !(seen_from(a, pos, t0) >> i & 1)) continue;
         const int at = t0 + i - a.page_div.div(t0 + i) * a.page_size;
+        if constexpr (KV4) {
+          const char* const from = v_words + ((uint64_t)((uint32_t)page * a.kb) << 4) + at * (D / 16);
+#pragma unroll
+          for (int d = 0; d < kDims; ++d)
+            if ((reinterpret_cast<const uint16_t*>(from)[d / 2] & 0x7F80u) == 0x7F80u)
+              o[d] = f32x4{__builtin_nanf(""), __builtin_nanf(""), __builtin_nanf(""), __builtin_nanf("")};
+          continue;
+        }
         const char* const v = a.v + kv * a.vh +
                               ((uint64_t)((uint32_t)page * a.vb + (uint32_t)at * a.vt) << 4);
 #pragma unroll
@@ -1189,15 +1206,15 @@ paged_rows_kernel(PagedArgs a) {
   __syncthreads();
   constexpr int kLanes = D / 4;
   const int at = threadIdx.x % kLanes;
-  for (int row = threadIdx.x / kLanes; row < rows; row += 64 * kRowWaves / kLanes) {
+  for (int row = threadIdx.x / kLanes; row < rows; row += 64 * W / kLanes) {
     float top = kNegInf;
 #pragma unroll
-    for (int w = 0; w < kRowWaves; ++w) top = fmaxf(top, merge[w * (S::kMerge / 4) + 16 * D + row]);
+    for (int w = 0; w < W; ++w) top = fmaxf(top, merge[w * (S::kMerge / 4) + 16 * D + row]);
     const float from = top == kNegInf ? 0.0f : top;
     f32x4 acc = {0, 0, 0, 0};
     float total = 0.0f;
 #pragma unroll
-    for (int w = 0; w < kRowWaves; ++w) {
+    for (int w = 0; w < W; ++w) {
       const float* const part = merge + w * (S::kMerge / 4);
       const float f = fast_exp2(part[16 * D + row] - from);
       total += f * part[16 * D + 16 + row];
@@ -1228,12 +1245,15 @@ paged_rows_kernel(PagedArgs a) {
 
 // Joins the pieces of requests of few rows in order, D / 4 lanes a head and WAYS times
 // as many that take every WAYS-th piece.
+template <int WAYS>
+constexpr int kMergeThreads = WAYS == 32 ? 1024 : 256;
 template <int D, int WAYS>
-__global__ __launch_bounds__(256) void paged_rows_merge_kernel(PagedArgs a, int rows_each,
-                                                               int head_groups) {
-  constexpr int kLanes = D / 4, kHeads = 256 / kLanes / WAYS, kAhead = 4;
-  __shared__ f32x4 acc_lds[256 / kLanes][kLanes];
-  __shared__ float top_lds[256 / kLanes], sum_lds[256 / kLanes];
+__global__ __launch_bounds__(kMergeThreads<WAYS>) void paged_rows_merge_kernel(PagedArgs a, int rows_each,
+                                                                               int head_groups) {
+  constexpr int kLanes = D / 4, kAhead = WAYS == 1 ? 4 : 8;
+  constexpr int kGroups = kMergeThreads<WAYS> / kLanes, kHeads = kGroups / WAYS;
+  __shared__ f32x4 acc_lds[kGroups][kLanes];
+  __shared__ float top_lds[kGroups], sum_lds[kGroups];
   const int hg = blockIdx.x % head_groups;
   const int bi = blockIdx.x / head_groups, b = bi / rows_each, i = bi - b * rows_each;
   const int first_piece = a.row_pieces[2 * b], pieces = a.row_pieces[2 * b + 1];
@@ -1315,7 +1335,7 @@ __global__ __launch_bounds__(256) void paged_rows_merge_kernel(PagedArgs a, int 
 struct PagedPlan {
   int waves, splits;   // of the tiles
   int64_t tiles;       // of all requests, at most; 0: no launch
-  int requests, few, few_groups;
+  int requests, few, few_groups, few_waves;
   int64_t few_units;   // requests of few rows and kv heads, at most; 0: no launch
 };
 
@@ -1338,8 +1358,14 @@ PagedPlan make_plan(bool kv4, int rows, int requests, int num_q_heads, int num_k
   if (group <= kFew && (most <= kFew || rows < all)) {
     p.few = kFew;
     p.few_units = (int64_t)requests * num_kv_heads;
-    const int64_t blocks = (seen(kFew / group) + 31) / 32;
-    if (blocks > kMinBlocks && p.few_units <= 16 * kCUs)
+    const int64_t blocks = seen(kFew / group) / (kv4 ? 64 : 32) + 1;
+    // Workgroups of 4 waves, pieces of a block a wave at least: 11.4 us for one request of
+    // 700 .. 4000 tokens, 12.4 from 4 bits. Where 8 waves have 3 blocks each at most (2 from
+    // 4 bits) they are the whole launch: 8.3 us on 300 tokens, 10.3 on 500, 11.7 on 1000
+    // from 4 bits, 14.6 and 17.4 at twice that.
+    const bool whole = p.few_units <= kCUs && blocks <= (kv4 ? 16 : 24);
+    p.few_waves = whole ? 8 : 4;
+    if (!whole && blocks > p.few_waves && p.few_units <= 16 * kCUs)
       p.few_groups = (int)std::max<int64_t>(2 * kCUs, 2 * p.few_units);
   }
   if (most > p.few) {
@@ -1382,13 +1408,20 @@ hipError_t launch_tiles(const PagedArgs& a, int64_t tiles, hipStream_t stream) {
   hipLaunchKernelGGL((paged_merge_kernel<D, W>), dim3((unsigned)a.rows), dim3(256), 0, stream, a);
   return hipGetLastError();
 }
+template <int D, bool KV4, int W>
+hipError_t launch_rows(const PagedArgs& a, int64_t grid, hipStream_t stream) {
+  constexpr int kLds = RowShape<D, KV4, W>::kLds;
+  static_assert(kLds <= 163840, "of a CU");
+  hipLaunchKernelGGL((paged_rows_kernel<D, KV4, W>), dim3((unsigned)grid), dim3(64 * W), kLds, stream, a);
+  return hipGetLastError();
+}
 template <int D, int WAYS>
 hipError_t launch_rows_merge(const PagedArgs& a, int rows_each, hipStream_t stream) {
-  constexpr int kHeads = 256 / (D / 4) / WAYS;
+  constexpr int kHeads = kMergeThreads<WAYS> / (D / 4) / WAYS;
   const int head_groups = (a.num_q_heads + kHeads - 1) / kHeads;
   hipLaunchKernelGGL((paged_rows_merge_kernel<D, WAYS>),
-                     dim3((unsigned)((int64_t)a.requests * rows_each * head_groups)), dim3(256), 0,
-                     stream, a, rows_each, head_groups);
+                     dim3((unsigned)((int64_t)a.requests * rows_each * head_groups)),
+                     dim3(kMergeThreads<WAYS>), 0, stream, a, rows_each, head_groups);
   return hipGetLastError();
 }
 template <int D, bool KV4>
@@ -1397,7 +1430,7 @@ hipError_t launch_paged(const PagedArgs& a, const PagedPlan& p, hipStream_t stre
   const int64_t grid = p.few_groups ? p.few_groups : p.few_units;
   const int rows_each = std::min(a.max_rows, kFew / std::min(a.group, kFew));
   if (!fits(p.tiles * std::max(p.splits, 1) * a.kv_heads, 64 * 8) || !fits(a.rows, 256) ||
-      !fits(grid, 256) || !fits((int64_t)a.requests * rows_each * a.num_q_heads, 256))
+      !fits(grid, 512) || !fits((int64_t)a.requests * rows_each * a.num_q_heads, 1024))
     return kTooLarge;
   if (p.tiles) {
     const hipError_t err = p.waves == 2   ? launch_tiles<D, 2, KV4>(a, p.tiles, stream)
@@ -1406,16 +1439,14 @@ hipError_t launch_paged(const PagedArgs& a, const PagedPlan& p, hipStream_t stre
     if (err != hipSuccess) return err;
   }
   if (!p.few_units) return hipSuccess;
-  constexpr int kLds = RowShape<D, KV4>::kLds;
-  static_assert(kLds <= 65536, "no attribute to set");
-  hipLaunchKernelGGL((paged_rows_kernel<D, KV4>), dim3((unsigned)grid), dim3(64 * kRowWaves), kLds,
-                     stream, a);
-  const hipError_t err = hipGetLastError();
+  const hipError_t err = p.few_waves == 8 ? launch_rows<D, KV4, 8>(a, grid, stream)
+                                          : launch_rows<D, KV4, 4>(a, grid, stream);
   if (err != hipSuccess || !p.few_groups) return err;
-  // Few (row, head)s are joined 8 ways.
-  return (int64_t)a.requests * rows_each * a.num_q_heads <= 2048
-             ? launch_rows_merge<D, 8>(a, rows_each, stream)
-             : launch_rows_merge<D, 1>(a, rows_each, stream);
+  // The fewer (row, head)s, the more pieces have each.
+  const int64_t heads = (int64_t)a.requests * rows_each * a.num_q_heads;
+  return heads <= 256    ? launch_rows_merge<D, 32>(a, rows_each, stream)
+         : heads <= 2048 ? launch_rows_merge<D, 8>(a, rows_each, stream)
+                         : launch_rows_merge<D, 1>(a, rows_each, stream);
 }
 
 bool aligned16(const void* p) { return ((uintptr_t)p & 15u) == 0; }
@@ -1493,6 +1524,7 @@ int run_paged(const std::string& name, PagedArgs a, bool kv4, const void* q, int
   a.tiles = (int)plan.tiles;
   a.few = plan.few;
   a.few_groups = plan.few_groups;
+  a.few_waves = plan.few_waves;
   a.scale_log2 = 1.4426950408889634f / sqrtf((float)head_dim);
   hipStream_t s = static_cast<hipStream_t>(stream);
   const hipError_t err = head_dim == 128 ? (kv4 ? launch_paged<128, true>(a, plan, s)
