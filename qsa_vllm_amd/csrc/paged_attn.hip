@@ -245,22 +245,24 @@ __device__ __forceinline__ float add_pair(uint32_t pair, float c) {
 template <bool K>
 __device__ __forceinline__ u32x4 values4(uint32_t codes, uint32_t word) {
   const float s = __builtin_bit_cast(float, (word & 0xFFF0u) << 16);
-  const float z = (float)(word & 15u);
+  const float zs = -(float)(word & 15u) * s;
+  const uint32_t even = codes & 0x0F0F0F0Fu, odd = codes >> 4 & 0x0F0F0F0Fu;  // a code a byte
   u32x4 r;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const float c0 = (float)(codes >> (K ? 4 * i : 8 * i) & 15u);
-    const float c1 = (float)(codes >> (K ? 4 * i + 16 : 8 * i + 4) & 15u);
-    // (exact in bf16, so the packing truncates nothing)
-    r[i] = perm_b32(__builtin_bit_cast(uint32_t, (c1 - z) * s),
-                    __builtin_bit_cast(uint32_t, (c0 - z) * s), 0x07060302u);
+    const uint32_t b0 = K ? (i % 2 ? odd : even) >> 8 * (i / 2) : even >> 8 * i;
+    const uint32_t b1 = K ? b0 >> 16 : odd >> 8 * i;
+    // (All exact, and exact in bf16, so the packing truncates nothing.)
+    r[i] = perm_b32(__builtin_bit_cast(uint32_t, __builtin_fmaf((float)(b1 & 255u), s, zs)),
+                    __builtin_bit_cast(uint32_t, __builtin_fmaf((float)(b0 & 255u), s, zs)),
+                    0x07060302u);
   }
   return r;
 }
 
+// Workgroup `block` of a tiles' launch.
 template <int D, int W, bool KV4>
-__global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(2, 2))) void
-paged_tile_kernel(PagedArgs a) {
+__device__ __forceinline__ void paged_tile(const PagedArgs& a, int block) {
   constexpr int R = 32 * W;          // rows of the tile
   constexpr int U = D / 8;           // 16-byte units of a row
   constexpr int kSteps = D / 16;     // products of a score
@@ -275,9 +277,9 @@ paged_tile_kernel(PagedArgs a) {
   const int n = lane & 31, h = lane >> 5;
 
   // Which tile: kv heads innermost, then the pieces, then the tiles.
-  const int kv = blockIdx.x % a.kv_heads;
-  const int split = blockIdx.x / a.kv_heads % a.splits;
-  const int tile_id = blockIdx.x / a.kv_heads / a.splits;
+  const int kv = block % a.kv_heads;
+  const int split = block / a.kv_heads % a.splits;
+  const int tile_id = block / a.kv_heads / a.splits;
   int tile = tile_id;
   const int b = locate(a, tile, [&](const Request& r) { return tiles_of<R>(a, r); });
   if (b >= a.requests) return;
@@ -611,6 +613,12 @@ paged_tile_kernel(PagedArgs a) {
     }
 }
 
+template <int D, int W, bool KV4>
+__global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(2, 2))) void
+paged_tile_kernel(PagedArgs a) {
+  paged_tile<D, W, KV4>(a, blockIdx.x);
+}
+
 // Joins a tile's pieces in order: a workgroup for a row, D / 4 lanes a head.
 template <int D, int W>
 __global__ __launch_bounds__(256) void paged_merge_kernel(PagedArgs a) {
@@ -729,8 +737,7 @@ __device__ __forceinline__ int piece_blocks(const PagedArgs& a, int blocks, int 
 }
 // False where the launch has no such workgroup.
 template <int T>
-__device__ __forceinline__ bool find_share(const PagedArgs& a, Share& s) {
-  int place = blockIdx.x;
+__device__ __forceinline__ bool find_share(const PagedArgs& a, int place, Share& s) {
   if (a.requests == 1) {
     s.rq = uniform_request(a, 0);
     if (s.rq.rows <= 0 || !is_few(a, s.rq)) return false;
@@ -834,9 +841,9 @@ __device__ __forceinline__ int v4_at(int tok, int unit) {
   return tok * (D / 2) + (unit ^ (D == 128 ? tok >> 2 & 3 : tok >> 3 & 1)) * 16;
 }
 
+// Workgroup `place` of a launch for requests of few rows.
 template <int D, bool KV4, int W>
-__global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(2, 3))) void
-paged_rows_kernel(PagedArgs a) {
+__device__ __forceinline__ void paged_rows(const PagedArgs& a, int place) {
   typedef RowShape<D, KV4, W> S;
   constexpr int T = S::kBlock;
   constexpr int U = D / 8;
@@ -848,7 +855,7 @@ paged_rows_kernel(PagedArgs a) {
   const int n = lane & 15, g = lane >> 4;
 
   Share share;
-  if (!find_share<T>(a, share)) return;
+  if (!find_share<T>(a, place, share)) return;
   const Request rq = share.rq;
   const int kv = share.kv, pieces = share.pieces;
   if (a.few_groups && kv == 0 && share.piece == 0 && threadIdx.x == 0) {
@@ -1226,7 +1233,7 @@ paged_rows_kernel(PagedArgs a) {
 #pragma unroll
     for (int r = 0; r < 4; ++r) acc[r] *= inv;
     if (pieces > 1) {
-      const int64_t slot = (int64_t)blockIdx.x * kFew + row;
+      const int64_t slot = (int64_t)place * kFew + row;
       *reinterpret_cast<f32x4*>(a.row_out + slot * D + 4 * at) = acc;
       if (at == 0) a.row_lse[slot] = total == 0.0f ? kNegInf : top + __log2f(total);
       continue;
@@ -1241,6 +1248,22 @@ paged_rows_kernel(PagedArgs a) {
     u32x2 w = {pack_bf16x2(acc[0], acc[1]), pack_bf16x2(acc[2], acc[3])};
     __builtin_memcpy(a.out + r0 * a.out_row + h * a.out_head + 4 * at, &w, 8);
   }
+}
+
+template <int D, bool KV4, int W>
+__global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(2, 3))) void
+paged_rows_kernel(PagedArgs a) {
+  paged_rows<D, KV4, W>(a, blockIdx.x);
+}
+
+// Both in one launch, for a step of prompt chunks and single tokens: the tiles first, as
+// they take longest, and few rows on the CUs that they leave.
+template <int D, bool KV4>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void
+paged_both_kernel(PagedArgs a, int tiles) {
+  const int i = blockIdx.x;
+  if (i < tiles) paged_tile<D, 4, KV4>(a, i);
+  else paged_rows<D, KV4, 4>(a, i - tiles);
 }
 
 // Joins the pieces of requests of few rows in order, D / 4 lanes a head and WAYS times
@@ -1363,7 +1386,7 @@ PagedPlan make_plan(bool kv4, int rows, int requests, int num_q_heads, int num_k
     // 700 .. 4000 tokens, 12.4 from 4 bits. Where 8 waves have 3 blocks each at most (2 from
     // 4 bits) they are the whole launch: 8.3 us on 300 tokens, 10.3 on 500, 11.7 on 1000
     // from 4 bits, 14.6 and 17.4 at twice that.
-    const bool whole = p.few_units <= kCUs && blocks <= (kv4 ? 16 : 24);
+    const bool whole = most <= kFew && p.few_units <= kCUs && blocks <= (kv4 ? 16 : 24);
     p.few_waves = whole ? 8 : 4;
     if (!whole && blocks > p.few_waves && p.few_units <= 16 * kCUs)
       p.few_groups = (int)std::max<int64_t>(2 * kCUs, 2 * p.few_units);
@@ -1371,9 +1394,11 @@ PagedPlan make_plan(bool kv4, int rows, int requests, int num_q_heads, int num_k
   if (most > p.few) {
     // Tiles of 128 rows, two workgroups a CU; of fewer where requests have no more. Tiles
     // of 256 read K/V half as often and wait for their longest longer: 286 us for 259 on
-    // 8192 rows of 32 heads and a window of 4096. A 4-bit cache's are 256: its values are
-    // made once a tile, 297 us for 336 on 4 x 500 rows of 32 heads on 16k.
-    p.waves = most <= 64 ? 2 : most <= 128 || !kv4 ? 4 : 8;
+    // 8192 rows of 32 heads and a window of 4096. From a 4-bit cache, whose values are made
+    // once a tile, they are 256: 288 us for 343 on 4 x 500 rows of 16 heads on 8k .. 16k.
+    // Beside requests of few rows, in one launch, both have 4 waves.
+    p.waves = p.few_units || most > 64 ? 4 : 2;
+    if (kv4 && !p.few_units && most > 128) p.waves = 8;
     const int64_t tile_rows = 32 * p.waves;
     p.tiles = std::min<int64_t>((rows * group) / tile_rows + requests,
                                 requests * ((most + tile_rows - 1) / tile_rows));
@@ -1397,26 +1422,24 @@ size_t workspace_of(const PagedPlan& p, int num_kv_heads, int head_dim) {
 constexpr hipError_t kTooLarge = hipErrorInvalidConfiguration;
 bool fits(int64_t blocks, int threads) { return blocks <= UINT_MAX / threads; }
 
-template <int D, int W, bool KV4>
-hipError_t launch_tiles(const PagedArgs& a, int64_t tiles, hipStream_t stream) {
-  constexpr int kLds = 4 * kTok * D * 2;
-  static_assert(kLds <= 65536, "no attribute to set");
-  const int64_t grid = tiles * a.splits * a.kv_heads;
-  hipLaunchKernelGGL((paged_tile_kernel<D, W, KV4>), dim3((unsigned)grid), dim3(64 * W), kLds, stream, a);
-  const hipError_t err = hipGetLastError();
-  if (err != hipSuccess || a.splits <= 1) return err;
+template <int D>
+constexpr int kTileLds = 4 * kTok * D * 2;
+
+template <int D, int W>
+hipError_t launch_tile_merge(const PagedArgs& a, hipStream_t stream) {
+  if (a.splits <= 1) return hipSuccess;
   hipLaunchKernelGGL((paged_merge_kernel<D, W>), dim3((unsigned)a.rows), dim3(256), 0, stream, a);
   return hipGetLastError();
 }
-template <int D, bool KV4, int W>
-hipError_t launch_rows(const PagedArgs& a, int64_t grid, hipStream_t stream) {
-  constexpr int kLds = RowShape<D, KV4, W>::kLds;
-  static_assert(kLds <= 163840, "of a CU");
-  hipLaunchKernelGGL((paged_rows_kernel<D, KV4, W>), dim3((unsigned)grid), dim3(64 * W), kLds, stream, a);
-  return hipGetLastError();
+template <int D, int W, bool KV4>
+hipError_t launch_tiles(const PagedArgs& a, int64_t grid, hipStream_t stream) {
+  hipLaunchKernelGGL((paged_tile_kernel<D, W, KV4>), dim3((unsigned)grid), dim3(64 * W), kTileLds<D>,
+                     stream, a);
+  const hipError_t err = hipGetLastError();
+  return err != hipSuccess ? err : launch_tile_merge<D, W>(a, stream);
 }
 template <int D, int WAYS>
-hipError_t launch_rows_merge(const PagedArgs& a, int rows_each, hipStream_t stream) {
+hipError_t launch_rows_merge_ways(const PagedArgs& a, int rows_each, hipStream_t stream) {
   constexpr int kHeads = kMergeThreads<WAYS> / (D / 4) / WAYS;
   const int head_groups = (a.num_q_heads + kHeads - 1) / kHeads;
   hipLaunchKernelGGL((paged_rows_merge_kernel<D, WAYS>),
@@ -1424,29 +1447,48 @@ hipError_t launch_rows_merge(const PagedArgs& a, int rows_each, hipStream_t stre
                      dim3(kMergeThreads<WAYS>), 0, stream, a, rows_each, head_groups);
   return hipGetLastError();
 }
+template <int D>
+hipError_t launch_rows_merge(const PagedArgs& a, int rows_each, hipStream_t stream) {
+  if (!a.few_groups) return hipSuccess;
+  // The fewer (row, head)s, the more pieces have each.
+  const int64_t heads = (int64_t)a.requests * rows_each * a.num_q_heads;
+  return heads <= 256    ? launch_rows_merge_ways<D, 32>(a, rows_each, stream)
+         : heads <= 2048 ? launch_rows_merge_ways<D, 8>(a, rows_each, stream)
+                         : launch_rows_merge_ways<D, 1>(a, rows_each, stream);
+}
+template <int D, bool KV4, int W>
+hipError_t launch_rows(const PagedArgs& a, int64_t grid, int rows_each, hipStream_t stream) {
+  constexpr int kLds = RowShape<D, KV4, W>::kLds;
+  static_assert(kLds <= 163840, "of a CU");
+  hipLaunchKernelGGL((paged_rows_kernel<D, KV4, W>), dim3((unsigned)grid), dim3(64 * W), kLds, stream, a);
+  const hipError_t err = hipGetLastError();
+  return err != hipSuccess ? err : launch_rows_merge<D>(a, rows_each, stream);
+}
+template <int D, bool KV4>
+hipError_t launch_both(const PagedArgs& a, int64_t tiles, int64_t few, int rows_each, hipStream_t stream) {
+  constexpr int kLds = std::max(kTileLds<D>, RowShape<D, KV4, 4>::kLds);
+  hipLaunchKernelGGL((paged_both_kernel<D, KV4>), dim3((unsigned)(tiles + few)), dim3(256), kLds, stream,
+                     a, (int)tiles);
+  hipError_t err = hipGetLastError();
+  if (err == hipSuccess) err = launch_tile_merge<D, 4>(a, stream);
+  return err != hipSuccess ? err : launch_rows_merge<D>(a, rows_each, stream);
+}
 template <int D, bool KV4>
 hipError_t launch_paged(const PagedArgs& a, const PagedPlan& p, hipStream_t stream) {
   // All launches' sizes before the first: a call that is refused has written nothing.
-  const int64_t grid = p.few_groups ? p.few_groups : p.few_units;
+  const int64_t few = p.few_groups ? p.few_groups : p.few_units;
+  const int64_t tiles = p.tiles * std::max(p.splits, 1) * a.kv_heads;
   const int rows_each = std::min(a.max_rows, kFew / std::min(a.group, kFew));
-  if (!fits(p.tiles * std::max(p.splits, 1) * a.kv_heads, 64 * 8) || !fits(a.rows, 256) ||
-      !fits(grid, 512) || !fits((int64_t)a.requests * rows_each * a.num_q_heads, 1024))
+  if (!fits(tiles + few, 64 * 8) || !fits(a.rows, 256) ||
+      !fits((int64_t)a.requests * rows_each * a.num_q_heads, 1024))
     return kTooLarge;
-  if (p.tiles) {
-    const hipError_t err = p.waves == 2   ? launch_tiles<D, 2, KV4>(a, p.tiles, stream)
-                           : p.waves == 4 ? launch_tiles<D, 4, KV4>(a, p.tiles, stream)
-                                          : launch_tiles<D, 8, KV4>(a, p.tiles, stream);
-    if (err != hipSuccess) return err;
-  }
-  if (!p.few_units) return hipSuccess;
-  const hipError_t err = p.few_waves == 8 ? launch_rows<D, KV4, 8>(a, grid, stream)
-                                          : launch_rows<D, KV4, 4>(a, grid, stream);
-  if (err != hipSuccess || !p.few_groups) return err;
-  // The fewer (row, head)s, the more pieces have each.
-  const int64_t heads = (int64_t)a.requests * rows_each * a.num_q_heads;
-  return heads <= 256    ? launch_rows_merge<D, 32>(a, rows_each, stream)
-         : heads <= 2048 ? launch_rows_merge<D, 8>(a, rows_each, stream)
-                         : launch_rows_merge<D, 1>(a, rows_each, stream);
+  if (tiles && few) return launch_both<D, KV4>(a, tiles, few, rows_each, stream);
+  if (few)
+    return p.few_waves == 4 ? launch_rows<D, KV4, 4>(a, few, rows_each, stream)
+                            : launch_rows<D, KV4, 8>(a, few, rows_each, stream);
+  return p.waves == 2   ? launch_tiles<D, 2, KV4>(a, tiles, stream)
+         : p.waves == 4 ? launch_tiles<D, 4, KV4>(a, tiles, stream)
+                        : launch_tiles<D, KV4 ? 8 : 4, KV4>(a, tiles, stream);
 }
 
 bool aligned16(const void* p) { return ((uintptr_t)p & 15u) == 0; }
