@@ -15,8 +15,10 @@
 // so that the range is covered whatever the rounding of s.
 //
 // D / 8 lanes share a row, 8 dims a lane: one 16-byte load and store, sums and
-// rotation partners by lane exchange. Bound by memory for many tokens, by the
-// launch and one chain of loads for few.
+// rotation partners by lane exchange. Bound by memory for many tokens (8304 of 20
+// heads of 128, 87 MB, in 16.7 us: 5.2 TB/s; 8191 of 48 heads of 64 into 4 bits, 108
+// MB, in 23.1: 4.7), by the launch and one chain of loads for few (1 token 2.6 us, 112
+// into 4 bits 4.1, of the 7 that the host needs for a call).
 #include "qsa_common.h"
 #include "../../include/qsa_hip.h"
 #include "kv4.h"
@@ -28,7 +30,9 @@ namespace qsa {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kSmall = 4096;  // rows up to which each has its own lanes
+// Heads of a group of lanes. With one each, 8304 tokens take 27 us for 16.7 (the
+// position's row is loaded for every head); for few tokens it is the same.
+constexpr int kQRows = 4, kKvRows = 2;
 
 struct Rows {  // [tokens, heads, D] bf16, strides in elements
   uint16_t* p;
@@ -235,17 +239,17 @@ __device__ __forceinline__ void take_heads(const HeadRopeArgs& a, int part, int 
   }
 }
 
-// Groups of lanes: first those of the queries (ROWS heads each), from workgroup q_blocks
+// Groups of lanes: first those of the queries (kQRows heads each), from workgroup q_blocks
 // on those of all keys, then of all values, so that a wave's groups have the same to do.
-template <int D, int BITS, int ROWS>
+template <int D, int BITS>
 __global__ __launch_bounds__(kThreads) void head_rope_kernel(HeadRopeArgs a) {
-  constexpr int kLanes = D / 8, kPer = kThreads / kLanes, kKvRows = ROWS > 2 ? 2 : ROWS;
+  constexpr int kLanes = D / 8, kPer = kThreads / kLanes;
   const int j = threadIdx.x % kLanes, group = threadIdx.x / kLanes;
   if ((int)blockIdx.x < a.q_blocks) {
     const int item = blockIdx.x * kPer + group;
     if (item >= a.q_items) return;
     const int token = a.q_div.div(item);
-    take_heads<D, BITS, ROWS>(a, 0, token, (item - token * a.q_div.divisor) * ROWS, j);
+    take_heads<D, BITS, kQRows>(a, 0, token, (item - token * a.q_div.divisor) * kQRows, j);
   } else {
     int item = (blockIdx.x - a.q_blocks) * kPer + group;
     if (item >= a.kv_parts * a.kv_items) return;
@@ -258,24 +262,19 @@ __global__ __launch_bounds__(kThreads) void head_rope_kernel(HeadRopeArgs a) {
 
 bool aligned16(const void* p) { return ((uintptr_t)p & 15u) == 0; }
 
-template <int D, int ROWS>
+template <int D>
 void launch_head_rope(HeadRopeArgs& a, int tokens, int bits, hipStream_t stream) {
-  constexpr int kPer = kThreads / (D / 8), kKvRows = ROWS > 2 ? 2 : ROWS;
-  const int q = (a.q_heads + ROWS - 1) / ROWS, kv = (a.kv_heads + kKvRows - 1) / kKvRows;
+  constexpr int kPer = kThreads / (D / 8);
+  const int q = (a.q_heads + kQRows - 1) / kQRows, kv = (a.kv_heads + kKvRows - 1) / kKvRows;
   a.q_div = FastDiv::make(std::max(q, 1));
   a.kv_div = FastDiv::make(std::max(kv, 1));
   a.q_items = q * tokens;
   a.kv_items = kv * tokens;
   a.q_blocks = (a.q_items + kPer - 1) / kPer;
   const dim3 grid((unsigned)(a.q_blocks + (a.kv_parts * a.kv_items + kPer - 1) / kPer)), block(kThreads);
-  if (bits == 0) hipLaunchKernelGGL((head_rope_kernel<D, 0, ROWS>), grid, block, 0, stream, a);
-  else if (bits == 16) hipLaunchKernelGGL((head_rope_kernel<D, 16, ROWS>), grid, block, 0, stream, a);
-  else hipLaunchKernelGGL((head_rope_kernel<D, 4, ROWS>), grid, block, 0, stream, a);
-}
-template <int D>
-void launch_rows(HeadRopeArgs& a, int tokens, int bits, hipStream_t stream) {
-  if ((int64_t)(a.q_heads + a.kv_parts * a.kv_heads) * tokens <= kSmall) launch_head_rope<D, 1>(a, tokens, bits, stream);
-  else launch_head_rope<D, 4>(a, tokens, bits, stream);
+  if (bits == 0) hipLaunchKernelGGL((head_rope_kernel<D, 0>), grid, block, 0, stream, a);
+  else if (bits == 16) hipLaunchKernelGGL((head_rope_kernel<D, 16>), grid, block, 0, stream, a);
+  else hipLaunchKernelGGL((head_rope_kernel<D, 4>), grid, block, 0, stream, a);
 }
 
 }  // namespace
@@ -338,7 +337,11 @@ extern "C" int qsa_qk_norm_rope(
                                         "strides of multiples of 8 elements");
   const int64_t rows = (int64_t)num_q_heads + num_kv_heads * (value ? 2 : 1);
   if (rows == 0) return QSA_OK;
-  if (rows * tokens > INT_MAX - 4096) return fail(QSA_ERR_UNSUPPORTED, name + ": too many rows");
+  const int64_t groups = (num_q_heads + (int64_t)kQRows - 1) / kQRows +
+                         (num_kv_heads + (int64_t)kKvRows - 1) / kKvRows * (value ? 2 : 1);
+  // (32-bit counts of rows, and a launch of less than 2^32 threads)
+  if (rows * tokens > INT_MAX - 4096 || groups * tokens * (head_dim / 8) > UINT_MAX - 4096)
+    return fail(QSA_ERR_UNSUPPORTED, name + ": too many rows");
   HeadRopeArgs a = {};
   auto view = [](const void* p, int64_t token, int64_t head) {
     return Rows{static_cast<uint16_t*>(const_cast<void*>(p)), token, head};
@@ -373,7 +376,7 @@ extern "C" int qsa_qk_norm_rope(
   a.num_slots = (int64_t)num_blocks * page_size;
   a.page_div = FastDiv::make(std::max(page_size, 1));
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (head_dim == 128) launch_rows<128>(a, tokens, cache_bits, s);
-  else launch_rows<64>(a, tokens, cache_bits, s);
+  if (head_dim == 128) launch_head_rope<128>(a, tokens, cache_bits, s);
+  else launch_head_rope<64>(a, tokens, cache_bits, s);
   return check_launch("qsa_qk_norm_rope launch");
 }

@@ -119,6 +119,10 @@ def test_norm_rope_refuses_before_a_launch():
         assert _rope(**change) == status, change
         assert b"qsa_qk_norm_rope" in _lib.load().qsa_last_error()
     assert _rope(tokens=0) == 0
+    # A launch of 2^32 threads and more, of fewer than 2^31 rows.
+    for change in (dict(tokens=1 << 28, hq=1, hkv=0), dict(tokens=(1 << 28) // 3 + 1, hkv=1)):
+        assert _rope(**change) == -2
+        assert b"too many rows" in _lib.load().qsa_last_error()
 
 
 def test_cpu_tensors_are_refused():
