@@ -635,9 +635,9 @@ int qsa_qk_norm_rope(const void* query, int64_t q_token_stride, int64_t q_head_s
  * ones are not computed); max_seq_len should bound seq_lens: it shapes the launch only.
  * q and the caches are 16-byte aligned with strides of multiples of 8 elements; a cache
  * spans less than 64 GiB from its first row to its last. head_dim 64 or 128. The
- * workspace (0 bytes: none) holds the call's partial results until its work is done:
- * calls that may overlap need one each. qsa_int4_kv_attention: the same over a 4-bit
- * cache (block and head strides in bytes). */
+ * workspace (0 bytes: none; enough for either cache) holds the call's partial results
+ * until its work is done: calls that may overlap need one each. qsa_int4_kv_attention:
+ * the same over a 4-bit cache (block and head strides in bytes). */
 size_t qsa_paged_attention_workspace_bytes(int rows, int requests, int num_q_heads,
                                            int num_kv_heads, int head_dim, int window,
                                            int sink_tokens, int max_query_len, int max_seq_len);
