@@ -1041,6 +1041,7 @@ __device__ __forceinline__ void paged_rows(const PagedArgs& a, int place) {
           if (__builtin_bit_cast(uint32_t, vs[s * T + lane]) >= 0x7F800000u) vs[s * T + lane] = 0.0f;
         poisoned = true;
       }
+      asm volatile("" ::: "memory");  // other lanes read it: a wave's LDS accesses stay in order
 #pragma unroll
       for (int u = 0; u < S::kSub; ++u) {
         if constexpr (D == 128) {

@@ -125,6 +125,63 @@ def test_freed_and_missing_pages(bits):
     assert (got[4] == 0).all()
 
 
+@pytest.mark.parametrize("bits", [16, 4])
+@pytest.mark.parametrize("ctx,new,heads,kv_heads,dim,page,window,sinks", [
+    ([50, 2000, 0, 700, 3, 4100, 90], [1, 40, 1, 2, 300, 1, 0], 16, 2, 128, 16, 600, 3),
+    ([900, 5000, 17], [1, 1, 200], 8, 1, 64, 48, None, 0),       # a long piece beside tiles
+    ([3000, 0, 64], [3, 129, 20], 4, 4, 64, 16, None, 0),        # heads of their own
+    ([700, 800], [1, 33], 16, 1, 128, 272, 300, 70),             # 16 heads: one row is all of a few
+    ([10, 20], [2, 5], 20, 1, 128, 16, None, 0),                 # 20 heads: none is of few rows
+    ([int(37 * i % 1500) for i in range(70)], [1] * 66 + [0, 30, 2, 5], 16, 2, 128, 16, None, 0),
+])
+def test_steps_of_both(ctx, new, heads, kv_heads, dim, page, window, sinks, bits):
+    """Chunks and single tokens in one call: tiles and few rows side by side, pieces of
+    both, more requests than lanes, empty ones among them."""
+    print(ctx[:7], new[:7], heads, kv_heads, dim, page, window, bits, flush=True)
+    c = Case(ctx, new, heads, kv_heads, dim, page, window, sinks, gate=True, seed=sum(new), bits=bits)
+    c.check(c.run())
+    table = c.table.clone()       # and with pages missing from all of them
+    table[:, 1::5] = -1
+    c.check(c.run(table=table), table=table)
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+@pytest.mark.parametrize("requests,heads,dim", [(1, 16, 128), (1, 8, 64), (20, 16, 128), (150, 16, 64)])
+def test_single_tokens_in_pieces(requests, heads, dim, bits):
+    """Each way of joining pieces, by the number of heads in the call."""
+    gen = torch.Generator().manual_seed(requests)
+    ctx = torch.randint(1500, 3000, (requests,), generator=gen).tolist()
+    c = Case(ctx, [1] * requests, heads, 2, dim, gate=True, seed=heads, bits=bits)
+    c.check(c.run(max_seq_len=max(c.lens)))
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+@pytest.mark.parametrize("new", [[1], [2], [1, 50]])
+def test_values_that_are_not_finite_in_pieces(new, bits):
+    """V of a token that all rows see, in a whole block and in the last one: its dims and
+    no others, whichever piece holds it. In the last row's own token: that row alone."""
+    c = Case([3000, 2500][:len(new)], new, heads=8, kv_heads=2, bits=bits, seed=8)
+    clean = c.run()
+    for pos in (700, c.lens[0] - new[0] - 1, c.lens[0] - 1):
+        block, place = int(c.table[0, pos // 16]), pos % 16
+        saved, words = c.kv.clone(), [w.copy() for w in c.words] if bits == 4 else None
+        if bits == 4:
+            c.words[1][block, place, 0, 2] = 0x7FC0
+        c.kv[block, place, 0, 128 + 64:128 + 96] = float("nan")
+        got = c.run()
+        c.kv = saved
+        if bits == 4:
+            c.words = words
+        for r in range(c.starts[-1]):
+            if r >= new[0] or pos > c.lens[0] - new[0] + r:
+                assert torch.equal(got[r], clean[r])
+                continue
+            assert torch.isnan(got[r, :4, 64:96]).all()
+            assert torch.equal(got[r, 4:], clean[r, 4:])
+            rest = torch.cat((got[r, :4, :64], got[r, :4, 96:]), -1)
+            assert torch.equal(rest, torch.cat((clean[r, :4, :64], clean[r, :4, 96:]), -1))
+
+
 def test_lengths_that_do_not_fit():
     """Lengths past the table, under the rows, zero and negative: what is there is seen."""
     c = Case([100, 40, 3, 0], [2, 5, 1, 2], heads=4, window=None)
