@@ -627,12 +627,90 @@ paged_tile_kernel(PagedArgs a) {
   paged_tile<D, W, KV4>(a, blockIdx.x);
 }
 
-// Joins a tile's pieces in order: a workgroup for a row, D / 4 lanes a head.
-template <int D, int W>
-__global__ __launch_bounds__(256) void paged_merge_kernel(PagedArgs a) {
-  constexpr int R = 32 * W, kLanes = D / 4;
+// Joining of pieces in a fixed order, D / 4 lanes a (row, head) and WAYS times as many
+// that take every WAYS-th piece, some of them in flight together.
+template <int WAYS>
+constexpr int kMergeThreads = WAYS == 32 ? 1024 : 256;
+template <int D, int WAYS>
+constexpr int kMergeHeads = kMergeThreads<WAYS> / (D / 4) / WAYS;  // of a workgroup
+
+// `pieces` of a (row, head), `stride` rows apart from `first` on, times the gate, to dst.
+// All of a workgroup's threads come here; `write`: whether the head is one of the row's.
+template <int D, int WAYS>
+__device__ __forceinline__ void join_pieces(const float* out, const float* lses, int64_t first,
+                                            int64_t stride, int pieces, bool write, uint16_t* dst,
+                                            const uint16_t* gate, int64_t gate_dim) {
+  constexpr int kLanes = D / 4, kAhead = WAYS == 1 ? 4 : 8, kGroups = kMergeThreads<WAYS> / kLanes;
+  __shared__ f32x4 acc_lds[kGroups][kLanes];
+  __shared__ float top_lds[kGroups], sum_lds[kGroups];
+  const int lane = threadIdx.x % kLanes, grp = threadIdx.x / kLanes, way = grp % WAYS;
+  // Running maximum and sum over the way's pieces.
+  float top = kNegInf, sum = 0.0f;
+  f32x4 acc = {0, 0, 0, 0};
+  for (int s = way; s < pieces; s += WAYS * kAhead) {
+    float lse[kAhead];
+    f32x4 part[kAhead];
+#pragma unroll
+    for (int e = 0; e < kAhead; ++e) {
+      const int64_t at = first + min(s + e * WAYS, pieces - 1) * stride;
+      lse[e] = lses[at];
+      part[e] = *reinterpret_cast<const f32x4*>(out + at * D + 4 * lane);
+    }
+#pragma unroll
+    for (int e = 0; e < kAhead; ++e) {
+      if (s + e * WAYS >= pieces) break;
+      const float to = fmaxf(top, lse[e]);
+      const float from = to == kNegInf ? 0.0f : to;
+      const float old = fast_exp2(top - from), f = fast_exp2(lse[e] - from);
+      top = to;
+      sum = sum * old + f;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) acc[r] = acc[r] * old + f * part[e][r];
+    }
+  }
+  if constexpr (WAYS > 1) {
+    acc_lds[grp][lane] = acc;
+    if (lane == 0) {
+      top_lds[grp] = top;
+      sum_lds[grp] = sum;
+    }
+    __syncthreads();
+    if (way > 0) return;
+    float all = top;
+#pragma unroll
+    for (int w = 1; w < WAYS; ++w) all = fmaxf(all, top_lds[grp + w]);
+    const float from = all == kNegInf ? 0.0f : all;
+    const float own = fast_exp2(top - from);
+    sum *= own;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) acc[r] *= own;
+#pragma unroll
+    for (int w = 1; w < WAYS; ++w) {
+      const float f = fast_exp2(top_lds[grp + w] - from);
+      sum += f * sum_lds[grp + w];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) acc[r] += f * acc_lds[grp + w][lane][r];
+    }
+  }
+  if (!write) return;
+  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+  float y[4];
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    y[r] = acc[r] * inv;
+    if (gate) y[r] *= gate_factor(gate[(4 * lane + r) * gate_dim]);
+  }
+  u32x2 w = {pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3])};
+  __builtin_memcpy(dst + 4 * lane, &w, 8);
+}
+
+// A tile's pieces: a workgroup for some heads of a row.
+template <int D, int W, int WAYS>
+__global__ __launch_bounds__(kMergeThreads<WAYS>) void paged_merge_kernel(PagedArgs a, int head_groups) {
+  constexpr int R = 32 * W, kHeads = kMergeHeads<D, WAYS>;
   // The row's request: rows past the last one are of none.
-  const int row = blockIdx.x, wave_lane = threadIdx.x & 63;
+  const int hg = blockIdx.x % head_groups, row = blockIdx.x / head_groups;
+  const int wave_lane = threadIdx.x & 63;
   int tiles = 0, b = -1;
   for (int b0 = 0; b0 < a.requests; b0 += 64) {
     Request r = {0, 0, 0, 0};
@@ -651,36 +729,17 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedArgs a) {
   if (b < 0) return;
   const Request rq = uniform_request(a, b);
   if (is_few(a, rq)) return;
-  for (int head = threadIdx.x / kLanes; head < a.num_q_heads; head += 256 / kLanes) {
-    const int lane = threadIdx.x % kLanes;
-    const int kv = a.group_div.div(head);
-    const int m = (row - rq.row0) * a.group + head - kv * a.group;
-    const int tile = tiles + tiles_of<R>(a, rq) - 1 - m / R;
-    if (tile >= a.tiles) return;  // (requests whose rows overlap)
-    const int64_t first = ((int64_t)tile * a.kv_heads + kv) * a.splits * R + m % R;
-    float top = kNegInf;
-    for (int s = 0; s < a.splits; ++s) top = fmaxf(top, a.part_lse[first + (int64_t)s * R]);
-    const float base = top == kNegInf ? 0.0f : top;
-    float sum = 0.0f;
-    f32x4 acc = {0, 0, 0, 0};
-    for (int s = 0; s < a.splits; ++s) {
-      const int64_t at = first + (int64_t)s * R;
-      const float f = fast_exp2(a.part_lse[at] - base);
-      const f32x4 part = *reinterpret_cast<const f32x4*>(a.part_out + at * D + 4 * lane);
-      sum += f;
-#pragma unroll
-      for (int r = 0; r < 4; ++r) acc[r] += f * part[r];
-    }
-    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-    float y[4];
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      y[r] = acc[r] * inv;
-      if (a.gate) y[r] *= gate_factor(a.gate[row * a.g_row + head * a.g_head + (4 * lane + r) * a.g_dim]);
-    }
-    u32x2 w = {pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3])};
-    __builtin_memcpy(a.out + row * a.out_row + head * a.out_head + 4 * lane, &w, 8);
-  }
+  const int of_group = threadIdx.x / (D / 4) / WAYS;
+  const int head = min(hg * kHeads + of_group, a.num_q_heads - 1);
+  const int kv = a.group_div.div(head);
+  const int m = (row - rq.row0) * a.group + head - kv * a.group;
+  // (Requests whose rows overlap may have more tiles than the launch.)
+  const int tile = tiles + tiles_of<R>(a, rq) - 1 - m / R;
+  const int64_t first = ((int64_t)min(tile, a.tiles - 1) * a.kv_heads + kv) * a.splits * R + m % R;
+  join_pieces<D, WAYS>(a.part_out, a.part_lse, first, R, a.splits,
+                       tile < a.tiles && hg * kHeads + of_group < a.num_q_heads,
+                       a.out + row * a.out_row + head * a.out_head,
+                       a.gate ? a.gate + row * a.g_row + head * a.g_head : nullptr, a.g_dim);
 }
 
 // ---------------------------------------------------------------------------
@@ -1282,17 +1341,11 @@ paged_both_kernel(PagedArgs a, int tiles) {
   else paged_rows<D, KV4, 4>(a, i - tiles);
 }
 
-// Joins the pieces of requests of few rows in order, D / 4 lanes a head and WAYS times
-// as many that take every WAYS-th piece.
-template <int WAYS>
-constexpr int kMergeThreads = WAYS == 32 ? 1024 : 256;
+// The pieces of requests of few rows: a workgroup for some heads of a row.
 template <int D, int WAYS>
 __global__ __launch_bounds__(kMergeThreads<WAYS>) void paged_rows_merge_kernel(PagedArgs a, int rows_each,
                                                                                int head_groups) {
-  constexpr int kLanes = D / 4, kAhead = WAYS == 1 ? 4 : 8;
-  constexpr int kGroups = kMergeThreads<WAYS> / kLanes, kHeads = kGroups / WAYS;
-  __shared__ f32x4 acc_lds[kGroups][kLanes];
-  __shared__ float top_lds[kGroups], sum_lds[kGroups];
+  constexpr int kHeads = kMergeHeads<D, WAYS>;
   const int hg = blockIdx.x % head_groups;
   const int bi = blockIdx.x / head_groups, b = bi / rows_each, i = bi - b * rows_each;
   const int first_piece = a.row_pieces[2 * b], pieces = a.row_pieces[2 * b + 1];
@@ -1301,70 +1354,14 @@ __global__ __launch_bounds__(kMergeThreads<WAYS>) void paged_rows_merge_kernel(P
   if (i >= rq.rows || !is_few(a, rq) || pieces <= 1) return;
   if (first_piece < 0 || first_piece + (int64_t)pieces * a.kv_heads > a.few_groups)
     return;  // (requests whose rows overlap: some have no workgroup)
-  const int row = rq.row0 + i, lane = threadIdx.x % kLanes;
-  const int grp = threadIdx.x / kLanes, way = grp % WAYS;
-  const int head = min(hg * kHeads + grp / WAYS, a.num_q_heads - 1);
+  const int row = rq.row0 + i, of_group = threadIdx.x / (D / 4) / WAYS;
+  const int head = min(hg * kHeads + of_group, a.num_q_heads - 1);
   const int kv = a.group_div.div(head);
   const int m = i * a.group + head - kv * a.group;
-  const int64_t first = ((int64_t)first_piece + (int64_t)kv * pieces) * kFew + m;
-  // Running maximum and sum over the way's pieces, some of them in flight together.
-  float top = kNegInf, sum = 0.0f;
-  f32x4 acc = {0, 0, 0, 0};
-  for (int s = way; s < pieces; s += WAYS * kAhead) {
-    float lse[kAhead];
-    f32x4 part[kAhead];
-#pragma unroll
-    for (int e = 0; e < kAhead; ++e) {
-      const int64_t at = first + (int64_t)min(s + e * WAYS, pieces - 1) * kFew;
-      lse[e] = a.row_lse[at];
-      part[e] = *reinterpret_cast<const f32x4*>(a.row_out + at * D + 4 * lane);
-    }
-#pragma unroll
-    for (int e = 0; e < kAhead; ++e) {
-      if (s + e * WAYS >= pieces) break;
-      const float to = fmaxf(top, lse[e]);
-      const float from = to == kNegInf ? 0.0f : to;
-      const float old = fast_exp2(top - from), f = fast_exp2(lse[e] - from);
-      top = to;
-      sum = sum * old + f;
-#pragma unroll
-      for (int r = 0; r < 4; ++r) acc[r] = acc[r] * old + f * part[e][r];
-    }
-  }
-  if constexpr (WAYS > 1) {
-    acc_lds[grp][lane] = acc;
-    if (lane == 0) {
-      top_lds[grp] = top;
-      sum_lds[grp] = sum;
-    }
-    __syncthreads();
-    if (way > 0) return;
-    float all = top;
-#pragma unroll
-    for (int w = 1; w < WAYS; ++w) all = fmaxf(all, top_lds[grp + w]);
-    const float from = all == kNegInf ? 0.0f : all;
-    const float own = fast_exp2(top - from);
-    sum *= own;
-#pragma unroll
-    for (int r = 0; r < 4; ++r) acc[r] *= own;
-#pragma unroll
-    for (int w = 1; w < WAYS; ++w) {
-      const float f = fast_exp2(top_lds[grp + w] - from);
-      sum += f * sum_lds[grp + w];
-#pragma unroll
-      for (int r = 0; r < 4; ++r) acc[r] += f * acc_lds[grp + w][lane][r];
-    }
-  }
-  if (hg * kHeads + grp / WAYS >= a.num_q_heads) return;
-  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-  float y[4];
-#pragma unroll
-  for (int r = 0; r < 4; ++r) {
-    y[r] = acc[r] * inv;
-    if (a.gate) y[r] *= gate_factor(a.gate[row * a.g_row + head * a.g_head + (4 * lane + r) * a.g_dim]);
-  }
-  u32x2 w = {pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3])};
-  __builtin_memcpy(a.out + row * a.out_row + head * a.out_head + 4 * lane, &w, 8);
+  join_pieces<D, WAYS>(a.row_out, a.row_lse, ((int64_t)first_piece + (int64_t)kv * pieces) * kFew + m,
+                       kFew, pieces, hg * kHeads + of_group < a.num_q_heads,
+                       a.out + row * a.out_row + head * a.out_head,
+                       a.gate ? a.gate + row * a.g_row + head * a.g_head : nullptr, a.g_dim);
 }
 
 // ---------------------------------------------------------------------------
@@ -1445,11 +1442,19 @@ bool fits(int64_t blocks, int threads) { return blocks <= UINT_MAX / threads; }
 template <int D>
 constexpr int kTileLds = 4 * kTok * D * 2;
 
+template <int D, int W, int WAYS>
+hipError_t launch_tile_merge_ways(const PagedArgs& a, hipStream_t stream) {
+  constexpr int kHeads = kMergeHeads<D, WAYS>;
+  const int head_groups = (a.num_q_heads + kHeads - 1) / kHeads;
+  hipLaunchKernelGGL((paged_merge_kernel<D, W, WAYS>), dim3((unsigned)((int64_t)a.rows * head_groups)),
+                     dim3(kMergeThreads<WAYS>), 0, stream, a, head_groups);
+  return hipGetLastError();
+}
 template <int D, int W>
 hipError_t launch_tile_merge(const PagedArgs& a, hipStream_t stream) {
   if (a.splits <= 1) return hipSuccess;
-  hipLaunchKernelGGL((paged_merge_kernel<D, W>), dim3((unsigned)a.rows), dim3(256), 0, stream, a);
-  return hipGetLastError();
+  return (int64_t)a.rows * a.num_q_heads <= 2048 ? launch_tile_merge_ways<D, W, 8>(a, stream)
+                                                 : launch_tile_merge_ways<D, W, 1>(a, stream);
 }
 template <int D, int W, bool KV4>
 hipError_t launch_tiles(const PagedArgs& a, int64_t grid, hipStream_t stream) {
@@ -1460,7 +1465,7 @@ hipError_t launch_tiles(const PagedArgs& a, int64_t grid, hipStream_t stream) {
 }
 template <int D, int WAYS>
 hipError_t launch_rows_merge_ways(const PagedArgs& a, int rows_each, hipStream_t stream) {
-  constexpr int kHeads = kMergeThreads<WAYS> / (D / 4) / WAYS;
+  constexpr int kHeads = kMergeHeads<D, WAYS>;
   const int head_groups = (a.num_q_heads + kHeads - 1) / kHeads;
   hipLaunchKernelGGL((paged_rows_merge_kernel<D, WAYS>),
                      dim3((unsigned)((int64_t)a.requests * rows_each * head_groups)),
@@ -1501,7 +1506,7 @@ hipError_t launch_paged(const PagedArgs& a, const PagedPlan& p, hipStream_t stre
   const int64_t few = p.few_groups ? p.few_groups : p.few_units;
   const int64_t tiles = p.tiles * std::max(p.splits, 1) * a.kv_heads;
   const int rows_each = std::min(a.max_rows, kFew / std::min(a.group, kFew));
-  if (!fits(tiles + few, 64 * 8) || !fits(a.rows, 256) ||
+  if (!fits(tiles + few, 64 * 8) || !fits((int64_t)a.rows * a.num_q_heads, 256) ||
       !fits((int64_t)a.requests * rows_each * a.num_q_heads, 1024))
     return kTooLarge;
   if (tiles && few) return launch_both<D, KV4>(a, tiles, few, rows_each, stream);
