@@ -1417,11 +1417,14 @@ PagedPlan make_plan(bool kv4, int rows, int requests, int num_q_heads, int num_k
                                 requests * ((most + tile_rows - 1) / tile_rows));
     const int64_t stages = (seen(tile_rows / group + 1) + kTok - 1) / kTok;
     const int64_t units = std::max<int64_t>(p.tiles * num_kv_heads, 1);
-    // Pieces for two workgroups a CU. One of 8 waves fills a CU: two in turn even out
-    // tiles of unlike lengths (four requests on 8k .. 16k 278 us for 341, a prompt of 4096
-    // 121 for 167), alike ones need one (500 rows on 8192 69 us for 86).
+    // Pieces of four stages at least, for two workgroups a CU; of two for one a CU (32 rows
+    // on 2000 15.2 us for 17.4, but 1000 on themselves from 4 bits 44 for 31, in two rounds).
+    // A workgroup of 8 waves fills a CU: two in turn even out tiles of unlike lengths (four
+    // requests on 8k .. 16k 278 us for 341, a prompt of 4096 121 for 167), alike ones need
+    // one (500 rows on 8192 69 us for 86).
     const bool alike = p.waves == 8 && requests == 1 && 4 * (int64_t)max_query_len <= max_seq_len;
-    p.splits = (int)std::max<int64_t>(1, std::min((alike ? kCUs : 2 * kCUs) / units, stages / 4));
+    const int64_t most_pieces = std::max(stages / 4, std::min(kCUs / units, stages / 2));
+    p.splits = (int)std::max<int64_t>(1, std::min((alike ? kCUs : 2 * kCUs) / units, most_pieces));
   }
   return p;
 }
