@@ -1401,8 +1401,13 @@ PagedPlan make_plan(bool kv4, int rows, int requests, int num_q_heads, int num_k
     // from 4 bits, 14.6 and 17.4 at twice that.
     const bool whole = most <= kFew && p.few_units <= kCUs && blocks <= (kv4 ? 16 : 24);
     p.few_waves = whole ? 8 : 4;
+    // As many pieces as two workgroups a CU take (one: 2 us less for a single request, but
+    // 51 us for 31 for 64 on 1024 .. 8192 of 4 bits), and more than the units, so that long
+    // ones are cut: four each up to one a CU (128 requests 130 us for 147 with two, 60 for
+    // 68 from 4 bits), two past that (512 requests on 512 .. 2048 145 us for 175 with four).
     if (!whole && blocks > p.few_waves && p.few_units <= 16 * kCUs)
-      p.few_groups = (int)std::max<int64_t>(2 * kCUs, 2 * p.few_units);
+      p.few_groups =
+          (int)std::max<int64_t>(2 * kCUs, (p.few_units <= kCUs ? 4 : 2) * p.few_units);
   }
   if (most > p.few) {
     // Tiles of 128 rows, two workgroups a CU; of fewer where requests have no more. Tiles
