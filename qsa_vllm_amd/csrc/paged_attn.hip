@@ -1421,7 +1421,18 @@ PagedPlan make_plan(bool kv4, int rows, int requests, int num_q_heads, int num_k
     p.tiles = std::min<int64_t>((rows * group) / tile_rows + requests,
                                 requests * ((most + tile_rows - 1) / tile_rows));
     const int64_t stages = (seen(tile_rows / group + 1) + kTok - 1) / kTok;
-    const int64_t units = std::max<int64_t>(p.tiles * num_kv_heads, 1);
+    // The tiles that there likely are: beside requests of few rows those of the longest
+    // allowed, the others being single tokens (64 tokens on 1000 .. 8000 and 4 chunks of 512
+    // 161 us, 212 with the bound's pieces; from 4 bits 203 and 338). Many more would fit the
+    // bounds, whose workgroups end at once; their pieces' room is kept to 2048 tiles.
+    int64_t likely = p.tiles;
+    if (p.few_units) {
+      const int64_t more = rows - requests;  // rows past the first of each request
+      const int64_t chunks = std::max<int64_t>(more / std::max(max_query_len - 1, 1), 1);
+      likely = std::min(likely, chunks * (((more / chunks + 1) * group + tile_rows - 1) / tile_rows));
+    }
+    const int64_t room = std::max<int64_t>(8 * kCUs / std::max<int64_t>(p.tiles * num_kv_heads, 1), 1);
+    const int64_t units = std::max<int64_t>(likely * num_kv_heads, 1);
     // Pieces of four stages at least, for two workgroups a CU; of two for one a CU (32 rows
     // on 2000 15.2 us for 17.4, but 1000 on themselves from 4 bits 44 for 31, in two rounds).
     // A workgroup of 8 waves fills a CU: two in turn even out tiles of unlike lengths (four
@@ -1429,7 +1440,8 @@ PagedPlan make_plan(bool kv4, int rows, int requests, int num_q_heads, int num_k
     // one (500 rows on 8192 69 us for 86).
     const bool alike = p.waves == 8 && requests == 1 && 4 * (int64_t)max_query_len <= max_seq_len;
     const int64_t most_pieces = std::max(stages / 4, std::min(kCUs / units, stages / 2));
-    p.splits = (int)std::max<int64_t>(1, std::min((alike ? kCUs : 2 * kCUs) / units, most_pieces));
+    p.splits = (int)std::max<int64_t>(
+        1, std::min({(alike ? kCUs : 2 * kCUs) / units, most_pieces, room}));
   }
   return p;
 }
