@@ -16,9 +16,9 @@
 //
 // D / 8 lanes share a row, 8 dims a lane: one 16-byte load and store, sums and
 // rotation partners by lane exchange. Bound by memory for many tokens (8304 of 20
-// heads of 128, 87 MB, in 16.7 us: 5.2 TB/s; 8191 of 48 heads of 64 into 4 bits, 108
-// MB, in 23.1: 4.7), by the launch and one chain of loads for few (1 token 2.6 us, 112
-// into 4 bits 4.1, of the 7 that the host needs for a call).
+// heads of 128, 87 MB, in 16.5 us: 5.3 TB/s; 8191 of 48 heads of 64 into 4 bits, 108
+// MB, in 22.5: 4.8), by the launch and one chain of loads for few (1 token 2.8 us, 112
+// into 4 bits 3.9, of the 7 that the host needs for a call).
 #include "qsa_common.h"
 #include "../../include/qsa_hip.h"
 #include "kv4.h"
@@ -30,9 +30,10 @@ namespace qsa {
 namespace {
 
 constexpr int kThreads = 256;
-// Heads of a group of lanes. With one each, 8304 tokens take 27 us for 16.7 (the
-// position's row is loaded for every head); for few tokens it is the same.
-constexpr int kQRows = 4, kKvRows = 2;
+// Rows up to which each has its own group of lanes; past that a group takes four query
+// heads or two of K or V of a token, whose position's row is loaded once: 8304 tokens of
+// 20 heads 16.7 us for 27, but one token 3.7 for 2.6 and 112 into 4 bits 5.0 for 4.1.
+constexpr int kSmall = 4096;
 
 struct Rows {  // [tokens, heads, D] bf16, strides in elements
   uint16_t* p;
@@ -239,17 +240,17 @@ __device__ __forceinline__ void take_heads(const HeadRopeArgs& a, int part, int 
   }
 }
 
-// Groups of lanes: first those of the queries (kQRows heads each), from workgroup q_blocks
+// Groups of lanes: first those of the queries (ROWS heads each), from workgroup q_blocks
 // on those of all keys, then of all values, so that a wave's groups have the same to do.
-template <int D, int BITS>
+template <int D, int BITS, int ROWS>
 __global__ __launch_bounds__(kThreads) void head_rope_kernel(HeadRopeArgs a) {
-  constexpr int kLanes = D / 8, kPer = kThreads / kLanes;
+  constexpr int kLanes = D / 8, kPer = kThreads / kLanes, kKvRows = ROWS > 2 ? 2 : ROWS;
   const int j = threadIdx.x % kLanes, group = threadIdx.x / kLanes;
   if ((int)blockIdx.x < a.q_blocks) {
     const int item = blockIdx.x * kPer + group;
     if (item >= a.q_items) return;
     const int token = a.q_div.div(item);
-    take_heads<D, BITS, kQRows>(a, 0, token, (item - token * a.q_div.divisor) * kQRows, j);
+    take_heads<D, BITS, ROWS>(a, 0, token, (item - token * a.q_div.divisor) * ROWS, j);
   } else {
     int item = (blockIdx.x - a.q_blocks) * kPer + group;
     if (item >= a.kv_parts * a.kv_items) return;
@@ -262,19 +263,25 @@ __global__ __launch_bounds__(kThreads) void head_rope_kernel(HeadRopeArgs a) {
 
 bool aligned16(const void* p) { return ((uintptr_t)p & 15u) == 0; }
 
-template <int D>
-void launch_head_rope(HeadRopeArgs& a, int tokens, int bits, hipStream_t stream) {
-  constexpr int kPer = kThreads / (D / 8);
-  const int q = (a.q_heads + kQRows - 1) / kQRows, kv = (a.kv_heads + kKvRows - 1) / kKvRows;
+template <int D, int ROWS>
+void launch_rows(HeadRopeArgs& a, int tokens, int bits, hipStream_t stream) {
+  constexpr int kPer = kThreads / (D / 8), kKvRows = ROWS > 2 ? 2 : ROWS;
+  const int q = (a.q_heads + ROWS - 1) / ROWS, kv = (a.kv_heads + kKvRows - 1) / kKvRows;
   a.q_div = FastDiv::make(std::max(q, 1));
   a.kv_div = FastDiv::make(std::max(kv, 1));
   a.q_items = q * tokens;
   a.kv_items = kv * tokens;
   a.q_blocks = (a.q_items + kPer - 1) / kPer;
   const dim3 grid((unsigned)(a.q_blocks + (a.kv_parts * a.kv_items + kPer - 1) / kPer)), block(kThreads);
-  if (bits == 0) hipLaunchKernelGGL((head_rope_kernel<D, 0>), grid, block, 0, stream, a);
-  else if (bits == 16) hipLaunchKernelGGL((head_rope_kernel<D, 16>), grid, block, 0, stream, a);
-  else hipLaunchKernelGGL((head_rope_kernel<D, 4>), grid, block, 0, stream, a);
+  if (bits == 0) hipLaunchKernelGGL((head_rope_kernel<D, 0, ROWS>), grid, block, 0, stream, a);
+  else if (bits == 16) hipLaunchKernelGGL((head_rope_kernel<D, 16, ROWS>), grid, block, 0, stream, a);
+  else hipLaunchKernelGGL((head_rope_kernel<D, 4, ROWS>), grid, block, 0, stream, a);
+}
+template <int D>
+void launch_head_rope(HeadRopeArgs& a, int tokens, int bits, hipStream_t stream) {
+  const int64_t rows = (int64_t)(a.q_heads + a.kv_parts * a.kv_heads) * tokens;
+  if (rows <= kSmall) launch_rows<D, 1>(a, tokens, bits, stream);
+  else launch_rows<D, 4>(a, tokens, bits, stream);
 }
 
 }  // namespace
@@ -337,8 +344,8 @@ extern "C" int qsa_qk_norm_rope(
                                         "strides of multiples of 8 elements");
   const int64_t rows = (int64_t)num_q_heads + num_kv_heads * (value ? 2 : 1);
   if (rows == 0) return QSA_OK;
-  const int64_t groups = (num_q_heads + (int64_t)kQRows - 1) / kQRows +
-                         (num_kv_heads + (int64_t)kKvRows - 1) / kKvRows * (value ? 2 : 1);
+  const int64_t groups =
+      (num_q_heads + (int64_t)3) / 4 + (num_kv_heads + (int64_t)1) / 2 * (value ? 2 : 1);
   // (32-bit counts of rows, and a launch of less than 2^32 threads)
   if (rows * tokens > INT_MAX - 4096 || groups * tokens * (head_dim / 8) > UINT_MAX - 4096)
     return fail(QSA_ERR_UNSUPPORTED, name + ": too many rows");

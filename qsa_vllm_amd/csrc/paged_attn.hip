@@ -26,8 +26,8 @@
 // values, exactly, and the rest is the same.
 //
 // Bound by the matrix cores: 8192 rows of 16 heads of 128 in a window of 4096 are 206
-// Gflop and take 253 us, 0.81 Pflop/s (the card's large bf16 product reaches 1.2). A
-// stage is 32 products of a wave and 220 vector instructions (masks, exponentials,
+// Gflop and take 256 us, 0.80 Pflop/s (the card's large bf16 product reaches 1.2). A
+// stage is 32 products of a wave and 210 vector instructions (masks, exponentials,
 // packing, addresses), and two waves a SIMD, of workgroups of their own, hide each
 // other's by two thirds. Tried and slower: two groups of four waves in turns in one
 // workgroup (313 us), 64 rows a wave (380: too few registers), raised priority around
@@ -755,7 +755,7 @@ __global__ __launch_bounds__(kMergeThreads<WAYS>) void paged_merge_kernel(PagedA
 //
 // Work is shared out by blocks: requests of more blocks than an equal share of the
 // whole launch are cut into pieces, found on the device, which a second kernel joins.
-// 112 tokens in windows of 4096 of a bf16 cache take 96 us with the joining, 472 MB at
+// 112 tokens in windows of 4096 of a bf16 cache take 98 us with the joining, 472 MB at
 // the rate of a large copy. A wave has its next block on the way in registers; a second
 // one behind it made all cases slower (130 us here: registers spilled, and short pieces
 // load blocks that they do not have).
