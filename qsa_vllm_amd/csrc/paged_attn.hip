@@ -1412,7 +1412,7 @@ PagedPlan make_plan(bool kv4, int rows, int requests, int num_q_heads, int num_k
   if (most > p.few) {
     // Tiles of 128 rows, two workgroups a CU; of fewer where requests have no more. Tiles
     // of 256 read K/V half as often and wait for their longest longer: 286 us for 259 on
-    // 8192 rows of 32 heads and a window of 4096. From a 4-bit cache, whose values are made
+    // 8192 rows of 16 heads and a window of 4096. From a 4-bit cache, whose values are made
     // once a tile, they are 256: 288 us for 343 on 4 x 500 rows of 16 heads on 8k .. 16k.
     // Beside requests of few rows, in one launch, both have 4 waves.
     p.waves = p.few_units || most > 64 ? 4 : 2;
