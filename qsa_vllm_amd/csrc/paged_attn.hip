@@ -1082,9 +1082,8 @@ __device__ __forceinline__ void paged_rows(const PagedArgs& a, int place) {
         ks[s * T + lane] = scale;
         zero_at[s] = perm_b32(__builtin_bit_cast(uint32_t, scale * (float)(kw & 15u)),
                               __builtin_bit_cast(uint32_t, scale * 16.0f), 0x07060302u);
-        const uint32_t v_scale = (vw & 0xFFF0u) << 16;
-        bad |= v_scale >= 0x7F800000u;  // (NaN: the only one past the finite)
-        vs[s * T + lane] = __builtin_bit_cast(float, v_scale);
+        bad |= (vw & 0x7F80u) == 0x7F80u;  // no finite scale, of either sign
+        vs[s * T + lane] = __builtin_bit_cast(float, (vw & 0xFFF0u) << 16);
         // Token 16 u + 4 g' + r at the place of its code in the other operand.
         const int u = lane >> 4, gt = lane >> 2 & 3, r = lane & 3;
         vz[((s * 2 + u / 2) * 4 + gt) * 8 + r * 2 + u % 2] = (uint16_t)(0x4180u | (vw & 15u) << 3);
@@ -1097,7 +1096,8 @@ __device__ __forceinline__ void paged_rows(const PagedArgs& a, int place) {
         // V may be NaN where a row must not see it: as in the tiles' kernel.
 #pragma unroll
         for (int s = 0; s < kGroups; ++s)
-          if (__builtin_bit_cast(uint32_t, vs[s * T + lane]) >= 0x7F800000u) vs[s * T + lane] = 0.0f;
+          if ((__builtin_bit_cast(uint32_t, vs[s * T + lane]) & 0x7F800000u) == 0x7F800000u)
+            vs[s * T + lane] = 0.0f;
         poisoned = true;
       }
       asm volatile("" ::: "memory");  // other lanes read it: a wave's LDS accesses stay in order
