@@ -583,9 +583,10 @@ int qsa_process_logits(const void* logits, int logits_type, int64_t logits_row_s
  * words and the V words (a 16-bit word for each group of 32 dims, little end
  * first), both word blocks filled up to 16 bytes. A group's word: zero point z in
  * the low four bits, the others a bf16 scale s of four significant bits, of either
- * sign; the values are (code - z) * s, bf16 values exactly. Code words of 8 dims, 32
- * bits: V's word w holds dims 8 w .., 4 bits a dim in order; K's word b * head_dim / 32
- * + a holds dims 32 a + 8 b .., dim 2 i in bits 4 i .., dim 2 i + 1 in bits 16 + 4 i ...
+ * sign; the values are (code - z) * s, bf16 values exactly, NaN where s is not finite.
+ * Code words of 8 dims, 32 bits: V's word w holds dims 8 w .., 4 bits a dim in order;
+ * K's word b * head_dim / 32 + a holds dims 32 a + 8 b .., dim 2 i in bits 4 i .., dim
+ * 2 i + 1 in bits 16 + 4 i ...
  * qsa_kv4_page_bytes: the bytes of such a page (0 for head dims but 64 and 128). */
 int64_t qsa_kv4_page_bytes(int page_size, int head_dim);
 

@@ -71,6 +71,7 @@ class Int4KVCache:
             w = self.data[:, :, first:first + words].reshape(blocks, heads, page, -1, 2).to(torch.int32)
             w = w[..., 0] | (w[..., 1] << 8)
             scale = ((w & 0xFFF0) << 16).view(torch.float32)
+            scale = torch.where(scale.isfinite(), scale, torch.nan)  # as the attention reads it
             x = (c.unflatten(-1, (-1, _GROUP)) - (w & 15).float()[..., None]) * scale[..., None]
             out.append(x.flatten(-2).to(torch.bfloat16).transpose(1, 2))
         return out[0], out[1]
