@@ -632,7 +632,10 @@ int qsa_qk_norm_rope(const void* query, int64_t q_token_stride, int64_t q_head_s
  * nothing. Rows of no request are not written. Infinities and NaN in K or V reach the
  * rows that see them, as arithmetic has it (an infinite score gives NaN, an infinite
  * value an infinity or NaN), and no others. A score of minus infinity weighs nothing; a
- * row that has no other gets zeros. max_query_len bounds a request's rows (further
+ * row that has no other gets zeros. Scores and weighted sums are held in fp32: V's
+ * largest magnitude times the tokens that a row sees must be under 2^117, and the sum of
+ * a query's magnitudes times K's largest under 2^125 (past that finite K and V may give
+ * infinities or NaN). max_query_len bounds a request's rows (further
  * ones are not computed); max_seq_len should bound seq_lens: it shapes the launch only.
  * q and the caches are 16-byte aligned with strides of multiples of 8 elements; a cache
  * spans less than 64 GiB from its first row to its last. head_dim 64 or 128. The

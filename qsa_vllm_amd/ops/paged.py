@@ -52,8 +52,10 @@ def qsa_window_paged_attention(
     Positions without a page (an entry of ``block_table`` that is no block, such as -1
     for pages that left every window and were freed) are not seen, and a row that sees
     nothing gets zeros. Infinities and NaN in K or V reach the rows that see them, as
-    arithmetic has it, and no others; a score of minus infinity weighs nothing. Rows of
-    no request (past ``query_start_loc[-1]``) are not written. The caches must span less
+    arithmetic has it, and no others; a score of minus infinity weighs nothing. Scores and
+    weighted sums are held in fp32: V's largest magnitude times the tokens that a row sees
+    must be under 2^117, the sum of a query's magnitudes times K's largest under 2^125
+    (past that finite values may give infinities or NaN). Rows of no request (past ``query_start_loc[-1]``) are not written. The caches must span less
     than 64 GiB each. ``max_query_len`` must be at least every request's row count
     (further rows are not computed); ``max_seq_len`` should be at least every length: it
     shapes the launch, not the result. Captured into a graph, both hold for its replays."""
