@@ -638,7 +638,10 @@ int qsa_qk_norm_rope(const void* query, int64_t q_token_stride, int64_t q_head_s
  * infinities or NaN). max_query_len bounds a request's rows (further
  * ones are not computed); max_seq_len should bound seq_lens: it shapes the launch only.
  * q and the caches are 16-byte aligned with strides of multiples of 8 elements; a cache
- * spans less than 64 GiB from its first row to its last. head_dim 64 or 128. The
+ * spans less than 64 GiB from its first row to its last. head_dim 64 or 128. rows *
+ * num_q_heads of 2^30 and more are refused, and launches of 2^32 threads (which take
+ * more than 2^22 requests times kv heads, or a q of 2^24 rows of 8 heads a few of which
+ * belong to requests). The
  * workspace (0 bytes: none; enough for either cache) holds the call's partial results
  * until its work is done: calls that may overlap need one each. qsa_int4_kv_attention:
  * the same over a 4-bit cache (block and head strides in bytes). */

@@ -1464,10 +1464,14 @@ bool fits(int64_t blocks, int threads) { return blocks <= UINT_MAX / threads; }
 template <int D>
 constexpr int kTileLds = 4 * kTok * D * 2;
 
+// Workgroups of a row of a joining launch.
+template <int D, int WAYS>
+int head_groups_of(const PagedArgs& a) {
+  return (a.num_q_heads + kMergeHeads<D, WAYS> - 1) / kMergeHeads<D, WAYS>;
+}
 template <int D, int W, int WAYS>
 hipError_t launch_tile_merge_ways(const PagedArgs& a, hipStream_t stream) {
-  constexpr int kHeads = kMergeHeads<D, WAYS>;
-  const int head_groups = (a.num_q_heads + kHeads - 1) / kHeads;
+  const int head_groups = head_groups_of<D, WAYS>(a);
   hipLaunchKernelGGL((paged_merge_kernel<D, W, WAYS>), dim3((unsigned)((int64_t)a.rows * head_groups)),
                      dim3(kMergeThreads<WAYS>), 0, stream, a, head_groups);
   return hipGetLastError();
@@ -1487,8 +1491,7 @@ hipError_t launch_tiles(const PagedArgs& a, int64_t grid, hipStream_t stream) {
 }
 template <int D, int WAYS>
 hipError_t launch_rows_merge_ways(const PagedArgs& a, int rows_each, hipStream_t stream) {
-  constexpr int kHeads = kMergeHeads<D, WAYS>;
-  const int head_groups = (a.num_q_heads + kHeads - 1) / kHeads;
+  const int head_groups = head_groups_of<D, WAYS>(a);
   hipLaunchKernelGGL((paged_rows_merge_kernel<D, WAYS>),
                      dim3((unsigned)((int64_t)a.requests * rows_each * head_groups)),
                      dim3(kMergeThreads<WAYS>), 0, stream, a, rows_each, head_groups);
@@ -1524,12 +1527,15 @@ hipError_t launch_both(const PagedArgs& a, int64_t tiles, int64_t few, int rows_
 }
 template <int D, bool KV4>
 hipError_t launch_paged(const PagedArgs& a, const PagedPlan& p, hipStream_t stream) {
-  // All launches' sizes before the first: a call that is refused has written nothing.
+  // All launches' sizes before the first: a call that is refused has written nothing. (Only
+  // few (row, head)s are joined more than one way.)
   const int64_t few = p.few_groups ? p.few_groups : p.few_units;
   const int64_t tiles = p.tiles * std::max(p.splits, 1) * a.kv_heads;
   const int rows_each = std::min(a.max_rows, kFew / std::min(a.group, kFew));
-  if (!fits(tiles + few, 64 * 8) || !fits((int64_t)a.rows * a.num_q_heads, 256) ||
-      !fits((int64_t)a.requests * rows_each * a.num_q_heads, 1024))
+  const int64_t head_groups = head_groups_of<D, 1>(a);
+  if (!fits(tiles + few, 64 * std::max(p.waves, p.few_waves)) ||
+      (p.splits > 1 && !fits(a.rows * head_groups, kMergeThreads<1>)) ||
+      (p.few_groups && !fits(a.requests * rows_each * head_groups, kMergeThreads<1>)))
     return kTooLarge;
   if (tiles && few) return launch_both<D, KV4>(a, tiles, few, rows_each, stream);
   if (few)
