@@ -262,7 +262,7 @@ class QSAAttention:
 class WindowAttention:
     """Causal attention over a sliding window and the first tokens, gated."""
 
-    def __init__(self, cfg: HybridConfig, init: _Init, num_blocks: int, max_position: int,
+    def __init__(self, cfg: HybridConfig, init: _Init, num_blocks: int, cos_sin: torch.Tensor,
                  cache_std: float):
         d = cfg.head_dim
         self.heads, self.kv_heads, self.head_dim = cfg.heads, cfg.kv_heads, d
@@ -275,7 +275,7 @@ class WindowAttention:
         self.q_norm = torch.ones(d, dtype=torch.bfloat16, device=init.device)
         self.k_norm = torch.ones(d, dtype=torch.bfloat16, device=init.device)
         self.o_proj = _stored(cfg, init.normal(cfg.hidden_size, self.heads * d))
-        self.cos_sin = rotary_table(max_position, cfg.rope_dim, cfg.rope_theta, init.device)
+        self.cos_sin = cos_sin   # all layers'
         kv = init.normal(num_blocks, cfg.page_size, self.kv_heads, 2 * d, std=cache_std)
         if cfg.window_kv_bits == 16:
             self.cache = kv[..., :d], kv[..., d:]
@@ -454,6 +454,8 @@ class HybridDecoder:
         self.embed_tokens = init.normal(cfg.vocab_size, cfg.hidden_size)
         self.layers = []
         d, dx = cfg.head_dim, cfg.indexer_head_dim
+        if cfg.window_layers:
+            cos_sin = rotary_table(max_position, cfg.rope_dim, cfg.rope_theta, init.device)
         for kind in cfg.layer_types():
             if kind == "full_attention":
                 kv = init.normal(num_blocks, cfg.page_size, cfg.kv_heads, 2 * d, std=cache_std)
@@ -462,7 +464,7 @@ class HybridDecoder:
                 mixer = QSAAttention(cfg, init, kv.permute(0, 2, 1, 3), ring, comp, max_tokens,
                                      max_position)
             elif kind == "sliding_attention":
-                mixer = WindowAttention(cfg, init, num_blocks, max_position, cache_std)
+                mixer = WindowAttention(cfg, init, num_blocks, cos_sin, cache_std)
             else:
                 mixer = GatedDeltaNet(cfg, init, state_slots, state_std)
             self.layers.append(DecoderLayer(kind, mixer, cfg, init))
