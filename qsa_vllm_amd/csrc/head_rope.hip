@@ -230,7 +230,7 @@ __device__ __forceinline__ void take_heads(const HeadRopeArgs& a, int part, int 
               4 * (part == 1 ? j % 4 * (D / 32) + j / 4 : j)) = packed;
           if (j % 4 == 0)
             *reinterpret_cast<uint16_t*>(to + (part == 1 ? lay.k_words() : lay.v_words()) +
-                                         place * lay.words() + j / 4 * 2) = (uint16_t)word;
+                                         (int64_t)place * lay.words() + j / 4 * 2) = (uint16_t)word;
         }
         x[r] = pack8(f);
       }

@@ -1252,7 +1252,8 @@ __device__ __forceinline__ void paged_rows(const PagedArgs& a, int place) {
         if (page < 0 || page >= a.num_blocks || !(seen_from(a, pos, t0) >> i & 1)) continue;
         const int at = t0 + i - a.page_div.div(t0 + i) * a.page_size;
         if constexpr (KV4) {
-          const char* const from = v_words + ((uint64_t)((uint32_t)page * a.kb) << 4) + at * (D / 16);
+          const char* const from =
+              v_words + ((uint64_t)((uint32_t)page * a.kb) << 4) + (int64_t)at * (D / 16);
 #pragma unroll
           for (int d = 0; d < kDims; ++d)
             if ((reinterpret_cast<const uint16_t*>(from)[d / 2] & 0x7F80u) == 0x7F80u)
