@@ -1734,7 +1734,9 @@ extern "C" int qsa_int4_kv_attention(
   if (!aligned16(cache) || block_stride < 0 || head_stride < 0 || ((block_stride | head_stride) & 15))
     return fail(QSA_ERR_INVALID, name + ": the cache needs 16-byte alignment and strides of "
                                         "multiples of 16 bytes");
-  if (block_stride / 16 >= kNoToken || (int64_t)num_blocks * (block_stride / 16) >= kNoToken)
+  // The kernel's offsets are 32-bit counts of 16 bytes.
+  const int64_t page_units = Kv4Page{page_size, head_dim}.bytes() / 16, stride = block_stride / 16;
+  if (stride >= kNoToken || std::max(num_blocks - 1, 0) * stride + page_units >= kNoToken)
     return fail(QSA_ERR_UNSUPPORTED, name + ": the cache must span under 64 GiB");
   PagedArgs a = {};
   a.k = static_cast<const char*>(cache);
