@@ -1536,7 +1536,7 @@ hipError_t launch_paged(const PagedArgs& a, const PagedPlan& p, hipStream_t stre
   const int64_t head_groups = head_groups_of<D, 1>(a);
   if (!fits(tiles + few, 64 * std::max(p.waves, p.few_waves)) ||
       (p.splits > 1 && !fits(a.rows * head_groups, kMergeThreads<1>)) ||
-      (p.few_groups && !fits(a.requests * rows_each * head_groups, kMergeThreads<1>)))
+      (p.few_groups && !fits((int64_t)a.requests * rows_each * head_groups, kMergeThreads<1>)))
     return kTooLarge;
   if (tiles && few) return launch_both<D, KV4>(a, tiles, few, rows_each, stream);
   if (few)

@@ -45,3 +45,12 @@ def test_a_join_past_the_largest():
     assert need > 0
     for name in NAMES:
         assert _attention(name, ws=16, ws_bytes=need, **args) == UNSUPPORTED
+
+
+def test_more_requests_than_rows():
+    """A join counts all requests, of rows or not, in 64 bits."""
+    args = dict(rows=8, requests=1 << 29, hq=4, hkv=2, most=8, longest=1 << 20)
+    need = _lib.load().qsa_paged_attention_workspace_bytes(8, 1 << 29, 4, 2, 128, 0, 0, 8, 1 << 20)
+    assert need > 0
+    for name in NAMES:
+        assert _attention(name, ws=16, ws_bytes=need, **args) == UNSUPPORTED
