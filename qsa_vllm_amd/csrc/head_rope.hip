@@ -32,7 +32,7 @@ namespace {
 constexpr int kThreads = 256;
 // Rows up to which each has its own group of lanes; past that a group takes four query
 // heads or two of K or V of a token, whose position's row is loaded once: 8304 tokens of
-// 20 heads 16.7 us for 27, but one token 3.7 for 2.6 and 112 into 4 bits 5.0 for 4.1.
+// 20 heads 16.5 us for 27, but one token 3.7 for 2.8 and 112 into 4 bits 5.0 for 3.9.
 constexpr int kSmall = 4096;
 
 struct Rows {  // [tokens, heads, D] bf16, strides in elements

@@ -19,19 +19,22 @@
 // registers; V^T comes from row-major V rows in LDS by the transposing LDS read. The
 // exponentials are rounded to bf16, the matrix cores' type (2^-8 of a weight at
 // most), and the rounded ones are what is summed, in fp32: the weights that meet V
-// add up to 1. They are taken from a base that follows the row's maximum only when
-// that has passed it by 2^8, so that most stages rescale nothing.
+// add up to 1 (but not those of few rows from 4 bits, below). They are taken from a
+// base that follows the row's maximum only when that has passed it by 2^8, so that
+// most stages rescale nothing.
 //
 // A 4-bit cache (kv4.h) is taken apart on the way into LDS: its values are bf16
 // values, exactly, and the rest is the same.
 //
-// Bound by the matrix cores: 8192 rows of 16 heads of 128 in a window of 4096 are 206
-// Gflop and take 256 us, 0.80 Pflop/s (the card's large bf16 product reaches 1.2). A
-// stage is 32 products of a wave and 210 vector instructions (masks, exponentials,
-// packing, addresses), and two waves a SIMD, of workgroups of their own, hide each
-// other's by two thirds. Tried and slower: two groups of four waves in turns in one
-// workgroup (313 us), 64 rows a wave (380: too few registers), raised priority around
-// the products (274), maxima and sums in four chains each (268).
+// 8192 rows of 16 heads of 128 in a window of 4096 are 206 Gflop and take 256 us, 0.80
+// Pflop/s (the card's large bf16 product reaches 1.2). No unit is full: by the counters
+// the matrix cores are busy for 0.44 of the waves' time and the vector unit for 0.47 (from
+// 4 bits, in tiles of 256 rows, 0.33 and 0.51). A stage is 32 products of a wave and 210
+// vector instructions (masks, exponentials, packing, addresses), which follow each other
+// in a wave; two waves a SIMD, of workgroups of their own, overlap them in part. Tried and
+// slower: two groups of four waves in turns in one workgroup (313 us), 64 rows a wave
+// (380: too few registers), raised priority around the products (274), maxima and sums in
+// four chains each (268).
 #include "qsa_common.h"
 #include "../../include/qsa_hip.h"
 #include "kv4.h"
@@ -751,7 +754,8 @@ __global__ __launch_bounds__(kMergeThreads<WAYS>) void paged_merge_kernel(PagedA
 // of a workgroup take blocks of positions in turn, each on its own: K goes from memory
 // into the matrix cores' operand registers, V through the wave's own LDS, so that no
 // wave waits for another until they join their results at the end. The scores are the
-// transposed products of 16 rows, mfma_f32_16x16x32_bf16, weights and sums as above.
+// transposed products of 16 rows, mfma_f32_16x16x32_bf16, weights and sums as above
+// from a bf16 cache.
 //
 // Work is shared out by blocks: requests of more blocks than an equal share of the
 // whole launch are cut into pieces, found on the device, which a second kernel joins.
@@ -768,12 +772,15 @@ __global__ __launch_bounds__(kMergeThreads<WAYS>) void paged_merge_kernel(PagedA
 //   o_d += sum_t (p_t s_tG) (16 + c_td)  -  sum_t (p_t s_tG) (16 + z_tG)
 //
 // the last sums by one more product each: 16 s and s z are bf16 numbers (of 4 and 8
-// bits), the sums of q are split in three. p_t s_tG is rounded to bf16 for both. Over n
-// tokens the sums reach 2^8 n 31 s, where s is at most 0.15 of V's largest magnitude: under
-// 2^128 for magnitudes of 2^117 / n, which is the range that the interface states. Bound by
-// the vector unit, 860 instructions for 64 positions (the codes' bits 256, scales of K
-// and V 128, exponentials 50): 64 tokens on 1024 .. 8192, 82 MB, take 30 us with the
-// joining, one on 131071 24 us (values of fp32 taken apart first: 208 and 330).
+// bits), the sums of q are split in three. p_t s_tG is rounded to bf16 for both (2^-8 of
+// a weight at most); the weights p_t that are summed are not, as a group's scale is not
+// theirs. Over n tokens the sums reach 2^8 n 31 s, where s is at most 0.15 of V's largest
+// magnitude: under 2^128 for magnitudes of 2^117 / n, which is the range that the interface
+// states. 64 tokens on 1024 .. 8192, 82 MB, take 30 us with the joining, one on 131071 24
+// us (values of fp32 taken apart first: 208 and 330). 64 positions are 860 vector
+// instructions (the codes' bits 256, scales of K and V 128, exponentials 50), and the vector
+// unit is busy for 0.59 of the waves' time, the matrix cores for 0.13: the rest is waiting,
+// with two waves a SIMD (206 registers) and one block on its way for each.
 
 constexpr int kFew = 16;
 
@@ -1417,7 +1424,10 @@ PagedPlan make_plan(bool kv4, int rows, int requests, int num_q_heads, int num_k
     // of 256 read K/V half as often and wait for their longest longer: 286 us for 259 on
     // 8192 rows of 16 heads and a window of 4096. From a 4-bit cache, whose values are made
     // once a tile, they are 256: 288 us for 343 on 4 x 500 rows of 16 heads on 8k .. 16k.
-    // Beside requests of few rows, in one launch, both have 4 waves.
+    // Beside requests of few rows, in one launch, both have 4 waves; so have chunks of unlike
+    // lengths, which may hold such requests (500, 500, 500 and 499 rows 330 us, 4 x 500 275).
+    // More than 16 heads a kv head are tiles of 64 rows for single tokens too: 64 tokens of 24
+    // heads of one kv head on 1024 .. 8192 48 us, where memory takes 30.
     p.waves = p.few_units || most > 64 ? 4 : 2;
     if (kv4 && !p.few_units && most > 128) p.waves = 8;
     const int64_t tile_rows = 32 * p.waves;
@@ -1440,7 +1450,7 @@ PagedPlan make_plan(bool kv4, int rows, int requests, int num_q_heads, int num_k
     // on 2000 15.2 us for 17.4, but 1000 on themselves from 4 bits 44 for 31, in two rounds).
     // A workgroup of 8 waves fills a CU: two in turn even out tiles of unlike lengths (four
     // requests on 8k .. 16k 278 us for 341, a prompt of 4096 121 for 167), alike ones need
-    // one (500 rows on 8192 69 us for 86).
+    // one (500 rows on 8192 69 us for 86; measured for one request, as the rule has it).
     const bool alike = p.waves == 8 && requests == 1 && 4 * (int64_t)max_query_len <= max_seq_len;
     const int64_t most_pieces = std::max(stages / 4, std::min(kCUs / units, stages / 2));
     p.splits = (int)std::max<int64_t>(
@@ -1503,7 +1513,8 @@ hipError_t launch_rows_merge(const PagedArgs& a, int rows_each, hipStream_t stre
   if (!a.few_groups) return hipSuccess;
   // The fewer (row, head)s, the more pieces have each: a call of one token on 131071 takes
   // 24 us with 32 ways, 30 with 8, 100 with one; of 64 tokens on 1024 .. 8192 43, 31 and 32;
-  // of 512 on 512 .. 2048 143, 85 and 81.
+  // of 512 on 512 .. 2048 143, 85 and 81. (With 32 ways the last sum spills 19 registers of
+  // 128, 30 at dim 64, and a launch is few workgroups.)
   const int64_t heads = (int64_t)a.requests * rows_each * a.num_q_heads;
   return heads <= 256    ? launch_rows_merge_ways<D, 32>(a, rows_each, stream)
          : heads <= 2048 ? launch_rows_merge_ways<D, 8>(a, rows_each, stream)
