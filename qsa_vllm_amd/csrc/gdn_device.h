@@ -32,14 +32,6 @@ struct GdnRecurLds {
   float sg[kRecTokens], sb[kRecTokens];
 };
 
-__device__ __forceinline__ void unpack8(const u32x4& v, float (&f)[8]) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    f[2 * i] = bf16_lo(v[i]);
-    f[2 * i + 1] = bf16_hi(v[i]);
-  }
-}
-
 // The per-token rule for (sequence, value head) number `block`, 4 waves:
 // sequences shorter than chunk_min.
 __device__ __forceinline__ void gdn_recurrence_block(const GdnRecurArgs& a, int block, GdnRecurLds& L) {

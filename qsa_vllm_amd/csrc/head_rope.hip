@@ -61,20 +61,6 @@ struct HeadRopeArgs {
   FastDiv page_div;
 };
 
-__device__ __forceinline__ void unpack8(const u32x4& v, float (&f)[8]) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    f[2 * i] = bf16_lo(v[i]);
-    f[2 * i + 1] = bf16_hi(v[i]);
-  }
-}
-__device__ __forceinline__ u32x4 pack8(const float (&f)[8]) {
-  u32x4 v;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) v[i] = pack_bf16x2(f[2 * i], f[2 * i + 1]);
-  return v;
-}
-
 // x / d correctly rounded, for the rounded reciprocal r of d: the quotient's residual is
 // exact (Markstein's division step). No operand here is near the type's ends.
 __device__ __forceinline__ float divide(float x, float d, float r) {
@@ -260,8 +246,6 @@ __global__ __launch_bounds__(kThreads) void head_rope_kernel(HeadRopeArgs a) {
     take_heads<D, BITS, kKvRows>(a, part, token, (item - token * a.kv_div.divisor) * kKvRows, j);
   }
 }
-
-bool aligned16(const void* p) { return ((uintptr_t)p & 15u) == 0; }
 
 template <int D, int ROWS>
 void launch_rows(HeadRopeArgs& a, int tokens, int bits, hipStream_t stream) {

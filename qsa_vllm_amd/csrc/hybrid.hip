@@ -52,13 +52,6 @@ __device__ __forceinline__ float sigmoid_f(float x) {
 }
 __device__ __forceinline__ float silu_f(float x) { return x * sigmoid_f(x); }
 
-__device__ __forceinline__ u32x4 pack8(const float (&f)[8]) {
-  u32x4 v;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) v[i] = pack_bf16x2(f[2 * i], f[2 * i + 1]);
-  return v;
-}
-
 // c + a[0] b[0] + a[1] b[1] of bf16 pairs, in fp32.
 __device__ __forceinline__ float dot2(uint32_t a, uint32_t b, float c) {
   typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
@@ -1010,8 +1003,6 @@ bool gdn_shape(int key_heads, int value_heads, int head_dim, int kernel, GdnShap
   }
   return true;
 }
-
-bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 }  // namespace
 }  // namespace qsa

@@ -35,7 +35,7 @@
 // slower: two groups of four waves in turns in one workgroup (313 us), 64 rows a wave
 // (380: too few registers), raised priority around the products (274), maxima and sums in
 // four chains each (268).
-#include "qsa_common.h"
+#include "paged_stage.h"
 #include "../../include/qsa_hip.h"
 #include "kv4.h"
 
@@ -45,17 +45,9 @@
 namespace qsa {
 namespace {
 
-constexpr float kNegInf = -__builtin_huge_valf();
 constexpr int kCUs = 256;
 constexpr int kTok = 64;  // tokens of a stage
-constexpr uint32_t kNoToken = 0xFFFFFFFFu;
 constexpr int kNoWindow = INT_MAX / 2;  // past every position
-constexpr float kSlack = 8.0f;  // log2: how far scores may pass the exponents' base
-// s_waitcnt for the vector-memory counter alone (gfx9 encoding), at 0.
-constexpr int kLoadsDone = (7 << 4) | (15 << 8);
-
-typedef short s16x4 __attribute__((ext_vector_type(4)));
-typedef short s16x8 __attribute__((ext_vector_type(8)));
 
 struct PagedArgs {
   const uint16_t* q;
@@ -94,8 +86,6 @@ struct PagedArgs {
   int few_waves;   // of such a workgroup
   float scale_log2;
 };
-
-__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
 // One request's rows and tokens, kept within the query tensor and the page table
 // whatever the device arrays say.
@@ -187,42 +177,6 @@ __device__ __forceinline__ uint64_t below(int n) {
 __device__ __forceinline__ uint64_t seen_from(const PagedArgs& a, int p, int base) {
   return below(p + 1 - base) & (~below(p - a.window + 1 - base) | below(a.sinks - base));
 }
-// sigmoid(g), 0 and 1 at the infinities. The hardware's exponential and reciprocal:
-// off by 2^-20 for gates to 10, by 2^-17 for the least: far inside the output's 2^-8.
-__device__ __forceinline__ float gate_factor(uint16_t g) {
-  return __builtin_amdgcn_rcpf(1.0f + __expf(-bf16_lo(g)));
-}
-
-// Byte offset of 16-byte unit `unit` of token `tok`'s row in a K stage: units are
-// permuted by the token so that 8 tokens' same unit (what one pass of the A
-// operand's read takes) lie in different banks.
-template <int D>
-__device__ __forceinline__ int k_swizzle(int tok) {
-  return D == 128 ? tok & 15 : (tok >> 1) & 7;
-}
-template <int D>
-__device__ __forceinline__ int k_at(int tok, int unit) {
-  return (tok * (D / 8) + (unit ^ k_swizzle<D>(tok))) * 16;
-}
-// The same for V, permuted in 32-byte units (what the transposing read takes).
-template <int D>
-__device__ __forceinline__ int v_swizzle(int tok) {
-  return D == 128 ? (tok & 7) << 1 : ((tok >> 1) & 3) << 1;
-}
-template <int D>
-__device__ __forceinline__ int v_at(int tok, int unit) {
-  return (tok * (D / 8) + (unit ^ v_swizzle<D>(tok))) * 16;
-}
-
-// Lane i of 16 passes the address of 4 dims of token i / 4 and gets dim i of the four.
-__device__ __forceinline__ s16x4 read_transposed(const char* p) {
-  return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p);
-}
-__device__ __forceinline__ void load_to_lds(const char* src, char* dst) {  // 16 bytes a lane
-  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src,
-                                   (__attribute__((address_space(3))) void*)dst, 16, 0, 0);
-}
-
 // Whether any of eight bf16 values is an infinity or NaN; and 0 in their place.
 __device__ __forceinline__ bool not_finite(const u32x4& v) {
   bool bad = false;
@@ -239,12 +193,6 @@ __device__ __forceinline__ u32x4 finite_or_zero(u32x4 v) {
   return v;
 }
 
-// max over the two lanes of a query row.
-__device__ __forceinline__ float max_over_halves(float v) {
-  const uint32_t b = __builtin_bit_cast(uint32_t, v);
-  const auto r = __builtin_amdgcn_permlane32_swap(b, b, false, false);
-  return fmaxf(__builtin_bit_cast(float, (uint32_t)r[0]), __builtin_bit_cast(float, (uint32_t)r[1]));
-}
 // c + both halves of a pair of bf16 values.
 __device__ __forceinline__ float add_pair(uint32_t pair, float c) {
   typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
@@ -883,13 +831,6 @@ __device__ __forceinline__ bool find_share(const PagedArgs& a, int place, Share&
   return s.kv < a.kv_heads;
 }
 
-// max over the four lanes of a query row.
-__device__ __forceinline__ float max_over_quarters(float v) {
-  v = max_over_halves(v);
-  const uint32_t b = __builtin_bit_cast(uint32_t, v);
-  const auto r = __builtin_amdgcn_permlane16_swap(b, b, false, false);
-  return fmaxf(__builtin_bit_cast(float, (uint32_t)r[0]), __builtin_bit_cast(float, (uint32_t)r[1]));
-}
 __device__ __forceinline__ float sum_over_quarters(float v) {
   v = sum_wave_halves(v);
   const uint32_t b = __builtin_bit_cast(uint32_t, v);
@@ -1556,17 +1497,6 @@ hipError_t launch_paged(const PagedArgs& a, const PagedPlan& p, hipStream_t stre
   return p.waves == 2   ? launch_tiles<D, 2, KV4>(a, tiles, stream)
          : p.waves == 4 ? launch_tiles<D, 4, KV4>(a, tiles, stream)
                         : launch_tiles<D, KV4 ? 8 : 4, KV4>(a, tiles, stream);
-}
-
-bool aligned16(const void* p) { return ((uintptr_t)p & 15u) == 0; }
-
-// Elements from a cache's first token row to its last, -1 if a stride is negative or
-// the span past 2^62.
-int64_t cache_span(int64_t blocks, int64_t block_stride, int64_t page, int64_t token_stride) {
-  if (block_stride < 0 || token_stride < 0 || block_stride >= INT64_MAX / 4 / (blocks + 1) ||
-      token_stride >= INT64_MAX / 4 / page)
-    return -1;
-  return blocks > 0 ? (blocks - 1) * block_stride + (page - 1) * token_stride : 0;
 }
 
 // What both entry points check and set; the caches are theirs.

@@ -48,21 +48,6 @@ struct NormRope {
   int rotary;
 };
 
-__device__ __forceinline__ void unpack8(const u32x4& v, float (&f)[8]) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    f[2 * i] = bf16_lo(v[i]);
-    f[2 * i + 1] = bf16_hi(v[i]);
-  }
-}
-
-__device__ __forceinline__ u32x4 pack8(const float (&f)[8]) {
-  u32x4 v;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) v[i] = pack_bf16x2(f[2 * i], f[2 * i + 1]);
-  return v;
-}
-
 __device__ __forceinline__ float round_bf16(float x) { return bf16_lo(pack_bf16x2(x, 0.0f)); }
 
 // Sum over the 16 lanes of a row group (lanes 16 k .. 16 k + 15).
@@ -550,8 +535,6 @@ int check_norm_rope(int dim, int rotary, int max_positions, const void* weight, 
     return fail(QSA_ERR_INVALID, std::string(name) + ": weight and rotary cache must be 16-byte aligned");
   return QSA_OK;
 }
-
-bool aligned16(const void* p) { return ((uintptr_t)p & 15u) == 0; }
 
 }  // namespace
 }  // namespace qsa

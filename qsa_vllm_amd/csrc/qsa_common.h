@@ -25,6 +25,8 @@ void set_error(const std::string& message);
 int fail(int status, const std::string& message);
 int check_launch(const char* what);
 
+inline bool aligned16(const void* p) { return ((uintptr_t)p & 15u) == 0; }
+
 // ---------------------------------------------------------------------------
 // Device helpers.
 // ---------------------------------------------------------------------------
@@ -46,6 +48,21 @@ __device__ __forceinline__ float bf16_lo(uint32_t pair) {
 }
 __device__ __forceinline__ float bf16_hi(uint32_t pair) {
   return __builtin_bit_cast(float, pair & 0xffff0000u);
+}
+
+// 8 bf16 values as fp32, and fp32 values rounded to bf16.
+__device__ __forceinline__ void unpack8(const u32x4& v, float (&f)[8]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    f[2 * i] = bf16_lo(v[i]);
+    f[2 * i + 1] = bf16_hi(v[i]);
+  }
+}
+__device__ __forceinline__ u32x4 pack8(const float (&f)[8]) {
+  u32x4 v;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = pack_bf16x2(f[2 * i], f[2 * i + 1]);
+  return v;
 }
 
 __device__ __forceinline__ float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }

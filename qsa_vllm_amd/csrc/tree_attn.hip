@@ -49,7 +49,7 @@
 // 64 nodes on 131072 tokens, 103 us, the matrix cores with the softmax between
 // them (0.67 PFLOP/s; 1.4 in a large library product). One request of 8 nodes on
 // 500 tokens, 14.5 us, is two launches' chains of loads.
-#include "qsa_common.h"
+#include "paged_stage.h"
 #include "../../include/qsa_hip.h"
 
 #include <algorithm>
@@ -60,17 +60,9 @@ namespace {
 
 constexpr int kWaves = 4;
 constexpr int kCUs = 256;
-constexpr float kNegInf = -__builtin_huge_valf();
 
 constexpr int kTok = 64;         // tokens of a stage
 constexpr int kTileRows = 128;  // (node, head) rows of a workgroup
-constexpr uint32_t kNoToken = 0xFFFFFFFFu;
-constexpr float kSlack = 8.0f;   // log2: how far scores may pass the exponents' base
-// s_waitcnt for the vector-memory counter alone (gfx9 encoding), at 0.
-constexpr int kLoadsDone = (7 << 4) | (15 << 8);
-
-typedef short s16x4 __attribute__((ext_vector_type(4)));
-typedef short s16x8 __attribute__((ext_vector_type(8)));
 
 struct TreeArgs {
   const uint16_t* q;
@@ -127,7 +119,6 @@ __device__ __forceinline__ Request uniform_request(const TreeArgs& a, int b) {  
   return make_request(a, load_uniform(a.query_start_loc + b), load_uniform(a.query_start_loc + b + 1),
                       load_uniform(a.context_lens + b));
 }
-__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 __device__ __forceinline__ int tiles_of(const TreeArgs& a, const Request& r) {
   return (r.nodes * a.group + kTileRows - 1) / kTileRows;
 }
@@ -204,40 +195,6 @@ __device__ __forceinline__ int locate(const TreeArgs& a, int tile, int& place) {
   return a.requests;
 }
 
-// sigmoid(g), 0 and 1 at the infinities. The hardware's exponential and reciprocal:
-// off by 2^-20 for gates to 10, by 2^-17 for the least: far inside the output's 2^-8.
-__device__ __forceinline__ float gate_factor(uint16_t g) {
-  return __builtin_amdgcn_rcpf(1.0f + __expf(-__builtin_bit_cast(float, (uint32_t)g << 16)));
-}
-
-// Byte offset of 16-byte unit `unit` of token `tok`'s row in a K stage: units
-// are permuted by the token so that 16 tokens' same unit (the A operand's
-// read) lie in different banks.
-template <int D>
-__device__ __forceinline__ int k_swizzle(int tok) {
-  return D == 128 ? tok & 15 : (tok >> 1) & 7;
-}
-template <int D>
-__device__ __forceinline__ int k_at(int tok, int unit) {
-  return (tok * (D / 8) + (unit ^ k_swizzle<D>(tok))) * 16;
-}
-// The same for V, permuted in 32-byte units (what the transposing read takes
-// of a token).
-template <int D>
-__device__ __forceinline__ int v_swizzle(int tok) {
-  return D == 128 ? (tok & 7) << 1 : ((tok >> 1) & 3) << 1;
-}
-template <int D>
-__device__ __forceinline__ int v_at(int tok, int unit) {
-  return (tok * (D / 8) + (unit ^ v_swizzle<D>(tok))) * 16;
-}
-
-// Lane l (group g = l / 16, member n) passes the address of 4 dims of token
-// 4 g + n / 4 and gets dim n of the group's four tokens.
-__device__ __forceinline__ s16x4 read_transposed(const char* p) {
-  return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p);
-}
-
 // c += A B over 32 tokens (two subtiles' operands) or, when the wave has a
 // single subtile, over its 16.
 template <int SUB>
@@ -269,11 +226,6 @@ struct Shape {
   static constexpr size_t kLds = 4 * kStage > kMerge ? 4 * kStage : kMerge;
 };
 
-__device__ __forceinline__ void load_to_lds(const char* src, char* dst) {  // 16 bytes a lane
-  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src,
-                                   (__attribute__((address_space(3))) void*)dst, 16, 0, 0);
-}
-
 // Which 16-bit halves hold an infinity or NaN (bf16), as bits; and 0 in their place.
 __device__ __forceinline__ uint32_t not_finite(const u32x4& v) {
   uint32_t bits = 0;
@@ -290,16 +242,6 @@ __device__ __forceinline__ u32x4 finite_or_zero(u32x4 v) {
   for (int w = 0; w < 4; ++w)
     v[w] &= (bits >> (2 * w) & 1 ? 0u : 0xFFFFu) | (bits >> (2 * w + 1) & 1 ? 0u : 0xFFFF0000u);
   return v;
-}
-
-// max over the four lanes (n, 0 .. 3) of a query row.
-__device__ __forceinline__ float max_over_groups(float v) {
-  uint32_t b = __builtin_bit_cast(uint32_t, v);
-  auto r = __builtin_amdgcn_permlane32_swap(b, b, false, false);
-  v = fmaxf(__builtin_bit_cast(float, (uint32_t)r[0]), __builtin_bit_cast(float, (uint32_t)r[1]));
-  b = __builtin_bit_cast(uint32_t, v);
-  r = __builtin_amdgcn_permlane16_swap(b, b, false, false);
-  return fmaxf(__builtin_bit_cast(float, (uint32_t)r[0]), __builtin_bit_cast(float, (uint32_t)r[1]));
 }
 
 // What a row sees of 64 positions: bit i for drafted node j + i, set for the
@@ -494,7 +436,7 @@ __device__ __forceinline__ void attend_tile(const TreeArgs& a, const Request& rq
       if (__any(top > base[i] + slack)) {
         // Only the rows that passed it: a row's bits are its own. (A row that has
         // seen nothing yet has -inf, and so has one whose scores are NaN.)
-        const float row_top = max_over_groups(top);
+        const float row_top = max_over_quarters(top);
         const float m = row_top > base[i] + slack ? row_top : base[i];
         const float shrink =
             m == kNegInf ? 1.0f : fast_exp2((base[i] - m) * a.scale_log2);
@@ -885,17 +827,6 @@ hipError_t launch_tree(const TreeArgs& a, const TreePlan& plan, int max_nodes, h
   return pairs * a.requests <= 2048 ? launch_merge<D, 8>(a, pairs, stream)
                                     : launch_merge<D, 1>(a, pairs, stream);
 }
-
-// Elements from a cache's first token row to its last, -1 if a stride is negative
-// or the span past 2^62.
-int64_t cache_span(int64_t blocks, int64_t block_stride, int64_t page, int64_t token_stride) {
-  if (block_stride < 0 || token_stride < 0 || block_stride >= INT64_MAX / 4 / (blocks + 1) ||
-      token_stride >= INT64_MAX / 4 / page)
-    return -1;
-  return blocks > 0 ? (blocks - 1) * block_stride + (page - 1) * token_stride : 0;
-}
-
-bool aligned16(const void* p) { return ((uintptr_t)p & 15u) == 0; }
 
 }  // namespace
 }  // namespace qsa
